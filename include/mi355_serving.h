@@ -295,6 +295,84 @@ int mi355_fmha_fwd_ws(const void* Q, const void* K, const void* V, void* O, floa
 int mi355_fmha_fwd_noalloc(const void* Q, const void* K, const void* V, void* O, float* LSE, int B, int Hq, int Hkv, int Sq,
                            int Sk, int D, float scale, int causal, int kv_valid_len, const int64_t* strides, void* stream);
 
+/*
+ * ---- A key-value cache in pages -------------------------------------------------------------------------------------------
+ *
+ * A pool of pages that the sequences of a batch share. A page holds page_size tokens of Hkv key heads followed by Hkv value heads, 128 wide:
+ * element [page][head][slot][d] lies at pages + page*page_stride + head*head_stride + slot*row_stride + d (16-bit elements; strides
+ * positive multiples of 8, pages 16-byte aligned). page_size is a multiple of 16. Key j of sequence b lies in page block_table[b*table_stride +
+ * j / page_size], slot j % page_size; entries outside [0, n_pages) hold no keys (they are masked where keys are read, and nothing is
+ * written there). seq_lens[b] counts the keys of sequence b, those of this call's tokens among them, which are its last ones; it is cut to
+ * [0, max_pages * page_size]. new_lens[b] (may be NULL) says how many of the S rows of a padded batch are tokens, the first ones: row i
+ * of `new` tokens is key seq_lens[b] - new + i and sees the keys up to that one; rows behind them give O = 0 and LSE = -inf. A
+ * sequence of length 0 gives the same.
+ *
+ * weights (fp32) and key_positions (int32), [n_pages][Hkv][page_size] contiguous, hold what eviction goes by: the attention each key has
+ * had from the queries of its kv head, and the position of its token in the text. Both may be NULL where a call does not need them.
+ *
+ * Lengths, table and positions are read on the device: no call waits for it, and a captured call serves what the tensors hold when it
+ * is replayed. No page may belong to two sequences of a call that write it. B * Hkv <= 65535.
+ *
+ * The library allocates nothing for these calls: what *_workspace_bytes says (0: NULL will do) is the caller's, 16-byte aligned, its
+ * contents irrelevant before and after; calls that share a workspace must be ordered on one stream. The reference has no counterpart: its caller grows
+ * one tensor a layer (`past_key_value.update`, benchmarks/flashattn-cuda/modeling_llama.py:664-668).
+ */
+typedef struct mi355_paged_kv {
+    void* pages;
+    const int32_t* block_table;
+    const int32_t* seq_lens;
+    const int32_t* new_lens;
+    float* weights;
+    int32_t* key_positions;
+    int64_t page_stride, head_stride, row_stride, table_stride; /* elements */
+    int32_t n_pages, page_size, max_pages; /* pages of the pool, tokens of a page, entries of a sequence's row of the table */
+    int32_t B, Hkv, dtype;                 /* MI355_DTYPE_FP16 or MI355_DTYPE_BF16 */
+} mi355_paged_kv;
+
+/*
+ * Attention of S rows (the new token of a generation step; a few drafted ones; a chunk of a prompt) of every sequence over its pages:
+ * O = softmax(scale * Q K^T + mask) V, LSE [B, Hq, S] (may be NULL) its natural log-sum-exp. Q and O are [B, Hq, S, 128] with `strides` = q_batch,
+ * q_head, q_row, o_batch, o_head, o_row in elements (multiples of 8, not negative; NULL: contiguous). Query head h reads kv head h / (Hq / Hkv).
+ * Where cache->weights is given, each key's probabilities, summed over the query heads of its kv head and the rows, are added to
+ * it. Sums and statistics are fp32, in an order that depends on the sizes and lengths alone; the probabilities are rounded to the element type for
+ * the second product. What a row does not see has no influence on it, infinities and NaN included. new_lens of NULL with S rows and
+ * a sequence shorter than S: its first rows see nothing.
+ */
+size_t mi355_fmha_paged_workspace_bytes(const mi355_paged_kv* cache, int Hq, int S, int want_lse);
+int mi355_fmha_paged(const mi355_paged_kv* cache, const void* Q, void* O, float* LSE, int Hq, int S, const int64_t* strides, float scale,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * mi355_rope_qkv for a cache in pages: token (b, t) of the fused projection qkv ([q_heads | Hkv key heads | Hkv value heads] of 128 at
+ * qkv + b*x_batch + t*x_row) has its queries rotated in place; its rotated keys and its values go to key seq_lens[b] - new + t of its sequence,
+ * whose weight becomes 0 and whose key_positions entry positions[b*pos_batch + t] where those are given. keep_keys != 0: the
+ * rotated keys are stored in qkv as well (for an attention that reads them there). Tables, positions (clamped for the tables only) and arithmetic as
+ * mi355_rope. Rows behind the new tokens are left as they are.
+ */
+int mi355_rope_paged(const mi355_paged_kv* cache, void* qkv, int S, int q_heads, int keep_keys, int64_t x_batch, int64_t x_row,
+                     const float* cos_table, const float* sin_table, const int32_t* positions, int64_t pos_batch, int n_positions, void* stream);
+
+/*
+ * What a prompt's rows attended to: for every key, cache->weights += the sum over the query heads of its kv head and the rows that see it of
+ * exp(scale * q k - LSE), LSE [B, Hq, S] being what the attention over the same keys left. last_rows > 0: only the last `last_rows` tokens of
+ * each sequence count. Rows whose LSE is -inf add nothing. q_strides: batch, head, row (NULL: contiguous [B, Hq, S, 128]).
+ */
+size_t mi355_fmha_key_weights_workspace_bytes(const mi355_paged_kv* cache, int Hq, int S, int last_rows);
+int mi355_fmha_key_weights(const mi355_paged_kv* cache, const void* Q, const float* LSE, int Hq, int S, const int64_t* q_strides,
+                           int last_rows, float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Eviction: every kv head of a sequence longer than `budget` (>= 1) keeps `budget` keys: first those whose position is within `recent` of
+ * the largest position that the kv head holds (position > largest - recent), then those of the largest weights (NaN lowest); of equals, the
+ * lowest slots. The kept keys that lie behind the budget move, in order, into the slots of the dropped ones in front of it, with their
+ * values, weights and positions, so the sequence is `budget` long afterwards and its keys lie in no particular order; each kv head keeps keys of its own. Slots
+ * from `budget` on are left as they are. lens_out[b] = min(seq_lens[b], budget); lens_out may not overlap seq_lens, which is not written. Both
+ * weights and key_positions are needed; new_lens is not read.
+ */
+size_t mi355_cache_evict_workspace_bytes(const mi355_paged_kv* cache, int budget);
+int mi355_cache_evict(const mi355_paged_kv* cache, int budget, int recent, int32_t* lens_out, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
 /* Thread-local text for the last non-zero return of this thread ("" if none). */
 const char* mi355_last_error(void);
 

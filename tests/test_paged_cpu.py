@@ -1,0 +1,113 @@
+"""CPU-only checks of the paged key-value cache's entry points: what they refuse, before anything is launched."""
+import ctypes
+
+import pytest
+import torch
+
+import fmha_unified
+
+ops = fmha_unified.ops
+P = 0x10000   # an address that nothing reads
+
+
+def cache(lib, **other):
+    c = dict(pages=P, block_table=P, seq_lens=P, new_lens=None, weights=P, key_positions=P, page_stride=16 * 16 * 128, head_stride=16 * 128, row_stride=128,
+             table_stride=8, n_pages=32, page_size=16, max_pages=8, B=4, Hkv=8, dtype=0)
+    c.update(other)
+    return lib.PagedKV(**c)
+
+
+BAD_CACHES = [dict(pages=None), dict(block_table=None), dict(seq_lens=None), dict(pages=P + 8), dict(B=0), dict(Hkv=0), dict(n_pages=0), dict(max_pages=0),
+              dict(page_size=0), dict(page_size=8), dict(page_size=24), dict(dtype=2), dict(table_stride=7), dict(page_stride=0), dict(head_stride=64),
+              dict(row_stride=129), dict(row_stride=-128), dict(row_stride=1 << 24), dict(page_size=1 << 20, row_stride=1 << 20), dict(B=9000),
+              dict(max_pages=1 << 28, table_stride=1 << 28), dict(max_pages=1 << 22, table_stride=1 << 22, B=1000, Hkv=10)]
+
+
+@pytest.mark.parametrize("bad", BAD_CACHES, ids=lambda d: "-".join("%s=%s" % x for x in d.items()))
+def test_every_entry_point_refuses_a_bad_cache(lib, bad):
+    cdll, c = lib.load(), cache(lib, **bad)
+    big = 1 << 60   # a workspace that is large enough whatever it is asked to be
+    for rc in (cdll.mi355_fmha_paged(c, P, P, P, 32, 1, None, 0.1, P, big, None),
+               cdll.mi355_rope_paged(c, P, 1, 32, 0, 48 * 128, 48 * 128, P, P, P, 0, 100, None),
+               cdll.mi355_fmha_key_weights(c, P, P, 32, 1, None, 0, 0.1, P, big, None),
+               cdll.mi355_cache_evict(c, 10, 5, P * 16, P, big, None)):
+        assert rc in (lib.ERR_BAD_ARGUMENT, lib.ERR_UNSUPPORTED)
+        assert cdll.mi355_last_error()
+    assert cdll.mi355_fmha_paged(None, P, P, P, 32, 1, None, 0.1, P, big, None) == lib.ERR_BAD_ARGUMENT
+
+
+def test_attention_refuses_bad_arguments(lib):
+    cdll, c, big = lib.load(), cache(lib), 1 << 60
+
+    def call(Q=P, O=P, Hq=32, S=1, strides=None, scale=0.1, ws=P, size=big):
+        st = None if strides is None else (ctypes.c_int64 * 6)(*strides)
+        return cdll.mi355_fmha_paged(c, Q, O, P, Hq, S, st, scale, ws, size, None)
+
+    ok = [4096, 128, 128, 4096, 128, 128]
+    for kw in (dict(Q=None), dict(O=None), dict(Q=P + 2), dict(O=P + 2), dict(Hq=0), dict(Hq=31), dict(S=0), dict(scale=0.0), dict(scale=float("nan")),
+               dict(scale=float("inf")), dict(S=16384), dict(strides=[-8] + ok[1:]), dict(strides=[4] + ok[1:]), dict(strides=ok[:2] + [1 << 24] + ok[3:]),
+               dict(strides=ok[:4] + [64, 128]), dict(strides=ok[:3] + [0, 128, 128])):
+        assert call(**kw) in (lib.ERR_BAD_ARGUMENT, lib.ERR_UNSUPPORTED), kw
+    # a workspace is needed for the scores that the account is made from
+    need = cdll.mi355_fmha_paged_workspace_bytes(c, 32, 1, 1)
+    assert need > 0
+    for kw in (dict(ws=None), dict(size=need - 1), dict(ws=P + 4)):
+        assert call(**kw) == lib.ERR_BAD_ARGUMENT
+        assert b"workspace" in cdll.mi355_last_error()
+    # none without an account, up to 512 keys
+    assert cdll.mi355_fmha_paged_workspace_bytes(cache(lib, weights=None), 32, 1, 1) == 0
+
+
+def test_the_other_entry_points_refuse_bad_arguments(lib):
+    cdll, c, big = lib.load(), cache(lib), 1 << 60
+    row = 48 * 128
+
+    def rope(qkv=P, S=2, q_heads=32, x_batch=2 * row, x_row=row, cos=P, sin=P, pos=P, pos_batch=0, n=100):
+        return cdll.mi355_rope_paged(c, qkv, S, q_heads, 0, x_batch, x_row, cos, sin, pos, pos_batch, n, None)
+
+    for kw in (dict(qkv=None), dict(cos=None), dict(sin=None), dict(pos=None), dict(qkv=P + 2), dict(cos=P + 4), dict(S=0), dict(q_heads=-1), dict(n=0),
+               dict(x_row=row - 8), dict(x_row=row + 4), dict(x_batch=row - 8), dict(x_batch=-8), dict(pos_batch=1), dict(S=1 << 30)):
+        assert rope(**kw) in (lib.ERR_BAD_ARGUMENT, lib.ERR_UNSUPPORTED), kw
+
+    def kw_call(Q=P, LSE=P, Hq=32, S=4, strides=None, last=0, scale=0.1, cc=c):
+        st = None if strides is None else (ctypes.c_int64 * 3)(*strides)
+        return cdll.mi355_fmha_key_weights(cc, Q, LSE, Hq, S, st, last, scale, P, big, None)
+
+    for kw in (dict(Q=None), dict(LSE=None), dict(Hq=31), dict(S=0), dict(last=-1), dict(scale=-1.0), dict(strides=[8, 8, 4]), dict(cc=cache(lib, weights=None))):
+        assert kw_call(**kw) in (lib.ERR_BAD_ARGUMENT, lib.ERR_UNSUPPORTED), kw
+
+    def evict(budget=10, recent=5, out=P * 16, ws=P, size=big, cc=c):
+        return cdll.mi355_cache_evict(cc, budget, recent, out, ws, size, None)
+
+    need = cdll.mi355_cache_evict_workspace_bytes(c, 10)
+    for kw in (dict(budget=0), dict(recent=-1), dict(out=None), dict(out=P), dict(out=P + 12), dict(out=P - 12), dict(ws=None), dict(size=need - 1),
+               dict(cc=cache(lib, weights=None)), dict(cc=cache(lib, key_positions=None))):
+        assert evict(**kw) == lib.ERR_BAD_ARGUMENT, kw
+
+
+def tensors(B=2, Hq=8, Hkv=2, S=1, page=16, n_pages=5, max_pages=2):
+    kv = torch.zeros(n_pages, 2 * Hkv, page, 128, dtype=torch.float16)
+    table, lens = torch.zeros(B, max_pages, dtype=torch.int32), torch.zeros(B, dtype=torch.int32)
+    return dict(q=torch.zeros(B, Hq, S, 128, dtype=torch.float16), kv_pages=kv, block_table=table, seq_lens=lens)
+
+
+def test_operators_refuse_what_is_not_on_the_gpu_and_wrong_shapes():
+    t = tensors()
+    w, pos = torch.zeros(5, 2, 16), torch.zeros(5, 2, 16, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="GPU tensor"):
+        ops.fine_fmha_paged(**t)
+    with pytest.raises(RuntimeError, match="GPU tensor"):
+        ops.fine_evict_paged(t["kv_pages"], t["block_table"], t["seq_lens"], w, pos, 4, 2)
+    for name, bad in (("kv_pages", torch.zeros(5, 3, 16, 128, dtype=torch.float16)), ("kv_pages", torch.zeros(5, 4, 16, 64, dtype=torch.float16)),
+                      ("kv_pages", torch.zeros(5, 4, 16, 128)), ("kv_pages", torch.zeros(0, 4, 16, 128, dtype=torch.float16)),
+                      ("kv_pages", torch.zeros(5, 4, 128, 16, dtype=torch.float16).transpose(2, 3)), ("block_table", torch.zeros(2, dtype=torch.int32)),
+                      ("block_table", torch.zeros(2, 0, dtype=torch.int32))):
+        with pytest.raises(RuntimeError, match=name):
+            ops.fine_fmha_paged(**dict(t, **{name: bad}))
+
+
+def test_operators_name_what_they_write():
+    for name, written in (("finefmha_paged", ["weights"]), ("finefmha_paged_lse", ["weights"]), ("rope_paged", ["qkv", "kv_pages", "weights", "key_positions"]),
+                          ("key_weights", ["weights"]), ("evict_paged", ["kv_pages", "weights", "key_positions"])):
+        schema = getattr(torch.ops.fmha_unified, name).default._schema
+        assert [a.name for a in schema.arguments if a.alias_info is not None and a.alias_info.is_write] == written

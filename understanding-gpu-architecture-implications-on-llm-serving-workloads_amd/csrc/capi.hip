@@ -435,6 +435,132 @@ int mi355_internal_step_gate_up(const void* x, const void* norm_weight, float ep
 }
 
 
+// ---- the paged key-value cache ----
+static int paged_checked(const char* fn, const mi355_paged_kv* c) {
+    if (!c || !c->pages || !c->block_table || !c->seq_lens) return fail(MI355_ERR_BAD_ARGUMENT, "%s: null pointer", fn);
+    if (c->dtype != MI355_DTYPE_FP16 && c->dtype != MI355_DTYPE_BF16) return fail(MI355_ERR_BAD_ARGUMENT, "%s: unknown dtype %d", fn, c->dtype);
+    if (c->B < 1 || c->Hkv < 1 || c->n_pages < 1 || c->max_pages < 1)
+        return fail(MI355_ERR_BAD_ARGUMENT, "%s: B, Hkv, n_pages and max_pages must be >= 1 (got %d, %d, %d, %d)", fn, c->B, c->Hkv, c->n_pages, c->max_pages);
+    if (c->page_size < 16 || c->page_size % 16 != 0)
+        return fail(MI355_ERR_UNSUPPORTED, "%s: page_size must be a positive multiple of 16 (got %d)", fn, c->page_size);
+    const int64_t pairs = (int64_t)c->B * c->Hkv, max_len = (int64_t)c->max_pages * c->page_size;
+    if (pairs > 65535) return fail(MI355_ERR_UNSUPPORTED, "%s: B * Hkv must be at most 65535 (got %lld)", fn, (long long)pairs);
+    if (max_len > INT32_MAX - 1024 || pairs * (max_len / 32 + 1) > INT32_MAX)
+        return fail(MI355_ERR_UNSUPPORTED, "%s: %d sequences of up to %lld keys of %d heads are more than a call takes", fn, c->B, (long long)max_len, c->Hkv);
+    if (c->B > 1 && c->table_stride < c->max_pages)
+        return fail(MI355_ERR_BAD_ARGUMENT, "%s: rows of the block table overlap (stride %lld, %d entries)", fn, (long long)c->table_stride, c->max_pages);
+    const int64_t strides[3] = {c->page_stride, c->head_stride, c->row_stride};
+    for (int64_t x : strides)
+        if (x < 128 || x % 8 != 0)
+            return fail(MI355_ERR_BAD_ARGUMENT, "%s: strides of the pages must be multiples of 8 elements, 128 or more (got %lld, %lld, %lld)", fn,
+                        (long long)strides[0], (long long)strides[1], (long long)strides[2]);
+    if (c->row_stride >= (1 << 24) || c->row_stride * 2 * c->page_size > INT32_MAX)
+        return fail(MI355_ERR_UNSUPPORTED, "%s: row stride %lld of the pages is too large", fn, (long long)c->row_stride);
+    if (!aligned16(c->pages)) return fail(MI355_ERR_BAD_ARGUMENT, "%s: pages must be 16-byte aligned", fn);
+    return 0;
+}
+
+static int paged_queries_checked(const char* fn, const mi355_paged_kv* c, const void* Q, int Hq, int S, const int64_t* strides, int n, float scale) {
+    if (!Q) return fail(MI355_ERR_BAD_ARGUMENT, "%s: null pointer", fn);
+    if (Hq < 1 || S < 1) return fail(MI355_ERR_BAD_ARGUMENT, "%s: Hq and S must be >= 1", fn);
+    if (Hq % c->Hkv != 0) return fail(MI355_ERR_BAD_ARGUMENT, "%s: Hq (%d) must be a multiple of Hkv (%d)", fn, Hq, c->Hkv);
+    if ((int64_t)(Hq / c->Hkv) * S > 65535)
+        return fail(MI355_ERR_UNSUPPORTED, "%s: Hq / Hkv * S must be at most 65535 (got %d / %d * %d)", fn, Hq, c->Hkv, S);
+    if (!(scale > 0.f) || scale > 3.0e38f) return fail(MI355_ERR_BAD_ARGUMENT, "%s: scale must be positive and finite (got %g)", fn, (double)scale);
+    if (!aligned16(Q)) return fail(MI355_ERR_BAD_ARGUMENT, "%s: Q must be 16-byte aligned", fn);
+    for (int i = 0; i < n; ++i)
+        if (strides[i] < 0 || strides[i] % 8 != 0)
+            return fail(MI355_ERR_BAD_ARGUMENT, "%s: stride %d is %lld; strides must be non-negative multiples of 8 elements", fn, i, (long long)strides[i]);
+    if (strides[2] >= (1 << 24)) return fail(MI355_ERR_UNSUPPORTED, "%s: the row stride of Q must be below 2^24 elements (got %lld)", fn, (long long)strides[2]);
+    return 0;
+}
+
+static int workspace_checked(const char* fn, size_t need, const void* workspace, size_t bytes) {
+    if (need > 0 && (workspace == nullptr || bytes < need || !aligned16(workspace)))
+        return fail(MI355_ERR_BAD_ARGUMENT, "%s: workspace of %zu bytes at %p; this call needs %zu bytes, 16-byte aligned (%s_workspace_bytes)", fn, bytes,
+                    workspace, need, fn);
+    return 0;
+}
+
+size_t mi355_fmha_paged_workspace_bytes(const mi355_paged_kv* cache, int Hq, int S, int want_lse) {
+    if (!cache || cache->B < 1 || cache->Hkv < 1 || Hq < cache->Hkv || S < 1 || cache->max_pages < 1 || cache->page_size < 1) return 0;
+    return mi355::fmha_paged_workspace(*cache, Hq, S, want_lse != 0);
+}
+
+int mi355_fmha_paged(const mi355_paged_kv* cache, const void* Q, void* O, float* LSE, int Hq, int S, const int64_t* strides, float scale,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+    const char* fn = "mi355_fmha_paged";
+    if (int rc = paged_checked(fn, cache)) return rc;
+    if (!O) return fail(MI355_ERR_BAD_ARGUMENT, "%s: null pointer", fn);
+    const int64_t dense[6] = {(int64_t)Hq * S * 128, (int64_t)S * 128, 128, (int64_t)Hq * S * 128, (int64_t)S * 128, 128};
+    const int64_t* st = strides ? strides : dense;
+    if (int rc = paged_queries_checked(fn, cache, Q, Hq, S, st, 6, scale)) return rc;
+    if (!aligned16(O)) return fail(MI355_ERR_BAD_ARGUMENT, "%s: O must be 16-byte aligned", fn);
+    if ((S > 1 && st[5] < 128) || (Hq > 1 && st[4] < 128) || (cache->B > 1 && st[3] < 128))
+        return fail(MI355_ERR_BAD_ARGUMENT, "%s: rows of O overlap (o strides %lld, %lld, %lld)", fn, (long long)st[3], (long long)st[4], (long long)st[5]);
+    if (int rc = workspace_checked(fn, mi355::fmha_paged_workspace(*cache, Hq, S, LSE != nullptr), workspace, workspace_bytes)) return rc;
+    const long l[6] = {(long)st[0], (long)st[1], (long)st[2], (long)st[3], (long)st[4], (long)st[5]};
+    const hipError_t e = mi355::fmha_paged_dispatch(*cache, Q, O, LSE, Hq, S, l, scale, workspace, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? 0 : hip_fail(e, fn);
+}
+
+int mi355_rope_paged(const mi355_paged_kv* cache, void* qkv, int S, int q_heads, int keep_keys, int64_t x_batch, int64_t x_row,
+                     const float* cos_table, const float* sin_table, const int32_t* positions, int64_t pos_batch, int n_positions, void* stream) {
+    const char* fn = "mi355_rope_paged";
+    if (int rc = paged_checked(fn, cache)) return rc;
+    if (!qkv || !cos_table || !sin_table || !positions) return fail(MI355_ERR_BAD_ARGUMENT, "%s: null pointer", fn);
+    if (S < 1 || q_heads < 0 || n_positions < 1) return fail(MI355_ERR_BAD_ARGUMENT, "%s: S, n_positions >= 1 and q_heads >= 0 required", fn);
+    const int64_t heads = (int64_t)q_heads + 2 * (int64_t)cache->Hkv;
+    if ((int64_t)cache->B * S > INT32_MAX || heads > 65535 * 32) return fail(MI355_ERR_UNSUPPORTED, "%s: too many tokens or heads", fn);
+    if (x_row < heads * 128 || x_row % 8 || x_batch < 0 || x_batch % 8 || (cache->B > 1 && x_batch < heads * 128))
+        return fail(MI355_ERR_BAD_ARGUMENT, "%s: rows of qkv overlap or strides are no multiples of 8 (batch %lld, row %lld, %lld heads)", fn,
+                    (long long)x_batch, (long long)x_row, (long long)heads);
+    if (pos_batch != 0 && pos_batch < S) return fail(MI355_ERR_BAD_ARGUMENT, "%s: pos_batch must be 0 or >= S (got %lld)", fn, (long long)pos_batch);
+    if (!aligned16(qkv) || !aligned16(cos_table) || !aligned16(sin_table))
+        return fail(MI355_ERR_BAD_ARGUMENT, "%s: pointers must be 16-byte aligned", fn);
+    const hipError_t e = mi355::rope_paged_dispatch(*cache, qkv, S, q_heads, keep_keys, (long)x_batch, (long)x_row, cos_table, sin_table, positions,
+                                                    (long)pos_batch, n_positions, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? 0 : hip_fail(e, fn);
+}
+
+size_t mi355_fmha_key_weights_workspace_bytes(const mi355_paged_kv* cache, int Hq, int S, int last_rows) {
+    if (!cache || cache->B < 1 || cache->Hkv < 1 || Hq < cache->Hkv || S < 1 || cache->max_pages < 1 || cache->page_size < 1) return 0;
+    return mi355::key_weights_workspace(*cache, Hq, S, last_rows);
+}
+
+int mi355_fmha_key_weights(const mi355_paged_kv* cache, const void* Q, const float* LSE, int Hq, int S, const int64_t* q_strides,
+                           int last_rows, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* fn = "mi355_fmha_key_weights";
+    if (int rc = paged_checked(fn, cache)) return rc;
+    if (!LSE || !cache->weights) return fail(MI355_ERR_BAD_ARGUMENT, "%s: null pointer", fn);
+    if (last_rows < 0) return fail(MI355_ERR_BAD_ARGUMENT, "%s: last_rows must be >= 0 (got %d)", fn, last_rows);
+    const int64_t dense[3] = {(int64_t)Hq * S * 128, (int64_t)S * 128, 128};
+    const int64_t* st = q_strides ? q_strides : dense;
+    if (int rc = paged_queries_checked(fn, cache, Q, Hq, S, st, 3, scale)) return rc;
+    if (int rc = workspace_checked(fn, mi355::key_weights_workspace(*cache, Hq, S, last_rows), workspace, workspace_bytes)) return rc;
+    const long l[3] = {(long)st[0], (long)st[1], (long)st[2]};
+    const hipError_t e = mi355::key_weights_dispatch(*cache, Q, LSE, Hq, S, l, last_rows, scale, workspace, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? 0 : hip_fail(e, fn);
+}
+
+size_t mi355_cache_evict_workspace_bytes(const mi355_paged_kv* cache, int budget) {
+    if (!cache || cache->B < 1 || cache->Hkv < 1 || budget < 1 || cache->max_pages < 1 || cache->page_size < 1) return 0;
+    return mi355::evict_workspace(*cache, budget);
+}
+
+int mi355_cache_evict(const mi355_paged_kv* cache, int budget, int recent, int32_t* lens_out, void* workspace, size_t workspace_bytes,
+                      void* stream) {
+    const char* fn = "mi355_cache_evict";
+    if (int rc = paged_checked(fn, cache)) return rc;
+    if (!cache->weights || !cache->key_positions || !lens_out) return fail(MI355_ERR_BAD_ARGUMENT, "%s: null pointer", fn);
+    if (budget < 1 || recent < 0) return fail(MI355_ERR_BAD_ARGUMENT, "%s: budget >= 1 and recent >= 0 required (got %d, %d)", fn, budget, recent);
+    if (lens_out < cache->seq_lens + cache->B && cache->seq_lens < lens_out + cache->B)
+        return fail(MI355_ERR_BAD_ARGUMENT, "%s: lens_out overlaps seq_lens", fn);
+    if (int rc = workspace_checked(fn, mi355::evict_workspace(*cache, budget), workspace, workspace_bytes)) return rc;
+    const hipError_t e = mi355::evict_dispatch(*cache, budget, recent, lens_out, workspace, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? 0 : hip_fail(e, fn);
+}
+
 const char* mi355_last_error(void) { return g_err; }
 
 int mi355_serving_version(void) { return MI355_SERVING_VERSION; }

@@ -1,0 +1,643 @@
+// Attention of one new token (or a few) of every sequence over a paged key-value cache, for gfx950 (MI355X).
+//
+//   s = scale q k^T over the keys j <= i + len - new of the sequence (row i of `new` tokens, which are its last ones)
+//   O = softmax(s) V,  LSE = log sum exp s,  and where the cache keeps account: weights[page][kv head][slot] += sum over the query heads of the
+//   kv head and the rows of exp(s - LSE)
+//
+// Bound by the one read of K and V from HBM (512 bytes a key and kv head for 4 * 128 flops a query row). The lengths of a batch differ and
+// are known to the device only, so the cut of the work is made there: the key tiles (32 keys) of all (sequence, kv head) pairs
+// lie one behind the other on one axis, and each of a fixed number of workgroups takes an equal piece of it, whatever pairs
+// the piece touches. A part of a pair leaves an unnormalised partial result (O~ [128], m, l a column, fp32); a second kernel joins the
+// parts of a pair. Where a pair is walked by one workgroup it writes O and LSE itself.
+//
+// Inside a part: the query rows of all heads of the kv head are the columns of S^T = K Q^T (MFMA 16x16x32), so K and V are read
+// once per kv head. The waves cut the part into contiguous pieces; each streams its tiles through two private LDS stages with
+// direct-to-LDS copies, no barriers, and keeps a running maximum and sum. 16 keys lie in one page: a lane works out the
+// address of one such half tile of the next 64, and the scalar unit picks them up one after the other.
+#include <algorithm>
+
+#include "paged.h"
+
+namespace mi355 {
+
+namespace pdec {
+constexpr int D = 128;
+constexpr int TK = 32;                       // keys per tile
+constexpr int ROW_BYTES = D * 2;             // 256
+constexpr int TILE_BYTES = TK * ROW_BYTES;   // 8 KiB
+constexpr int STAGE_BYTES = 2 * TILE_BYTES;  // K + V
+constexpr int WAVES = 4, NSTAGE = 2;
+constexpr int NTHREADS = WAVES * 64;
+constexpr int WAVE_BYTES = NSTAGE * STAGE_BYTES;
+constexpr int LDS_BYTES = WAVES * WAVE_BYTES;   // 128 KiB
+constexpr int COPIES = 2 * (TILE_BYTES / 1024);
+constexpr int WINDOW = 32;                   // tiles whose addresses a wave holds at a time (64 half tiles, one a lane)
+constexpr float kLazyLog2 = 8.f;             // rescale only when a column maximum grows by more than 2^8
+constexpr int PART_STRIDE = D + 4;           // floats per (part, column): O~[128], m, l, 2 pad (keeps rows 16-byte aligned)
+constexpr int kWorkgroups = 256;             // one per CU
+constexpr int kMinTiles = 4;                 // of a workgroup: one per wave
+constexpr int kDirectLen = 512;              // up to this many keys a workgroup per (sequence, kv head) walks them all
+
+__device__ __forceinline__ int swz_k(int row) { return row & 15; }
+__device__ __forceinline__ int swz_v(int row) { return (row & 7) << 1; }
+__device__ __forceinline__ float quad_max(float x) {
+    x = fmaxf(x, __shfl_xor(x, 16, 64));
+    return fmaxf(x, __shfl_xor(x, 32, 64));
+}
+__device__ __forceinline__ float quad_sum(float x) {
+    x += __shfl_xor(x, 16, 64);
+    return x + __shfl_xor(x, 32, 64);
+}
+}  // namespace pdec
+
+struct PagedAttn {
+    const void* Q;
+    void* O;
+    float* LSE;       // may be nullptr
+    float* part;      // [workgroup + pair][column of a block][PART_STRIDE] per block of columns
+    float* scores;    // [pair][max_tiles][ncols][32], where the cache keeps account
+    long q_batch, q_head, q_row, o_batch, o_head, o_row;
+    long part_block;  // floats of `part` per block of columns
+    int Hq, Sq, group, ncols, col_block;   // columns of a kv head, and of a workgroup
+    int workgroups, min_tiles, direct, max_tiles;
+    float scale_log2;
+    Divisor by_sq, by_hkv;
+};
+
+namespace pdec {
+
+// Where the work is cut: `quota` tiles a workgroup over the axis of all pairs' tiles.
+struct Cut {
+    int total, quota;
+};
+// One sequence on that axis: its number, its length, its tiles and those of the sequences in front of it (per kv head).
+struct Where {
+    int b, len, tiles, before;
+};
+__device__ __forceinline__ int tiles_of(int len) { return (len + TK - 1) / TK; }
+
+// The lengths of up to 64 sequences at a time, one a lane. With up to 64 of them both functions work on the same registers.
+struct Lengths {
+    const PagedKv& kv;
+    int lane, len, incl;   // of sequence `first + lane`
+    int first;
+    __device__ __forceinline__ Lengths(const PagedKv& kv_) : kv(kv_), lane(threadIdx.x & 63), first(-1) {}
+    __device__ __forceinline__ void load(int b0) {
+        if (first == b0) return;
+        first = b0;
+        const int b = b0 + lane;
+        len = b < kv.B ? paged_len(kv, b) : 0;
+        incl = wave_inclusive_sum(tiles_of(len));
+    }
+    __device__ __forceinline__ Cut cut(const PagedAttn& a) {
+        int total = 0;
+        for (int b0 = 0; b0 < kv.B; b0 += 64) {
+            load(b0);
+            total += __builtin_amdgcn_readlane(incl, 63);
+        }
+        total *= kv.Hkv;
+        return {total, max((int)((uint32_t)(total + a.workgroups - 1) / (uint32_t)a.workgroups), a.min_tiles)};
+    }
+    __device__ __forceinline__ Where pick(int i, int before) const {
+        const int n = __builtin_amdgcn_readlane(len, i), t = tiles_of(n);
+        return {first + i, n, t, before + __builtin_amdgcn_readlane(incl, i) - t};
+    }
+    // the sequence that tile f of the axis belongs to (f < total)
+    __device__ __forceinline__ Where find(int f) {
+        int before = 0;
+        for (int b0 = 0;; b0 += 64) {
+            load(b0);
+            const uint64_t past = __builtin_amdgcn_ballot_w64(f < (before + incl) * kv.Hkv);
+            if (past != 0) return pick(__builtin_ctzll(past), before);
+            before += __builtin_amdgcn_readlane(incl, 63);
+            if (b0 + 64 >= kv.B) return {kv.B - 1, 0, 0, before};   // (not reached for f < total)
+        }
+    }
+    // sequence b
+    __device__ __forceinline__ Where at(int b) {
+        int before = 0;
+        for (int b0 = 0;; b0 += 64) {
+            load(b0);
+            if (b < b0 + 64) return pick(b - b0, before);
+            before += __builtin_amdgcn_readlane(incl, 63);
+        }
+    }
+};
+
+}  // namespace pdec
+
+// Grid: (workgroups, blocks of columns). NB: blocks of 16 columns of a workgroup. SCORES: the scores are kept for
+// paged_weights_kernel.
+template <typename T, int NB, bool SCORES>
+__global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, PagedAttn a) {
+    using namespace pdec;
+    using V8 = typename Elem<T>::v8;
+    extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    MI355_LDS char* wbase = (MI355_LDS char*)smem_raw + wave * WAVE_BYTES;
+    const int g = lane >> 4;
+    const int c16 = lane & 15;
+    const int col0 = blockIdx.y * a.col_block;
+    const int ncols = min(a.col_block, a.ncols - col0);   // of this workgroup, <= 16 NB
+    const T* Q = (const T*)a.Q;
+    T* O = (T*)a.O;
+
+    Lengths lengths(kv);
+    Where seq;
+    int f = 0, f_end = 0, hkv, tile0;
+    if (a.direct) {
+        const int b = divide(blockIdx.x, a.by_hkv);
+        hkv = blockIdx.x - b * kv.Hkv;
+        const int len = __builtin_amdgcn_readfirstlane(paged_len(kv, b));
+        seq = {b, len, tiles_of(len), 0};
+        tile0 = 0;
+        f_end = seq.tiles;
+    } else {
+        const Cut cut = lengths.cut(a);
+        f = blockIdx.x * cut.quota;
+        f_end = min(f + cut.quota, cut.total);
+        if (f >= f_end) return;
+        seq = lengths.find(f);
+        const int rest = f - seq.before * kv.Hkv;
+        hkv = (int)((uint32_t)rest / (uint32_t)seq.tiles);
+        tile0 = rest - hkv * seq.tiles;
+    }
+
+    for (;;) {   // the parts of this workgroup: tiles tile0 .. tile0 + n - 1 of (seq.b, hkv)
+        const int n = min(seq.tiles - tile0, f_end - f);
+        const int per_wave = (n + WAVES - 1) / WAVES;
+        const int t_begin = tile0 + min(wave * per_wave, n);
+        const int n_loc = tile0 + min((wave + 1) * per_wave, n) - t_begin;
+        const int b = seq.b, len = seq.len;
+        const int* table = kv.table + (long)b * kv.table_stride;
+        const char* heads = kv.pages + (long)hkv * kv.head_bytes;
+        const long v_off = (long)kv.Hkv * kv.head_bytes;
+
+        // half tile h of the window (a lane's own): the address of its 16 keys; a lane without keys or with a page outside the pool
+        // has its bit in `bad` and the pool's first page to read
+        uint32_t adr_lo = 0, adr_hi = 0;
+        uint64_t bad = 0;
+        auto load_window = [&](int first_tile) {
+            const int key = (first_tile * 2 + lane) * 16;
+            int page = 0, slot = 0;
+            bool ok = key < len;
+            if (ok) {
+                const int i = divide(key, kv.by_page);
+                page = table[i];
+                slot = key - i * kv.page_size;
+                ok = (uint32_t)page < (uint32_t)kv.n_pages;
+            }
+            bad = __builtin_amdgcn_ballot_w64(!ok);
+            const uint64_t adr = (uint64_t)(uintptr_t)heads + (ok ? (uint64_t)page * kv.page_bytes + (uint32_t)slot * kv.row_bytes : 0);
+            adr_lo = (uint32_t)adr;
+            adr_hi = (uint32_t)(adr >> 32);
+        };
+        // tile i of this wave's piece into stage `slot`: copy c covers rows 4c + lane / 16 of the tile, chunk lane % 16; rows behind
+        // the last key repeat it (masked later)
+        const int c_row = lane >> 4;
+        const uint32_t chunk = lane & 15;
+        uint64_t bad_next = 0;   // halves (bit 0, 1) of the tile issued last that hold no keys at all
+        auto issue_stage = [&](int i, int slot) {
+            if ((i & (WINDOW - 1)) == 0) load_window(t_begin + i);
+            MI355_LDS char* st = wbase + slot * STAGE_BYTES;
+            const int w = (i & (WINDOW - 1)) * 2;
+            bad_next = (bad >> w) & 3;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const char* kb = (const char*)(uintptr_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)adr_lo, w + h) |
+                                                          (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)adr_hi, w + h) << 32);
+                const char* vb = kb + v_off;
+                const int last = max(min(len - 1 - ((t_begin + i) * 2 + h) * 16, 15), 0);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int row = 4 * c + c_row;
+                    copy16_global_to_lds(kb, (uint32_t)min(row, last) * kv.row_bytes + ((chunk ^ swz_k(row)) << 4), st + (4 * h + c) * 1024);
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int row = 4 * c + c_row;
+                    copy16_global_to_lds(vb, (uint32_t)min(row, last) * kv.row_bytes + ((chunk ^ swz_v(row)) << 4),
+                                         st + TILE_BYTES + (4 * h + c) * 1024);
+                }
+            }
+        };
+        const int k_base = c16 * ROW_BYTES + ((g ^ c16) << 4);   // xor (ks << 6), + kb * 16 rows
+        const int v_row = 4 * g + (c16 >> 2);
+        const int v_base = TILE_BYTES + v_row * ROW_BYTES + ((((c16 & 3) >> 1) ^ swz_v(v_row)) << 4) + (c16 & 1) * 8;  // xor (db << 5)
+
+        float4v o[NB][8];
+        float m_run[NB], l_run[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            m_run[nb] = -INFINITY;
+            l_run[nb] = 0.f;
+#pragma unroll
+            for (int db = 0; db < 8; ++db) o[nb][db] = float4v{0.f, 0.f, 0.f, 0.f};
+        }
+        uint64_t bad_of[NSTAGE];   // of the tile in each stage
+        if (n_loc > 0) issue_stage(0, 0);
+        bad_of[0] = bad_next;
+        bad_of[1] = 0;
+        // queries behind the first copies: column c of the kv head = (its query head c / Sq, row c % Sq)
+        const int n_new = paged_new(kv, b, a.Sq);
+        int lim[NB];      // last visible key of this lane's column(s); -1: none
+        int qrow[NB];
+        V8 qf[NB][4];     // Q[column][32 ks + 8 g .. +7]
+        int lim_min = len - 1, lim_max = -1;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const int col = col0 + min(16 * nb + c16, ncols - 1);
+            const int head = divide(col, a.by_sq);
+            const int qi = col - head * a.Sq;
+            const T* qp = Q + b * a.q_batch + (long)(hkv * a.group + head) * a.q_head + qi * a.q_row + 8 * g;
+            qrow[nb] = qi;
+            lim[nb] = qi < n_new ? min(len - 1, qi + len - n_new) : -1;
+            lim_min = min(lim_min, lim[nb]);
+            lim_max = max(lim_max, lim[nb]);
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) qf[nb][ks] = *(const V8*)(qp + ks * 32);
+        }
+        int row_min = a.Sq, row_max = -1;   // rows of the columns of this wave
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) row_min = min(row_min, qrow[nb]), row_max = max(row_max, qrow[nb]);
+#pragma unroll
+        for (int off = 8; off >= 1; off >>= 1) {
+            lim_min = min(lim_min, __shfl_xor(lim_min, off, 64));
+            lim_max = max(lim_max, __shfl_xor(lim_max, off, 64));
+            row_min = min(row_min, __shfl_xor(row_min, off, 64));
+            row_max = max(row_max, __shfl_xor(row_max, off, 64));
+        }
+        lim_min = __builtin_amdgcn_readfirstlane(lim_min);
+        lim_max = __builtin_amdgcn_readfirstlane(lim_max);
+        row_min = __builtin_amdgcn_readfirstlane(row_min);
+        row_max = __builtin_amdgcn_readfirstlane(row_max);
+        // a use of the query fragments in front of the loop: their first use inside it would make the compiler wait there, on every
+        // iteration, for everything in flight
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) asm volatile("" : "+v"(qf[nb][0]), "+v"(qf[nb][1]), "+v"(qf[nb][2]), "+v"(qf[nb][3]));
+
+        for (int i = 0; i < n_loc; ++i) {
+            const int slot = i & 1;
+            if (i + 1 < n_loc) {
+                issue_stage(i + 1, slot ^ 1);
+                bad_of[slot ^ 1] = bad_next;
+                wait_vmcnt<COPIES>();   // everything but the newest tile has landed
+            } else {
+                wait_vmcnt<0>();
+            }
+            MI355_LDS char* st = wbase + slot * STAGE_BYTES;
+            const int key0 = (t_begin + i) * TK;
+            const uint64_t no_keys = bad_of[slot];
+
+            // S^T = K Q^T: lane holds keys 16 kb + 4 g + 0..3 of its column
+            float4v s[NB][2];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) s[nb][0] = s[nb][1] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) {
+                    V8 kf = Elem<T>::frag(lds_read_b128(st + ((k_base ^ (ks << 6)) + kb * 16 * ROW_BYTES)));
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) s[nb][kb] = Elem<T>::mfma16(kf, qf[nb][ks], s[nb][kb]);
+                }
+            const bool masked = key0 + TK - 1 > lim_min || no_keys != 0;
+            if (masked) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (key0 + 16 * (e >> 2) + 4 * g + (e & 3) > lim[nb] || ((no_keys >> (e >> 2)) & 1)) s[nb][e >> 2][e & 3] = -INFINITY;
+            }
+            if constexpr (SCORES) {
+                float* sp = a.scores + (((long)b * kv.Hkv + hkv) * a.max_tiles + t_begin + i) * (a.ncols * TK);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+                    if (16 * nb + c16 < ncols) {
+                        *(float4v*)(sp + (16 * nb + c16) * TK + 4 * g) = s[nb][0];
+                        *(float4v*)(sp + (16 * nb + c16) * TK + 16 + 4 * g) = s[nb][1];
+                    }
+            }
+            // lazy rescaling: m_run is the exponent reference of the running sums and only moves (with O and l rescaled) when
+            // some score exceeds it by more than 2^kLazyLog2
+            float mx[NB];
+            bool raise = false;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                mx[nb] = fmaxf(fmaxf(fmaxf(s[nb][0][0], s[nb][0][1]), fmaxf(s[nb][0][2], s[nb][0][3])),
+                               fmaxf(fmaxf(s[nb][1][0], s[nb][1][1]), fmaxf(s[nb][1][2], s[nb][1][3])));
+                raise = raise || (mx[nb] - m_run[nb]) * a.scale_log2 > kLazyLog2;  // -inf - -inf = NaN compares false
+            }
+            if (__builtin_amdgcn_ballot_w64(raise) != 0) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    const float m_new = fmaxf(m_run[nb], quad_max(mx[nb]));
+                    const float m_use = (m_new == -INFINITY) ? 0.f : m_new;
+                    const float alpha = __builtin_amdgcn_exp2f((m_run[nb] - m_use) * a.scale_log2);
+                    m_run[nb] = m_new;
+                    l_run[nb] *= alpha;
+#pragma unroll
+                    for (int db = 0; db < 8; ++db) o[nb][db] *= alpha;
+                }
+            }
+            V8 pf[NB];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                const float neg_ms = (m_run[nb] == -INFINITY) ? 0.f : -m_run[nb] * a.scale_log2;
+                float psum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nb][e >> 2][e & 3], a.scale_log2, neg_ms));
+                    psum += p;
+                    pf[nb][e] = (T)p;   // the second product's operand: 16 bits, at most half a step off each
+                }
+                l_run[nb] += psum;
+            }
+            // O^T += V^T P^T; the 8 keys of a lane of P are 4 g + 0..3 and 16 + 4 g + 0..3, V^T is gathered in that order
+            if (!masked) {
+#pragma unroll
+                for (int db = 0; db < 8; ++db) {
+                    MI355_LDS char* vp = st + (v_base ^ (db << 5));
+                    V8 vf = Elem<T>::frag(concat(lds_read_tr16_b64(vp), lds_read_tr16_b64(vp + 16 * ROW_BYTES)));
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) o[nb][db] = Elem<T>::mfma16(vf, pf[nb], o[nb][db]);
+                }
+            } else if (key0 <= lim_max) {
+                // A product with p = 0 is not nothing where v is infinite or NaN: what a row does not see is taken out of V, row by
+                // row, and the sum is taken over for that row's columns alone.
+                for (int r = row_min; r <= row_max; ++r) {
+                    const int last = r < n_new ? min(len - 1, r + len - n_new) : -1;
+#pragma unroll
+                    for (int db = 0; db < 8; ++db) {
+                        MI355_LDS char* vp = st + (v_base ^ (db << 5));
+                        V8 vf = Elem<T>::frag(concat(lds_read_tr16_b64(vp), lds_read_tr16_b64(vp + 16 * ROW_BYTES)));
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (key0 + 16 * (e >> 2) + 4 * g + (e & 3) > last || ((no_keys >> (e >> 2)) & 1)) vf[e] = (T)0.f;
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) {   // (of the row's own columns)
+                            const float4v sum = Elem<T>::mfma16(vf, pf[nb], o[nb][db]);
+                            if (qrow[nb] == r) o[nb][db] = sum;
+                        }
+                    }
+                }
+            }
+            wait_lgkmcnt<0>();  // the reads of this slot are complete before a later copy refills it
+        }
+
+        // ---- the waves' results meet in LDS (their stages are free): per wave O~ [ncols][128] floats, then m [32], l [32] ----
+        __syncthreads();
+        MI355_LDS float* cmb = (MI355_LDS float*)smem_raw;
+        const int wave_floats = ncols * D + 64;
+        {
+            MI355_LDS float* mine = cmb + wave * wave_floats;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                const int col = 16 * nb + c16;
+                const float l_tot = quad_sum(l_run[nb]);
+                if (col < ncols) {
+#pragma unroll
+                    for (int db = 0; db < 8; ++db) *(MI355_LDS float4v*)(mine + col * D + db * 16 + 4 * g) = o[nb][db];
+                    if (g == 0) {
+                        mine[ncols * D + col] = m_run[nb];
+                        mine[ncols * D + 32 + col] = l_tot;
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        const bool whole = n == seq.tiles;   // this part is all of its pair
+        float* part = a.part + (whole ? 0 : blockIdx.y * a.part_block + (long)(blockIdx.x + b * kv.Hkv + hkv) * (a.col_block * PART_STRIDE));
+        for (int e4 = tid; e4 < ncols * (D / 4); e4 += NTHREADS) {   // output elements (column e4 / 32, d 4 (e4 % 32) .. +3)
+            const int c = e4 >> 5, d = (e4 & 31) * 4;
+            float mw[WAVES], lw[WAVES];
+            float4v ow[WAVES];
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                mw[w] = cmb[w * wave_floats + ncols * D + c];
+                lw[w] = cmb[w * wave_floats + ncols * D + 32 + c];
+                ow[w] = *(MI355_LDS const float4v*)(cmb + w * wave_floats + 4 * e4);
+            }
+            float m = -INFINITY, l = 0.f;
+            float4v acc = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) m = fmaxf(m, mw[w]);
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                // a wave without a visible key has no weight
+                const float wgt = (mw[w] == -INFINITY) ? 0.f : __builtin_amdgcn_exp2f((mw[w] - m) * a.scale_log2);
+                acc += wgt * ow[w];
+                l += wgt * lw[w];
+            }
+            if (whole) {
+                const float inv = l != 0.f ? 1.f / l : 0.f;
+                const int head = divide(col0 + c, a.by_sq), qi = col0 + c - head * a.Sq, hq = hkv * a.group + head;
+                typename Elem<T>::v4 ov;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) ov[e] = (T)(acc[e] * inv);
+                *(typename Elem<T>::v4*)(O + b * a.o_batch + (long)hq * a.o_head + qi * a.o_row + d) = ov;
+                if (a.LSE != nullptr && d == 0)
+                    a.LSE[((long)b * a.Hq + hq) * a.Sq + qi] = l != 0.f ? (m * a.scale_log2 + __builtin_log2f(l)) * 0.69314718055994531f : -INFINITY;
+            } else {
+                *(float4v*)(part + c * PART_STRIDE + d) = acc;
+                if (d == 0) {
+                    part[c * PART_STRIDE + D] = m;
+                    part[c * PART_STRIDE + D + 1] = l;
+                }
+            }
+        }
+        f += n;
+        if (f >= f_end || n == 0) return;
+        __syncthreads();   // the next part's copies overwrite what was read above
+        // the next pair: tiles are left in front of f_end, so one with tiles follows
+        tile0 = 0;
+        if (++hkv == kv.Hkv) {
+            hkv = 0;
+            seq = lengths.find(f);
+        }
+    }
+}
+
+// Joins the parts of each (pair, column): grid (pairs, columns of all blocks). O = sum_p 2^((m_p - m) c) O~_p / sum_p 2^((m_p - m) c) l_p. Pairs without a key
+// get zeros, those of one part were written by its workgroup.
+template <typename T>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedKv kv, PagedAttn a) {
+    using namespace pdec;
+    __shared__ __attribute__((aligned(16))) float sums[8][D + 4];
+    const int b = divide(blockIdx.x, a.by_hkv), hkv = blockIdx.x - b * kv.Hkv;
+    Lengths lengths(kv);
+    const Cut cut = lengths.cut(a);
+    const Where seq = lengths.at(b);
+    const int f = seq.before * kv.Hkv + hkv * seq.tiles;
+    const int first = (int)((uint32_t)f / (uint32_t)cut.quota);
+    const int n = seq.tiles == 0 ? 0 : (int)((uint32_t)(f + seq.tiles - 1) / (uint32_t)cut.quota) - first + 1;
+    if (n == 1) return;
+    const int col = blockIdx.y, cb = (int)((uint32_t)col / (uint32_t)a.col_block), c = col - cb * a.col_block;
+    const int head = divide(col, a.by_sq), qi = col - head * a.Sq, hq = hkv * a.group + head;
+    const int part0 = threadIdx.x >> 5, d = (threadIdx.x & 31) * 4;
+    const long stride = (long)a.col_block * PART_STRIDE;
+    const float* base = a.part + cb * a.part_block + (long)(first + blockIdx.x) * stride + c * PART_STRIDE;
+    float m = -INFINITY, l = 0.f;
+    float4v acc = float4v{0.f, 0.f, 0.f, 0.f};
+    for (int p = part0; p < n; p += 8) {
+        const float* pp = base + p * stride;
+        const float4v v = *(const float4v*)(pp + d);
+        const float mp = pp[D], lp = pp[D + 1];
+        const float m_new = fmaxf(m, mp);
+        if (mp != -INFINITY) {
+            const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - m_new) * a.scale_log2);
+            const float wgt = __builtin_amdgcn_exp2f((mp - m_new) * a.scale_log2);
+            acc = acc * keep + v * wgt;
+            l = l * keep + lp * wgt;
+            m = m_new;
+        } else {   // no score above minus infinity: nothing, or NaN
+            acc += v;
+            l += lp;
+        }
+    }
+    *(float4v*)&sums[part0][d] = acc;
+    if (d == 0) sums[part0][D] = m, sums[part0][D + 1] = l;
+    __syncthreads();
+    if (threadIdx.x >= 32) return;
+    float m_all = -INFINITY;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) m_all = fmaxf(m_all, sums[p][D]);
+    acc = float4v{0.f, 0.f, 0.f, 0.f};
+    l = 0.f;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+        const float mp = sums[p][D];
+        const float wgt = mp == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mp - m_all) * a.scale_log2);
+        acc += *(const float4v*)&sums[p][d] * wgt;
+        l += sums[p][D + 1] * wgt;
+    }
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    typename Elem<T>::v4 ov;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ov[e] = (T)(acc[e] * inv);
+    *(typename Elem<T>::v4*)((T*)a.O + b * a.o_batch + (long)hq * a.o_head + qi * a.o_row + d) = ov;
+    if (a.LSE != nullptr && d == 0)
+        a.LSE[((long)b * a.Hq + hq) * a.Sq + qi] = l != 0.f ? (m_all * a.scale_log2 + __builtin_log2f(l)) * 0.69314718055994531f : -INFINITY;
+}
+
+// weights[page][kv head][slot] += sum over the pair's columns of 2^(s c - LSE): grid (tiles / 8, pairs), a thread per key
+__global__ __launch_bounds__(256) void paged_weights_kernel(PagedKv kv, PagedAttn a) {
+    using namespace pdec;
+    __shared__ float lse[32];
+    const int b = divide(blockIdx.y, a.by_hkv), hkv = blockIdx.y - b * kv.Hkv;
+    const int len = paged_len(kv, b);
+    const int key = blockIdx.x * 256 + threadIdx.x;
+    if ((int)(blockIdx.x * 256) >= len) return;
+    if ((int)threadIdx.x < a.ncols) {
+        const float x = a.LSE[((long)b * a.Hq + hkv * a.group) * a.Sq + threadIdx.x];   // columns are consecutive rows
+        lse[threadIdx.x] = x == -INFINITY ? INFINITY : x * 1.4426950408889634f;         // a row that sees no key adds nothing
+    }
+    __syncthreads();
+    if (key >= len) return;
+    const float* sp = a.scores + ((long)blockIdx.y * a.max_tiles + (key >> 5)) * (a.ncols * TK) + (key & 31);
+    float sum = 0.f;
+    for (int c = 0; c < a.ncols; ++c) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(sp[c * TK], a.scale_log2, -lse[c]));
+    const int i = divide(key, kv.by_page);
+    const int page = kv.table[(long)b * kv.table_stride + i];
+    if ((uint32_t)page >= (uint32_t)kv.n_pages) return;
+    float* w = kv.weights + ((long)page * kv.Hkv + hkv) * kv.page_size + (key - i * kv.page_size);
+    *w += sum;
+}
+
+// What a call takes of its workspace
+struct PagedPlan {
+    int nb, col_block, blocks, workgroups, direct, max_tiles, scores;
+    size_t part_bytes, score_bytes, lse_bytes;
+};
+static PagedPlan paged_plan(int B, int Hkv, int max_len, int Hq, int Sq, bool weights, bool lse) {
+    using namespace pdec;
+    PagedPlan p = {};
+    const int ncols = Hq / Hkv * Sq;
+    const long pairs = (long)B * Hkv;
+    p.nb = ncols > 16 ? 2 : 1;
+    p.col_block = std::min(ncols, 32);
+    p.blocks = (ncols + p.col_block - 1) / p.col_block;
+    p.max_tiles = (max_len + TK - 1) / TK;
+    p.direct = max_len <= kDirectLen;
+    p.workgroups = p.direct ? (int)pairs : (int)std::min<long>(kWorkgroups, (pairs * p.max_tiles + kMinTiles - 1) / kMinTiles);
+    if (!p.direct) p.part_bytes = sizeof(float) * (size_t)p.blocks * (p.workgroups + pairs) * p.col_block * PART_STRIDE;
+    p.scores = weights && ncols <= 32;
+    if (p.scores) p.score_bytes = sizeof(float) * (size_t)pairs * p.max_tiles * ncols * TK;
+    if (weights && !lse) p.lse_bytes = (sizeof(float) * (size_t)B * Hq * Sq + 15) & ~size_t(15);
+    return p;
+}
+
+size_t fmha_paged_workspace(const mi355_paged_kv& c, int Hq, int Sq, bool lse) {
+    const PagedPlan p = paged_plan(c.B, c.Hkv, c.max_pages * c.page_size, Hq, Sq, c.weights != nullptr, lse);
+    size_t key_weights = 0;
+    if (c.weights != nullptr && !p.scores) key_weights = key_weights_workspace(c, Hq, Sq, 0);
+    return std::max(p.part_bytes, key_weights) + p.score_bytes + p.lse_bytes;
+}
+
+template <typename T, int NB, bool SCORES>
+static hipError_t launch_paged(const PagedKv& kv, const PagedAttn& a, const PagedPlan& p, hipStream_t stream) {
+    using namespace pdec;
+    static DynamicLdsOnce once;
+    const hipError_t e = once.ensure(reinterpret_cast<const void*>(fmha_paged_kernel<T, NB, SCORES>), LDS_BYTES);
+    if (e != hipSuccess) return e;
+    fmha_paged_kernel<T, NB, SCORES><<<dim3(p.workgroups, p.blocks), dim3(NTHREADS), LDS_BYTES, stream>>>(kv, a);
+    return hipGetLastError();
+}
+
+template <typename T>
+static hipError_t fmha_paged_t(const PagedKv& kv, const PagedAttn& a, const PagedPlan& p, hipStream_t stream) {
+    const unsigned pairs = (unsigned)(kv.B * kv.Hkv);
+    hipError_t e = p.nb == 1 ? (p.scores ? launch_paged<T, 1, true>(kv, a, p, stream) : launch_paged<T, 1, false>(kv, a, p, stream))
+                             : (p.scores ? launch_paged<T, 2, true>(kv, a, p, stream) : launch_paged<T, 2, false>(kv, a, p, stream));
+    if (e == hipSuccess && !p.direct) {
+        paged_join_kernel<T><<<dim3(pairs, a.ncols), dim3(256), 0, stream>>>(kv, a);
+        e = hipGetLastError();
+    }
+    if (e == hipSuccess && p.scores) {
+        paged_weights_kernel<<<dim3((kv.max_len + 255) / 256, pairs), dim3(256), 0, stream>>>(kv, a);
+        e = hipGetLastError();
+    }
+    return e;
+}
+
+hipError_t fmha_paged_dispatch(const mi355_paged_kv& c, const void* Q, void* O, float* LSE, int Hq, int Sq, const long* strides, float scale,
+                               void* workspace, hipStream_t stream) {
+    const PagedKv kv = paged_from(c);
+    const PagedPlan p = paged_plan(kv.B, kv.Hkv, kv.max_len, Hq, Sq, kv.weights != nullptr, LSE != nullptr);
+    char* ws = (char*)workspace;
+    PagedAttn a = {};
+    a.Q = Q;
+    a.O = O;
+    if (p.lse_bytes) {   // the account needs the log-sum-exp even where the caller does not
+        a.LSE = (float*)ws;
+        ws += p.lse_bytes;
+    } else {
+        a.LSE = LSE;
+    }
+    a.scores = (float*)ws;
+    ws += p.score_bytes;
+    a.part = (float*)ws;
+    a.q_batch = strides[0], a.q_head = strides[1], a.q_row = strides[2];
+    a.o_batch = strides[3], a.o_head = strides[4], a.o_row = strides[5];
+    a.Hq = Hq;
+    a.Sq = Sq;
+    a.group = Hq / kv.Hkv;
+    a.ncols = a.group * Sq;
+    a.col_block = p.col_block;
+    a.workgroups = p.workgroups;
+    a.min_tiles = pdec::kMinTiles;
+    a.direct = p.direct;
+    a.max_tiles = p.max_tiles;
+    a.part_block = (long)(p.workgroups + kv.B * kv.Hkv) * p.col_block * pdec::PART_STRIDE;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.by_sq = divisor_of(Sq);
+    a.by_hkv = divisor_of(kv.Hkv);
+    hipError_t e = c.dtype == MI355_DTYPE_BF16 ? fmha_paged_t<bf16_t>(kv, a, p, stream) : fmha_paged_t<half_t>(kv, a, p, stream);
+    if (e == hipSuccess && kv.weights != nullptr && !p.scores)   // many rows: from the log-sum-exp, with the scores worked out again
+        e = key_weights_dispatch(c, Q, a.LSE, Hq, Sq, strides, 0, scale, ws, stream);
+    return e;
+}
+
+}  // namespace mi355

@@ -181,6 +181,19 @@ hipError_t rope_dispatch(const void* x, void* out, int B, int S, int inplace_hea
 hipError_t silu_mul_dispatch(const void* in, void* out, long rows, int inter, int block, long ld_in, long ld_out, int dtype,
                              hipStream_t stream);
 
+// The paged key-value cache (arguments as the entry points' after validation). `strides`: q (batch, head, row), o (batch, head, row).
+// `workspace` holds what the *_workspace functions say.
+size_t fmha_paged_workspace(const mi355_paged_kv& cache, int Hq, int Sq, bool lse);
+hipError_t fmha_paged_dispatch(const mi355_paged_kv& cache, const void* Q, void* O, float* LSE, int Hq, int Sq, const long* strides, float scale,
+                               void* workspace, hipStream_t stream);
+size_t key_weights_workspace(const mi355_paged_kv& cache, int Hq, int Sq, int last_rows);
+hipError_t key_weights_dispatch(const mi355_paged_kv& cache, const void* Q, const float* LSE, int Hq, int Sq, const long* q_strides, int last_rows,
+                                float scale, void* workspace, hipStream_t stream);
+hipError_t rope_paged_dispatch(const mi355_paged_kv& cache, void* qkv, int S, int q_heads, int keep_keys, long x_batch, long x_row, const float* cos_t,
+                               const float* sin_t, const int* positions, long pos_batch, int n_pos, hipStream_t stream);
+size_t evict_workspace(const mi355_paged_kv& cache, int budget);
+hipError_t evict_dispatch(const mi355_paged_kv& cache, int budget, int recent, int* lens_out, void* workspace, hipStream_t stream);
+
 }  // namespace mi355
 
 // Test and tuning hooks: exported from the shared library but not part of its public header. They take the kernel

@@ -19,7 +19,9 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
+#include <algorithm>
 #include <cmath>
+#include <optional>
 #include <tuple>
 
 #include "mi355_serving.h"
@@ -105,6 +107,166 @@ std::tuple<at::Tensor, at::Tensor> finefmha_fwd_lse(const at::Tensor& q, const a
     return run_fmha(q, k, v, causal, is_decode, decode_length, true);
 }
 
+// ---- a key-value cache in pages (include/mi355_serving.h: mi355_paged_kv) -----------------------------------------------
+
+void check_like(const char* name, const char* what, const at::Tensor& t, const at::Tensor& like, at::ScalarType type) {
+    TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, ": ", what, " must be a GPU tensor on the device of kv_pages");
+    TORCH_CHECK(t.scalar_type() == type, name, ": ", what, " must be ", type, ", got ", t.scalar_type());
+}
+
+mi355_paged_kv paged_kv(const char* name, const at::Tensor& kv_pages, const at::Tensor& block_table, const at::Tensor& seq_lens,
+                        const std::optional<at::Tensor>& new_lens, const std::optional<at::Tensor>& weights, const std::optional<at::Tensor>& key_positions) {
+    TORCH_CHECK(kv_pages.dim() == 4 && kv_pages.size(3) == 128 && kv_pages.size(1) % 2 == 0 && kv_pages.numel() > 0, name,
+                ": kv_pages must be [n_pages, 2 * Hkv, page_size, 128], got ", kv_pages.sizes());
+    const bool bf16 = kv_pages.scalar_type() == at::kBFloat16;
+    TORCH_CHECK(kv_pages.scalar_type() == at::kHalf || bf16, name, ": kv_pages must be float16 or bfloat16, got ", kv_pages.scalar_type());
+    TORCH_CHECK(kv_pages.stride(3) == 1, name, ": the last dimension of kv_pages must be contiguous");
+    TORCH_CHECK(block_table.dim() == 2 && block_table.numel() > 0, name, ": block_table must be [B, max_pages], got ", block_table.sizes());
+    const int64_t B = block_table.size(0), Hkv = kv_pages.size(1) / 2;
+    TORCH_CHECK(kv_pages.is_cuda(), name, ": kv_pages must be a GPU tensor");
+    check_like(name, "block_table", block_table, kv_pages, at::kInt);
+    TORCH_CHECK(block_table.stride(1) == 1 || block_table.size(1) == 1, name, ": the rows of block_table must be contiguous");
+    const auto lengths = [&](const at::Tensor& t, const char* what) {
+        check_like(name, what, t, kv_pages, at::kInt);
+        TORCH_CHECK(t.dim() == 1 && t.size(0) == B && t.is_contiguous(), name, ": ", what, " must be a contiguous [", B, "] tensor, got ", t.sizes());
+        return t.data_ptr<int32_t>();
+    };
+    const auto account = [&](const std::optional<at::Tensor>& t, const char* what, at::ScalarType type) -> void* {
+        if (!t.has_value()) return nullptr;
+        check_like(name, what, *t, kv_pages, type);
+        TORCH_CHECK(t->dim() == 3 && t->size(0) == kv_pages.size(0) && t->size(1) == Hkv && t->size(2) == kv_pages.size(2) && t->is_contiguous(), name, ": ", what,
+                    " must be a contiguous [", kv_pages.size(0), ", ", Hkv, ", ", kv_pages.size(2), "] tensor, got ", t->sizes());
+        return t->data_ptr();
+    };
+    TORCH_CHECK(kv_pages.size(0) <= INT32_MAX && kv_pages.size(2) <= INT32_MAX && block_table.size(1) <= INT32_MAX && B <= INT32_MAX, name, ": dimension exceeds int32");
+    mi355_paged_kv c = {};
+    c.pages = kv_pages.data_ptr();
+    c.block_table = block_table.data_ptr<int32_t>();
+    c.seq_lens = lengths(seq_lens, "seq_lens");
+    c.new_lens = new_lens.has_value() ? lengths(*new_lens, "new_lens") : nullptr;
+    c.weights = static_cast<float*>(account(weights, "weights", at::kFloat));
+    c.key_positions = static_cast<int32_t*>(account(key_positions, "key_positions", at::kInt));
+    // (a dimension of one element may have any stride)
+    c.row_stride = kv_pages.size(2) > 1 ? kv_pages.stride(2) : 128;
+    c.head_stride = kv_pages.stride(1);
+    c.page_stride = kv_pages.size(0) > 1 ? kv_pages.stride(0) : std::max<int64_t>(kv_pages.stride(0), 128);
+    c.table_stride = block_table.stride(0);
+    c.n_pages = (int32_t)kv_pages.size(0);
+    c.page_size = (int32_t)kv_pages.size(2);
+    c.max_pages = (int32_t)block_table.size(1);
+    c.B = (int32_t)B;
+    c.Hkv = (int32_t)Hkv;
+    c.dtype = bf16 ? MI355_DTYPE_BF16 : MI355_DTYPE_FP16;
+    return c;
+}
+
+// queries [B, Hq, S, 128] of the pages' type and device
+at::Tensor paged_queries(const char* name, const at::Tensor& q, const at::Tensor& kv_pages, const mi355_paged_kv& c) {
+    TORCH_CHECK(q.dim() == 4 && q.size(0) == c.B && q.size(3) == 128 && q.numel() > 0, name, ": q must be [", c.B, ", Hq, S, 128], got ", q.sizes());
+    check_like(name, "q", q, kv_pages, kv_pages.scalar_type());
+    TORCH_CHECK(q.size(1) <= INT32_MAX && q.size(2) <= INT32_MAX, name, ": dimension exceeds int32");
+    return readable_in_place(q) ? q : q.contiguous();
+}
+
+at::Tensor workspace_of(size_t bytes, const at::Tensor& like) {
+    return bytes > 0 ? gpu_empty({static_cast<int64_t>(bytes)}, at::kByte, like) : at::Tensor();
+}
+
+std::tuple<at::Tensor, at::Tensor> run_paged(const at::Tensor& q, const at::Tensor& kv_pages, const at::Tensor& block_table, const at::Tensor& seq_lens,
+                                             const std::optional<at::Tensor>& new_lens, const std::optional<at::Tensor>& weights, bool want_lse) {
+    const char* name = "finefmha_paged";
+    const mi355_paged_kv c = paged_kv(name, kv_pages, block_table, seq_lens, new_lens, weights, std::nullopt);
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(kv_pages.device());
+    const at::Tensor qc = paged_queries(name, q, kv_pages, c);
+    const int64_t Hq = q.size(1), S = q.size(2);
+    at::Tensor o = gpu_empty(q.sizes(), q.scalar_type(), q), lse;
+    if (want_lse) lse = gpu_empty({c.B, Hq, S}, at::kFloat, q);
+    const size_t need = mi355_fmha_paged_workspace_bytes(&c, (int)Hq, (int)S, want_lse ? 1 : 0);
+    const at::Tensor ws = workspace_of(need, q);
+    const int64_t strides[6] = {qc.stride(0), qc.stride(1), qc.stride(2), o.stride(0), o.stride(1), o.stride(2)};
+    hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+    const int rc = mi355_fmha_paged(&c, qc.data_ptr(), o.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr, (int)Hq, (int)S, strides,
+                                    1.0f / std::sqrt(128.0f), need > 0 ? ws.data_ptr() : nullptr, need, stream);
+    TORCH_CHECK(rc == 0, name, ": ", mi355_last_error(), " (code ", rc, ")");
+    return {o, lse};
+}
+
+at::Tensor finefmha_paged(const at::Tensor& q, const at::Tensor& kv_pages, const at::Tensor& block_table, const at::Tensor& seq_lens,
+                          const std::optional<at::Tensor>& new_lens, const std::optional<at::Tensor>& weights) {
+    return std::get<0>(run_paged(q, kv_pages, block_table, seq_lens, new_lens, weights, false));
+}
+
+std::tuple<at::Tensor, at::Tensor> finefmha_paged_lse(const at::Tensor& q, const at::Tensor& kv_pages, const at::Tensor& block_table,
+                                                      const at::Tensor& seq_lens, const std::optional<at::Tensor>& new_lens,
+                                                      const std::optional<at::Tensor>& weights) {
+    return run_paged(q, kv_pages, block_table, seq_lens, new_lens, weights, true);
+}
+
+void rope_paged(const at::Tensor& qkv, const at::Tensor& kv_pages, const at::Tensor& block_table, const at::Tensor& seq_lens, const at::Tensor& cos,
+                const at::Tensor& sin, const at::Tensor& positions, int64_t q_heads, const std::optional<at::Tensor>& new_lens,
+                const std::optional<at::Tensor>& weights, const std::optional<at::Tensor>& key_positions, bool keep_keys) {
+    const char* name = "fine_rope_paged";
+    const mi355_paged_kv c = paged_kv(name, kv_pages, block_table, seq_lens, new_lens, weights, key_positions);
+    TORCH_CHECK(q_heads >= 0 && qkv.dim() == 4 && qkv.size(0) == c.B && qkv.size(2) == q_heads + 2 * (int64_t)c.Hkv && qkv.size(3) == 128 && qkv.numel() > 0, name,
+                ": qkv must be [", c.B, ", S, ", q_heads + 2 * (int64_t)c.Hkv, ", 128], got ", qkv.sizes());
+    check_like(name, "qkv", qkv, kv_pages, kv_pages.scalar_type());
+    TORCH_CHECK(qkv.stride(3) == 1 && qkv.stride(2) == 128, name, ": the heads of a token of qkv must lie side by side");
+    const int64_t B = c.B, S = qkv.size(1);
+    for (const at::Tensor* t : {&cos, &sin}) {
+        check_like(name, "cos and sin", *t, kv_pages, at::kFloat);
+        TORCH_CHECK(t->dim() == 2 && t->size(0) >= 1 && t->size(1) == 64 && t->is_contiguous() && t->sizes() == cos.sizes(), name,
+                    ": cos and sin must be contiguous [n_positions, 64] tensors");
+    }
+    check_like(name, "positions", positions, kv_pages, at::kInt);
+    TORCH_CHECK(positions.is_contiguous() && ((positions.dim() == 2 && positions.size(0) == B && positions.size(1) == S) ||
+                                              (positions.dim() == 1 && positions.size(0) == S)), name, ": positions must be a contiguous [", B, ", ", S, "] or [", S,
+                "] tensor, got ", positions.sizes());
+    TORCH_CHECK(S <= INT32_MAX && q_heads <= INT32_MAX && cos.size(0) <= INT32_MAX, name, ": dimension exceeds int32");
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(kv_pages.device());
+    hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+    const int64_t row = S > 1 ? qkv.stride(1) : (q_heads + 2 * (int64_t)c.Hkv) * 128;
+    const int rc = mi355_rope_paged(&c, qkv.data_ptr(), (int)S, (int)q_heads, keep_keys ? 1 : 0, qkv.stride(0), row, cos.data_ptr<float>(),
+                                    sin.data_ptr<float>(), positions.data_ptr<int32_t>(), positions.dim() == 2 ? S : 0, (int)cos.size(0), stream);
+    TORCH_CHECK(rc == 0, name, ": ", mi355_last_error(), " (code ", rc, ")");
+}
+
+void key_weights(const at::Tensor& q, const at::Tensor& lse, const at::Tensor& kv_pages, const at::Tensor& block_table, const at::Tensor& seq_lens,
+                 const at::Tensor& weights, const std::optional<at::Tensor>& new_lens, int64_t last_rows) {
+    const char* name = "fine_key_weights";
+    const mi355_paged_kv c = paged_kv(name, kv_pages, block_table, seq_lens, new_lens, weights, std::nullopt);
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(kv_pages.device());
+    const at::Tensor qc = paged_queries(name, q, kv_pages, c);
+    const int64_t Hq = q.size(1), S = q.size(2);
+    check_like(name, "lse", lse, kv_pages, at::kFloat);
+    TORCH_CHECK(lse.dim() == 3 && lse.size(0) == c.B && lse.size(1) == Hq && lse.size(2) == S && lse.is_contiguous(), name, ": lse must be a contiguous [", c.B, ", ",
+                Hq, ", ", S, "] tensor, got ", lse.sizes());
+    TORCH_CHECK(last_rows >= 0, name, ": last_rows must not be negative, got ", last_rows);
+    const int last = (int)std::min<int64_t>(last_rows, INT32_MAX);
+    const size_t need = mi355_fmha_key_weights_workspace_bytes(&c, (int)Hq, (int)S, last);
+    const at::Tensor ws = workspace_of(need, q);
+    const int64_t strides[3] = {qc.stride(0), qc.stride(1), qc.stride(2)};
+    hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+    const int rc = mi355_fmha_key_weights(&c, qc.data_ptr(), lse.data_ptr<float>(), (int)Hq, (int)S, strides, last, 1.0f / std::sqrt(128.0f),
+                                          need > 0 ? ws.data_ptr() : nullptr, need, stream);
+    TORCH_CHECK(rc == 0, name, ": ", mi355_last_error(), " (code ", rc, ")");
+}
+
+at::Tensor evict_paged(const at::Tensor& kv_pages, const at::Tensor& block_table, const at::Tensor& seq_lens, const at::Tensor& weights,
+                       const at::Tensor& key_positions, int64_t budget, int64_t recent) {
+    const char* name = "fine_evict_paged";
+    const mi355_paged_kv c = paged_kv(name, kv_pages, block_table, seq_lens, std::nullopt, weights, key_positions);
+    TORCH_CHECK(budget >= 1 && recent >= 0, name, ": budget >= 1 and recent >= 0 required, got ", budget, " and ", recent);
+    const int keep = (int)std::min<int64_t>(budget, INT32_MAX), fresh = (int)std::min<int64_t>(recent, INT32_MAX);
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(kv_pages.device());
+    at::Tensor lens = gpu_empty({c.B}, at::kInt, kv_pages);
+    const size_t need = mi355_cache_evict_workspace_bytes(&c, keep);
+    const at::Tensor ws = workspace_of(need, kv_pages);
+    hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+    const int rc = mi355_cache_evict(&c, keep, fresh, lens.data_ptr<int32_t>(), need > 0 ? ws.data_ptr() : nullptr, need, stream);
+    TORCH_CHECK(rc == 0, name, ": ", mi355_last_error(), " (code ", rc, ")");
+    return lens;
+}
+
 }  // namespace
 
 // Defines the operators (the first eight schema strings are the reference's).
@@ -118,6 +280,12 @@ TORCH_LIBRARY(fmha_unified, m) {
     m.def("finefmha_6(Tensor q, Tensor k, Tensor v, bool causal, bool is_decode, int decode_length) -> Tensor");
     m.def("finefmha_7(Tensor q, Tensor k, Tensor v, bool causal, bool is_decode, int decode_length) -> Tensor");
     m.def("finefmha_fwd_lse(Tensor q, Tensor k, Tensor v, bool causal, bool is_decode, int decode_length) -> (Tensor, Tensor)");
+    m.def("finefmha_paged(Tensor q, Tensor kv_pages, Tensor block_table, Tensor seq_lens, Tensor? new_lens, Tensor(a!)? weights) -> Tensor");
+    m.def("finefmha_paged_lse(Tensor q, Tensor kv_pages, Tensor block_table, Tensor seq_lens, Tensor? new_lens, Tensor(a!)? weights) -> (Tensor, Tensor)");
+    m.def("rope_paged(Tensor(a!) qkv, Tensor(b!) kv_pages, Tensor block_table, Tensor seq_lens, Tensor cos, Tensor sin, Tensor positions, int q_heads, "
+          "Tensor? new_lens, Tensor(c!)? weights, Tensor(d!)? key_positions, bool keep_keys) -> ()");
+    m.def("key_weights(Tensor q, Tensor lse, Tensor kv_pages, Tensor block_table, Tensor seq_lens, Tensor(a!) weights, Tensor? new_lens, int last_rows) -> ()");
+    m.def("evict_paged(Tensor(a!) kv_pages, Tensor block_table, Tensor seq_lens, Tensor(b!) weights, Tensor(c!) key_positions, int budget, int recent) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(fmha_unified, CUDA, m) {
@@ -130,6 +298,11 @@ TORCH_LIBRARY_IMPL(fmha_unified, CUDA, m) {
     m.impl("finefmha_6", &finefmha);
     m.impl("finefmha_7", &finefmha);
     m.impl("finefmha_fwd_lse", &finefmha_fwd_lse);
+    m.impl("finefmha_paged", &finefmha_paged);
+    m.impl("finefmha_paged_lse", &finefmha_paged_lse);
+    m.impl("rope_paged", &rope_paged);
+    m.impl("key_weights", &key_weights);
+    m.impl("evict_paged", &evict_paged);
 }
 
 // The same functions under the CPU key: CPU tensors then reach the argument validation above and are
@@ -144,6 +317,11 @@ TORCH_LIBRARY_IMPL(fmha_unified, CPU, m) {
     m.impl("finefmha_6", &finefmha);
     m.impl("finefmha_7", &finefmha);
     m.impl("finefmha_fwd_lse", &finefmha_fwd_lse);
+    m.impl("finefmha_paged", &finefmha_paged);
+    m.impl("finefmha_paged_lse", &finefmha_paged_lse);
+    m.impl("rope_paged", &rope_paged);
+    m.impl("key_weights", &key_weights);
+    m.impl("evict_paged", &evict_paged);
 }
 
 }  // namespace fmha_unified

@@ -19,6 +19,8 @@ EXPORTED_SYMBOLS = ("mi355_hgemm", "mi355_fmha_fwd", "mi355_fmha_fwd_strided", "
                     "mi355_gemm_bf16", "mi355_gemm_silu_mul_bf16", "mi355_gemm_add_bf16", "mi355_rmsnorm_bf16", "mi355_rope_bf16", "mi355_rope_qkv_bf16", "mi355_silu_mul_bf16",
                     "mi355_gemm_workspace_bytes", "mi355_gemm_ws",
                     "mi355_fmha_fwd_workspace_bytes", "mi355_fmha_fwd_ws", "mi355_fmha_fwd_noalloc",
+                    "mi355_fmha_paged_workspace_bytes", "mi355_fmha_paged", "mi355_rope_paged", "mi355_fmha_key_weights_workspace_bytes",
+                    "mi355_fmha_key_weights", "mi355_cache_evict_workspace_bytes", "mi355_cache_evict",
                     "mi355_last_error", "mi355_serving_version")
 # exported for tests and tuning runs, declared in csrc/mi355_serving_internal.h and not in the public header
 INTERNAL_SYMBOLS = ("mi355_internal_hgemm_variant", "mi355_internal_hgemm_add_variant", "mi355_internal_hgemm_choice", "mi355_internal_hgemm_wide_ranges", "mi355_internal_hgemm_direct_choice",
@@ -27,6 +29,13 @@ INTERNAL_SYMBOLS = ("mi355_internal_hgemm_variant", "mi355_internal_hgemm_add_va
                     "mi355_internal_fmha_decode_plan", "mi355_internal_step_qkv", "mi355_internal_step_gate_up")
 
 _lib = None
+
+
+class PagedKV(ctypes.Structure):
+    """mi355_paged_kv: a key-value cache in pages, as the C ABI takes it (include/mi355_serving.h). `paged_kv` fills one from tensors."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("pages", "block_table", "seq_lens", "new_lens", "weights", "key_positions")] +
+                [(n, ctypes.c_int64) for n in ("page_stride", "head_stride", "row_stride", "table_stride")] +
+                [(n, ctypes.c_int32) for n in ("n_pages", "page_size", "max_pages", "B", "Hkv", "dtype")])
 
 
 class Mi355Error(RuntimeError):
@@ -92,6 +101,21 @@ def load():
     lib.mi355_fmha_fwd_ws.restype = i32
     lib.mi355_fmha_fwd_noalloc.argtypes = lib.mi355_fmha_fwd_strided.argtypes
     lib.mi355_fmha_fwd_noalloc.restype = i32
+    cache, size = ctypes.POINTER(PagedKV), ctypes.c_size_t
+    lib.mi355_fmha_paged_workspace_bytes.argtypes = [cache, i32, i32, i32]
+    lib.mi355_fmha_paged_workspace_bytes.restype = size
+    lib.mi355_fmha_paged.argtypes = [cache, vp, vp, vp, i32, i32, ctypes.POINTER(i64), f32, vp, size, vp]
+    lib.mi355_fmha_paged.restype = i32
+    lib.mi355_rope_paged.argtypes = [cache, vp, i32, i32, i32, i64, i64, vp, vp, vp, i64, i32, vp]
+    lib.mi355_rope_paged.restype = i32
+    lib.mi355_fmha_key_weights_workspace_bytes.argtypes = [cache, i32, i32, i32]
+    lib.mi355_fmha_key_weights_workspace_bytes.restype = size
+    lib.mi355_fmha_key_weights.argtypes = [cache, vp, vp, i32, i32, ctypes.POINTER(i64), i32, f32, vp, size, vp]
+    lib.mi355_fmha_key_weights.restype = i32
+    lib.mi355_cache_evict_workspace_bytes.argtypes = [cache, i32]
+    lib.mi355_cache_evict_workspace_bytes.restype = size
+    lib.mi355_cache_evict.argtypes = [cache, i32, i32, vp, vp, size, vp]
+    lib.mi355_cache_evict.restype = i32
     lib.mi355_internal_hgemm_variant.argtypes = [vp, vp, vp, i32, i32, i32, i64, i64, i64, i32, i32, i32, vp]
     lib.mi355_internal_hgemm_variant.restype = i32
     lib.mi355_internal_hgemm_add_variant.argtypes = [vp, vp, vp, vp, i32, i32, i32, i64, i64, i64, i64, i32, i32, i32, vp]
@@ -353,6 +377,16 @@ def silu_mul(gate_up, out=None, interleave=0):
     _check(entry(_ptr(gate_up), _ptr(out), rows, inter, int(interleave), gate_up.stride(0), out.stride(0),
                                  _stream_of(gate_up)))
     return out
+
+
+def paged_kv(kv_pages, block_table, seq_lens, new_lens=None, weights=None, key_positions=None):
+    """The PagedKV of a pool [n_pages, 2 * Hkv, page_size, 128] (any strides with a contiguous last dimension), a block table [B, max_pages] and
+    lengths [B] (both int32). It holds addresses: the tensors have to outlive its calls."""
+    import torch
+    return PagedKV(_ptr(kv_pages), _ptr(block_table), _ptr(seq_lens), _ptr(new_lens), _ptr(weights), _ptr(key_positions),
+                   kv_pages.stride(0), kv_pages.stride(1), kv_pages.stride(2), block_table.stride(0), kv_pages.shape[0], kv_pages.shape[2],
+                   block_table.shape[1], block_table.shape[0], kv_pages.shape[1] // 2,
+                   DTYPE_BF16 if kv_pages.dtype == torch.bfloat16 else DTYPE_FP16)
 
 
 GATE_UP_BLOCK = 32  # columns per gate / up group in the operand of mi355_hgemm_silu_mul
