@@ -307,7 +307,7 @@ int mi355_fmha_fwd_noalloc(const void* Q, const void* K, const void* V, void* O,
  * of `new` tokens is key seq_lens[b] - new + i and sees the keys up to that one; rows behind them give O = 0 and LSE = -inf. A
  * sequence of length 0 gives the same.
  *
- * weights (fp32) and key_positions (int32), [n_pages][Hkv][page_size] contiguous, hold what eviction goes by: the attention each key has
+ * weights (fp32) and key_positions (int32), [n_pages][Hkv][page_size] contiguous, 16-byte aligned, hold what eviction goes by: the attention each key has
  * had from the queries of its kv head, and the position of its token in the text. Both may be NULL where a call does not need them.
  *
  * Lengths, table and positions are read on the device: no call waits for it, and a captured call serves what the tensors hold when it

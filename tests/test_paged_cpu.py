@@ -17,7 +17,7 @@ def cache(lib, **other):
     return lib.PagedKV(**c)
 
 
-BAD_CACHES = [dict(pages=None), dict(block_table=None), dict(seq_lens=None), dict(pages=P + 8), dict(B=0), dict(Hkv=0), dict(n_pages=0), dict(max_pages=0),
+BAD_CACHES = [dict(pages=None), dict(block_table=None), dict(seq_lens=None), dict(pages=P + 8), dict(weights=P + 4), dict(key_positions=P + 8), dict(B=0), dict(Hkv=0), dict(n_pages=0), dict(max_pages=0),
               dict(page_size=0), dict(page_size=8), dict(page_size=24), dict(dtype=2), dict(table_stride=7), dict(page_stride=0), dict(head_stride=64),
               dict(row_stride=129), dict(row_stride=-128), dict(row_stride=1 << 24), dict(page_size=1 << 20, row_stride=1 << 20), dict(B=9000),
               dict(max_pages=1 << 28, table_stride=1 << 28), dict(max_pages=1 << 22, table_stride=1 << 22, B=1000, Hkv=10)]

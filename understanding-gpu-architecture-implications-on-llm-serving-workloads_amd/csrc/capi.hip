@@ -445,7 +445,7 @@ static int paged_checked(const char* fn, const mi355_paged_kv* c) {
         return fail(MI355_ERR_UNSUPPORTED, "%s: page_size must be a positive multiple of 16 (got %d)", fn, c->page_size);
     const int64_t pairs = (int64_t)c->B * c->Hkv, max_len = (int64_t)c->max_pages * c->page_size;
     if (pairs > 65535) return fail(MI355_ERR_UNSUPPORTED, "%s: B * Hkv must be at most 65535 (got %lld)", fn, (long long)pairs);
-    if (max_len > INT32_MAX - 1024 || pairs * (max_len / 32 + 1) > INT32_MAX)
+    if (max_len > INT32_MAX - 8192 || pairs * (max_len / 32 + 1) > INT32_MAX)
         return fail(MI355_ERR_UNSUPPORTED, "%s: %d sequences of up to %lld keys of %d heads are more than a call takes", fn, c->B, (long long)max_len, c->Hkv);
     if (c->B > 1 && c->table_stride < c->max_pages)
         return fail(MI355_ERR_BAD_ARGUMENT, "%s: rows of the block table overlap (stride %lld, %d entries)", fn, (long long)c->table_stride, c->max_pages);
@@ -456,7 +456,8 @@ static int paged_checked(const char* fn, const mi355_paged_kv* c) {
                         (long long)strides[0], (long long)strides[1], (long long)strides[2]);
     if (c->row_stride >= (1 << 24) || c->row_stride * 2 * c->page_size > INT32_MAX)
         return fail(MI355_ERR_UNSUPPORTED, "%s: row stride %lld of the pages is too large", fn, (long long)c->row_stride);
-    if (!aligned16(c->pages)) return fail(MI355_ERR_BAD_ARGUMENT, "%s: pages must be 16-byte aligned", fn);
+    if (!aligned16(c->pages) || !aligned16(c->weights) || !aligned16(c->key_positions))
+        return fail(MI355_ERR_BAD_ARGUMENT, "%s: pages, weights and key_positions must be 16-byte aligned", fn);
     return 0;
 }
 

@@ -1,7 +1,6 @@
 // What fills a paged key-value cache and what keeps it short, for gfx950 (MI355X): rotary embedding of a fused projection with its keys and values
 // filed into their pages, and eviction by accumulated attention weight. Memory-bound, or bound by their chains of memory round trips.
 #include <algorithm>
-#include <type_traits>
 
 #include "paged.h"
 
@@ -74,9 +73,10 @@ __global__ __launch_bounds__(pcache::THREADS) void rope_paged_kernel(PagedKv kv,
 // as are dropped (closing ranks would move most of the cache for one dropped key).
 namespace evict {
 constexpr int THREADS = 1024, WAVES = THREADS / 64;
-constexpr int BINS = 2048;                    // of 11, 11 and 10 bits
-constexpr int kLdsKeys = 36864;               // ranks kept in LDS up to this many keys (144 KiB), behind that in the workspace
-constexpr int MOVES = 64;                     // of a workgroup of the moving kernel
+constexpr int BINS = 2048, COPIES = 4;        // of 11, 11 and 10 bits; of the histogram, a lane's own: many weights are alike in their upper bits
+constexpr int kMostChunks = 8;                // of 4 keys whose ranks stay in a thread's registers (32768 keys)
+constexpr int kMovesHere = 256;               // up to this many moves are made by the selecting workgroup
+constexpr int MOVES = 32;                     // of a workgroup of the moving kernel, 8 at a time side by side
 
 // a weight as a whole number of the same order; NaN and the slots of pages outside the pool lowest, minus infinity next
 __device__ __forceinline__ uint32_t rank_of(float w) {
@@ -91,152 +91,259 @@ struct Evict {
     int budget, recent, cap;   // cap: the most moves of a (sequence, kv head)
     int* counts;               // [pair]
     int* moves;                // [pair][2][cap]: slots of the dropped keys, of those that take them
-    uint32_t* ranks;           // [pair][max_len], where they do not fit LDS
+    uint4* ranks;              // [pair][2][max_len / 4]: ranks and positions, where registers do not hold them
     int* lens_out;
     Divisor by_hkv;
 };
 
-// One workgroup per (sequence, kv head)
-template <bool IN_LDS>
+namespace evict {
+
+// sum of one value a thread over the threads in front of this one; `sums` is free again behind the caller's next barrier
+__device__ __forceinline__ int block_before(int x, int (&sums)[WAVES], int& total) {
+    const int incl = wave_inclusive_sum(x), wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 63) sums[wave] = incl;
+    __syncthreads();
+    int before = incl - x;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        const int n = sums[w];
+        before += w < wave ? n : 0;
+        total += n;
+    }
+    return before;
+}
+
+// Moves n0, n0 + step, .. of those listed: 32 threads a move, four in flight each
+template <typename List>
+__device__ __forceinline__ void move_keys(const PagedKv& kv, int b, int hkv, List to, List from, int n0, int step, int count) {
+    const int* table = kv.table + (long)b * kv.table_stride;
+    const int l32 = threadIdx.x & 31;
+    const long head = (long)(hkv + (l32 >> 4) * kv.Hkv) * kv.head_bytes + (l32 & 15) * 16;
+    constexpr int N = 4;
+    if (n0 >= count) return;
+    int d[N], s[N], dp[N], sp[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int n = min(n0 + step * k, count - 1);   // (the last move again behind the end: not stored)
+        d[k] = to[n];
+        s[k] = from[n];
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int di = divide(d[k], kv.by_page), si = divide(s[k], kv.by_page);
+        dp[k] = table[di];
+        sp[k] = table[si];
+        d[k] -= di * kv.page_size;
+        s[k] -= si * kv.page_size;
+    }
+    int4v row[N];
+    int other[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        // a page outside the pool has no keys: nothing comes from it, nothing goes there
+        if (n0 + step * k >= count || (uint32_t)dp[k] >= (uint32_t)kv.n_pages || (uint32_t)sp[k] >= (uint32_t)kv.n_pages) dp[k] = -1;
+        if (dp[k] < 0) continue;
+        row[k] = *(const int4v*)(kv.pages + (long)sp[k] * kv.page_bytes + head + (uint32_t)s[k] * kv.row_bytes);
+        const long sa = ((long)sp[k] * kv.Hkv + hkv) * kv.page_size + s[k];
+        if (l32 == 0) other[k] = __builtin_bit_cast(int, kv.weights[sa]);
+        if (l32 == 16) other[k] = kv.key_positions[sa];
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        if (dp[k] < 0) continue;
+        *(int4v*)(kv.pages + (long)dp[k] * kv.page_bytes + head + (uint32_t)d[k] * kv.row_bytes) = row[k];
+        const long da = ((long)dp[k] * kv.Hkv + hkv) * kv.page_size + d[k];
+        if (l32 == 0) kv.weights[da] = __builtin_bit_cast(float, other[k]);
+        if (l32 == 16) kv.key_positions[da] = other[k];
+    }
+}
+
+}  // namespace evict
+
+// One workgroup per (sequence, kv head). A thread owns 4 * chunks slots side by side (4 lie in one page and are read with one access), so that
+// what has to be counted in the order of the slots is one sum over the threads. Their ranks stay in M chunks of registers or, M == 0, in
+// the workspace, where only their thread reads them again. Bound by its chain of about ten steps, a memory round trip or a pass over the
+// workgroup each.
+template <int M>
 __global__ __launch_bounds__(evict::THREADS) void evict_select_kernel(PagedKv kv, Evict a) {
     using namespace evict;
-    __shared__ int hist[BINS];
-    __shared__ int wave_sums[WAVES], wave_sums2[WAVES];
+    __shared__ int hist[BINS * COPIES];
+    __shared__ int sums[4][WAVES];
     __shared__ int found[2];
-    extern __shared__ uint32_t lds_ranks[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ int list[2][kMovesHere];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int b = divide(blockIdx.x, a.by_hkv), hkv = blockIdx.x - b * kv.Hkv;
-    const int len = paged_len(kv, b);
+    const int len = __builtin_amdgcn_readfirstlane(paged_len(kv, b));
     if (hkv == 0 && tid == 0) a.lens_out[b] = min(len, a.budget);
     if (len <= a.budget) {
         if (tid == 0) a.counts[blockIdx.x] = 0;
         return;
     }
-    uint32_t* ranks = IN_LDS ? lds_ranks : a.ranks + (long)blockIdx.x * kv.max_len;
     const int* table = kv.table + (long)b * kv.table_stride;
-    const auto place = [&](int j) -> long {   // of the account of key j; -1: its page is outside the pool
-        const int i = divide(j, kv.by_page);
-        const int page = table[i];
-        return (uint32_t)page < (uint32_t)kv.n_pages ? ((long)page * kv.Hkv + hkv) * kv.page_size + (j - i * kv.page_size) : -1L;
-    };
+    const int chunks = (len + 4 * THREADS - 1) / (4 * THREADS);   // <= M, where that is given
+    const int j0 = tid * 4 * chunks;   // (up to 4096 behind the last key: max_len leaves that much below 2^31)
+    constexpr int REGS = M > 0 ? M : 1;
+    uint4 rank[REGS], position[REGS];
+    uint4* kept_ranks = a.ranks + (long)blockIdx.x * 2 * ((kv.max_len + 3) / 4 + THREADS);
+    uint4* kept_positions = kept_ranks + (kv.max_len + 3) / 4 + THREADS;
+#pragma unroll
+    for (int i = 0; i < BINS * COPIES / THREADS; ++i) hist[i * THREADS + tid] = 0;
 
-    // the largest position
+    // Positions and the weights' ranks; the largest position. `there`: a bit for each key of a chunk that the sequence has, in a page of the pool
+    const auto there_of = [&](int j, int page) -> uint32_t {
+        return (uint32_t)page < (uint32_t)kv.n_pages && (uint32_t)j < (uint32_t)len ? (len - j >= 4 ? 15u : (1u << (len - j)) - 1u) : 0u;
+    };
+    const auto get = [&](const uint4& v, int e) { return e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w; };
     int newest = INT32_MIN;
-    for (int j = tid; j < len; j += THREADS) {
-        const long at = place(j);
-        if (at >= 0) newest = max(newest, kv.key_positions[at]);
+    const auto load = [&](int c, uint4& r, uint4& p) {
+        const int j = min(j0 + 4 * c, kv.max_len - 4), i = divide(j, kv.by_page);
+        const int page = table[i];
+        const uint32_t there = c < chunks && j == j0 + 4 * c ? there_of(j, page) : 0u;
+        const long at = ((long)(there ? page : 0) * kv.Hkv + hkv) * kv.page_size + (j - i * kv.page_size);
+        p = *(const uint4*)(kv.key_positions + at);
+        const float4v w = *(const float4v*)(kv.weights + at);
+        uint32_t x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[e] = (there >> e) & 1 ? rank_of(w[e]) : 0u;
+            newest = (there >> e) & 1 ? max(newest, (int)get(p, e)) : newest;
+        }
+        r = uint4{x[0], x[1], x[2], x[3]};
+        return there;
+    };
+    uint32_t present = 0;   // of the chunks in registers, 4 bits each
+    if constexpr (M > 0) {
+#pragma unroll
+        for (int c = 0; c < M; ++c) present |= load(c, rank[c], position[c]) << (4 * c);
+    } else {
+        for (int c = 0; c < chunks; ++c) {
+            uint4 r, p;
+            load(c, r, p);
+            kept_ranks[c * THREADS + tid] = r;
+            kept_positions[c * THREADS + tid] = p;
+        }
     }
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) newest = max(newest, __shfl_xor(newest, off, 64));
-    if (lane == 0) wave_sums[wave] = newest;
+    if (lane == 0) sums[0][wave] = newest;
     __syncthreads();
-    for (int w = 0; w < WAVES; ++w) newest = max(newest, wave_sums[w]);
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) newest = max(newest, sums[0][w]);
     const long old = (long)newest - a.recent;   // positions up to here are not recent
-    // the ranks
-    for (int j = tid; j < len; j += THREADS) {
-        const long at = place(j);
-        ranks[j] = at < 0 ? 0u : kv.key_positions[at] > old ? kRecent : rank_of(kv.weights[at]);
-    }
-    // the budget-th largest: 11 bits, 11, then 10; `want` of those whose upper bits are `prefix`
-    uint32_t prefix = 0;
-    int want = a.budget;
-    for (int pass = 0; pass < 3; ++pass) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-        const int above = pass == 0 ? 32 : pass == 1 ? 21 : 10;   // bits that are known
-        const uint32_t mask = pass == 2 ? 1023u : 2047u;
-        __syncthreads();
-        hist[tid] = 0;
-        hist[tid + THREADS] = 0;
-        __syncthreads();
-        for (int j = tid; j < len; j += THREADS) {
-            const uint32_t r = ranks[j];
-            if (pass == 0 || (r >> above) == prefix) atomicAdd(&hist[(r >> shift) & mask], 1);
+    int recent = 0;
+    const auto mark = [&](uint32_t there, uint4& r, const uint4& p) {
+        uint32_t x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool is = ((there >> e) & 1) && (int)get(p, e) > old;
+            x[e] = is ? kRecent : get(r, e);
+            recent += is;
         }
-        __syncthreads();
-        // thread t: the bins 2047 - 2t and 2046 - 2t; sums from the top
-        const int h0 = hist[BINS - 1 - 2 * tid], h1 = hist[BINS - 2 - 2 * tid];
-        int incl = wave_inclusive_sum(h0 + h1);
-        if (lane == 63) wave_sums2[wave] = incl;
-        __syncthreads();
-        for (int w = 0; w < wave; ++w) incl += wave_sums2[w];
-        const int before = incl - h0 - h1;
-        if (before < want && want <= before + h0) found[0] = BINS - 1 - 2 * tid, found[1] = want - before;
-        else if (before + h0 < want && want <= incl) found[0] = BINS - 2 - 2 * tid, found[1] = want - before - h0;
-        __syncthreads();
-        prefix = pass == 0 ? (uint32_t)found[0] : (prefix << (pass == 1 ? 11 : 10)) | (uint32_t)found[0];
-        want = found[1];
-    }
-    // `want` of the keys of rank `prefix` are kept, the first ones. A wave owns a run of slots and goes through it three times:
-    // how many such keys, how many holes and moving keys, then the lists.
-    const int run = (((len + WAVES - 1) / WAVES) + 63) & ~63;
-    const int j0 = min(wave * run, len), j1 = min(j0 + run, len);
-    int ties = 0;
-    for (int j = j0; j < j1; j += 64) ties += __popcll(__builtin_amdgcn_ballot_w64(j + lane < j1 && ranks[j + lane] == prefix));
-    __syncthreads();
-    if (lane == 0) wave_sums[wave] = ties;
-    __syncthreads();
-    int tie0 = 0;
-    for (int w = 0; w < wave; ++w) tie0 += wave_sums[w];
-    const auto kept = [&](int j, int& tie) {   // of key j + lane; `tie`: such keys in front of this call's
-        const bool there = j + lane < j1;
-        const uint32_t r = there ? ranks[j + lane] : 0u;
-        const uint64_t equal = __builtin_amdgcn_ballot_w64(there && r == prefix);
-        const int mine = tie + __popcll(equal & ((1ULL << lane) - 1));
-        tie += __popcll(equal);
-        return there && (r > prefix || (r == prefix && mine < want));
+        r = uint4{x[0], x[1], x[2], x[3]};
     };
+    // f(key, rank) for this thread's keys in order
+    const auto each = [&](auto&& f) {
+        if constexpr (M > 0) {
+#pragma unroll
+            for (int c = 0; c < M; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c < chunks && j0 + 4 * c + e < len) f(j0 + 4 * c + e, get(rank[c], e));
+        } else {
+            for (int c = 0; c < chunks && j0 + 4 * c < len; ++c) {
+                const uint4 r = kept_ranks[c * THREADS + tid];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (j0 + 4 * c + e < len) f(j0 + 4 * c + e, get(r, e));
+            }
+        }
+    };
+    if constexpr (M > 0) {
+#pragma unroll
+        for (int c = 0; c < M; ++c) mark((present >> (4 * c)) & 15, rank[c], position[c]);
+    } else {
+        for (int c = 0; c < chunks; ++c) {
+            const int j = j0 + 4 * c;
+            if (j >= len) break;
+            uint4 r = kept_ranks[c * THREADS + tid];
+            const int page = table[divide(j, kv.by_page)];
+            mark(there_of(j, page), r, kept_positions[c * THREADS + tid]);
+            kept_ranks[c * THREADS + tid] = r;
+        }
+    }
+    int all_recent;
+    block_before(recent, sums[1], all_recent);
+
+    // The rank of the last kept key, and how many keys of it are kept (`want`, the first ones). The recent ones are counted above (in the
+    // histogram they would all fall on one counter); of the others the want-th largest: 11 bits, 11, then 10.
+    uint32_t last = kRecent;
+    int want = a.budget;
+    if (all_recent < a.budget) {
+        want -= all_recent;
+        last = 0;
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+            const int known = pass == 1 ? 21 : 10;   // bits below those that are known (pass 0: none are)
+            const uint32_t mask = pass == 2 ? 1023u : 2047u;
+            each([&](int, uint32_t r) {
+                if (r != kRecent && (pass == 0 || (r >> known) == last)) atomicAdd(&hist[((r >> shift) & mask) * COPIES + (lane & (COPIES - 1))], 1);
+            });
+            __syncthreads();
+            // thread t: the bins 2047 - 2t and 2046 - 2t; sums from the top
+            int4v* at = (int4v*)(hist + (BINS - 2 - 2 * tid) * COPIES);
+            const int4v lo = at[0], hi = at[1];
+            at[0] = at[1] = int4v{0, 0, 0, 0};
+            const int h0 = hi[0] + hi[1] + hi[2] + hi[3], h1 = lo[0] + lo[1] + lo[2] + lo[3];
+            int unused;
+            const int before = block_before(h0 + h1, sums[2 + (pass & 1)], unused);
+            if (before < want && want <= before + h0) found[0] = BINS - 1 - 2 * tid, found[1] = want - before;
+            else if (before + h0 < want && want <= before + h0 + h1) found[0] = BINS - 2 - 2 * tid, found[1] = want - before - h0;
+            __syncthreads();
+            last = pass == 0 ? (uint32_t)found[0] : (last << (pass == 1 ? 11 : 10)) | (uint32_t)found[0];
+            want = found[1];
+        }
+    }
+    int ties = 0, unused;
+    each([&](int, uint32_t r) { ties += r == last; });
+    const int tie0 = block_before(ties, sums[0], unused);
     int holes = 0, movers = 0, tie = tie0;
-    for (int j = j0; j < j1; j += 64) {
-        const bool keep = kept(j, tie);
-        holes += __popcll(__builtin_amdgcn_ballot_w64(j + lane < j1 && !keep && j + lane < a.budget));
-        movers += __popcll(__builtin_amdgcn_ballot_w64(keep && j + lane >= a.budget));
-    }
-    if (lane == 0) wave_sums2[wave] = holes;
-    __syncthreads();
-    if (lane == 0) wave_sums[wave] = movers;
-    __syncthreads();
-    int hole0 = 0, mover0 = 0, total = 0;
-    for (int w = 0; w < WAVES; ++w) {
-        if (w < wave) hole0 += wave_sums2[w], mover0 += wave_sums[w];
-        total += wave_sums2[w];
-    }
-    if (tid == 0) a.counts[blockIdx.x] = total;
+    each([&](int j, uint32_t r) {
+        const bool keep = r > last || (r == last && tie < want);
+        tie += r == last;
+        holes += !keep && j < a.budget;
+        movers += keep && j >= a.budget;
+    });
+    int total;
+    int hole = block_before(holes, sums[1], total), mover = block_before(movers, sums[2], unused);
+    const bool here = a.cap <= kMovesHere;
+    if (tid == 0) a.counts[blockIdx.x] = here ? 0 : total;
     int* to = a.moves + (long)blockIdx.x * 2 * a.cap;
     int* from = to + a.cap;
     tie = tie0;
-    for (int j = j0; j < j1; j += 64) {
-        const bool keep = kept(j, tie);
-        const bool hole = j + lane < j1 && !keep && j + lane < a.budget, mover = keep && j + lane >= a.budget;
-        const uint64_t hm = __builtin_amdgcn_ballot_w64(hole), mm = __builtin_amdgcn_ballot_w64(mover);
-        const uint64_t below = (1ULL << lane) - 1;
-        if (hole) to[hole0 + __popcll(hm & below)] = j + lane;
-        if (mover) from[mover0 + __popcll(mm & below)] = j + lane;
-        hole0 += __popcll(hm);
-        mover0 += __popcll(mm);
-    }
+    each([&](int j, uint32_t r) {
+        const bool keep = r > last || (r == last && tie < want);
+        tie += r == last;
+        if (!keep && j < a.budget) {
+            if (here) list[0][hole++] = j;
+            else to[hole++] = j;
+        }
+        if (keep && j >= a.budget) {
+            if (here) list[1][mover++] = j;
+            else from[mover++] = j;
+        }
+    });
+    if (!here) return;
+    __syncthreads();
+    for (int n = 0; n < total; n += 4 * THREADS / 32) move_keys(kv, b, hkv, list[0], list[1], n + (tid >> 5), THREADS / 32, total);
 }
 
-// Grid (moves / 64, pairs): 32 threads move a key, its value, its weight and its position
+// Grid (moves / 32, pairs)
 __global__ __launch_bounds__(256) void evict_move_kernel(PagedKv kv, Evict a) {
-    using namespace evict;
     const int count = a.counts[blockIdx.y];
     const int b = divide(blockIdx.y, a.by_hkv), hkv = blockIdx.y - b * kv.Hkv;
-    const int* table = kv.table + (long)b * kv.table_stride;
     const int* to = a.moves + (long)blockIdx.y * 2 * a.cap;
-    const int l32 = threadIdx.x & 31;
-    for (int n = blockIdx.x * MOVES + (threadIdx.x >> 5); n < min(count, (int)(blockIdx.x + 1) * MOVES); n += 8) {
-        const int d = to[n], s = to[a.cap + n];
-        const int di = divide(d, kv.by_page), si = divide(s, kv.by_page);
-        const int dp = table[di], sp = table[si];
-        if ((uint32_t)dp >= (uint32_t)kv.n_pages || (uint32_t)sp >= (uint32_t)kv.n_pages) continue;
-        const int ds = d - di * kv.page_size, ss = s - si * kv.page_size;
-        const long head = (long)(hkv + (l32 >> 4) * kv.Hkv) * kv.head_bytes + (l32 & 15) * 16;
-        *(int4v*)(kv.pages + (long)dp * kv.page_bytes + head + (uint32_t)ds * kv.row_bytes) =
-            *(const int4v*)(kv.pages + (long)sp * kv.page_bytes + head + (uint32_t)ss * kv.row_bytes);
-        const long da = ((long)dp * kv.Hkv + hkv) * kv.page_size + ds, sa = ((long)sp * kv.Hkv + hkv) * kv.page_size + ss;
-        if (l32 == 0) kv.weights[da] = kv.weights[sa];
-        if (l32 == 16) kv.key_positions[da] = kv.key_positions[sa];
-    }
+    evict::move_keys(kv, b, hkv, to, to + a.cap, blockIdx.x * evict::MOVES + (threadIdx.x >> 5), 8, count);
 }
 
 hipError_t rope_paged_dispatch(const mi355_paged_kv& c, void* qkv, int S, int q_heads, int keep_keys, long x_batch, long x_row, const float* cos_t,
@@ -255,10 +362,14 @@ hipError_t rope_paged_dispatch(const mi355_paged_kv& c, void* qkv, int S, int q_
 
 static int evict_cap(int max_len, int budget) { return std::max(0, std::min(budget, max_len - budget)); }
 
+// ints: the counts and lists, then (16-byte aligned) the ranks and positions of long sequences
+static size_t evict_lists(size_t pairs, int cap) { return (pairs + pairs * 2 * cap + 3) / 4 * 4; }
+
 size_t evict_workspace(const mi355_paged_kv& c, int budget) {
     const int max_len = c.max_pages * c.page_size;
     const size_t pairs = (size_t)c.B * c.Hkv;
-    return 4 * (pairs + pairs * 2 * evict_cap(max_len, budget) + (max_len > evict::kLdsKeys ? pairs * max_len : 0));
+    const bool long_ones = max_len > evict::kMostChunks * 4 * evict::THREADS;
+    return 4 * evict_lists(pairs, evict_cap(max_len, budget)) + (long_ones ? 16 * pairs * 2 * ((size_t)(max_len + 3) / 4 + evict::THREADS) : 0);
 }
 
 hipError_t evict_dispatch(const mi355_paged_kv& c, int budget, int recent, int* lens_out, void* workspace, hipStream_t stream) {
@@ -271,19 +382,18 @@ hipError_t evict_dispatch(const mi355_paged_kv& c, int budget, int recent, int* 
     a.cap = evict_cap(kv.max_len, budget);
     a.counts = (int*)workspace;
     a.moves = a.counts + pairs;
-    a.ranks = (uint32_t*)(a.moves + (size_t)pairs * 2 * a.cap);
+    a.ranks = (uint4*)((int*)workspace + evict_lists(pairs, a.cap));
     a.lens_out = lens_out;
     a.by_hkv = divisor_of(kv.Hkv);
-    if (kv.max_len > kLdsKeys) {
-        evict_select_kernel<false><<<dim3(pairs), dim3(THREADS), 0, stream>>>(kv, a);
-    } else {
-        static DynamicLdsOnce once;
-        const hipError_t e = once.ensure(reinterpret_cast<const void*>(evict_select_kernel<true>), kLdsKeys * 4);
-        if (e != hipSuccess) return e;
-        evict_select_kernel<true><<<dim3(pairs), dim3(THREADS), (size_t)kv.max_len * 4, stream>>>(kv, a);
-    }
+    const dim3 grid(pairs), block(THREADS);
+    const int chunks = (int)(((long)kv.max_len + 4 * THREADS - 1) / (4 * THREADS));
+    if (chunks <= 1) evict_select_kernel<1><<<grid, block, 0, stream>>>(kv, a);
+    else if (chunks <= 2) evict_select_kernel<2><<<grid, block, 0, stream>>>(kv, a);
+    else if (chunks <= 4) evict_select_kernel<4><<<grid, block, 0, stream>>>(kv, a);
+    else if (chunks <= kMostChunks) evict_select_kernel<kMostChunks><<<grid, block, 0, stream>>>(kv, a);
+    else evict_select_kernel<0><<<grid, block, 0, stream>>>(kv, a);
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess || a.cap == 0) return e;
+    if (e != hipSuccess || a.cap <= kMovesHere) return e;
     evict_move_kernel<<<dim3((a.cap + MOVES - 1) / MOVES, pairs), dim3(256), 0, stream>>>(kv, a);
     return hipGetLastError();
 }
