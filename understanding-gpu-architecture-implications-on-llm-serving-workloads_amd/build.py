@@ -42,8 +42,8 @@ SOURCE_PARTS = {"csrc/hgemm.hip": [(t + "." + l.lower(), ["-DMI355_HGEMM_T=%s_t"
                                     (["-DMI355_HGEMM_STEP"] if l == "NT" else []))
                                    for t in ("fp16", "bf16") for l in ("NN", "NT", "TN")]}
 # Per-source additions. The GEMM keeps its MFMA accumulators in ordinary VGPRs: left to itself the compiler moves part of
-# them to AGPRs in the 4-wave kernels and then shuffles them back and forth inside the K loop.
-SOURCE_FLAGS = {src: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for src in ("csrc/hgemm.hip", "csrc/hgemm_direct.hip")}
+# them to AGPRs in the 4-wave kernels and then shuffles them back and forth inside the K loop; the attention over pages likewise.
+SOURCE_FLAGS = {src: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for src in ("csrc/hgemm.hip", "csrc/hgemm_direct.hip", "csrc/fmha_paged.hip")}
 
 
 def check_archs():

@@ -11,8 +11,9 @@
 // parts of a pair. Where a pair is walked by one workgroup it writes O and LSE itself.
 //
 // Inside a part: the query rows of all heads of the kv head are the columns of S^T = K Q^T (MFMA 16x16x32), so K and V are read
-// once per kv head. The waves cut the part into contiguous pieces; each streams its tiles through two private LDS stages with
-// direct-to-LDS copies, no barriers, and keeps a running maximum and sum. 16 keys lie in one page: a lane works out the
+// once per kv head. The waves take the part's tiles in turn; each streams its own through two private LDS stages with
+// direct-to-LDS copies, no barriers, and keeps a running maximum and sum; the next part's first tiles are requested in front of the last ones'
+// arithmetic. 16 keys lie in one page: a lane works out the
 // address of one such half tile of the next 64, and the scalar unit picks them up one after the other.
 #include <algorithm>
 
@@ -30,6 +31,7 @@ constexpr int WAVES = 4, NSTAGE = 2;
 constexpr int NTHREADS = WAVES * 64;
 constexpr int WAVE_BYTES = NSTAGE * STAGE_BYTES;
 constexpr int LDS_BYTES = WAVES * WAVE_BYTES;   // 128 KiB
+constexpr int kMeetBytes = 31 << 10;           // the rest of a CU's 160 KiB, less what the compiler may want
 constexpr int COPIES = 2 * (TILE_BYTES / 1024);
 constexpr int WINDOW = 32;                   // tiles whose addresses a wave holds at a time (64 half tiles, one a lane)
 constexpr float kLazyLog2 = 8.f;             // rescale only when a column maximum grows by more than 2^8
@@ -60,6 +62,7 @@ struct PagedAttn {
     long part_block;  // floats of `part` per block of columns
     int Hq, Sq, group, ncols, col_block;   // columns of a kv head, and of a workgroup
     int workgroups, min_tiles, direct, max_tiles;
+    int apart;        // the waves' results meet behind the stages
     float scale_log2;
     Divisor by_sq, by_hkv;
 };
@@ -144,85 +147,112 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
     const T* Q = (const T*)a.Q;
     T* O = (T*)a.O;
 
+    // Part of this workgroup: tiles tile0 .. tile0 + n - 1 of (seq.b, hkv); wave w takes every fourth from tile0 + w on
+    struct Part {
+        Where seq;
+        int hkv, tile0, n;
+    };
     Lengths lengths(kv);
-    Where seq;
-    int f = 0, f_end = 0, hkv, tile0;
+    Part now;
+    int f = 0, f_end = 0;
     if (a.direct) {
         const int b = divide(blockIdx.x, a.by_hkv);
-        hkv = blockIdx.x - b * kv.Hkv;
         const int len = __builtin_amdgcn_readfirstlane(paged_len(kv, b));
-        seq = {b, len, tiles_of(len), 0};
-        tile0 = 0;
-        f_end = seq.tiles;
+        now = {{b, len, tiles_of(len), 0}, (int)blockIdx.x - b * kv.Hkv, 0, tiles_of(len)};
+        f_end = now.n;
     } else {
         const Cut cut = lengths.cut(a);
         f = blockIdx.x * cut.quota;
         f_end = min(f + cut.quota, cut.total);
         if (f >= f_end) return;
-        seq = lengths.find(f);
-        const int rest = f - seq.before * kv.Hkv;
-        hkv = (int)((uint32_t)rest / (uint32_t)seq.tiles);
-        tile0 = rest - hkv * seq.tiles;
+        now.seq = lengths.find(f);
+        const int rest = f - now.seq.before * kv.Hkv;
+        now.hkv = (int)((uint32_t)rest / (uint32_t)now.seq.tiles);
+        now.tile0 = rest - now.hkv * now.seq.tiles;
+        now.n = min(now.seq.tiles - now.tile0, f_end - f);
     }
 
-    for (;;) {   // the parts of this workgroup: tiles tile0 .. tile0 + n - 1 of (seq.b, hkv)
-        const int n = min(seq.tiles - tile0, f_end - f);
-        const int per_wave = (n + WAVES - 1) / WAVES;
-        const int t_begin = tile0 + min(wave * per_wave, n);
-        const int n_loc = tile0 + min((wave + 1) * per_wave, n) - t_begin;
-        const int b = seq.b, len = seq.len;
-        const int* table = kv.table + (long)b * kv.table_stride;
-        const char* heads = kv.pages + (long)hkv * kv.head_bytes;
-        const long v_off = (long)kv.Hkv * kv.head_bytes;
+    // The tiles in flight: of `ahead` (the part whose tiles are being requested), window of 32 of this wave's tiles. Half tile h of it is
+    // lane h's: the address of its 16 keys; a half without keys or with a page outside the pool has its bit in `bad` and the pool's
+    // first page to read.
+    Part ahead = now;
+    uint32_t adr_lo = 0, adr_hi = 0;
+    uint64_t bad = 0;
+    const long v_off = (long)kv.Hkv * kv.head_bytes;
+    auto load_window = [&](int i) {
+        const int key = ((ahead.tile0 + wave + (i + (lane >> 1)) * WAVES) * 2 + (lane & 1)) * 16;
+        const int index = divide(key, kv.by_page);
+        const int page = kv.table[(long)ahead.seq.b * kv.table_stride + min(index, kv.max_pages - 1)];
+        const bool ok = key < ahead.seq.len && (uint32_t)page < (uint32_t)kv.n_pages;
+        bad = __builtin_amdgcn_ballot_w64(!ok);
+        const uint64_t adr = (uint64_t)(uintptr_t)kv.pages + (uint64_t)ahead.hkv * kv.head_bytes +
+                             (ok ? (uint64_t)page * kv.page_bytes + (uint32_t)(key - index * kv.page_size) * kv.row_bytes : 0);
+        adr_lo = (uint32_t)adr;
+        adr_hi = (uint32_t)(adr >> 32);
+    };
+    // this wave's tile i of `ahead` into stage `slot`: copy c covers rows 4c + lane / 16 of a half tile, chunk lane % 16 (the rows' swizzles
+    // repeat every 16); rows behind the last key repeat it (masked later)
+    const int c_row = lane >> 4;
+    uint32_t k_lane[4], v_lane[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        const int row = 4 * c + c_row;
+        k_lane[c] = (uint32_t)row * kv.row_bytes + ((uint32_t)(c16 ^ swz_k(row)) << 4);
+        v_lane[c] = (uint32_t)row * kv.row_bytes + ((uint32_t)(c16 ^ swz_v(row)) << 4);
+    }
+    uint32_t bad_stage0 = 0, bad_stage1 = 0;   // halves (bits 0, 1) of the tile in each stage that hold no keys at all
+    auto issue_tile = [&](int i, int slot) {
+        if ((i & (WINDOW - 1)) == 0) load_window(i);
+        MI355_LDS char* st = wbase + slot * STAGE_BYTES;
+        const int w = (i & (WINDOW - 1)) * 2;
+        const uint32_t none = (uint32_t)(bad >> w) & 3;
+        if (slot == 0) bad_stage0 = none;
+        else bad_stage1 = none;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const char* kb = (const char*)(uintptr_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)adr_lo, w + h) |
+                                                      (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)adr_hi, w + h) << 32);
+            const char* vb = kb + v_off;
+            const int last = ahead.seq.len - 1 - ((ahead.tile0 + wave + i * WAVES) * 2 + h) * 16;
+            if (last >= 15) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) copy16_global_to_lds(kb, k_lane[c], st + (4 * h + c) * 1024);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) copy16_global_to_lds(vb, v_lane[c], st + TILE_BYTES + (4 * h + c) * 1024);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int row = 4 * c + c_row;
+                    copy16_global_to_lds(kb, k_lane[c] - (uint32_t)(row - min(row, max(last, 0))) * kv.row_bytes, st + (4 * h + c) * 1024);
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int row = 4 * c + c_row;
+                    copy16_global_to_lds(vb, v_lane[c] - (uint32_t)(row - min(row, max(last, 0))) * kv.row_bytes, st + TILE_BYTES + (4 * h + c) * 1024);
+                }
+            }
+        }
+    };
+    const auto count_of = [&](const Part& p) { return max((p.n - wave + WAVES - 1) / WAVES, 0); };
+    // The part behind `now` becomes `ahead` and its first tile is requested. (Tiles are left in front of f_end, so the sequences that follow
+    // have some.)
+    auto begin_next = [&](int slot) {
+        ahead.tile0 = 0;
+        if (++ahead.hkv == kv.Hkv) {
+            ahead.hkv = 0;
+            ahead.seq = lengths.find(f + now.n);
+        }
+        ahead.n = min(ahead.seq.tiles, f_end - f - now.n);
+        const bool any = count_of(ahead) > 0;
+        if (any) issue_tile(0, slot);
+        return any;
+    };
 
-        // half tile h of the window (a lane's own): the address of its 16 keys; a lane without keys or with a page outside the pool
-        // has its bit in `bad` and the pool's first page to read
-        uint32_t adr_lo = 0, adr_hi = 0;
-        uint64_t bad = 0;
-        auto load_window = [&](int first_tile) {
-            const int key = (first_tile * 2 + lane) * 16;
-            int page = 0, slot = 0;
-            bool ok = key < len;
-            if (ok) {
-                const int i = divide(key, kv.by_page);
-                page = table[i];
-                slot = key - i * kv.page_size;
-                ok = (uint32_t)page < (uint32_t)kv.n_pages;
-            }
-            bad = __builtin_amdgcn_ballot_w64(!ok);
-            const uint64_t adr = (uint64_t)(uintptr_t)heads + (ok ? (uint64_t)page * kv.page_bytes + (uint32_t)slot * kv.row_bytes : 0);
-            adr_lo = (uint32_t)adr;
-            adr_hi = (uint32_t)(adr >> 32);
-        };
-        // tile i of this wave's piece into stage `slot`: copy c covers rows 4c + lane / 16 of the tile, chunk lane % 16; rows behind
-        // the last key repeat it (masked later)
-        const int c_row = lane >> 4;
-        const uint32_t chunk = lane & 15;
-        uint64_t bad_next = 0;   // halves (bit 0, 1) of the tile issued last that hold no keys at all
-        auto issue_stage = [&](int i, int slot) {
-            if ((i & (WINDOW - 1)) == 0) load_window(t_begin + i);
-            MI355_LDS char* st = wbase + slot * STAGE_BYTES;
-            const int w = (i & (WINDOW - 1)) * 2;
-            bad_next = (bad >> w) & 3;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const char* kb = (const char*)(uintptr_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)adr_lo, w + h) |
-                                                          (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)adr_hi, w + h) << 32);
-                const char* vb = kb + v_off;
-                const int last = max(min(len - 1 - ((t_begin + i) * 2 + h) * 16, 15), 0);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int row = 4 * c + c_row;
-                    copy16_global_to_lds(kb, (uint32_t)min(row, last) * kv.row_bytes + ((chunk ^ swz_k(row)) << 4), st + (4 * h + c) * 1024);
-                }
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int row = 4 * c + c_row;
-                    copy16_global_to_lds(vb, (uint32_t)min(row, last) * kv.row_bytes + ((chunk ^ swz_v(row)) << 4),
-                                         st + TILE_BYTES + (4 * h + c) * 1024);
-                }
-            }
-        };
+    if (count_of(now) > 0) issue_tile(0, 0);
+    int slot = 0;   // stage of the next tile
+    for (;;) {      // the parts
+        const int n = now.n, n_loc = count_of(now), hkv = now.hkv, b = now.seq.b, len = now.seq.len;
+        const bool more = f + n < f_end;
         const int k_base = c16 * ROW_BYTES + ((g ^ c16) << 4);   // xor (ks << 6), + kb * 16 rows
         const int v_row = 4 * g + (c16 >> 2);
         const int v_base = TILE_BYTES + v_row * ROW_BYTES + ((((c16 & 3) >> 1) ^ swz_v(v_row)) << 4) + (c16 & 1) * 8;  // xor (db << 5)
@@ -236,10 +266,6 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
 #pragma unroll
             for (int db = 0; db < 8; ++db) o[nb][db] = float4v{0.f, 0.f, 0.f, 0.f};
         }
-        uint64_t bad_of[NSTAGE];   // of the tile in each stage
-        if (n_loc > 0) issue_stage(0, 0);
-        bad_of[0] = bad_next;
-        bad_of[1] = 0;
         // queries behind the first copies: column c of the kv head = (its query head c / Sq, row c % Sq)
         const int n_new = paged_new(kv, b, a.Sq);
         int lim[NB];      // last visible key of this lane's column(s); -1: none
@@ -278,18 +304,24 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) asm volatile("" : "+v"(qf[nb][0]), "+v"(qf[nb][1]), "+v"(qf[nb][2]), "+v"(qf[nb][3]));
 
+        bool begun = false;   // the next part's first tile has been requested
         for (int i = 0; i < n_loc; ++i) {
-            const int slot = i & 1;
+            bool newer = true;
             if (i + 1 < n_loc) {
-                issue_stage(i + 1, slot ^ 1);
-                bad_of[slot ^ 1] = bad_next;
-                wait_vmcnt<COPIES>();   // everything but the newest tile has landed
+                issue_tile(i + 1, slot ^ 1);
+            } else if (a.apart && more) {
+                newer = begin_next(slot ^ 1);
+                begun = true;
             } else {
-                wait_vmcnt<0>();
+                newer = false;
             }
+            if (newer) wait_vmcnt<COPIES>();   // everything but the newest tile has landed
+            else wait_vmcnt<0>();
             MI355_LDS char* st = wbase + slot * STAGE_BYTES;
-            const int key0 = (t_begin + i) * TK;
-            const uint64_t no_keys = bad_of[slot];
+            const int tile = now.tile0 + wave + i * WAVES;
+            const int key0 = tile * TK;
+            const uint32_t no_keys = slot == 0 ? bad_stage0 : bad_stage1;
+            slot ^= 1;
 
             // S^T = K Q^T: lane holds keys 16 kb + 4 g + 0..3 of its column
             float4v s[NB][2];
@@ -312,7 +344,7 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
                         if (key0 + 16 * (e >> 2) + 4 * g + (e & 3) > lim[nb] || ((no_keys >> (e >> 2)) & 1)) s[nb][e >> 2][e & 3] = -INFINITY;
             }
             if constexpr (SCORES) {
-                float* sp = a.scores + (((long)b * kv.Hkv + hkv) * a.max_tiles + t_begin + i) * (a.ncols * TK);
+                float* sp = a.scores + (((long)b * kv.Hkv + hkv) * a.max_tiles + tile) * (a.ncols * TK);
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
                     if (16 * nb + c16 < ncols) {
@@ -387,9 +419,11 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
             wait_lgkmcnt<0>();  // the reads of this slot are complete before a later copy refills it
         }
 
-        // ---- the waves' results meet in LDS (their stages are free): per wave O~ [ncols][128] floats, then m [32], l [32] ----
+        if (a.apart && more && !begun) begin_next(slot);   // (a wave without a tile of this part)
+        // ---- the waves' results meet in LDS, behind the stages where there is room (a.apart: the next part's first tiles are on their way into
+        // those), otherwise in them: per wave O~ [ncols][128] floats, then m [32], l [32] ----
         __syncthreads();
-        MI355_LDS float* cmb = (MI355_LDS float*)smem_raw;
+        MI355_LDS float* cmb = (MI355_LDS float*)(smem_raw + (a.apart ? LDS_BYTES : 0));
         const int wave_floats = ncols * D + 64;
         {
             MI355_LDS float* mine = cmb + wave * wave_floats;
@@ -408,7 +442,7 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
             }
         }
         __syncthreads();
-        const bool whole = n == seq.tiles;   // this part is all of its pair
+        const bool whole = n == now.seq.tiles;   // this part is all of its pair
         float* part = a.part + (whole ? 0 : blockIdx.y * a.part_block + (long)(blockIdx.x + b * kv.Hkv + hkv) * (a.col_block * PART_STRIDE));
         for (int e4 = tid; e4 < ncols * (D / 4); e4 += NTHREADS) {   // output elements (column e4 / 32, d 4 (e4 % 32) .. +3)
             const int c = e4 >> 5, d = (e4 & 31) * 4;
@@ -448,15 +482,13 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
                 }
             }
         }
-        f += n;
-        if (f >= f_end || n == 0) return;
-        __syncthreads();   // the next part's copies overwrite what was read above
-        // the next pair: tiles are left in front of f_end, so one with tiles follows
-        tile0 = 0;
-        if (++hkv == kv.Hkv) {
-            hkv = 0;
-            seq = lengths.find(f);
+        if (!more) return;
+        if (!a.apart) {
+            __syncthreads();   // the next part's copies overwrite what was read above
+            begin_next(slot);
         }
+        f += n;
+        now = ahead;
     }
 }
 
@@ -548,7 +580,7 @@ __global__ __launch_bounds__(256) void paged_weights_kernel(PagedKv kv, PagedAtt
 
 // What a call takes of its workspace
 struct PagedPlan {
-    int nb, col_block, blocks, workgroups, direct, max_tiles, scores;
+    int nb, col_block, blocks, workgroups, direct, max_tiles, scores, lds;
     size_t part_bytes, score_bytes, lse_bytes;
 };
 static PagedPlan paged_plan(int B, int Hkv, int max_len, int Hq, int Sq, bool weights, bool lse) {
@@ -564,6 +596,8 @@ static PagedPlan paged_plan(int B, int Hkv, int max_len, int Hq, int Sq, bool we
     p.workgroups = p.direct ? (int)pairs : (int)std::min<long>(kWorkgroups, (pairs * p.max_tiles + kMinTiles - 1) / kMinTiles);
     if (!p.direct) p.part_bytes = sizeof(float) * (size_t)p.blocks * (p.workgroups + pairs) * p.col_block * PART_STRIDE;
     p.scores = weights && ncols <= 32;
+    const int meet = WAVES * (p.col_block * D + 64) * (int)sizeof(float);
+    p.lds = LDS_BYTES + (meet <= kMeetBytes ? meet : 0);
     if (p.scores) p.score_bytes = sizeof(float) * (size_t)pairs * p.max_tiles * ncols * TK;
     if (weights && !lse) p.lse_bytes = (sizeof(float) * (size_t)B * Hq * Sq + 15) & ~size_t(15);
     return p;
@@ -580,9 +614,9 @@ template <typename T, int NB, bool SCORES>
 static hipError_t launch_paged(const PagedKv& kv, const PagedAttn& a, const PagedPlan& p, hipStream_t stream) {
     using namespace pdec;
     static DynamicLdsOnce once;
-    const hipError_t e = once.ensure(reinterpret_cast<const void*>(fmha_paged_kernel<T, NB, SCORES>), LDS_BYTES);
+    const hipError_t e = once.ensure(reinterpret_cast<const void*>(fmha_paged_kernel<T, NB, SCORES>), LDS_BYTES + kMeetBytes);
     if (e != hipSuccess) return e;
-    fmha_paged_kernel<T, NB, SCORES><<<dim3(p.workgroups, p.blocks), dim3(NTHREADS), LDS_BYTES, stream>>>(kv, a);
+    fmha_paged_kernel<T, NB, SCORES><<<dim3(p.workgroups, p.blocks), dim3(NTHREADS), p.lds, stream>>>(kv, a);
     return hipGetLastError();
 }
 
@@ -629,6 +663,7 @@ hipError_t fmha_paged_dispatch(const mi355_paged_kv& c, const void* Q, void* O, 
     a.workgroups = p.workgroups;
     a.min_tiles = pdec::kMinTiles;
     a.direct = p.direct;
+    a.apart = p.lds > pdec::LDS_BYTES;
     a.max_tiles = p.max_tiles;
     a.part_block = (long)(p.workgroups + kv.B * kv.Hkv) * p.col_block * pdec::PART_STRIDE;
     a.scale_log2 = scale * 1.4426950408889634f;

@@ -315,7 +315,16 @@ __global__ __launch_bounds__(evict::THREADS) void evict_select_kernel(PagedKv kv
         movers += keep && j >= a.budget;
     });
     int total;
-    int hole = block_before(holes, sums[1], total), mover = block_before(movers, sums[2], unused);
+    int hole, mover;
+    if constexpr (M > 0) {   // at most 16384 of each: one sum for both
+        hole = block_before(holes | movers << 16, sums[1], total);
+        mover = hole >> 16;
+        hole &= 0xffff;
+        total &= 0xffff;
+    } else {
+        hole = block_before(holes, sums[1], total);
+        mover = block_before(movers, sums[2], unused);
+    }
     const bool here = a.cap <= kMovesHere;
     if (tid == 0) a.counts[blockIdx.x] = here ? 0 : total;
     int* to = a.moves + (long)blockIdx.x * 2 * a.cap;
