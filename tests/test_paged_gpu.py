@@ -612,6 +612,28 @@ def test_a_captured_step_is_replayed_as_the_lengths_go_on(gpu):
             assert torch.equal(x.nan_to_num(7.0), y.nan_to_num(7.0))
 
 
+@pytest.mark.parametrize("Hq,Hkv,S", [(1, 1, 1), (4, 2, 1), (32, 8, 1), (64, 8, 1), (16, 2, 4), (40, 4, 7)])
+def test_captured_and_eager_calls_give_the_same_bits(gpu, Hq, Hkv, S):
+    """Parts of long caches are joined by the last workgroup, or by a launch of their own in a captured call."""
+    cache = Cache([9000, 17, 0, 3000], Hkv, 32)
+    q = queries(cache, Hq, S)
+    weights = cache.weights.clone()
+    eager = [ops.fine_fmha_paged_with_lse(q, *cache.args, weights=weights) for _ in range(3)]
+    check_attention(cache, q, *eager[0])
+    for o, lse in eager[1:]:
+        assert torch.equal(o, eager[0][0]) and torch.equal(lse, eager[0][1])
+    other = cache.weights.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = ops.fine_fmha_paged_with_lse(q, *cache.args, weights=other)
+    for _ in range(3):
+        g.replay()
+        again = ops.fine_fmha_paged(q, *cache.args)
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], eager[0][0]) and torch.equal(out[1], eager[0][1]) and torch.equal(again, out[0])
+    assert torch.equal(other.nan_to_num(7.0), weights.nan_to_num(7.0))
+
+
 def test_calls_on_two_streams_at_once(gpu):
     loops = [Loop(seed=s) for s in (1, 2)]
     alone = [Loop(seed=s) for s in (1, 2)]

@@ -22,6 +22,7 @@
 namespace mi355 {
 
 namespace pdec {
+typedef float float2v __attribute__((ext_vector_type(2)));
 constexpr int D = 128;
 constexpr int TK = 32;                       // keys per tile
 constexpr int ROW_BYTES = D * 2;             // 256
@@ -492,12 +493,17 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
     }
 }
 
-// Joins the parts of each (pair, column): grid (pairs, columns of all blocks). O = sum_p 2^((m_p - m) c) O~_p / sum_p 2^((m_p - m) c) l_p. Pairs without a key
-// get zeros, those of one part were written by its workgroup.
+// Joins the parts of each (pair, column): grid (pairs, columns of all blocks). O = sum_p w_p O~_p / sum_p w_p l_p with w_p = 2^((m_p - max m) c). Pairs
+// without a key get zeros, those of one part were written by its workgroup. Bound by its chain of memory round trips: the lengths, then
+// up to 32 parts at once (a thread takes 4 d of every eighth part, up to four of them in flight; the eight sums meet in LDS). The last
+// workgroup of a pair doing this inside the first launch, which takes loads and stores at device scope, was slower: 1 x 32/8 heads over 8191 keys 14.1
+// us with this launch, 15.5 without, 4 drafted tokens of 4 x 2048 keys 15.6 and 22.5.
 template <typename T>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedKv kv, PagedAttn a) {
+__global__ __launch_bounds__(pdec::NTHREADS) void paged_join_kernel(PagedKv kv, PagedAttn a) {
     using namespace pdec;
-    __shared__ __attribute__((aligned(16))) float sums[8][D + 4];
+    constexpr int ROUNDS = 4;
+    __shared__ __attribute__((aligned(16))) float sums[8][PART_STRIDE];
+    const int tid = threadIdx.x, part0 = tid >> 5, d = (tid & 31) * 4;
     const int b = divide(blockIdx.x, a.by_hkv), hkv = blockIdx.x - b * kv.Hkv;
     Lengths lengths(kv);
     const Cut cut = lengths.cut(a);
@@ -508,42 +514,53 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedKv kv, PagedAttn a
     if (n == 1) return;
     const int col = blockIdx.y, cb = (int)((uint32_t)col / (uint32_t)a.col_block), c = col - cb * a.col_block;
     const int head = divide(col, a.by_sq), qi = col - head * a.Sq, hq = hkv * a.group + head;
-    const int part0 = threadIdx.x >> 5, d = (threadIdx.x & 31) * 4;
     const long stride = (long)a.col_block * PART_STRIDE;
     const float* base = a.part + cb * a.part_block + (long)(first + blockIdx.x) * stride + c * PART_STRIDE;
     float m = -INFINITY, l = 0.f;
     float4v acc = float4v{0.f, 0.f, 0.f, 0.f};
-    for (int p = part0; p < n; p += 8) {
-        const float* pp = base + p * stride;
-        const float4v v = *(const float4v*)(pp + d);
-        const float mp = pp[D], lp = pp[D + 1];
-        const float m_new = fmaxf(m, mp);
-        if (mp != -INFINITY) {
-            const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - m_new) * a.scale_log2);
-            const float wgt = __builtin_amdgcn_exp2f((mp - m_new) * a.scale_log2);
-            acc = acc * keep + v * wgt;
-            l = l * keep + lp * wgt;
-            m = m_new;
-        } else {   // no score above minus infinity: nothing, or NaN
-            acc += v;
-            l += lp;
+    // of a part that saw no key: its outputs and l are 0 (or NaN, which stays)
+    const auto weight = [&](float x, float ref) { return x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((x - ref) * a.scale_log2); };
+    for (int p0 = part0; p0 < n; p0 += 8 * ROUNDS) {
+        float4v v[ROUNDS];
+        float2v ml[ROUNDS];
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r)
+            if (r == 0 || p0 + 8 * r < n) {
+                const float* pp = base + (long)(p0 + 8 * r) * stride;
+                v[r] = *(const float4v*)(pp + d);
+                ml[r] = *(const float2v*)(pp + D);
+            } else {
+                v[r] = float4v{0.f, 0.f, 0.f, 0.f};
+                ml[r] = float2v{-INFINITY, 0.f};
+            }
+        float m_new = m;
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r) m_new = fmaxf(m_new, ml[r][0]);
+        const float keep = weight(m, m_new);
+        acc *= keep;
+        l *= keep;
+        m = m_new;
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r) {
+            const float w = weight(ml[r][0], m);
+            acc += w * v[r];
+            l += w * ml[r][1];
         }
     }
     *(float4v*)&sums[part0][d] = acc;
     if (d == 0) sums[part0][D] = m, sums[part0][D + 1] = l;
     __syncthreads();
-    if (threadIdx.x >= 32) return;
-    float m_all = -INFINITY;
+    if (tid >= 32) return;
+    m = -INFINITY;
 #pragma unroll
-    for (int p = 0; p < 8; ++p) m_all = fmaxf(m_all, sums[p][D]);
+    for (int p = 0; p < 8; ++p) m = fmaxf(m, sums[p][D]);
     acc = float4v{0.f, 0.f, 0.f, 0.f};
     l = 0.f;
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
-        const float mp = sums[p][D];
-        const float wgt = mp == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mp - m_all) * a.scale_log2);
-        acc += *(const float4v*)&sums[p][d] * wgt;
-        l += sums[p][D + 1] * wgt;
+        const float w = weight(sums[p][D], m);
+        acc += w * *(const float4v*)&sums[p][d];
+        l += w * sums[p][D + 1];
     }
     const float inv = l != 0.f ? 1.f / l : 0.f;
     typename Elem<T>::v4 ov;
@@ -551,7 +568,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedKv kv, PagedAttn a
     for (int e = 0; e < 4; ++e) ov[e] = (T)(acc[e] * inv);
     *(typename Elem<T>::v4*)((T*)a.O + b * a.o_batch + (long)hq * a.o_head + qi * a.o_row + d) = ov;
     if (a.LSE != nullptr && d == 0)
-        a.LSE[((long)b * a.Hq + hq) * a.Sq + qi] = l != 0.f ? (m_all * a.scale_log2 + __builtin_log2f(l)) * 0.69314718055994531f : -INFINITY;
+        a.LSE[((long)b * a.Hq + hq) * a.Sq + qi] = l != 0.f ? (m * a.scale_log2 + __builtin_log2f(l)) * 0.69314718055994531f : -INFINITY;
 }
 
 // weights[page][kv head][slot] += sum over the pair's columns of 2^(s c - LSE): grid (tiles / 8, pairs), a thread per key
