@@ -8,7 +8,7 @@
 // are known to the device only, so the cut of the work is made there: the key tiles (32 keys) of all (sequence, kv head) pairs
 // lie one behind the other on one axis, and each of a fixed number of workgroups takes an equal piece of it, whatever pairs
 // the piece touches. A part of a pair leaves an unnormalised partial result (O~ [128], m, l a column, fp32); a second kernel joins the
-// parts of a pair. Where a pair is walked by one workgroup it writes O and LSE itself.
+// parts of a pair and, beside that, adds to the account from the scores that the first one left. Where a pair is walked by one workgroup it writes O and LSE itself.
 //
 // Inside a part: the query rows of all heads of the kv head are the columns of S^T = K Q^T (MFMA 16x16x32), so K and V are read
 // once per kv head. The waves take the part's tiles in turn; each streams its own through two private LDS stages with
@@ -65,7 +65,8 @@ struct PagedAttn {
     int workgroups, min_tiles, direct, max_tiles;
     int apart;        // the waves' results meet behind the stages
     float scale_log2;
-    Divisor by_sq, by_hkv;
+    int chunks;       // of 256 keys, of the longest sequence
+    Divisor by_sq, by_hkv, by_ncols, by_chunks;
 };
 
 namespace pdec {
@@ -130,8 +131,8 @@ struct Lengths {
 
 }  // namespace pdec
 
-// Grid: (workgroups, blocks of columns). NB: blocks of 16 columns of a workgroup. SCORES: the scores are kept for
-// paged_weights_kernel.
+// Grid: (workgroups, blocks of columns). NB: blocks of 16 columns of a workgroup. SCORES: the scores are kept for the
+// account.
 template <typename T, int NB, bool SCORES>
 __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, PagedAttn a) {
     using namespace pdec;
@@ -493,29 +494,36 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
     }
 }
 
-// Joins the parts of each (pair, column): grid (pairs, columns of all blocks). O = sum_p w_p O~_p / sum_p w_p l_p with w_p = 2^((m_p - max m) c). Pairs
+// The parts of a pair: how many, and the workgroup that has the first
+__device__ __forceinline__ int parts_of(const PagedKv& kv, const PagedAttn& a, int b, int hkv, int& first) {
+    using namespace pdec;
+    Lengths lengths(kv);
+    const Cut cut = lengths.cut(a);
+    const Where seq = lengths.at(b);
+    const int f = seq.before * kv.Hkv + hkv * seq.tiles;
+    first = (int)((uint32_t)f / (uint32_t)cut.quota);
+    return seq.tiles == 0 ? 0 : (int)((uint32_t)(f + seq.tiles - 1) / (uint32_t)cut.quota) - first + 1;
+}
+
+// Joins the parts of a (pair, column): O = sum_p w_p O~_p / sum_p w_p l_p with w_p = 2^((m_p - max m) c). Pairs
 // without a key get zeros, those of one part were written by its workgroup. Bound by its chain of memory round trips: the lengths, then
 // up to 32 parts at once (a thread takes 4 d of every eighth part, up to four of them in flight; the eight sums meet in LDS). The last
 // workgroup of a pair doing this inside the first launch, which takes loads and stores at device scope, was slower: 1 x 32/8 heads over 8191 keys 14.1
 // us with this launch, 15.5 without, 4 drafted tokens of 4 x 2048 keys 15.6 and 22.5.
 template <typename T>
-__global__ __launch_bounds__(pdec::NTHREADS) void paged_join_kernel(PagedKv kv, PagedAttn a) {
+__device__ __forceinline__ void join_parts(const PagedKv& kv, const PagedAttn& a, int pair, int col) {
     using namespace pdec;
     constexpr int ROUNDS = 4;
     __shared__ __attribute__((aligned(16))) float sums[8][PART_STRIDE];
     const int tid = threadIdx.x, part0 = tid >> 5, d = (tid & 31) * 4;
-    const int b = divide(blockIdx.x, a.by_hkv), hkv = blockIdx.x - b * kv.Hkv;
-    Lengths lengths(kv);
-    const Cut cut = lengths.cut(a);
-    const Where seq = lengths.at(b);
-    const int f = seq.before * kv.Hkv + hkv * seq.tiles;
-    const int first = (int)((uint32_t)f / (uint32_t)cut.quota);
-    const int n = seq.tiles == 0 ? 0 : (int)((uint32_t)(f + seq.tiles - 1) / (uint32_t)cut.quota) - first + 1;
+    const int b = divide(pair, a.by_hkv), hkv = pair - b * kv.Hkv;
+    int first;
+    const int n = parts_of(kv, a, b, hkv, first);
     if (n == 1) return;
-    const int col = blockIdx.y, cb = (int)((uint32_t)col / (uint32_t)a.col_block), c = col - cb * a.col_block;
+    const int cb = (int)((uint32_t)col / (uint32_t)a.col_block), c = col - cb * a.col_block;
     const int head = divide(col, a.by_sq), qi = col - head * a.Sq, hq = hkv * a.group + head;
     const long stride = (long)a.col_block * PART_STRIDE;
-    const float* base = a.part + cb * a.part_block + (long)(first + blockIdx.x) * stride + c * PART_STRIDE;
+    const float* base = a.part + cb * a.part_block + (long)(first + pair) * stride + c * PART_STRIDE;
     float m = -INFINITY, l = 0.f;
     float4v acc = float4v{0.f, 0.f, 0.f, 0.f};
     // of a part that saw no key: its outputs and l are 0 (or NaN, which stays)
@@ -571,28 +579,78 @@ __global__ __launch_bounds__(pdec::NTHREADS) void paged_join_kernel(PagedKv kv, 
         a.LSE[((long)b * a.Hq + hq) * a.Sq + qi] = l != 0.f ? (m * a.scale_log2 + __builtin_log2f(l)) * 0.69314718055994531f : -INFINITY;
 }
 
-// weights[page][kv head][slot] += sum over the pair's columns of 2^(s c - LSE): grid (tiles / 8, pairs), a thread per key
-__global__ __launch_bounds__(256) void paged_weights_kernel(PagedKv kv, PagedAttn a) {
+// weights[page][kv head][slot] += sum over the pair's columns of 2^(s c - LSE) for 256 keys, one a thread. The log-sum-exp comes from the parts'
+// statistics, so that this need not wait for the joining; a pair of one part has it in place.
+__device__ __forceinline__ void add_weights(const PagedKv& kv, const PagedAttn& a, int pair, int chunk) {
     using namespace pdec;
     __shared__ float lse[32];
-    const int b = divide(blockIdx.y, a.by_hkv), hkv = blockIdx.y - b * kv.Hkv;
+    const int tid = threadIdx.x;
+    const int b = divide(pair, a.by_hkv), hkv = pair - b * kv.Hkv;
     const int len = paged_len(kv, b);
-    const int key = blockIdx.x * 256 + threadIdx.x;
-    if ((int)(blockIdx.x * 256) >= len) return;
-    if ((int)threadIdx.x < a.ncols) {
-        const float x = a.LSE[((long)b * a.Hq + hkv * a.group) * a.Sq + threadIdx.x];   // columns are consecutive rows
-        lse[threadIdx.x] = x == -INFINITY ? INFINITY : x * 1.4426950408889634f;         // a row that sees no key adds nothing
+    const int key = chunk * 256 + tid;
+    if (chunk * 256 >= len) return;
+    int first = 0;
+    const int n = a.direct ? 1 : parts_of(kv, a, b, hkv, first);
+    // the first scores are fetched beside the statistics
+    const float* sp = a.scores + ((long)pair * a.max_tiles + (min(key, len - 1) >> 5)) * (a.ncols * TK) + (key & 31);
+    constexpr int AHEAD = 8;
+    float s[AHEAD];
+#pragma unroll
+    for (int c = 0; c < AHEAD; ++c) s[c] = sp[min(c, a.ncols - 1) * TK];
+    if (n == 1) {
+        if (tid < a.ncols) {
+            const float x = a.LSE[((long)b * a.Hq + hkv * a.group) * a.Sq + tid];   // columns are consecutive rows
+            lse[tid] = x * 1.4426950408889634f;
+        }
+    } else {
+        // 32 lanes a column
+        for (int c = tid >> 5; c < a.ncols; c += 8) {
+            const float* ps = a.part + (long)(first + pair) * (a.col_block * PART_STRIDE) + c * PART_STRIDE + D;
+            const long stride = (long)a.col_block * PART_STRIDE;
+            float m = -INFINITY, l = 0.f;
+            for (int p = tid & 31; p < n; p += 32) {
+                const float2v ml = *(const float2v*)(ps + p * stride);
+                const float m_new = fmaxf(m, ml[0]);
+                l = m_new == -INFINITY ? l + ml[1]   // (nothing yet, or NaN)
+                                       : l * __builtin_amdgcn_exp2f((m - m_new) * a.scale_log2) + ml[1] * __builtin_amdgcn_exp2f((ml[0] - m_new) * a.scale_log2);
+                m = m_new;
+            }
+            float m_all = m;
+#pragma unroll
+            for (int off = 16; off >= 1; off >>= 1) m_all = fmaxf(m_all, __shfl_xor(m_all, off, 64));
+            l = m_all == -INFINITY ? l : l * __builtin_amdgcn_exp2f((m - m_all) * a.scale_log2);
+#pragma unroll
+            for (int off = 16; off >= 1; off >>= 1) l += __shfl_xor(l, off, 64);
+            if ((tid & 31) == 0) lse[c] = l != 0.f ? m_all * a.scale_log2 + __builtin_log2f(l) : -INFINITY;
+        }
     }
     __syncthreads();
     if (key >= len) return;
-    const float* sp = a.scores + ((long)blockIdx.y * a.max_tiles + (key >> 5)) * (a.ncols * TK) + (key & 31);
     float sum = 0.f;
-    for (int c = 0; c < a.ncols; ++c) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(sp[c * TK], a.scale_log2, -lse[c]));
+    // a row that sees no key adds nothing
+    const auto add = [&](int c, float x) { sum += lse[c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(x, a.scale_log2, -lse[c])); };
+#pragma unroll
+    for (int c = 0; c < AHEAD; ++c)
+        if (c < a.ncols) add(c, s[c]);
+    for (int c = AHEAD; c < a.ncols; ++c) add(c, sp[c * TK]);
     const int i = divide(key, kv.by_page);
     const int page = kv.table[(long)b * kv.table_stride + i];
     if ((uint32_t)page >= (uint32_t)kv.n_pages) return;
-    float* w = kv.weights + ((long)page * kv.Hkv + hkv) * kv.page_size + (key - i * kv.page_size);
-    *w += sum;
+    kv.weights[((long)page * kv.Hkv + hkv) * kv.page_size + (key - i * kv.page_size)] += sum;
+}
+
+// What is left behind fmha_paged_kernel, side by side: a workgroup per (pair, column) joins parts (none where one workgroup walked all keys), then
+// one per (pair, 256 keys) adds to the account (none without one).
+template <typename T>
+__global__ __launch_bounds__(pdec::NTHREADS) void paged_finish_kernel(PagedKv kv, PagedAttn a) {
+    const int joins = a.direct ? 0 : kv.B * kv.Hkv * a.ncols;
+    if ((int)blockIdx.x < joins) {
+        const int pair = divide(blockIdx.x, a.by_ncols);
+        join_parts<T>(kv, a, pair, blockIdx.x - pair * a.ncols);
+    } else {
+        const int i = blockIdx.x - joins, pair = divide(i, a.by_chunks);
+        add_weights(kv, a, pair, i - pair * a.chunks);
+    }
 }
 
 // What a call takes of its workspace
@@ -639,15 +697,13 @@ static hipError_t launch_paged(const PagedKv& kv, const PagedAttn& a, const Page
 
 template <typename T>
 static hipError_t fmha_paged_t(const PagedKv& kv, const PagedAttn& a, const PagedPlan& p, hipStream_t stream) {
+    using namespace pdec;
     const unsigned pairs = (unsigned)(kv.B * kv.Hkv);
     hipError_t e = p.nb == 1 ? (p.scores ? launch_paged<T, 1, true>(kv, a, p, stream) : launch_paged<T, 1, false>(kv, a, p, stream))
                              : (p.scores ? launch_paged<T, 2, true>(kv, a, p, stream) : launch_paged<T, 2, false>(kv, a, p, stream));
-    if (e == hipSuccess && !p.direct) {
-        paged_join_kernel<T><<<dim3(pairs, a.ncols), dim3(256), 0, stream>>>(kv, a);
-        e = hipGetLastError();
-    }
-    if (e == hipSuccess && p.scores) {
-        paged_weights_kernel<<<dim3((kv.max_len + 255) / 256, pairs), dim3(256), 0, stream>>>(kv, a);
+    const unsigned rest = pairs * ((p.direct ? 0u : (unsigned)a.ncols) + (p.scores ? (unsigned)a.chunks : 0u));
+    if (e == hipSuccess && rest > 0) {
+        paged_finish_kernel<T><<<dim3(rest), dim3(NTHREADS), 0, stream>>>(kv, a);
         e = hipGetLastError();
     }
     return e;
@@ -686,6 +742,9 @@ hipError_t fmha_paged_dispatch(const mi355_paged_kv& c, const void* Q, void* O, 
     a.scale_log2 = scale * 1.4426950408889634f;
     a.by_sq = divisor_of(Sq);
     a.by_hkv = divisor_of(kv.Hkv);
+    a.chunks = (kv.max_len + 255) / 256;
+    a.by_ncols = divisor_of(a.ncols);
+    a.by_chunks = divisor_of(a.chunks);
     hipError_t e = c.dtype == MI355_DTYPE_BF16 ? fmha_paged_t<bf16_t>(kv, a, p, stream) : fmha_paged_t<half_t>(kv, a, p, stream);
     if (e == hipSuccess && kv.weights != nullptr && !p.scores)   // many rows: from the log-sum-exp, with the scores worked out again
         e = key_weights_dispatch(c, Q, a.LSE, Hq, Sq, strides, 0, scale, ws, stream);
