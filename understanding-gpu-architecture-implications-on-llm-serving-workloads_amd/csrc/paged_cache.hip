@@ -21,12 +21,12 @@ __global__ __launch_bounds__(pcache::THREADS) void rope_paged_kernel(PagedKv kv,
     const int head = blockIdx.y * 32 + (threadIdx.x >> 3);
     if (head >= q_heads + 2 * kv.Hkv) return;
     const int b = divide(blockIdx.x, by_s), t = blockIdx.x - b * S;
+    const int n_new = paged_new(kv, b, S);
+    if (t >= n_new) return;
     const int i0 = (threadIdx.x & 7) * 8;
     T* xp = qkv + b * x_batch + t * x_row + (long)head * 128 + i0;
     V8 lo = *(const V8*)xp;
     V8 hi = *(const V8*)(xp + 64);
-    const int n_new = paged_new(kv, b, S);
-    if (t >= n_new) return;
     const int place = positions[b * pos_batch + t];
     if (head < q_heads + kv.Hkv) {
         const int pos = min(max(place, 0), n_pos - 1);

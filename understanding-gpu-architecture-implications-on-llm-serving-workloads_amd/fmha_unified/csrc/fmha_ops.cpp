@@ -28,9 +28,6 @@
 
 namespace fmha_unified {
 
-// Registers _C as a Python extension module.
-PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {}
-
 namespace {
 
 // an uninitialised GPU tensor, without a trip through the dispatcher (0.4 us)
@@ -322,6 +319,18 @@ TORCH_LIBRARY_IMPL(fmha_unified, CPU, m) {
     m.impl("rope_paged", &rope_paged);
     m.impl("key_weights", &key_weights);
     m.impl("evict_paged", &evict_paged);
+}
+
+// _C as a Python extension module. The operators of the paged cache are functions of it as well: with eight to twelve arguments, most of them tensors, a call
+// through the dispatcher takes the host 1 us longer than one of these, and a step's calls are a few us long on the GPU (64 tokens filed, calls one
+// behind the other: 6.4 us each, 7.5 through the dispatcher).
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    const auto no_gil = py::call_guard<py::gil_scoped_release>();
+    m.def("finefmha_paged", &finefmha_paged, no_gil);
+    m.def("finefmha_paged_lse", &finefmha_paged_lse, no_gil);
+    m.def("rope_paged", &rope_paged, no_gil);
+    m.def("key_weights", &key_weights, no_gil);
+    m.def("evict_paged", &evict_paged, no_gil);
 }
 
 }  // namespace fmha_unified

@@ -9,6 +9,8 @@ from typing import Optional, Tuple
 import torch
 from torch import Tensor
 
+from . import _C
+
 __all__ = ["fine_fmha", "fine_fmha_with_lse", "fine_fmha_paged", "fine_fmha_paged_with_lse", "fine_rope_paged", "fine_key_weights",
            "fine_evict_paged"]
 
@@ -52,12 +54,8 @@ def fine_fmha_with_lse(q: Tensor, k: Tensor, v: Tensor, causal: bool, is_decode=
 # Everything is read on the device: no call waits for it, and a captured call serves the lengths and tables that its tensors hold
 # when the graph is replayed. The reference keeps one growing tensor a layer instead (benchmarks/flashattn-cuda/modeling_llama.py:664-668).
 
-_PAGED = torch.ops.fmha_unified.finefmha_paged.default
-_PAGED_LSE = torch.ops.fmha_unified.finefmha_paged_lse.default
-_ROPE_PAGED = torch.ops.fmha_unified.rope_paged.default
-_KEY_WEIGHTS = torch.ops.fmha_unified.key_weights.default
-_EVICT_PAGED = torch.ops.fmha_unified.evict_paged.default
-
+# The functions below call the extension module's own; `torch.ops.fmha_unified.{finefmha_paged, finefmha_paged_lse, rope_paged, key_weights,
+# evict_paged}` are the same through torch's dispatcher.
 
 def fine_fmha_paged(q: Tensor, kv_pages: Tensor, block_table: Tensor, seq_lens: Tensor, new_lens: Optional[Tensor] = None,
                     weights: Optional[Tensor] = None) -> Tensor:
@@ -65,13 +63,13 @@ def fine_fmha_paged(q: Tensor, kv_pages: Tensor, block_table: Tensor, seq_lens: 
     generation step, a few drafted ones, a chunk of a prompt. Row i of `new` tokens is key seq_lens[b] - new + i and sees the keys up to that
     one; a row that sees none, or is no token, gives zeros. With `weights`, each key's probabilities, summed over the query heads of its
     kv head and the rows, are added to it. The result is a new contiguous [B, Hq, S, 128] tensor."""
-    return _PAGED(q, kv_pages, block_table, seq_lens, new_lens, weights)
+    return _C.finefmha_paged(q, kv_pages, block_table, seq_lens, new_lens, weights)
 
 
 def fine_fmha_paged_with_lse(q: Tensor, kv_pages: Tensor, block_table: Tensor, seq_lens: Tensor, new_lens: Optional[Tensor] = None,
                              weights: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
     """As :func:`fine_fmha_paged`, also returning the fp32 log-sum-exp [B, Hq, S] of the scaled, masked scores."""
-    return _PAGED_LSE(q, kv_pages, block_table, seq_lens, new_lens, weights)
+    return _C.finefmha_paged_lse(q, kv_pages, block_table, seq_lens, new_lens, weights)
 
 
 def fine_rope_paged(qkv: Tensor, kv_pages: Tensor, block_table: Tensor, seq_lens: Tensor, cos: Tensor, sin: Tensor, positions: Tensor,
@@ -81,7 +79,7 @@ def fine_rope_paged(qkv: Tensor, kv_pages: Tensor, block_table: Tensor, seq_lens
     heads are rotated in place, token t becomes key seq_lens[b] - new + t. cos, sin: [n_positions, 64] fp32; positions: int32, [B, S] or [S]
     (shared by all sequences). Where they are given, the new keys' `weights` become zero and their `key_positions` the tokens'
     positions. keep_keys: the rotated keys are stored in qkv as well."""
-    _ROPE_PAGED(qkv, kv_pages, block_table, seq_lens, cos, sin, positions, q_heads, new_lens, weights, key_positions, keep_keys)
+    _C.rope_paged(qkv, kv_pages, block_table, seq_lens, cos, sin, positions, q_heads, new_lens, weights, key_positions, keep_keys)
 
 
 def fine_key_weights(q: Tensor, lse: Tensor, kv_pages: Tensor, block_table: Tensor, seq_lens: Tensor, weights: Tensor,
@@ -89,7 +87,7 @@ def fine_key_weights(q: Tensor, lse: Tensor, kv_pages: Tensor, block_table: Tens
     """What a prompt's rows attended to is added to `weights`: for every key the sum of exp(q k / sqrt(d) - lse) over the query heads of its
     kv head and the rows that see it. q [B, Hq, S, 128] and lse [B, Hq, S] are those of the attention over the same keys. last_rows > 0:
     only the last that many tokens of each sequence count."""
-    _KEY_WEIGHTS(q, lse, kv_pages, block_table, seq_lens, weights, new_lens, last_rows)
+    _C.key_weights(q, lse, kv_pages, block_table, seq_lens, weights, new_lens, last_rows)
 
 
 def fine_evict_paged(kv_pages: Tensor, block_table: Tensor, seq_lens: Tensor, weights: Tensor, key_positions: Tensor, budget: int,
@@ -98,4 +96,4 @@ def fine_evict_paged(kv_pages: Tensor, block_table: Tensor, seq_lens: Tensor, we
     largest, then those of the largest weights (NaN lowest), of equals the lowest slots. Kept keys that lie behind the budget move, in order,
     into the slots of dropped ones in front of it, with their values, weights and positions. Returns the new lengths, min(seq_lens,
     budget); seq_lens itself is left as it is, and so are the slots from `budget` on."""
-    return _EVICT_PAGED(kv_pages, block_table, seq_lens, weights, key_positions, budget, recent)
+    return _C.evict_paged(kv_pages, block_table, seq_lens, weights, key_positions, budget, recent)
