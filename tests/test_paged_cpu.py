@@ -111,3 +111,38 @@ def test_operators_name_what_they_write():
                           ("key_weights", ["weights"]), ("evict_paged", ["kv_pages", "weights", "key_positions"])):
         schema = getattr(torch.ops.fmha_unified, name).default._schema
         assert [a.name for a in schema.arguments if a.alias_info is not None and a.alias_info.is_write] == written
+
+
+def test_a_cache_hands_out_pages_and_takes_them_back():
+    from llama_layer import FinePagedKVCache
+    c = FinePagedKVCache(3, 10, 2, page_size=16, max_pages=4, device="cpu", account=True)
+
+    def consistent():
+        used = [p for row in c._pages for p in row]
+        assert len(set(used)) == len(used) and sorted(used + c._free) == list(range(10))
+        for b, row in enumerate(c._pages):
+            assert c.block_table[b].tolist() == row + [-1] * (4 - len(row)) and len(row) == -(-c.lengths[b] // 16)
+        assert c.seq_lens.tolist() == c.lengths and c.next_positions.tolist() == c.positions
+
+    c.extend([20, 0, 33])
+    consistent()
+    assert c.lengths == [20, 0, 33] and c.free_pages == 5
+    for new in ([0, 65, 0], [16, 64, 16], [1, 2], [-1, 0, 0]):      # a sequence, the pool, another batch, fewer than none
+        with pytest.raises(ValueError):
+            c.extend(new)
+        consistent()
+        assert c.lengths == [20, 0, 33]
+    c.extend([12, 1, 15])
+    consistent()
+    c.take_back([12, 1, 2])
+    consistent()
+    assert c.lengths == [20, 0, 46]
+    with pytest.raises(ValueError):
+        c.take_back([0, 1, 0])
+    c.release(2)
+    consistent()
+    assert c.lengths == [20, 0, 0] and c.positions == [20, 0, 0]
+    c.extend([1, 1, 1])
+    consistent()
+    with pytest.raises(ValueError, match="account"):
+        FinePagedKVCache(1, 4, 1, device="cpu").evict(3, 1)

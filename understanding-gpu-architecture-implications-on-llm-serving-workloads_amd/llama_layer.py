@@ -15,15 +15,18 @@ the gate/up epilogue does not apply, an MLP width that is no multiple of 32, and
     residual added in its epilogue.
 With up to 8 rows (a generation step) RoPE is part of the QKV product, and each norm of the product behind it where that pays (1 or 2 rows
 up to 7680 wide, 4 up to 4608, 8 up to 2560, fewer in front of a wide MLP: `norm_fits` in csrc/hgemm.hip): five to seven launches.
+With a cache in pages (FinePagedKVCache: sequences of different lengths) norm, QKV product and rotary embedding with filing are three launches; the
+attention is over the pages, or for a prompt over its projection, and what the keys were attended to is kept where eviction will ask for it.
 Weights keep the nn.Linear layout ([out_features, in_features]); nothing is transposed or repacked beyond
 concatenating q/k/v and interleaving gate/up along the output dimension once at construction.
 """
 import torch
 
 import mi355_serving as lib
+from fmha_unified.ops import fine_evict_paged
 from mi355_serving import _C
 
-__all__ = ["FineKVCache", "FineLlamaDecoderLayer", "rope_tables"]
+__all__ = ["FineKVCache", "FinePagedKVCache", "FineLlamaDecoderLayer", "rope_tables"]
 
 
 def rope_tables(n_positions, head_dim=128, base=10000.0, device="cuda"):
@@ -52,6 +55,102 @@ class FineKVCache:
 
     def rows(self, past, S):
         return self.kv[:, :, past:past + S].transpose(1, 2)
+
+
+class FinePagedKVCache:
+    """Key/value cache of one layer in pages, for sequences of different lengths that come and go: a pool `kv_pages` [n_pages, 2 * n_kv,
+    page_size, 128], of which each of `batch` sequences owns the pages in its row of `block_table` [batch, max_pages]. `seq_lens` and
+    `next_positions` (int32, on the device) hold each sequence's keys and the position of its next token; `lengths` and `positions` are the same
+    on the host, which hands out the pages. With `account`, `weights` and `key_positions` [n_pages, n_kv, page_size] keep what
+    `evict` goes by: the attention that each key has had, the position of its token.
+
+    The layer's forward makes room with `extend` and files its tokens; `evict` cuts long sequences, `release` frees one."""
+
+    def __init__(self, batch, n_pages, n_kv, page_size=32, max_pages=None, head_dim=128, device="cuda", dtype=torch.float16, account=False):
+        max_pages = n_pages if max_pages is None else max_pages
+        self.kv_pages = torch.zeros((n_pages, 2 * n_kv, page_size, head_dim), dtype=dtype, device=device)
+        self.block_table = torch.full((batch, max_pages), -1, dtype=torch.int32, device=device)
+        self.seq_lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.next_positions = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.weights = torch.zeros((n_pages, n_kv, page_size), device=device) if account else None
+        self.key_positions = torch.zeros((n_pages, n_kv, page_size), dtype=torch.int32, device=device) if account else None
+        self.lengths, self.positions = [0] * batch, [0] * batch
+        self._pages = [[] for _ in range(batch)]
+        self._free = list(range(n_pages - 1, -1, -1))
+
+    @property
+    def free_pages(self):
+        return len(self._free)
+
+    def extend(self, new):
+        """Room for new[b] more tokens of each sequence, whose lengths and positions go on by that many. ValueError, and nothing changed, where the
+        pool or the table has no more."""
+        page, width = self.kv_pages.shape[2], self.block_table.shape[1]
+        if len(new) != len(self.lengths) or any(n < 0 for n in new):
+            raise ValueError("new tokens of %d sequences expected, got %r" % (len(self.lengths), new))
+        lengths = [n + more for n, more in zip(self.lengths, new)]
+        wanted = [max(0, -(-n // page) - len(have)) for n, have in zip(lengths, self._pages)]
+        if sum(wanted) > len(self._free) or any(n > width * page for n in lengths):
+            raise ValueError("a cache of %d free pages of %d tokens, %d a sequence, cannot take %r more after %r" %
+                             (len(self._free), page, width, list(new), self.lengths))
+        for b, more in enumerate(wanted):
+            for _ in range(more):
+                self._pages[b].append(self._free.pop())
+        if any(wanted):
+            self._write_table([b for b, more in enumerate(wanted) if more])
+        self.lengths = lengths
+        self.positions = [n + more for n, more in zip(self.positions, new)]
+        step = new[0] if all(n == new[0] for n in new) else torch.tensor(new, dtype=torch.int32, device=self.seq_lens.device)
+        self.seq_lens += step
+        self.next_positions += step
+
+    def take_back(self, new):
+        """The last new[b] tokens of each sequence are no longer its own (a call that failed; drafted tokens that were not accepted). The account of
+        the others keeps what those added to it."""
+        if len(new) != len(self.lengths) or any(not 0 <= n <= have for n, have in zip(new, self.lengths)):
+            raise ValueError("cannot take %r tokens back from sequences of %r" % (new, self.lengths))
+        self.lengths = [n - less for n, less in zip(self.lengths, new)]
+        self.positions = [n - less for n, less in zip(self.positions, new)]
+        step = new[0] if all(n == new[0] for n in new) else torch.tensor(new, dtype=torch.int32, device=self.seq_lens.device)
+        self.seq_lens -= step
+        self.next_positions -= step
+        self._give_back(range(len(new)))
+
+    def evict(self, budget, recent):
+        """Cuts every sequence longer than `budget` to it (fmha_unified.ops.fine_evict_paged) and frees the pages behind it."""
+        if self.weights is None:
+            raise ValueError("eviction needs a cache made with account=True")
+        if all(n <= budget for n in self.lengths):
+            return
+        self.seq_lens.copy_(fine_evict_paged(self.kv_pages, self.block_table, self.seq_lens, self.weights, self.key_positions, budget, recent))
+        self.lengths = [min(n, budget) for n in self.lengths]
+        self._give_back(range(len(self.lengths)))
+
+    def release(self, b):
+        """Sequence b is done: its pages are free, its place may be taken by another."""
+        self.lengths[b] = self.positions[b] = 0
+        self.seq_lens[b] = 0
+        self.next_positions[b] = 0
+        self._give_back([b])
+
+    def _give_back(self, rows):
+        page, changed = self.kv_pages.shape[2], []
+        for b in rows:
+            keep = -(-self.lengths[b] // page)
+            if keep < len(self._pages[b]):
+                self._free.extend(reversed(self._pages[b][keep:]))
+                del self._pages[b][keep:]
+                changed.append(b)
+        if changed:
+            self._write_table(changed)
+
+    def _write_table(self, rows):
+        width = self.block_table.shape[1]
+        host = torch.tensor([self._pages[b] + [-1] * (width - len(self._pages[b])) for b in rows], dtype=torch.int32)
+        if len(rows) == self.block_table.shape[0]:
+            self.block_table.copy_(host)
+        else:
+            self.block_table[torch.tensor(rows, device=self.block_table.device)] = host.to(self.block_table.device)
 
 
 class FineLlamaDecoderLayer:
@@ -95,8 +194,14 @@ class FineLlamaDecoderLayer:
         base = getattr(config, "rope_theta", None) or (getattr(config, "rope_parameters", None) or {}).get("rope_theta", 10000.0)
         return cls(w, config.num_attention_heads, config.num_key_value_heads, config.rms_norm_eps, base, max_positions, dtype)
 
-    def forward(self, hidden_states, position_ids=None, kv_cache=None, time_attention=False):
+    def forward(self, hidden_states, position_ids=None, kv_cache=None, time_attention=False, new_lens=None):
+        """With a FinePagedKVCache `new_lens` (a list) may say how many of each sequence's S rows are tokens, the first ones (none: all); the rows behind
+        them must be finite and their results mean nothing. Its positions go on where each sequence's text is unless position_ids are given."""
         B, S, H = hidden_states.shape
+        if type(kv_cache) is FinePagedKVCache:
+            return self._forward_paged(hidden_states, position_ids, kv_cache, time_attention, new_lens)
+        if new_lens is not None:
+            raise ValueError("new_lens goes with a FinePagedKVCache")
         past, kv, first = 0, (), 0
         if kv_cache is not None:
             past = kv_cache.length
@@ -111,11 +216,37 @@ class FineLlamaDecoderLayer:
             pos = position_ids.to(torch.int32).reshape(-1, S).contiguous()   # [1, S] (shared) or [B, S]
             assert pos.shape[0] in (1, B)
         out, ms = _C.layer_forward(hidden_states, self.w_qkv, self.w_o, self.w_gu, self.w_d, self.ln1, self.ln2, self.cos, self.sin, pos,
-                                   first, kv, past, self.n_q, self.n_kv, self.eps, self.gu_block, time_attention)
+                                   first, kv, past, self.n_q, self.n_kv, self.eps, self.gu_block, time_attention, (), False)
         if kv_cache is not None:
             kv_cache.length = past + S
         if time_attention:
             self.attn_ms["decode" if (S == 1 and past > 0) else "prefill"].append(ms)
+        return out
+
+    def _forward_paged(self, hidden_states, position_ids, cache, time_attention, new_lens):
+        B, S, _ = hidden_states.shape
+        new = [S] * B if new_lens is None else [int(n) for n in new_lens]
+        if len(new) != B or len(cache.lengths) != B or not all(0 <= n <= S for n in new):
+            raise ValueError("%d sequences of up to %d new tokens, a cache of %d sequences and new_lens %r do not fit" % (B, S, len(cache.lengths), new_lens))
+        if position_ids is None:
+            if max(p + n for p, n in zip(cache.positions, new)) > self.cos.shape[0]:
+                raise ValueError("max_positions is %d" % self.cos.shape[0])
+            pos = cache.next_positions[:, None] + self.all_positions[:S]
+        else:
+            pos = position_ids.to(torch.int32).reshape(-1, S).contiguous()
+            assert pos.shape[0] in (1, B)
+        prompt = not any(cache.lengths)
+        cache.extend(new)
+        counts = None if all(n == S for n in new) else torch.tensor(new, dtype=torch.int32, device=hidden_states.device)
+        paged = (cache.kv_pages, cache.block_table, cache.seq_lens, counts, cache.weights, cache.key_positions)
+        try:
+            out, ms = _C.layer_forward(hidden_states, self.w_qkv, self.w_o, self.w_gu, self.w_d, self.ln1, self.ln2, self.cos, self.sin, pos,
+                                       0, (), 0, self.n_q, self.n_kv, self.eps, self.gu_block, time_attention, paged, prompt)
+        except Exception:
+            cache.take_back(new)
+            raise
+        if time_attention:
+            self.attn_ms["prefill" if prompt or S > 1 else "decode"].append(ms)
         return out
 
     __call__ = forward

@@ -15,6 +15,7 @@
 #include <vector>
 
 #include "mi355_serving.h"
+#include "../../csrc/paged_tensors.h"
 
 // of the same library (csrc/mi355_serving_internal.h)
 extern "C" size_t mi355_internal_gemm_copy_bytes(const void* A, const void* B, int M, int N, int K, int64_t lda, int64_t ldb, int layout);
@@ -65,12 +66,14 @@ void linear(const void* a, const at::Tensor& w, const void* r, void* c, int64_t 
 // int32, [S] for all batch rows or [B, S]. `kv`: empty without a cache; {cache} for a tensor [B, 2 n_kv, max_len, 128], whose rows
 // past .. past + S - 1 are written; or {rows, k, v} for a cache of any layout: the [B, S, 2 n_kv, 128] view of the new tokens,
 // which are written, and the [B, past + S or more, n_kv, 128] views of all keys and values. `gate_up_block`: 32 when w_gu alternates 32 gate rows with their 32 up rows, 0 when all
-// gate rows precede all up rows.
+// gate rows precede all up rows. `paged`: empty, or (with an empty `kv`) the tensors of a cache in pages: kv_pages, block_table, seq_lens (the new
+// tokens counted), new_lens, weights, key_positions, the last three or none; `prompt`: no sequence had a key before, so that the new tokens' attention is over
+// their own projection.
 std::tuple<at::Tensor, double> layer_forward(const at::Tensor& hidden_states, const at::Tensor& w_qkv, const at::Tensor& w_o,
                                              const at::Tensor& w_gu, const at::Tensor& w_d, const at::Tensor& ln1, const at::Tensor& ln2,
                                              const at::Tensor& cos, const at::Tensor& sin, const at::Tensor& positions, int64_t first_position,
                                              const std::vector<at::Tensor>& kv, int64_t past, int64_t n_q, int64_t n_kv, double eps,
-                                             int64_t gate_up_block, bool timed) {
+                                             int64_t gate_up_block, bool timed, const std::vector<std::optional<at::Tensor>>& paged, bool prompt) {
     constexpr int64_t D = 128;
     TORCH_CHECK(hidden_states.dim() == 3 && hidden_states.is_cuda(), "hidden_states must be a [B, S, H] GPU tensor");
     const int64_t B = hidden_states.size(0), S = hidden_states.size(1), H = hidden_states.size(2), rows = B * S;
@@ -166,15 +169,55 @@ std::tuple<at::Tensor, double> layer_forward(const at::Tensor& hidden_states, co
         if (rc != MI355_ERR_UNSUPPORTED) check(rc, "mi355_internal_step_qkv");
         return rc == 0;
     };
+    mi355_paged_kv pages = {};
+    if (!paged.empty()) {
+        TORCH_CHECK(kv.empty() && paged.size() == 6 && paged[0] && paged[1] && paged[2], "a cache in pages: kv_pages, block_table, seq_lens, new_lens, weights, key_positions");
+        pages = mi355::paged_kv("layer_forward", *paged[0], *paged[1], *paged[2], paged[3], paged[4], paged[5]);
+        TORCH_CHECK(pages.B == B && pages.Hkv == n_kv && paged[0]->scalar_type() == type && paged[0]->device() == x.device(),
+                    "the cache in pages must have the layer's sequences, kv heads, type and device");
+    }
     Events ev;
-    if (timed || rows > 8 || !step_qkv(x.data_ptr(), ln1.data_ptr())) {
+    const auto begin_timing = [&] {
+        if (!timed) return;
+        CHECK_HIP(hipEventCreate(&ev.begin));
+        CHECK_HIP(hipEventCreate(&ev.end));
+        CHECK_HIP(hipDeviceSynchronize());
+        CHECK_HIP(hipEventRecord(ev.begin, stream));
+    };
+    // Attention over a cache in pages: the new tokens are filed; a prompt's are then attended to where they are, in the projection (up to 32 rows
+    // a kv head by the pages' kernel, like those of any other call).
+    const auto paged_attention = [&] {
+        const bool here = prompt && n_q / n_kv * S > 32;
         norm(x.data_ptr(), ln1);
-        if (timed) {
-            CHECK_HIP(hipEventCreate(&ev.begin));
-            CHECK_HIP(hipEventCreate(&ev.end));
-            CHECK_HIP(hipDeviceSynchronize());
-            CHECK_HIP(hipEventRecord(ev.begin, stream));
+        begin_timing();
+        linear(h, w_qkv, nullptr, qkv, rows, dtype, stream);
+        check(mi355_rope_paged(&pages, qkv, (int)S, (int)n_q, here ? 1 : 0, S * row, row, cos_p, sin_p, pos, pos_batch, n_pos, stream), "mi355_rope_paged");
+        const float scale = 1.0f / std::sqrt((float)D);
+        const auto block_of = [&](size_t bytes) { return at::empty({(int64_t)bytes}, x.options().dtype(at::kByte)); };
+        if (!here) {
+            const int64_t strides[6] = {S * row, D, row, S * n_q * D, D, n_q * D};
+            const size_t need = mi355_fmha_paged_workspace_bytes(&pages, (int)n_q, (int)S, 0);
+            const at::Tensor ws = block_of(need);
+            check(mi355_fmha_paged(&pages, qkv, attn, nullptr, (int)n_q, (int)S, strides, scale, need > 0 ? ws.data_ptr() : nullptr, need, stream), "mi355_fmha_paged");
+            return;
         }
+        const int64_t strides[12] = {S * row, D, row, S * row, D, row, S * row, D, row, S * n_q * D, D, n_q * D};
+        const at::Tensor lse = pages.weights != nullptr ? at::empty({B, n_q, S}, x.options().dtype(at::kFloat)) : at::Tensor();
+        const auto entry = bf16 ? &mi355_fmha_fwd_bf16 : &mi355_fmha_fwd_strided;
+        check(entry(qkv, k.ptr, v.ptr, attn, lse.defined() ? lse.data_ptr<float>() : nullptr, (int)B, (int)n_q, (int)n_kv, (int)S, (int)S, (int)D, scale, 1,
+                    (int)S, strides, stream), "mi355_fmha_fwd");
+        if (lse.defined()) {
+            const size_t need = mi355_fmha_key_weights_workspace_bytes(&pages, (int)n_q, (int)S, 0);
+            const at::Tensor ws = block_of(need);
+            check(mi355_fmha_key_weights(&pages, qkv, lse.data_ptr<float>(), (int)n_q, (int)S, strides, 0, scale, need > 0 ? ws.data_ptr() : nullptr, need, stream),
+                  "mi355_fmha_key_weights");
+        }
+    };
+    if (!paged.empty()) {
+        paged_attention();
+    } else if (timed || rows > 8 || !step_qkv(x.data_ptr(), ln1.data_ptr())) {
+        norm(x.data_ptr(), ln1);
+        begin_timing();
         if (!step_qkv(h, nullptr)) {
             linear(h, w_qkv, nullptr, qkv, rows, dtype, stream);
             if (kv.empty()) {
@@ -188,7 +231,7 @@ std::tuple<at::Tensor, double> layer_forward(const at::Tensor& hidden_states, co
             }
         }
     }
-    {
+    if (paged.empty()) {
         const int64_t strides[12] = {S * row, D, row, k.batch, k.head, k.row, v.batch, v.head, v.row, S * n_q * D, D, n_q * D};
         const auto entry = bf16 ? &mi355_fmha_fwd_bf16 : &mi355_fmha_fwd_strided;
         check(entry(qkv, k.ptr, v.ptr, attn, nullptr, (int)B, (int)n_q, (int)n_kv, (int)S, (int)keys, (int)D, 1.0f / std::sqrt((float)D), 1, (int)keys,
