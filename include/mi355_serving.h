@@ -311,7 +311,9 @@ int mi355_fmha_fwd_noalloc(const void* Q, const void* K, const void* V, void* O,
  * had from the queries of its kv head, and the position of its token in the text. Both may be NULL where a call does not need them.
  *
  * Lengths, table and positions are read on the device: no call waits for it, and a captured call serves what the tensors hold when it
- * is replayed. No page may belong to two sequences of a call that write it. B * Hkv <= 65535.
+ * is replayed (they must not change while a call runs). No page may belong to two sequences of a call that writes it, to its weights among others.
+ * Launches and workspaces are sized for max_pages, whatever the lengths are: a caller whose table is much wider than its sequences are long passes
+ * the columns in use. B * Hkv <= 65535, max_pages * page_size <= 2^28.
  *
  * The library allocates nothing for these calls: what *_workspace_bytes says (0: NULL will do) is the caller's, 16-byte aligned, its
  * contents irrelevant before and after; calls that share a workspace must be ordered on one stream. The reference has no counterpart: its caller grows

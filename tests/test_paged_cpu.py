@@ -20,7 +20,7 @@ def cache(lib, **other):
 BAD_CACHES = [dict(pages=None), dict(block_table=None), dict(seq_lens=None), dict(pages=P + 8), dict(weights=P + 4), dict(key_positions=P + 8), dict(B=0), dict(Hkv=0), dict(n_pages=0), dict(max_pages=0),
               dict(page_size=0), dict(page_size=8), dict(page_size=24), dict(dtype=2), dict(table_stride=7), dict(page_stride=0), dict(head_stride=64),
               dict(row_stride=129), dict(row_stride=-128), dict(row_stride=1 << 24), dict(page_size=1 << 20, row_stride=1 << 20), dict(B=9000),
-              dict(max_pages=1 << 28, table_stride=1 << 28), dict(max_pages=1 << 22, table_stride=1 << 22, B=1000, Hkv=10)]
+              dict(max_pages=(1 << 24) + 1, table_stride=1 << 25), dict(max_pages=1 << 22, table_stride=1 << 22, B=1000, Hkv=10)]
 
 
 @pytest.mark.parametrize("bad", BAD_CACHES, ids=lambda d: "-".join("%s=%s" % x for x in d.items()))
@@ -48,6 +48,11 @@ def test_attention_refuses_bad_arguments(lib):
                dict(scale=float("inf")), dict(S=16384), dict(strides=[-8] + ok[1:]), dict(strides=[4] + ok[1:]), dict(strides=ok[:2] + [1 << 24] + ok[3:]),
                dict(strides=ok[:4] + [64, 128]), dict(strides=ok[:3] + [0, 128, 128])):
         assert call(**kw) in (lib.ERR_BAD_ARGUMENT, lib.ERR_UNSUPPORTED), kw
+    # launches of more workgroups than there may be
+    many = cache(lib, B=8000, table_stride=8)
+    assert cdll.mi355_fmha_paged(many, P, P, P, 32, 100, None, 0.1, P, big, None) == lib.ERR_UNSUPPORTED
+    far = cache(lib, max_pages=1 << 20, table_stride=1 << 20)
+    assert cdll.mi355_fmha_key_weights(far, P, P, 32, 16383, None, 0, 0.1, P, big, None) == lib.ERR_UNSUPPORTED
     # a workspace is needed for the scores that the account is made from
     need = cdll.mi355_fmha_paged_workspace_bytes(c, 32, 1, 1)
     assert need > 0
@@ -66,7 +71,7 @@ def test_the_other_entry_points_refuse_bad_arguments(lib):
         return cdll.mi355_rope_paged(c, qkv, S, q_heads, 0, x_batch, x_row, cos, sin, pos, pos_batch, n, None)
 
     for kw in (dict(qkv=None), dict(cos=None), dict(sin=None), dict(pos=None), dict(qkv=P + 2), dict(cos=P + 4), dict(S=0), dict(q_heads=-1), dict(n=0),
-               dict(x_row=row - 8), dict(x_row=row + 4), dict(x_batch=row - 8), dict(x_batch=-8), dict(pos_batch=1), dict(S=1 << 30)):
+               dict(x_row=row - 8), dict(x_row=row + 4), dict(x_batch=row - 8), dict(x_batch=-8), dict(pos_batch=1), dict(S=1 << 30), dict(S=1 << 22)):
         assert rope(**kw) in (lib.ERR_BAD_ARGUMENT, lib.ERR_UNSUPPORTED), kw
 
     def kw_call(Q=P, LSE=P, Hq=32, S=4, strides=None, last=0, scale=0.1, cc=c):

@@ -660,6 +660,63 @@ def test_calls_on_two_streams_at_once(gpu):
             assert torch.equal(x.nan_to_num(7.0), y.nan_to_num(7.0))
 
 
+def test_strides_that_mean_nothing_and_strides_that_are_too_large(gpu):
+    c = Cache([40], 2, 16, spare=0)
+    assert c.kv.shape[0] == 3
+    q = queries(c, 8, 1)
+    want = ops.fine_fmha_paged(q, *c.args)
+    # one sequence, one row: their strides may be anything
+    odd = torch.empty(8 * D + 5, dtype=torch.float16, device="cuda")[:8 * D].as_strided((1, 8, 1, D), (7, D, 3, 1))
+    odd.copy_(q)
+    table = c.table.as_strided(c.table.shape, (1, 1))
+    assert torch.equal(ops.fine_fmha_paged(odd, c.kv, table, c.lens), want)
+    # rows 2^24 elements apart, an unaligned start, a reversed order of dimensions
+    S = 3
+    q = queries(c, 8, S)
+    want, lse = ops.fine_fmha_paged_with_lse(q, *c.args)
+    w = [c.weights.clone() for _ in range(4)]
+    ops.fine_key_weights(q, lse, *c.args, w[0])
+    far = torch.empty((S - 1) * (1 << 24) + 8 * D, dtype=torch.float16, device="cuda").as_strided((1, 8, S, D), (8, D, 1 << 24, 1))
+    shifted = torch.empty(8 * S * D + 1, dtype=torch.float16, device="cuda")[1:].view(1, 8, S, D)
+    across = torch.empty(D, S, 8, 1, dtype=torch.float16, device="cuda").permute(3, 2, 1, 0)
+    for i, other in enumerate((far, shifted, across)):
+        other.copy_(q)
+        assert torch.equal(ops.fine_fmha_paged(other, *c.args), want)
+        ops.fine_key_weights(other, lse, *c.args, w[i + 1])
+        assert torch.equal(w[i + 1].nan_to_num(7.0), w[0].nan_to_num(7.0))
+    # a pool of one page
+    one = Cache([10], 2, 16, spare=0)
+    pool = one.kv.as_strided(one.kv.shape, (3,) + one.kv.stride()[1:])
+    q = queries(one, 8, 1)
+    assert torch.equal(ops.fine_fmha_paged(q, pool, one.table, one.lens), ops.fine_fmha_paged(q, *one.args))
+
+
+def test_operators_through_the_dispatcher_are_the_same(gpu):
+    cache = Cache([700, 31], 2, 16)
+    q = queries(cache, 8, 2)
+    direct, lse = ops.fine_fmha_paged_with_lse(q, *cache.args)
+    through = torch.ops.fmha_unified
+    assert torch.equal(through.finefmha_paged(q, *cache.args, None, None), direct)
+    o, l = through.finefmha_paged_lse(q, *cache.args, None, None)
+    assert torch.equal(o, direct) and torch.equal(l, lse)
+    w = [cache.weights.clone(), cache.weights.clone()]
+    ops.fine_key_weights(q, lse, *cache.args, w[0])
+    through.key_weights(q, lse, *cache.args, w[1], None, 0)
+    assert torch.equal(w[0].nan_to_num(7.0), w[1].nan_to_num(7.0))
+    positions_of(cache, 1)
+    a = [t.clone() for t in (cache.kv, cache.weights, cache.positions)]
+    b = [t.clone() for t in a]
+    assert torch.equal(ops.fine_evict_paged(a[0], cache.table, cache.lens, a[1], a[2], 20, 5),
+                       through.evict_paged(b[0], cache.table, cache.lens, b[1], b[2], 20, 5))
+    assert all(torch.equal(x.nan_to_num(7.0), y.nan_to_num(7.0)) for x, y in zip(a, b))
+    qkv = torch.randn(2, 3, 12, D, device="cuda").half()
+    t, pos = torch.rand(50, 64, device="cuda"), torch.arange(3, dtype=torch.int32, device="cuda")
+    x, y = qkv.clone(), qkv.clone()
+    ops.fine_rope_paged(x, a[0], cache.table, cache.lens, t, t, pos, 8)
+    through.rope_paged(y, b[0], cache.table, cache.lens, t, t, pos, 8, None, None, None, False)
+    assert torch.equal(x, y) and torch.equal(a[0].nan_to_num(7.0), b[0].nan_to_num(7.0))
+
+
 def test_operators_refuse_wrong_tensors_on_the_gpu(gpu):
     c = Cache([40, 20], 2, 16)
     q = queries(c, 8, 1)

@@ -445,7 +445,7 @@ static int paged_checked(const char* fn, const mi355_paged_kv* c) {
         return fail(MI355_ERR_UNSUPPORTED, "%s: page_size must be a positive multiple of 16 (got %d)", fn, c->page_size);
     const int64_t pairs = (int64_t)c->B * c->Hkv, max_len = (int64_t)c->max_pages * c->page_size;
     if (pairs > 65535) return fail(MI355_ERR_UNSUPPORTED, "%s: B * Hkv must be at most 65535 (got %lld)", fn, (long long)pairs);
-    if (max_len > INT32_MAX - 8192 || pairs * (max_len / 32 + 1) > INT32_MAX)
+    if (max_len > (1 << 28) || pairs * (max_len / 32 + 1) > INT32_MAX)
         return fail(MI355_ERR_UNSUPPORTED, "%s: %d sequences of up to %lld keys of %d heads are more than a call takes", fn, c->B, (long long)max_len, c->Hkv);
     if (c->B > 1 && c->table_stride < c->max_pages)
         return fail(MI355_ERR_BAD_ARGUMENT, "%s: rows of the block table overlap (stride %lld, %d entries)", fn, (long long)c->table_stride, c->max_pages);
@@ -476,6 +476,8 @@ static int paged_queries_checked(const char* fn, const mi355_paged_kv* c, const 
     return 0;
 }
 
+constexpr int64_t kMostWorkgroups = (1 << 24) - 1;   // of 256 threads in one launch
+
 static int workspace_checked(const char* fn, size_t need, const void* workspace, size_t bytes) {
     if (need > 0 && (workspace == nullptr || bytes < need || !aligned16(workspace)))
         return fail(MI355_ERR_BAD_ARGUMENT, "%s: workspace of %zu bytes at %p; this call needs %zu bytes, 16-byte aligned (%s_workspace_bytes)", fn, bytes,
@@ -497,6 +499,9 @@ int mi355_fmha_paged(const mi355_paged_kv* cache, const void* Q, void* O, float*
     const int64_t* st = strides ? strides : dense;
     if (int rc = paged_queries_checked(fn, cache, Q, Hq, S, st, 6, scale)) return rc;
     if (!aligned16(O)) return fail(MI355_ERR_BAD_ARGUMENT, "%s: O must be 16-byte aligned", fn);
+    if ((int64_t)cache->B * cache->Hkv * ((int64_t)(Hq / cache->Hkv) * S + (int64_t)cache->max_pages * cache->page_size / 256 + 1) > kMostWorkgroups)
+        return fail(MI355_ERR_UNSUPPORTED, "%s: %d sequences of %d rows over up to %lld keys are more than a call takes", fn, cache->B, S,
+                    (long long)cache->max_pages * cache->page_size);
     if ((S > 1 && st[5] < 128) || (Hq > 1 && st[4] < 128) || (cache->B > 1 && st[3] < 128))
         return fail(MI355_ERR_BAD_ARGUMENT, "%s: rows of O overlap (o strides %lld, %lld, %lld)", fn, (long long)st[3], (long long)st[4], (long long)st[5]);
     if (int rc = workspace_checked(fn, mi355::fmha_paged_workspace(*cache, Hq, S, LSE != nullptr), workspace, workspace_bytes)) return rc;
@@ -512,7 +517,7 @@ int mi355_rope_paged(const mi355_paged_kv* cache, void* qkv, int S, int q_heads,
     if (!qkv || !cos_table || !sin_table || !positions) return fail(MI355_ERR_BAD_ARGUMENT, "%s: null pointer", fn);
     if (S < 1 || q_heads < 0 || n_positions < 1) return fail(MI355_ERR_BAD_ARGUMENT, "%s: S, n_positions >= 1 and q_heads >= 0 required", fn);
     const int64_t heads = (int64_t)q_heads + 2 * (int64_t)cache->Hkv;
-    if ((int64_t)cache->B * S > INT32_MAX || heads > 65535 * 32) return fail(MI355_ERR_UNSUPPORTED, "%s: too many tokens or heads", fn);
+    if ((int64_t)cache->B * S > kMostWorkgroups || heads > 65535 * 32) return fail(MI355_ERR_UNSUPPORTED, "%s: too many tokens or heads", fn);
     if (x_row < heads * 128 || x_row % 8 || x_batch < 0 || x_batch % 8 || (cache->B > 1 && x_batch < heads * 128))
         return fail(MI355_ERR_BAD_ARGUMENT, "%s: rows of qkv overlap or strides are no multiples of 8 (batch %lld, row %lld, %lld heads)", fn,
                     (long long)x_batch, (long long)x_row, (long long)heads);
@@ -538,6 +543,9 @@ int mi355_fmha_key_weights(const mi355_paged_kv* cache, const void* Q, const flo
     const int64_t dense[3] = {(int64_t)Hq * S * 128, (int64_t)S * 128, 128};
     const int64_t* st = q_strides ? q_strides : dense;
     if (int rc = paged_queries_checked(fn, cache, Q, Hq, S, st, 3, scale)) return rc;
+    if (mi355::key_weights_workgroups(*cache, Hq, S, last_rows) > kMostWorkgroups / 2)
+        return fail(MI355_ERR_UNSUPPORTED, "%s: %d sequences of %d rows over up to %lld keys are more than a call takes", fn, cache->B, S,
+                    (long long)cache->max_pages * cache->page_size);
     if (int rc = workspace_checked(fn, mi355::key_weights_workspace(*cache, Hq, S, last_rows), workspace, workspace_bytes)) return rc;
     const long l[3] = {(long)st[0], (long)st[1], (long)st[2]};
     const hipError_t e = mi355::key_weights_dispatch(*cache, Q, LSE, Hq, S, l, last_rows, scale, workspace, static_cast<hipStream_t>(stream));

@@ -226,6 +226,12 @@ static KeyWeightsPlan key_weights_plan(const mi355_paged_kv& c, int Hq, int Sq, 
     return p;
 }
 
+// Workgroups of a launch: all blocks of keys of each (pair, range), which are dealt to the XCDs eight at a time
+long key_weights_workgroups(const mi355_paged_kv& c, int Hq, int Sq, int last_rows) {
+    const KeyWeightsPlan p = key_weights_plan(c, Hq, Sq, last_rows);
+    return ((long)c.B * c.Hkv * p.ranges + 7) / 8 * 8 * p.max_blocks;
+}
+
 size_t key_weights_workspace(const mi355_paged_kv& c, int Hq, int Sq, int last_rows) {
     const KeyWeightsPlan p = key_weights_plan(c, Hq, Sq, last_rows);
     return p.ranges == 1 ? 0 : sizeof(float) * (size_t)p.ranges * c.B * c.Hkv * p.max_blocks * kw::BLOCK;
@@ -254,9 +260,7 @@ hipError_t key_weights_dispatch(const mi355_paged_kv& c, const void* Q, const fl
     a.by_pairs = divisor_of(a.pairs);
     a.by_blocks = divisor_of(a.max_blocks);
     a.by_group = divisor_of(a.group);
-    const long groups = ((long)a.pairs * a.ranges + 7) / 8 * 8;
-    if (groups * a.max_blocks > INT32_MAX) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)(groups * a.max_blocks));
+    const dim3 grid((unsigned)key_weights_workgroups(c, Hq, Sq, last_rows));
     // Eight waves of 32 keys where there is no more than a workgroup per CU (us, eight / four waves: 64 rows of 32/8 heads over 8191 keys 11.3 /
     // 12.2), four of 64, which read the rows' tiles half as often, where several share one (2 x 32/8 heads, 4096 rows 164.6 / 159.9).
     const bool one_each = (long)a.max_blocks * a.pairs * a.ranges <= 256;

@@ -254,7 +254,7 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
     int slot = 0;   // stage of the next tile
     for (;;) {      // the parts
         const int n = now.n, n_loc = count_of(now), hkv = now.hkv, b = now.seq.b, len = now.seq.len;
-        const bool more = f + n < f_end;
+        const bool more = n > 0 && f + n < f_end;   // (a part of nothing ends the walk even where lengths change under the call)
         const int k_base = c16 * ROW_BYTES + ((g ^ c16) << 4);   // xor (ks << 6), + kb * 16 rows
         const int v_row = 4 * g + (c16 >> 2);
         const int v_base = TILE_BYTES + v_row * ROW_BYTES + ((((c16 & 3) >> 1) ^ swz_v(v_row)) << 4) + (c16 & 1) * 8;  // xor (db << 5)

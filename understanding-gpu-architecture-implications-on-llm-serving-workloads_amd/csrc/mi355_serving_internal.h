@@ -186,6 +186,7 @@ hipError_t silu_mul_dispatch(const void* in, void* out, long rows, int inter, in
 size_t fmha_paged_workspace(const mi355_paged_kv& cache, int Hq, int Sq, bool lse);
 hipError_t fmha_paged_dispatch(const mi355_paged_kv& cache, const void* Q, void* O, float* LSE, int Hq, int Sq, const long* strides, float scale,
                                void* workspace, hipStream_t stream);
+long key_weights_workgroups(const mi355_paged_kv& cache, int Hq, int Sq, int last_rows);
 size_t key_weights_workspace(const mi355_paged_kv& cache, int Hq, int Sq, int last_rows);
 hipError_t key_weights_dispatch(const mi355_paged_kv& cache, const void* Q, const float* LSE, int Hq, int Sq, const long* q_strides, int last_rows,
                                 float scale, void* workspace, hipStream_t stream);

@@ -182,7 +182,7 @@ __global__ __launch_bounds__(evict::THREADS) void evict_select_kernel(PagedKv kv
     }
     const int* table = kv.table + (long)b * kv.table_stride;
     const int chunks = (len + 4 * THREADS - 1) / (4 * THREADS);   // <= M, where that is given
-    const int j0 = tid * 4 * chunks;   // (up to 4096 behind the last key: max_len leaves that much below 2^31)
+    const int j0 = tid * 4 * chunks;   // (up to 4096 behind the last key)
     constexpr int REGS = M > 0 ? M : 1;
     uint4 rank[REGS], position[REGS];
     uint4* kept_ranks = a.ranks + (long)blockIdx.x * 2 * ((kv.max_len + 3) / 4 + THREADS);

@@ -3,7 +3,6 @@
 #pragma once
 #include <torch/extension.h>
 
-#include <algorithm>
 #include <optional>
 
 #include "mi355_serving.h"
@@ -50,7 +49,7 @@ inline mi355_paged_kv paged_kv(const char* name, const at::Tensor& kv_pages, con
     // (a dimension of one element may have any stride)
     c.row_stride = kv_pages.size(2) > 1 ? kv_pages.stride(2) : 128;
     c.head_stride = kv_pages.stride(1);
-    c.page_stride = kv_pages.size(0) > 1 ? kv_pages.stride(0) : std::max<int64_t>(kv_pages.stride(0), 128);
+    c.page_stride = kv_pages.size(0) > 1 ? kv_pages.stride(0) : 128;
     c.table_stride = block_table.stride(0);
     c.n_pages = (int32_t)kv_pages.size(0);
     c.page_size = (int32_t)kv_pages.size(2);

@@ -20,6 +20,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
 #include <algorithm>
+#include <array>
 #include <cmath>
 #include <optional>
 #include <tuple>
@@ -110,12 +111,20 @@ std::tuple<at::Tensor, at::Tensor> finefmha_fwd_lse(const at::Tensor& q, const a
 
 // ---- a key-value cache in pages (include/mi355_serving.h: mi355_paged_kv) -----------------------------------------------
 
+// batch, head and row stride of [B, H, S, 128] queries; of a dimension of one element it may be anything and is not used
+std::array<int64_t, 3> query_strides(const at::Tensor& q) {
+    return {q.size(0) > 1 ? q.stride(0) : 0, q.size(1) > 1 ? q.stride(1) : 0, q.size(2) > 1 ? q.stride(2) : 128};
+}
+
 // queries [B, Hq, S, 128] of the pages' type and device
 at::Tensor paged_queries(const char* name, const at::Tensor& q, const at::Tensor& kv_pages, const mi355_paged_kv& c) {
     TORCH_CHECK(q.dim() == 4 && q.size(0) == c.B && q.size(3) == 128 && q.numel() > 0, name, ": q must be [", c.B, ", Hq, S, 128], got ", q.sizes());
     check_like(name, "q", q, kv_pages, kv_pages.scalar_type());
     TORCH_CHECK(q.size(1) <= INT32_MAX && q.size(2) <= INT32_MAX, name, ": dimension exceeds int32");
-    return readable_in_place(q) ? q : q.contiguous();
+    const auto st = query_strides(q);
+    const bool in_place = q.stride(3) == 1 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0 && st[0] >= 0 && st[1] >= 0 && st[2] >= 0 &&
+                          (st[0] | st[1] | st[2]) % 8 == 0 && st[2] < (1 << 24);
+    return in_place ? q : q.clone(at::MemoryFormat::Contiguous);   // (contiguous() would hand back a contiguous tensor at an odd address)
 }
 
 at::Tensor workspace_of(size_t bytes, const at::Tensor& like) {
@@ -133,7 +142,8 @@ std::tuple<at::Tensor, at::Tensor> run_paged(const at::Tensor& q, const at::Tens
     if (want_lse) lse = gpu_empty({c.B, Hq, S}, at::kFloat, q);
     const size_t need = mi355_fmha_paged_workspace_bytes(&c, (int)Hq, (int)S, want_lse ? 1 : 0);
     const at::Tensor ws = workspace_of(need, q);
-    const int64_t strides[6] = {qc.stride(0), qc.stride(1), qc.stride(2), o.stride(0), o.stride(1), o.stride(2)};
+    const auto st = query_strides(qc);
+    const int64_t strides[6] = {st[0], st[1], st[2], o.stride(0), o.stride(1), o.stride(2)};
     hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
     const int rc = mi355_fmha_paged(&c, qc.data_ptr(), o.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr, (int)Hq, (int)S, strides,
                                     1.0f / std::sqrt(128.0f), need > 0 ? ws.data_ptr() : nullptr, need, stream);
@@ -175,7 +185,7 @@ void rope_paged(const at::Tensor& qkv, const at::Tensor& kv_pages, const at::Ten
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(kv_pages.device());
     hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
     const int64_t row = S > 1 ? qkv.stride(1) : (q_heads + 2 * (int64_t)c.Hkv) * 128;
-    const int rc = mi355_rope_paged(&c, qkv.data_ptr(), (int)S, (int)q_heads, keep_keys ? 1 : 0, qkv.stride(0), row, cos.data_ptr<float>(),
+    const int rc = mi355_rope_paged(&c, qkv.data_ptr(), (int)S, (int)q_heads, keep_keys ? 1 : 0, B > 1 ? qkv.stride(0) : 0, row, cos.data_ptr<float>(),
                                     sin.data_ptr<float>(), positions.data_ptr<int32_t>(), positions.dim() == 2 ? S : 0, (int)cos.size(0), stream);
     TORCH_CHECK(rc == 0, name, ": ", mi355_last_error(), " (code ", rc, ")");
 }
@@ -194,9 +204,9 @@ void key_weights(const at::Tensor& q, const at::Tensor& lse, const at::Tensor& k
     const int last = (int)std::min<int64_t>(last_rows, INT32_MAX);
     const size_t need = mi355_fmha_key_weights_workspace_bytes(&c, (int)Hq, (int)S, last);
     const at::Tensor ws = workspace_of(need, q);
-    const int64_t strides[3] = {qc.stride(0), qc.stride(1), qc.stride(2)};
+    const auto strides = query_strides(qc);
     hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
-    const int rc = mi355_fmha_key_weights(&c, qc.data_ptr(), lse.data_ptr<float>(), (int)Hq, (int)S, strides, last, 1.0f / std::sqrt(128.0f),
+    const int rc = mi355_fmha_key_weights(&c, qc.data_ptr(), lse.data_ptr<float>(), (int)Hq, (int)S, strides.data(), last, 1.0f / std::sqrt(128.0f),
                                           need > 0 ? ws.data_ptr() : nullptr, need, stream);
     TORCH_CHECK(rc == 0, name, ": ", mi355_last_error(), " (code ", rc, ")");
 }
