@@ -16,6 +16,7 @@
 // arithmetic. 16 keys lie in one page: a lane works out the
 // address of one such half tile of the next 64, and the scalar unit picks them up one after the other.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.h"
 
@@ -23,6 +24,7 @@ namespace mi355 {
 
 namespace pdec {
 typedef float float2v __attribute__((ext_vector_type(2)));
+typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
 constexpr int D = 128;
 constexpr int TK = 32;                       // keys per tile
 constexpr int ROW_BYTES = D * 2;             // 256
@@ -390,7 +392,20 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
                 l_run[nb] += psum;
             }
             // O^T += V^T P^T; the 8 keys of a lane of P are 4 g + 0..3 and 16 + 4 g + 0..3, V^T is gathered in that order
-            if (!masked) {
+            // A product with p = 0 is not nothing where v is infinite or NaN: a masked tile that holds such values takes the way below.
+            bool finite = true;
+            if (masked) {
+                ushort2v top = {0, 0};
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const int4v x = *(MI355_LDS const int4v*)(st + TILE_BYTES + c * 1024 + lane * 16);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(ushort2v, x[e] & 0x7fff7fff));
+                }
+                constexpr unsigned short kInfinity = std::is_same<T, half_t>::value ? 0x7c00 : 0x7f80;
+                finite = __builtin_amdgcn_ballot_w64(top[0] >= kInfinity || top[1] >= kInfinity) == 0;
+            }
+            if (finite) {
 #pragma unroll
                 for (int db = 0; db < 8; ++db) {
                     MI355_LDS char* vp = st + (v_base ^ (db << 5));
@@ -399,8 +414,7 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
                     for (int nb = 0; nb < NB; ++nb) o[nb][db] = Elem<T>::mfma16(vf, pf[nb], o[nb][db]);
                 }
             } else if (key0 <= lim_max) {
-                // A product with p = 0 is not nothing where v is infinite or NaN: what a row does not see is taken out of V, row by
-                // row, and the sum is taken over for that row's columns alone.
+                // What a row does not see is taken out of V, row by row, and the sum is taken over for that row's columns alone.
                 for (int r = row_min; r <= row_max; ++r) {
                     const int last = r < n_new ? min(len - 1, r + len - n_new) : -1;
 #pragma unroll
