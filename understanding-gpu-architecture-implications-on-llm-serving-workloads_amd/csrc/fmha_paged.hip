@@ -682,7 +682,9 @@ static PagedPlan paged_plan(int B, int Hkv, int max_len, int Hq, int Sq, bool we
     p.blocks = (ncols + p.col_block - 1) / p.col_block;
     p.max_tiles = (max_len + TK - 1) / TK;
     p.direct = max_len <= kDirectLen;
-    p.workgroups = p.direct ? (int)pairs : (int)std::min<long>(kWorkgroups, (pairs * p.max_tiles + kMinTiles - 1) / kMinTiles);
+    // One workgroup per CU over all blocks of columns: a part has a fixed cost of ~8 us (the first tiles' way, the waves' meeting), so with many
+    // blocks each is cut into fewer (512 rows of 32/8 heads over 8191 keys, 64 blocks: 256 workgroups each 666 us, 4 each 185).
+    p.workgroups = p.direct ? (int)pairs : (int)std::min<long>((kWorkgroups + p.blocks - 1) / p.blocks, (pairs * p.max_tiles + kMinTiles - 1) / kMinTiles);
     if (!p.direct) p.part_bytes = sizeof(float) * (size_t)p.blocks * (p.workgroups + pairs) * p.col_block * PART_STRIDE;
     p.scores = weights && ncols <= 32;
     const int meet = WAVES * (p.col_block * D + 64) * (int)sizeof(float);
