@@ -41,7 +41,7 @@ constexpr float kLazyLog2 = 8.f;             // rescale only when a column maxim
 constexpr int PART_STRIDE = D + 4;           // floats per (part, column): O~[128], m, l, 2 pad (keeps rows 16-byte aligned)
 constexpr int kWorkgroups = 256;             // one per CU
 constexpr int kMinTiles = 4;                 // of a workgroup: one per wave
-constexpr int kDirectLen = 512;              // up to this many keys a workgroup per (sequence, kv head) walks them all
+constexpr int kDirectLen = 512;              // up to this many keys a workgroup per (sequence, kv head) walks them all (paged_plan)
 
 __device__ __forceinline__ int swz_k(int row) { return row & 15; }
 __device__ __forceinline__ int swz_v(int row) { return (row & 7) << 1; }
@@ -681,7 +681,10 @@ static PagedPlan paged_plan(int B, int Hkv, int max_len, int Hq, int Sq, bool we
     p.col_block = std::min(ncols, 32);
     p.blocks = (ncols + p.col_block - 1) / p.col_block;
     p.max_tiles = (max_len + TK - 1) / TK;
-    p.direct = max_len <= kDirectLen;
+    // A workgroup per pair needs no joining, but walks the longest sequence alone. us, so / in equal shares, sequences as long as the table is wide: 8 pairs
+    // over 512 keys 7.9 / 8.5, over 768 9.4 / 8.5, over 1024 11.1 / 8.6; 128 pairs over 512 9.2 / 12.3, over 1024 14.1 / 17.4 (over 2048 23.0 / 26.6, but 17.5 / 9.1 where
+    // one sequence is that long and the others short).
+    p.direct = max_len <= kDirectLen || (max_len <= 2 * kDirectLen && pairs >= 128);
     // One workgroup per CU over all blocks of columns: a part has a fixed cost of ~8 us (the first tiles' way, the waves' meeting), so with many
     // blocks each is cut into fewer (512 rows of 32/8 heads over 8191 keys, 64 blocks: 256 workgroups each 666 us, 4 each 185).
     p.workgroups = p.direct ? (int)pairs : (int)std::min<long>((kWorkgroups + p.blocks - 1) / p.blocks, (pairs * p.max_tiles + kMinTiles - 1) / kMinTiles);
