@@ -10,7 +10,7 @@
 // hardly overlap: a software pipeline of product and exponentials took 162 us, 32x32x16 instructions (2 waves to a SIMD instead of 3) 177.
 //
 // A workgroup owns 256 keys of one (sequence, kv head), which stay in its waves' registers as the A operand of S^T = K Q^T;
-// tiles of 64 rows of a query head pass through LDS, two stages, and each wave adds its scores' exponentials up in registers: the sum over the
+// tiles of 64 rows of a query head pass through LDS, three stages, and each wave adds its scores' exponentials up in registers: the sum over the
 // columns of an accumulator tile is left for the end, where 16 lanes add theirs. The rows of all heads that see the keys are cut into
 // ranges of equally many tiles, a workgroup each (in a causal triangle the first keys have many, the last ones few), and a second kernel adds
 // the ranges up in order, so that the same call gives the same bits.
@@ -26,8 +26,9 @@ constexpr int D = 128;
 constexpr int BLOCK = 256;                    // keys of a workgroup
 constexpr int ROWS = 64;                      // of a tile
 constexpr int STAGE_BYTES = ROWS * D * 2;     // 16 KiB
+constexpr int NSTAGE = 3;                     // one being worked on, two on their way
 constexpr int kMinTiles = 4, kMaxTiles = 16;  // of a range
-constexpr int kWorkgroups = 768;              // that run at the same time
+constexpr int kWorkgroups = 700;              // a little less than run at the same time (three to a CU)
 }  // namespace kw
 
 struct KeyWeights {
@@ -57,8 +58,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void key_weights_kernel(PagedKv kv, 
     using V8 = typename Elem<T>::v8;
     constexpr int KEYS = BLOCK / WAVES, NKB = KEYS / 16;   // keys of a wave, blocks of 16 of them
     constexpr int COPIES = 16 / WAVES;                     // of 4 rows, of a wave and tile
-    __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE_BYTES];
-    __shared__ float refs[2][ROWS];
+    __shared__ __attribute__((aligned(1024))) char smem[NSTAGE * STAGE_BYTES];
+    __shared__ float refs[kMaxTiles * ROWS];   // the exponents' offsets of the range's rows
     MI355_LDS char* lds = (MI355_LDS char*)smem;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -85,7 +86,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void key_weights_kernel(PagedKv kv, 
         const T* Q = (const T*)a.Q + b * a.q_batch;
         const float* LSE = a.LSE + (long)b * a.Hq * a.Sq;
         // tile t: rows row .. row + 63 of a query head; rows in front of the first that counts repeat it and count for nothing. The waves
-        // share its copies (where all are there, to offsets worked out once); thread r < 64 has the log-sum-exp of row r.
+        // share its copies (where all are there, to offsets worked out once).
         const uint32_t q_row_bytes = (uint32_t)(a.q_row * 2);
         uint32_t offset[COPIES];
 #pragma unroll
@@ -93,12 +94,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void key_weights_kernel(PagedKv kv, 
             const int r = 4 * (COPIES * wave + c) + (lane >> 4);
             offset[c] = (uint32_t)r * q_row_bytes + (((lane & 15) ^ (r & 15)) << 4);
         }
-        float lse = 0.f;
         auto issue = [&](int t, int slot) {
             const int back = divide(t, a.by_group), hq = hkv * a.group + t - back * a.group, row = n_new - (back + 1) * ROWS;
             const int at = max(row, first), missing = at - row;
             const char* base = (const char*)(Q + (long)hq * a.q_head + (long)at * a.q_row);
-            if (threadIdx.x < ROWS) lse = (int)threadIdx.x >= missing ? LSE[(long)hq * a.Sq + at + (int)threadIdx.x - missing] : -INFINITY;
             MI355_LDS char* st = lds + slot * STAGE_BYTES + wave * (COPIES * 1024);
             if (missing == 0) {
 #pragma unroll
@@ -113,6 +112,15 @@ __global__ __launch_bounds__(WAVES * 64, 2) void key_weights_kernel(PagedKv kv, 
         };
         const int q_base = c16 * 256 + ((g ^ c16) << 4);   // xor (ks << 6), + 16 cb rows
         issue(t_begin, 0);
+        if (t_begin + 1 < t_end) issue(t_begin + 1, 1);
+        // All rows' offsets up front (a load among the copies would be waited for together with them). A row that sees no key (or is none)
+        // adds nothing: 2^(x - inf) = 0
+        for (int r = threadIdx.x; r < (t_end - t_begin) * ROWS; r += WAVES * 64) {
+            const int t = t_begin + r / ROWS, back = divide(t, a.by_group), hq = hkv * a.group + t - back * a.group;
+            const int row = n_new - (back + 1) * ROWS + r % ROWS;
+            const float lse = row >= first ? LSE[(long)hq * a.Sq + row] : -INFINITY;
+            refs[r] = lse == -INFINITY ? -INFINITY : -lse * 1.4426950408889634f;
+        }
         // this wave's keys: lane holds K[16 kb + c16][32 ks + 8 g .. +7]; keys behind the last repeat it, those of a page outside the
         // pool read its first one (neither is written out)
         V8 kf[NKB][4];
@@ -128,15 +136,16 @@ __global__ __launch_bounds__(WAVES * 64, 2) void key_weights_kernel(PagedKv kv, 
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) kf[kb][ks] = *(const V8*)(p + 64 * ks);
         }
+        int slot = 0;
         for (int t = t_begin; t < t_end; ++t) {
-            const int slot = (t - t_begin) & 1;
-            wait_vmcnt<0>();
-            // the exponent's offset of each row; one that sees no key (or is none) adds nothing: 2^(x - inf) = 0
-            if (threadIdx.x < ROWS) refs[slot][threadIdx.x] = lse == -INFINITY ? -INFINITY : -lse * 1.4426950408889634f;
-            __syncthreads();
-            if (t + 1 < t_end) issue(t + 1, slot ^ 1);
+            if (t + 1 < t_end) wait_vmcnt<COPIES>();   // everything but the newest tile has landed
+            else wait_vmcnt<0>();
+            __syncthreads();   // everybody's copies; the stage of the tile before is free
+            if (t + 2 < t_end) issue(t + 2, slot == 0 ? 2 : slot - 1);
             const int row = n_new - (divide(t, a.by_group) + 1) * ROWS;
             MI355_LDS char* st = lds + slot * STAGE_BYTES;
+            const float* ref_of = refs + (t - t_begin) * ROWS;
+            slot = slot == NSTAGE - 1 ? 0 : slot + 1;
             // 16 rows against this wave's 64 keys, four times. MASKED: the tile holds rows that do not see all of them (a body of its own:
             // the comparisons would double the vector instructions of the others)
             const auto tile = [&](auto mask) {
@@ -146,7 +155,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void key_weights_kernel(PagedKv kv, 
 #pragma unroll
                     for (int ks = 0; ks < 4; ++ks)
                         qf[ks] = Elem<T>::frag(lds_read_b128(st + (q_base ^ (ks << 6)) + 16 * cb * 256));
-                    const float ref = refs[slot][16 * cb + c16];
+                    const float ref = ref_of[16 * cb + c16];
                     float4v s[NKB];
 #pragma unroll
                     for (int kb = 0; kb < NKB; ++kb) s[kb] = float4v{0.f, 0.f, 0.f, 0.f};
@@ -208,7 +217,13 @@ __global__ __launch_bounds__(256) void key_weights_sum_kernel(PagedKv kv, KeyWei
     const int tiles = key_weights_tiles(a, paged_len(kv, b), paged_new(kv, b, a.Sq), blockIdx.x * 256);
     const int ranges = max((tiles + a.range_tiles - 1) / a.range_tiles, 1);
     float sum = 0.f;
-    for (int z = 0; z < ranges; ++z) sum += p[z * stride];
+    for (int z0 = 0; z0 < ranges; z0 += 8) {   // eight in flight
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = p[min(z0 + k, ranges - 1) * stride];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum += z0 + k < ranges ? x[k] : 0.f;
+    }
     kv.weights[((long)page * kv.Hkv + hkv) * kv.page_size + (key - i * kv.page_size)] += sum;
 }
 
@@ -219,9 +234,12 @@ static KeyWeightsPlan key_weights_plan(const mi355_paged_kv& c, int Hq, int Sq, 
     using namespace kw;
     KeyWeightsPlan p;
     p.max_blocks = (c.max_pages * c.page_size + BLOCK - 1) / BLOCK;
-    const int rows = last_rows > 0 ? std::min(last_rows, Sq) : Sq;
-    const long most = (long)(Hq / c.Hkv) * ((rows + ROWS - 1) / ROWS), all = most * c.B * c.Hkv * p.max_blocks;
-    p.range_tiles = (int)std::max<long>(kMinTiles, std::min<long>(kMaxTiles, all / kWorkgroups));
+    const int max_len = c.max_pages * c.page_size, rows = last_rows > 0 ? std::min(last_rows, Sq) : Sq;
+    const long most = (long)(Hq / c.Hkv) * ((rows + ROWS - 1) / ROWS);
+    // about as many workgroups as run at the same time, where that leaves them few enough tiles; of the tiles, those that the causal triangle
+    // of the longest sequence leaves
+    const long seen = most * c.B * c.Hkv * p.max_blocks * (2L * max_len - std::min(rows, max_len)) / (2L * max_len);
+    p.range_tiles = (int)std::max<long>(kMinTiles, std::min<long>(kMaxTiles, (seen + kWorkgroups - 1) / kWorkgroups));
     p.ranges = (int)((most + p.range_tiles - 1) / p.range_tiles);
     return p;
 }
@@ -261,12 +279,12 @@ hipError_t key_weights_dispatch(const mi355_paged_kv& c, const void* Q, const fl
     a.by_blocks = divisor_of(a.max_blocks);
     a.by_group = divisor_of(a.group);
     const dim3 grid((unsigned)key_weights_workgroups(c, Hq, Sq, last_rows));
-    // Eight waves of 32 keys where there is no more than a workgroup per CU (us, eight / four waves: 64 rows of 32/8 heads over 8191 keys 11.3 /
-    // 12.2), four of 64, which read the rows' tiles half as often, where several share one (2 x 32/8 heads, 4096 rows 164.6 / 159.9).
-    const bool one_each = (long)a.max_blocks * a.pairs * a.ranges <= 256;
+    // Eight waves of 32 keys where a CU has one or two workgroups (us, eight / four waves: 64 rows of 32/8 heads over 8191 keys 11.3 / 12.2, 1024
+    // rows 17.8 / 18.9), four of 64, which read the rows' tiles half as often, where more share one (2 x 32/8 heads, 4096 rows 164.6 / 159.9).
+    const bool few = (long)a.max_blocks * a.pairs * a.ranges <= 512;
     const auto launch = [&](auto type) {
         using T = decltype(type);
-        if (one_each) key_weights_kernel<T, 8><<<grid, dim3(512), 0, stream>>>(kv, a);
+        if (few) key_weights_kernel<T, 8><<<grid, dim3(512), 0, stream>>>(kv, a);
         else key_weights_kernel<T, 4><<<grid, dim3(256), 0, stream>>>(kv, a);
     };
     if (c.dtype == MI355_DTYPE_BF16) launch(bf16_t{});
