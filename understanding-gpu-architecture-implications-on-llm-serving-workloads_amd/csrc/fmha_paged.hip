@@ -603,14 +603,19 @@ __device__ __forceinline__ void add_weights(const PagedKv& kv, const PagedAttn& 
     const int len = paged_len(kv, b);
     const int key = chunk * 256 + tid;
     if (chunk * 256 >= len) return;
-    int first = 0;
-    const int n = a.direct ? 1 : parts_of(kv, a, b, hkv, first);
-    // the first scores are fetched beside the statistics
-    const float* sp = a.scores + ((long)pair * a.max_tiles + (min(key, len - 1) >> 5)) * (a.ncols * TK) + (key & 31);
+    // the account as it is and the first scores are fetched beside the statistics
+    const int at = min(key, len - 1), i = divide(at, kv.by_page);
+    const int page = kv.table[(long)b * kv.table_stride + i];
+    const bool there = key < len && (uint32_t)page < (uint32_t)kv.n_pages;
+    float* w = kv.weights + ((long)(there ? page : 0) * kv.Hkv + hkv) * kv.page_size + (at - i * kv.page_size);
+    const float* sp = a.scores + ((long)pair * a.max_tiles + (at >> 5)) * (a.ncols * TK) + (at & 31);
     constexpr int AHEAD = 8;
     float s[AHEAD];
 #pragma unroll
     for (int c = 0; c < AHEAD; ++c) s[c] = sp[min(c, a.ncols - 1) * TK];
+    const float old = *w;
+    int first = 0;
+    const int n = a.direct ? 1 : parts_of(kv, a, b, hkv, first);
     if (n == 1) {
         if (tid < a.ncols) {
             const float x = a.LSE[((long)b * a.Hq + hkv * a.group) * a.Sq + tid];   // columns are consecutive rows
@@ -639,7 +644,7 @@ __device__ __forceinline__ void add_weights(const PagedKv& kv, const PagedAttn& 
         }
     }
     __syncthreads();
-    if (key >= len) return;
+    if (!there) return;
     float sum = 0.f;
     // a row that sees no key adds nothing
     const auto add = [&](int c, float x) { sum += lse[c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(x, a.scale_log2, -lse[c])); };
@@ -647,10 +652,7 @@ __device__ __forceinline__ void add_weights(const PagedKv& kv, const PagedAttn& 
     for (int c = 0; c < AHEAD; ++c)
         if (c < a.ncols) add(c, s[c]);
     for (int c = AHEAD; c < a.ncols; ++c) add(c, sp[c * TK]);
-    const int i = divide(key, kv.by_page);
-    const int page = kv.table[(long)b * kv.table_stride + i];
-    if ((uint32_t)page >= (uint32_t)kv.n_pages) return;
-    kv.weights[((long)page * kv.Hkv + hkv) * kv.page_size + (key - i * kv.page_size)] += sum;
+    *w = old + sum;
 }
 
 // What is left behind fmha_paged_kernel, side by side: a workgroup per (pair, column) joins parts (none where one workgroup walked all keys), then
