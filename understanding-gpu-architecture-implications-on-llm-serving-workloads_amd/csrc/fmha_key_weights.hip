@@ -42,6 +42,18 @@ struct KeyWeights {
     Divisor by_hkv, by_pairs, by_blocks, by_group;
 };
 
+// sum over the 16 lanes of a row, in every lane (rotations within the row: no trip through LDS)
+__device__ __forceinline__ float sum_of_16(float x) {
+    const auto turned = [](float v, auto by) {
+        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + decltype(by)::value, 0xf, 0xf, true));
+    };
+    x += turned(x, std::integral_constant<int, 8>{});
+    x += turned(x, std::integral_constant<int, 4>{});
+    x += turned(x, std::integral_constant<int, 2>{});
+    x += turned(x, std::integral_constant<int, 1>{});
+    return x;
+}
+
 // Row i sees the keys up to i + len - n_new (a sequence shorter than its rows: its first rows see nothing). Tiles are counted from the last rows,
 // which see most, to the first that see any key of the block at block0, the heads of a tile's rows one after the other.
 __device__ __forceinline__ int key_weights_first(const KeyWeights& a, int n_new) { return a.last_rows > 0 ? max(n_new - a.last_rows, 0) : 0; }
@@ -180,10 +192,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void key_weights_kernel(PagedKv kv, 
 #pragma unroll
         for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-#pragma unroll
-                for (int off = 8; off >= 1; off >>= 1) acc[kb][e] += __shfl_xor(acc[kb][e], off, 64);
-            }
+            for (int e = 0; e < 4; ++e) acc[kb][e] = sum_of_16(acc[kb][e]);
     }
     // lane c16 = 4 kb + e of a group writes its key 16 kb + 4 g + e (with fewer keys the upper lanes have none)
     float out = 0.f;
