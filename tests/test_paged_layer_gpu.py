@@ -110,6 +110,13 @@ def test_steps_with_eviction_attend_to_what_is_kept(gpu):
                 for h in range(n_kv):
                     assert set(range(max(0, cache.positions[b] - 20), cache.positions[b])) <= set(where[:, h].tolist())
     assert cache.positions == [150, 70] and cache.lengths == [64, 64]
+    with pytest.raises(ValueError):
+        cache.take_back([1, 0])                       # cut a moment ago: the last slot is not the last token
+    layer(so.randn_fp16((B, 3, H), 300).to(gpu), kv_cache=cache)
+    with pytest.raises(ValueError):
+        cache.take_back([4, 0])
+    cache.take_back([2, 3])
+    assert cache.lengths == [65, 64] and cache.positions == [151, 70] and cache.seq_lens.tolist() == [65, 64]
 
 
 def test_layer_over_pages_refuses(gpu):

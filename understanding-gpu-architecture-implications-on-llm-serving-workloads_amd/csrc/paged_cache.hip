@@ -12,7 +12,8 @@ constexpr int THREADS = 256;
 
 // Token (b, t) of a fused projection [q_heads | Hkv key heads | Hkv value heads] of 128: queries rotated in place, rotated keys and the values to row
 // seq_lens[b] - new + t of the sequence; keep_keys: the rotated keys also where they were read. A thread owns 8 values of the
-// lower half of a head and their 8 partners; 8 threads a head, 32 heads a workgroup. The arithmetic is that of rope_kernel (glue.hip).
+// lower half of a head and their 8 partners; 8 threads a head, 32 heads a workgroup. The arithmetic is that of rope_kernel (glue.hip). Bound by
+// HBM for prompts (4 x 2048 rows, 60 % of them tokens, 32/8 heads: 29 us, 5.35 TB/s), by its chain of loads for a step (64 tokens: 3.2 us).
 template <typename T>
 __global__ __launch_bounds__(pcache::THREADS) void rope_paged_kernel(PagedKv kv, T* qkv, int S, Divisor by_s, int q_heads, int keep_keys, long x_batch,
                                                                      long x_row, const float* __restrict__ cos_t, const float* __restrict__ sin_t,
@@ -163,8 +164,9 @@ __device__ __forceinline__ void move_keys(const PagedKv& kv, int b, int hkv, Lis
 
 // One workgroup per (sequence, kv head). A thread owns 4 * chunks slots side by side (4 lie in one page and are read with one access), so that
 // what has to be counted in the order of the slots is one sum over the threads. Their ranks stay in M chunks of registers or, M == 0, in
-// the workspace, where only their thread reads them again. Bound by its chain of about ten steps, a memory round trip or a pass over the
-// workgroup each.
+// the workspace, where only their thread reads them again. Bound by its chain of about twelve steps, a memory round trip or a pass over the
+// workgroup each (128 workgroups, 2176 keys each: loads 1.5 us, ranks 1.1, three passes 1.1 each, what moves 2, 120 moves 3; with positions and weights read by loops and the ranks
+// in LDS it took 13.9 us without the moves).
 template <int M>
 __global__ __launch_bounds__(evict::THREADS) void evict_select_kernel(PagedKv kv, Evict a) {
     using namespace evict;
@@ -347,7 +349,7 @@ __global__ __launch_bounds__(evict::THREADS) void evict_select_kernel(PagedKv kv
     for (int n = 0; n < total; n += 4 * THREADS / 32) move_keys(kv, b, hkv, list[0], list[1], n + (tid >> 5), THREADS / 32, total);
 }
 
-// Grid (moves / 32, pairs)
+// Grid (moves / 32, pairs), for more moves than the selecting workgroup makes (32 pairs, ~1500 moves each: 8.9 us; with one move in flight a thread 16)
 __global__ __launch_bounds__(256) void evict_move_kernel(PagedKv kv, Evict a) {
     const int count = a.counts[blockIdx.y];
     const int b = divide(blockIdx.y, a.by_hkv), hkv = blockIdx.y - b * kv.Hkv;

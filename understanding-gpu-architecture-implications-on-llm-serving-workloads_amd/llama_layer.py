@@ -75,6 +75,7 @@ class FinePagedKVCache:
         self.weights = torch.zeros((n_pages, n_kv, page_size), device=device) if account else None
         self.key_positions = torch.zeros((n_pages, n_kv, page_size), dtype=torch.int32, device=device) if account else None
         self.lengths, self.positions = [0] * batch, [0] * batch
+        self._in_order = [0] * batch      # tokens at the end of each sequence that no eviction has moved
         self._pages = [[] for _ in range(batch)]
         self._free = list(range(n_pages - 1, -1, -1))
 
@@ -100,15 +101,17 @@ class FinePagedKVCache:
             self._write_table([b for b, more in enumerate(wanted) if more])
         self.lengths = lengths
         self.positions = [n + more for n, more in zip(self.positions, new)]
+        self._in_order = [n + more for n, more in zip(self._in_order, new)]
         step = new[0] if all(n == new[0] for n in new) else torch.tensor(new, dtype=torch.int32, device=self.seq_lens.device)
         self.seq_lens += step
         self.next_positions += step
 
     def take_back(self, new):
-        """The last new[b] tokens of each sequence are no longer its own (a call that failed; drafted tokens that were not accepted). The account of
-        the others keeps what those added to it."""
-        if len(new) != len(self.lengths) or any(not 0 <= n <= have for n, have in zip(new, self.lengths)):
-            raise ValueError("cannot take %r tokens back from sequences of %r" % (new, self.lengths))
+        """The last new[b] tokens of each sequence are no longer its own (a call that failed; drafted tokens that were not accepted); ValueError for more
+        than have come since it was cut, which leaves no order. The account of the others keeps what those added to it."""
+        if len(new) != len(self.lengths) or any(not 0 <= n <= have for n, have in zip(new, self._in_order)):
+            raise ValueError("cannot take %r tokens back where %r have come" % (new, self._in_order))
+        self._in_order = [n - less for n, less in zip(self._in_order, new)]
         self.lengths = [n - less for n, less in zip(self.lengths, new)]
         self.positions = [n - less for n, less in zip(self.positions, new)]
         step = new[0] if all(n == new[0] for n in new) else torch.tensor(new, dtype=torch.int32, device=self.seq_lens.device)
@@ -123,12 +126,13 @@ class FinePagedKVCache:
         if all(n <= budget for n in self.lengths):
             return
         self.seq_lens.copy_(fine_evict_paged(self.kv_pages, self.block_table, self.seq_lens, self.weights, self.key_positions, budget, recent))
+        self._in_order = [0 if n > budget else have for n, have in zip(self.lengths, self._in_order)]
         self.lengths = [min(n, budget) for n in self.lengths]
         self._give_back(range(len(self.lengths)))
 
     def release(self, b):
         """Sequence b is done: its pages are free, its place may be taken by another."""
-        self.lengths[b] = self.positions[b] = 0
+        self.lengths[b] = self.positions[b] = self._in_order[b] = 0
         self.seq_lens[b] = 0
         self.next_positions[b] = 0
         self._give_back([b])
