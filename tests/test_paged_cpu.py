@@ -63,6 +63,32 @@ def test_attention_refuses_bad_arguments(lib):
     assert cdll.mi355_fmha_paged_workspace_bytes(cache(lib, weights=None), 32, 1, 1) == 0
 
 
+def test_workspaces_of_refused_calls_are_zero_bytes(lib):
+    """Sizes whose products leave the range of an int, or are zero in it, among them."""
+    cdll = lib.load()
+    sizes = [dict(page_size=1 << 16, max_pages=1 << 16), dict(page_size=1 << 30, max_pages=4), dict(max_pages=(1 << 24) + 1), dict(B=1 << 16, Hkv=1 << 16), dict(page_size=24),
+             dict(page_size=0), dict(B=0)]
+    for bad in sizes:
+        c = cache(lib, **bad)
+        assert cdll.mi355_fmha_paged_workspace_bytes(c, 1 << 16, 4, 1) == 0
+        assert cdll.mi355_fmha_key_weights_workspace_bytes(c, 1 << 16, 4, 0) == 0
+        assert cdll.mi355_cache_evict_workspace_bytes(c, 32) == 0
+    for Hq, S in ((1 << 16, 1 << 16), (1 << 16, 1 << 15), (1 << 20, 1 << 30), (8, 1 << 16), (7, 4), (8, 0), (0, 4)):
+        for weights in (None, P):
+            c = cache(lib, weights=weights)
+            assert cdll.mi355_fmha_paged_workspace_bytes(c, Hq, S, 1) == 0
+            assert cdll.mi355_fmha_key_weights_workspace_bytes(c, Hq, S, 0) == 0
+    assert cdll.mi355_cache_evict_workspace_bytes(cache(lib), 0) == 0
+
+
+def test_an_account_of_more_rows_than_a_launch_takes_is_refused(lib):
+    cdll, big = lib.load(), 1 << 60
+    wide = dict(B=1, Hkv=1, max_pages=1 << 20, table_stride=1 << 20)   # 65536 blocks of keys, 16 tiles of rows a workgroup
+    assert cdll.mi355_fmha_paged(cache(lib, **wide), P, P, P, 4, 16000, None, 0.1, P, 0, None) == lib.ERR_BAD_ARGUMENT   # (no workspace: sizes are fine)
+    assert cdll.mi355_fmha_paged(cache(lib, **wide), P, P, P, 32768, 1, None, 0.1, P, big, None) == lib.ERR_UNSUPPORTED
+    assert b"more than a call takes" in cdll.mi355_last_error()
+
+
 def test_the_other_entry_points_refuse_bad_arguments(lib):
     cdll, c, big = lib.load(), cache(lib), 1 << 60
     row = 48 * 128

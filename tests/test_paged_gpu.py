@@ -614,7 +614,7 @@ def test_a_captured_step_is_replayed_as_the_lengths_go_on(gpu):
 
 @pytest.mark.parametrize("Hq,Hkv,S", [(1, 1, 1), (4, 2, 1), (32, 8, 1), (64, 8, 1), (16, 2, 4), (40, 4, 7)])
 def test_captured_and_eager_calls_give_the_same_bits(gpu, Hq, Hkv, S):
-    """Parts of long caches are joined by the last workgroup, or by a launch of their own in a captured call."""
+    """Long caches are cut into parts, joined in an order that the lengths alone decide."""
     cache = Cache([9000, 17, 0, 3000], Hkv, 32)
     q = queries(cache, Hq, S)
     weights = cache.weights.clone()

@@ -436,6 +436,14 @@ int mi355_internal_step_gate_up(const void* x, const void* norm_weight, float ep
 
 
 // ---- the paged key-value cache ----
+// Whether the counts (keys, tiles of keys, rows) of a cache and a call stay within what the kernels and their plans count in ints
+static bool paged_sizes(const mi355_paged_kv* c) {
+    if (!c || c->B < 1 || c->Hkv < 1 || c->max_pages < 1 || c->page_size < 16 || c->page_size % 16 != 0) return false;
+    const int64_t pairs = (int64_t)c->B * c->Hkv, max_len = (int64_t)c->max_pages * c->page_size;
+    return pairs <= 65535 && max_len <= (1 << 28) && pairs * (max_len / 32 + 1) <= INT32_MAX - 65536;
+}
+static bool paged_rows(const mi355_paged_kv* c, int Hq, int S) { return Hq >= c->Hkv && S >= 1 && (int64_t)(Hq / c->Hkv) * S <= 65535; }
+
 static int paged_checked(const char* fn, const mi355_paged_kv* c) {
     if (!c || !c->pages || !c->block_table || !c->seq_lens) return fail(MI355_ERR_BAD_ARGUMENT, "%s: null pointer", fn);
     if (c->dtype != MI355_DTYPE_FP16 && c->dtype != MI355_DTYPE_BF16) return fail(MI355_ERR_BAD_ARGUMENT, "%s: unknown dtype %d", fn, c->dtype);
@@ -443,9 +451,9 @@ static int paged_checked(const char* fn, const mi355_paged_kv* c) {
         return fail(MI355_ERR_BAD_ARGUMENT, "%s: B, Hkv, n_pages and max_pages must be >= 1 (got %d, %d, %d, %d)", fn, c->B, c->Hkv, c->n_pages, c->max_pages);
     if (c->page_size < 16 || c->page_size % 16 != 0)
         return fail(MI355_ERR_UNSUPPORTED, "%s: page_size must be a positive multiple of 16 (got %d)", fn, c->page_size);
-    const int64_t pairs = (int64_t)c->B * c->Hkv, max_len = (int64_t)c->max_pages * c->page_size;
-    if (pairs > 65535) return fail(MI355_ERR_UNSUPPORTED, "%s: B * Hkv must be at most 65535 (got %lld)", fn, (long long)pairs);
-    if (max_len > (1 << 28) || pairs * (max_len / 32 + 1) > INT32_MAX)
+    const int64_t max_len = (int64_t)c->max_pages * c->page_size;
+    if ((int64_t)c->B * c->Hkv > 65535) return fail(MI355_ERR_UNSUPPORTED, "%s: B * Hkv must be at most 65535 (got %d * %d)", fn, c->B, c->Hkv);
+    if (!paged_sizes(c))
         return fail(MI355_ERR_UNSUPPORTED, "%s: %d sequences of up to %lld keys of %d heads are more than a call takes", fn, c->B, (long long)max_len, c->Hkv);
     if (c->B > 1 && c->table_stride < c->max_pages)
         return fail(MI355_ERR_BAD_ARGUMENT, "%s: rows of the block table overlap (stride %lld, %d entries)", fn, (long long)c->table_stride, c->max_pages);
@@ -465,7 +473,7 @@ static int paged_queries_checked(const char* fn, const mi355_paged_kv* c, const 
     if (!Q) return fail(MI355_ERR_BAD_ARGUMENT, "%s: null pointer", fn);
     if (Hq < 1 || S < 1) return fail(MI355_ERR_BAD_ARGUMENT, "%s: Hq and S must be >= 1", fn);
     if (Hq % c->Hkv != 0) return fail(MI355_ERR_BAD_ARGUMENT, "%s: Hq (%d) must be a multiple of Hkv (%d)", fn, Hq, c->Hkv);
-    if ((int64_t)(Hq / c->Hkv) * S > 65535)
+    if (!paged_rows(c, Hq, S))
         return fail(MI355_ERR_UNSUPPORTED, "%s: Hq / Hkv * S must be at most 65535 (got %d / %d * %d)", fn, Hq, c->Hkv, S);
     if (!(scale > 0.f) || scale > 3.0e38f) return fail(MI355_ERR_BAD_ARGUMENT, "%s: scale must be positive and finite (got %g)", fn, (double)scale);
     if (!aligned16(Q)) return fail(MI355_ERR_BAD_ARGUMENT, "%s: Q must be 16-byte aligned", fn);
@@ -486,7 +494,7 @@ static int workspace_checked(const char* fn, size_t need, const void* workspace,
 }
 
 size_t mi355_fmha_paged_workspace_bytes(const mi355_paged_kv* cache, int Hq, int S, int want_lse) {
-    if (!cache || cache->B < 1 || cache->Hkv < 1 || Hq < cache->Hkv || S < 1 || cache->max_pages < 1 || cache->page_size < 1) return 0;
+    if (!paged_sizes(cache) || !paged_rows(cache, Hq, S)) return 0;   // (the call is refused)
     return mi355::fmha_paged_workspace(*cache, Hq, S, want_lse != 0);
 }
 
@@ -499,7 +507,9 @@ int mi355_fmha_paged(const mi355_paged_kv* cache, const void* Q, void* O, float*
     const int64_t* st = strides ? strides : dense;
     if (int rc = paged_queries_checked(fn, cache, Q, Hq, S, st, 6, scale)) return rc;
     if (!aligned16(O)) return fail(MI355_ERR_BAD_ARGUMENT, "%s: O must be 16-byte aligned", fn);
-    if ((int64_t)cache->B * cache->Hkv * ((int64_t)(Hq / cache->Hkv) * S + (int64_t)cache->max_pages * cache->page_size / 256 + 1) > kMostWorkgroups)
+    // (the account of many rows is made by mi355_fmha_key_weights' kernel)
+    if ((int64_t)cache->B * cache->Hkv * ((int64_t)(Hq / cache->Hkv) * S + (int64_t)cache->max_pages * cache->page_size / 256 + 1) > kMostWorkgroups ||
+        (cache->weights && !mi355::fmha_paged_keeps_scores(*cache, Hq, S) && mi355::key_weights_workgroups(*cache, Hq, S, 0) > kMostWorkgroups / 2))
         return fail(MI355_ERR_UNSUPPORTED, "%s: %d sequences of %d rows over up to %lld keys are more than a call takes", fn, cache->B, S,
                     (long long)cache->max_pages * cache->page_size);
     if ((S > 1 && st[5] < 128) || (Hq > 1 && st[4] < 128) || (cache->B > 1 && st[3] < 128))
@@ -530,7 +540,7 @@ int mi355_rope_paged(const mi355_paged_kv* cache, void* qkv, int S, int q_heads,
 }
 
 size_t mi355_fmha_key_weights_workspace_bytes(const mi355_paged_kv* cache, int Hq, int S, int last_rows) {
-    if (!cache || cache->B < 1 || cache->Hkv < 1 || Hq < cache->Hkv || S < 1 || cache->max_pages < 1 || cache->page_size < 1) return 0;
+    if (!paged_sizes(cache) || !paged_rows(cache, Hq, S)) return 0;   // (the call is refused)
     return mi355::key_weights_workspace(*cache, Hq, S, last_rows);
 }
 
@@ -553,7 +563,7 @@ int mi355_fmha_key_weights(const mi355_paged_kv* cache, const void* Q, const flo
 }
 
 size_t mi355_cache_evict_workspace_bytes(const mi355_paged_kv* cache, int budget) {
-    if (!cache || cache->B < 1 || cache->Hkv < 1 || budget < 1 || cache->max_pages < 1 || cache->page_size < 1) return 0;
+    if (!paged_sizes(cache) || budget < 1) return 0;   // (the call is refused)
     return mi355::evict_workspace(*cache, budget);
 }
 

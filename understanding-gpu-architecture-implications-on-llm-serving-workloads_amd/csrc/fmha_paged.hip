@@ -35,6 +35,7 @@ constexpr int NTHREADS = WAVES * 64;
 constexpr int WAVE_BYTES = NSTAGE * STAGE_BYTES;
 constexpr int LDS_BYTES = WAVES * WAVE_BYTES;   // 128 KiB
 constexpr int kMeetBytes = 31 << 10;           // the rest of a CU's 160 KiB, less what the compiler may want
+constexpr int kMostScores = 32;               // columns of a kv head whose scores are kept for the account
 constexpr int COPIES = 2 * (TILE_BYTES / 1024);
 constexpr int WINDOW = 32;                   // tiles whose addresses a wave holds at a time (64 half tiles, one a lane)
 constexpr float kLazyLog2 = 8.f;             // rescale only when a column maximum grows by more than 2^8
@@ -597,7 +598,7 @@ __device__ __forceinline__ void join_parts(const PagedKv& kv, const PagedAttn& a
 // statistics, so that this need not wait for the joining; a pair of one part has it in place.
 __device__ __forceinline__ void add_weights(const PagedKv& kv, const PagedAttn& a, int pair, int chunk) {
     using namespace pdec;
-    __shared__ float lse[32];
+    __shared__ float lse[kMostScores];
     const int tid = threadIdx.x;
     const int b = divide(pair, a.by_hkv), hkv = pair - b * kv.Hkv;
     const int len = paged_len(kv, b);
@@ -691,13 +692,15 @@ static PagedPlan paged_plan(int B, int Hkv, int max_len, int Hq, int Sq, bool we
     // blocks each is cut into fewer (512 rows of 32/8 heads over 8191 keys, 64 blocks: 256 workgroups each 666 us, 4 each 185).
     p.workgroups = p.direct ? (int)pairs : (int)std::min<long>((kWorkgroups + p.blocks - 1) / p.blocks, (pairs * p.max_tiles + kMinTiles - 1) / kMinTiles);
     if (!p.direct) p.part_bytes = sizeof(float) * (size_t)p.blocks * (p.workgroups + pairs) * p.col_block * PART_STRIDE;
-    p.scores = weights && ncols <= 32;
+    p.scores = weights && ncols <= kMostScores;
     const int meet = WAVES * (p.col_block * D + 64) * (int)sizeof(float);
     p.lds = LDS_BYTES + (meet <= kMeetBytes ? meet : 0);
     if (p.scores) p.score_bytes = sizeof(float) * (size_t)pairs * p.max_tiles * ncols * TK;
     if (weights && !lse) p.lse_bytes = (sizeof(float) * (size_t)B * Hq * Sq + 15) & ~size_t(15);
     return p;
 }
+
+bool fmha_paged_keeps_scores(const mi355_paged_kv& c, int Hq, int Sq) { return Hq / c.Hkv * Sq <= pdec::kMostScores; }
 
 size_t fmha_paged_workspace(const mi355_paged_kv& c, int Hq, int Sq, bool lse) {
     const PagedPlan p = paged_plan(c.B, c.Hkv, c.max_pages * c.page_size, Hq, Sq, c.weights != nullptr, lse);

@@ -184,6 +184,8 @@ hipError_t silu_mul_dispatch(const void* in, void* out, long rows, int inter, in
 // The paged key-value cache (arguments as the entry points' after validation). `strides`: q (batch, head, row), o (batch, head, row).
 // `workspace` holds what the *_workspace functions say.
 size_t fmha_paged_workspace(const mi355_paged_kv& cache, int Hq, int Sq, bool lse);
+// whether the account is made from the attention's own scores (otherwise by key_weights_dispatch)
+bool fmha_paged_keeps_scores(const mi355_paged_kv& cache, int Hq, int Sq);
 hipError_t fmha_paged_dispatch(const mi355_paged_kv& cache, const void* Q, void* O, float* LSE, int Hq, int Sq, const long* strides, float scale,
                                void* workspace, hipStream_t stream);
 long key_weights_workgroups(const mi355_paged_kv& cache, int Hq, int Sq, int last_rows);
