@@ -509,6 +509,7 @@ int mi355_fmha_paged(const mi355_paged_kv* cache, const void* Q, void* O, float*
     if (!aligned16(O)) return fail(MI355_ERR_BAD_ARGUMENT, "%s: O must be 16-byte aligned", fn);
     // (the account of many rows is made by mi355_fmha_key_weights' kernel)
     if ((int64_t)cache->B * cache->Hkv * ((int64_t)(Hq / cache->Hkv) * S + (int64_t)cache->max_pages * cache->page_size / 256 + 1) > kMostWorkgroups ||
+        (mi355::fmha_paged_many_rows(*cache, Hq, S) && !mi355::paged_rows_fits(*cache, Hq, S)) ||
         (cache->weights && !mi355::fmha_paged_keeps_scores(*cache, Hq, S) && mi355::key_weights_workgroups(*cache, Hq, S, 0) > kMostWorkgroups / 2))
         return fail(MI355_ERR_UNSUPPORTED, "%s: %d sequences of %d rows over up to %lld keys are more than a call takes", fn, cache->B, S,
                     (long long)cache->max_pages * cache->page_size);

@@ -688,8 +688,7 @@ static PagedPlan paged_plan(int B, int Hkv, int max_len, int Hq, int Sq, bool we
     // over 512 keys 7.9 / 8.5, over 768 9.4 / 8.5, over 1024 11.1 / 8.6; 128 pairs over 512 9.2 / 12.3, over 1024 14.1 / 17.4 (over 2048 23.0 / 26.6, but 17.5 / 9.1 where
     // one sequence is that long and the others short).
     p.direct = max_len <= kDirectLen || (max_len <= 2 * kDirectLen && pairs >= 128);
-    // One workgroup per CU over all blocks of columns: a part has a fixed cost of ~8 us (the first tiles' way, the waves' meeting), so with many
-    // blocks each is cut into fewer (512 rows of 32/8 heads over 8191 keys, 64 blocks: 256 workgroups each 666 us, 4 each 185).
+    // one workgroup per CU over the blocks of columns (two at most where the work is cut)
     p.workgroups = p.direct ? (int)pairs : (int)std::min<long>((kWorkgroups + p.blocks - 1) / p.blocks, (pairs * p.max_tiles + kMinTiles - 1) / kMinTiles);
     if (!p.direct) p.part_bytes = sizeof(float) * (size_t)p.blocks * (p.workgroups + pairs) * p.col_block * PART_STRIDE;
     p.scores = weights && ncols <= kMostScores;
@@ -700,13 +699,23 @@ static PagedPlan paged_plan(int B, int Hkv, int max_len, int Hq, int Sq, bool we
     return p;
 }
 
+// Whether the kernel of fmha_paged_rows.hip, whose waves share the keys, takes a call. This one's blocks of 32 columns walk them again and again, but cost
+// less where there is little to do. us, this kernel / that one, 32/8 heads: 8191 keys, 16 rows 19.1 / 25, 48 rows 53.8 / 28, 512 rows 197 / 94; 8 sequences
+// of 4096 keys, 16 rows 36.4 / 38, 24 rows 93 / 42; 32 of 2048, 16 rows 75 / 59; one of 500 keys, 64 rows 13.8 / 17.8, 300 rows 26.2 / 18.1.
+bool fmha_paged_many_rows(const mi355_paged_kv& c, int Hq, int Sq) {
+    const long ncols = Hq / c.Hkv * Sq, pairs = (long)c.B * c.Hkv;
+    if (ncols <= pdec::kMostScores) return false;
+    if (c.max_pages * c.page_size <= pdec::kDirectLen) return pairs * ((ncols + 31) / 32) > pdec::kWorkgroups;
+    return ncols > 64 || pairs > 64;
+}
+
 bool fmha_paged_keeps_scores(const mi355_paged_kv& c, int Hq, int Sq) { return Hq / c.Hkv * Sq <= pdec::kMostScores; }
 
 size_t fmha_paged_workspace(const mi355_paged_kv& c, int Hq, int Sq, bool lse) {
     const PagedPlan p = paged_plan(c.B, c.Hkv, c.max_pages * c.page_size, Hq, Sq, c.weights != nullptr, lse);
-    size_t key_weights = 0;
-    if (c.weights != nullptr && !p.scores) key_weights = key_weights_workspace(c, Hq, Sq, 0);
-    return std::max(p.part_bytes, key_weights) + p.score_bytes + p.lse_bytes;
+    size_t first = fmha_paged_many_rows(c, Hq, Sq) ? paged_rows_workspace(c, Hq, Sq) : p.part_bytes + p.score_bytes;
+    if (c.weights != nullptr && !p.scores) first = std::max(first, key_weights_workspace(c, Hq, Sq, 0));   // (one behind the other)
+    return first + p.lse_bytes;
 }
 
 template <typename T, int NB, bool SCORES>
@@ -769,7 +778,9 @@ hipError_t fmha_paged_dispatch(const mi355_paged_kv& c, const void* Q, void* O, 
     a.chunks = (kv.max_len + 255) / 256;
     a.by_ncols = divisor_of(a.ncols);
     a.by_chunks = divisor_of(a.chunks);
-    hipError_t e = c.dtype == MI355_DTYPE_BF16 ? fmha_paged_t<bf16_t>(kv, a, p, stream) : fmha_paged_t<half_t>(kv, a, p, stream);
+    hipError_t e = fmha_paged_many_rows(c, Hq, Sq) ? paged_rows_dispatch(c, Q, O, a.LSE, Hq, Sq, strides, scale, ws, stream)
+                   : c.dtype == MI355_DTYPE_BF16      ? fmha_paged_t<bf16_t>(kv, a, p, stream)
+                                                      : fmha_paged_t<half_t>(kv, a, p, stream);
     if (e == hipSuccess && kv.weights != nullptr && !p.scores)   // many rows: from the log-sum-exp, with the scores worked out again
         e = key_weights_dispatch(c, Q, a.LSE, Hq, Sq, strides, 0, scale, ws, stream);
     return e;

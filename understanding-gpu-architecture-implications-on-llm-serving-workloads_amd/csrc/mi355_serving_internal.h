@@ -188,6 +188,12 @@ size_t fmha_paged_workspace(const mi355_paged_kv& cache, int Hq, int Sq, bool ls
 bool fmha_paged_keeps_scores(const mi355_paged_kv& cache, int Hq, int Sq);
 hipError_t fmha_paged_dispatch(const mi355_paged_kv& cache, const void* Q, void* O, float* LSE, int Hq, int Sq, const long* strides, float scale,
                                void* workspace, hipStream_t stream);
+// whether the kernel for many query columns a kv head takes a call (fmha_paged_rows.hip), and whether its tiles can be counted in an int
+bool fmha_paged_many_rows(const mi355_paged_kv& cache, int Hq, int Sq);
+bool paged_rows_fits(const mi355_paged_kv& cache, int Hq, int Sq);
+size_t paged_rows_workspace(const mi355_paged_kv& cache, int Hq, int Sq);
+hipError_t paged_rows_dispatch(const mi355_paged_kv& cache, const void* Q, void* O, float* LSE, int Hq, int Sq, const long* strides, float scale,
+                               void* workspace, hipStream_t stream);
 long key_weights_workgroups(const mi355_paged_kv& cache, int Hq, int Sq, int last_rows);
 size_t key_weights_workspace(const mi355_paged_kv& cache, int Hq, int Sq, int last_rows);
 hipError_t key_weights_dispatch(const mi355_paged_kv& cache, const void* Q, const float* LSE, int Hq, int Sq, const long* q_strides, int last_rows,
