@@ -6,8 +6,8 @@
 // the workgroup that take tiles of 32 keys in turn and meet in LDS at the end. Per 32 keys and wave S^T = K Q^T and O^T += V^T P^T are 32 MFMA 16x16x32 with
 // the queries in registers; four LDS stages, filled by direct-to-LDS copies (each wave copies 8 rows of K and of V of a tile, which lie in one page).
 //
-// Bound by issue: the two waves of a SIMD issue some 400 instructions per 32 keys, of which 64 are the products (2048 rows of 32/8 heads over 8191 keys: 292 us,
-// 824 TFLOP/s, matrix pipes busy 40 % of the time). Their products and exponentials take turns (phases, below), which alone gave nothing before the
+// Bound by issue: the two waves of a SIMD issue some 400 instructions per 32 keys, of which 64 are the products (2048 rows of 32/8 heads over 8191 keys: 300 us,
+// 800 TFLOP/s, matrix pipes busy 40 % of the time). Their products and exponentials take turns (phases, below), which alone gave nothing before the
 // maximum was taken with v_max3 and the steps without masks had a loop of their own (104 -> 94 us for 512 rows). Reading V in front of the exponentials
 // and all of K in front of the products, three stages, one barrier a tile and no phases: 325 us. With masks and what infinities need inside the one
 // loop the registers did not suffice (506 us).
@@ -256,9 +256,7 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
                 }
             }
         };
-        for (int i = 0; i < NSTAGE - 1 && i < n_loc; ++i) issue(i);
-
-        // this wave's columns
+        // this wave's columns; their loads are under way together with the table's
         const int len = seq.len, n_new = seq.n_new;
         const int col0 = block * COLS + cw * WCOLS;
         V8 qf[NB][4];             // Q[column][32 ks + 8 g .. +7]
@@ -278,6 +276,8 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) qf[nb][ks] = *(const V8*)(qp + ks * 32);
         }
+        for (int i = 0; i < NSTAGE - 1 && i < n_loc; ++i) issue(i);
+
 #pragma unroll
         for (int off = 8; off >= 1; off >>= 1) {
             lim_min = min(lim_min, __shfl_xor(lim_min, off, 64));
