@@ -485,6 +485,30 @@ def test_eviction(gpu, lens, budget, recent, page, Hkv, kind):
         assert torch.equal(x.nan_to_num(7.0), y.nan_to_num(7.0))
 
 
+@pytest.mark.parametrize("outliers", [False, True], ids=["", "outliers"])
+@pytest.mark.parametrize("steps", [1, 40, 3000, 1 << 20])
+def test_eviction_of_weights_side_by_side(gpu, steps, outliers):
+    """All within `steps` neighbouring values of 32 bits, so that the border is among many that share their upper bits, and with infinities
+    and zeros so that those are few of the range's."""
+    lens, Hkv = [3000, 700, 9000], 2
+    for budget, recent in ((600, 0), (2900, 300), (1, 0)):
+        cache = Cache(lens, Hkv, 16, seed=3)
+        positions_of(cache, 5)
+        gen = torch.Generator().manual_seed(steps)
+        for b, n in enumerate(lens):
+            pg, sl = cache.at(b)
+            w = (0x3f5a0000 + torch.randint(0, steps, (n, Hkv), generator=gen, dtype=torch.int32)).view(torch.float32)
+            if outliers:
+                w[torch.randperm(n, generator=gen)[:5], 0] = torch.tensor([math.inf, -math.inf, 0.0, -3.0, float("nan")])
+                w[:7, 1] = 0.0
+            cache.weights[pg, :, sl] = w.cuda()
+        want = evicted(cache, budget, recent)
+        got = ops.fine_evict_paged(*cache.args, cache.weights, cache.positions, budget, recent)
+        assert got.tolist() == want[0]
+        for x, y in zip((cache.kv, cache.weights, cache.positions), want[1:]):
+            assert torch.equal(x.nan_to_num(7.0), y.nan_to_num(7.0))
+
+
 def test_eviction_with_positions_of_the_whole_range(gpu):
     cache = Cache([100], 1, 16)
     pg, sl = cache.at(0)

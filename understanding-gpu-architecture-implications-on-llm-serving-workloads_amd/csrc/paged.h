@@ -56,15 +56,34 @@ __device__ __forceinline__ int paged_new(const PagedKv& kv, int b, int S) {
     return kv.new_lens == nullptr ? S : min(max(kv.new_lens[b], 0), S);
 }
 
-// inclusive sum over the lanes of a wave (row shifts inside 16 lanes, then the rows' sums are handed on: 6 additions, no LDS)
-__device__ __forceinline__ int wave_inclusive_sum(int x) {
+// inclusive sum over each 16 lanes of a wave, and over all of them (row shifts inside 16 lanes, then the rows' sums are handed on: 6 additions, no LDS)
+__device__ __forceinline__ int row_inclusive_sum(int x) {
     x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);   // row_shr:1
     x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);   // row_shr:2
     x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);   // row_shr:4
     x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);   // row_shr:8
+    return x;
+}
+__device__ __forceinline__ int wave_inclusive_sum(int x) {
+    x = row_inclusive_sum(x);
     x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
     x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
     return x;
+}
+// the largest of the first 16 lanes' values, and of all lanes', in every lane (likewise)
+__device__ __forceinline__ int row_running_max(int x) {
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x111, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x112, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x114, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x118, 0xf, 0xf, false));
+    return x;
+}
+__device__ __forceinline__ int row_max(int x) { return __builtin_amdgcn_readlane(row_running_max(x), 15); }
+__device__ __forceinline__ int wave_max(int x) {
+    x = row_running_max(x);
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x142, 0xa, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x143, 0xc, 0xf, false));
+    return __builtin_amdgcn_readlane(x, 63);
 }
 
 }  // namespace mi355

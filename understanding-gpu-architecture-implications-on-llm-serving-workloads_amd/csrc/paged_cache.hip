@@ -74,7 +74,8 @@ __global__ __launch_bounds__(pcache::THREADS) void rope_paged_kernel(PagedKv kv,
 // as are dropped (closing ranks would move most of the cache for one dropped key).
 namespace evict {
 constexpr int THREADS = 1024, WAVES = THREADS / 64;
-constexpr int BINS = 2048, COPIES = 4;        // of 11, 11 and 10 bits; of the histogram, a lane's own: many weights are alike in their upper bits
+constexpr int BINS = 2048, COPIES = 2;        // of the histogram, even and odd lanes' own
+constexpr int kCompared = 64;                 // so many keys are compared with one another
 constexpr int kMostChunks = 8;                // of 4 keys whose ranks stay in a thread's registers (32768 keys)
 constexpr int kMovesHere = 256;               // up to this many moves are made by the selecting workgroup
 constexpr int MOVES = 32;                     // of a workgroup of the moving kernel, 8 at a time side by side
@@ -85,6 +86,8 @@ __device__ __forceinline__ uint32_t rank_of(float w) {
     if (w != w) return 0u;
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
+// the lowest n bits, n cut to 0 .. 32
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n > 0 ? (1u << n) - 1u : 0u; }
 constexpr uint32_t kRecent = 0xffffffffu;     // above plus infinity (0xff800000)
 }  // namespace evict
 
@@ -101,18 +104,13 @@ namespace evict {
 
 // sum of one value a thread over the threads in front of this one; `sums` is free again behind the caller's next barrier
 __device__ __forceinline__ int block_before(int x, int (&sums)[WAVES], int& total) {
-    const int incl = wave_inclusive_sum(x), wave = threadIdx.x >> 6;
+    const int incl = wave_inclusive_sum(x), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if ((threadIdx.x & 63) == 63) sums[wave] = incl;
     __syncthreads();
-    int before = incl - x;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-        const int n = sums[w];
-        before += w < wave ? n : 0;
-        total += n;
-    }
-    return before;
+    static_assert(WAVES == 16, "the waves' sums are summed up in a row of lanes");
+    const int waves = row_inclusive_sum(sums[threadIdx.x & 15]);
+    total = __builtin_amdgcn_readlane(waves, 15);
+    return incl - x + (wave > 0 ? __builtin_amdgcn_readlane(waves, wave - 1) : 0);
 }
 
 // Moves n0, n0 + step, .. of those listed: 32 threads a move, four in flight each
@@ -164,15 +162,16 @@ __device__ __forceinline__ void move_keys(const PagedKv& kv, int b, int hkv, Lis
 
 // One workgroup per (sequence, kv head). A thread owns 4 * chunks slots side by side (4 lie in one page and are read with one access), so that
 // what has to be counted in the order of the slots is one sum over the threads. Their ranks stay in M chunks of registers or, M == 0, in
-// the workspace, where only their thread reads them again. Bound by its chain of about twelve steps, a memory round trip or a pass over the
-// workgroup each (128 workgroups, 2176 keys each: loads 1.5 us, ranks 1.1, three passes 1.1 each, what moves 2, 120 moves 3; with positions and weights read by loops and the ranks
-// in LDS it took 13.9 us without the moves).
+// the workspace, where only their thread reads them again. Bound by its chain of about a dozen steps, a memory round trip or a pass over
+// the workgroup each (128 workgroups, 2176 keys each, 13.4 us with a copy of 2.5: length and loads 0.8 us, ranks and their range 0.8, the recent ones 0.6, histogram
+// 1.0, comparing 0.8, what is kept 0.9, lists 0.3, 120 moves 2.3). In registers the keys' comparisons become bits of one word, which took 8192 keys from 24.4 to
+// 21.3 us; adding the waves' sums up in a row of lanes, not by every thread, 0.5 us; three passes of 11, 11 and 10 bits instead of range and comparison 0.4.
 template <int M>
 __global__ __launch_bounds__(evict::THREADS) void evict_select_kernel(PagedKv kv, Evict a) {
     using namespace evict;
-    __shared__ int hist[BINS * COPIES];
+    __shared__ __attribute__((aligned(16))) int hist[BINS * COPIES];
     __shared__ int sums[4][WAVES];
-    __shared__ int found[2];
+    __shared__ int found[3], extent[2][WAVES], near, standing[kCompared];
     __shared__ int list[2][kMovesHere];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int b = divide(blockIdx.x, a.by_hkv), hkv = blockIdx.x - b * kv.Hkv;
@@ -198,6 +197,7 @@ __global__ __launch_bounds__(evict::THREADS) void evict_select_kernel(PagedKv kv
     };
     const auto get = [&](const uint4& v, int e) { return e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w; };
     int newest = INT32_MIN;
+    uint32_t lowest = 0xffffffffu, highest = 0;   // ranks
     const auto load = [&](int c, uint4& r, uint4& p) {
         const int j = min(j0 + 4 * c, kv.max_len - 4), i = divide(j, kv.by_page);
         const int page = table[i];
@@ -210,6 +210,10 @@ __global__ __launch_bounds__(evict::THREADS) void evict_select_kernel(PagedKv kv
         for (int e = 0; e < 4; ++e) {
             x[e] = (there >> e) & 1 ? rank_of(w[e]) : 0u;
             newest = (there >> e) & 1 ? max(newest, (int)get(p, e)) : newest;
+            const bool has = c < chunks && j0 + 4 * c + e < len;   // (in a page of the pool or not)
+            lowest = has ? min(lowest, x[e]) : lowest;
+            highest = max(highest, x[e]);
+            if (M > 0) x[e] = has ? x[e] : kRecent;   // (what the sequence does not have is outside every range)
         }
         r = uint4{x[0], x[1], x[2], x[3]};
         return there;
@@ -226,12 +230,14 @@ __global__ __launch_bounds__(evict::THREADS) void evict_select_kernel(PagedKv kv
             kept_positions[c * THREADS + tid] = p;
         }
     }
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) newest = max(newest, __shfl_xor(newest, off, 64));
-    if (lane == 0) sums[0][wave] = newest;
+    newest = wave_max(newest);
+    const int below = wave_max((int)(~lowest ^ 0x80000000u)), above = wave_max((int)(highest ^ 0x80000000u));
+    if (lane == 0) sums[0][wave] = newest, extent[0][wave] = below, extent[1][wave] = above;
+    if (tid == 0) near = 0;
+    if (tid < kCompared) standing[tid] = 0;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) newest = max(newest, sums[0][w]);
+    newest = row_max(sums[0][lane & 15]);
+    const int bottom = row_max(extent[0][lane & 15]), top = row_max(extent[1][lane & 15]);
     const long old = (long)newest - a.recent;   // positions up to here are not recent
     int recent = 0;
     const auto mark = [&](uint32_t there, uint4& r, const uint4& p) {
@@ -244,22 +250,23 @@ __global__ __launch_bounds__(evict::THREADS) void evict_select_kernel(PagedKv kv
         }
         r = uint4{x[0], x[1], x[2], x[3]};
     };
-    // f(key, rank) for this thread's keys in order
+    // f(key, rank) for this thread's keys in order (from the workspace)
     const auto each = [&](auto&& f) {
-        if constexpr (M > 0) {
+        for (int c = 0; c < chunks && j0 + 4 * c < len; ++c) {
+            const uint4 r = kept_ranks[c * THREADS + tid];
 #pragma unroll
-            for (int c = 0; c < M; ++c)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (c < chunks && j0 + 4 * c + e < len) f(j0 + 4 * c + e, get(rank[c], e));
-        } else {
-            for (int c = 0; c < chunks && j0 + 4 * c < len; ++c) {
-                const uint4 r = kept_ranks[c * THREADS + tid];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (j0 + 4 * c + e < len) f(j0 + 4 * c + e, get(r, e));
-            }
+            for (int e = 0; e < 4; ++e)
+                if (j0 + 4 * c + e < len) f(j0 + 4 * c + e, get(r, e));
         }
+    };
+    // a bit for each of them (in registers) of which f(rank) holds
+    const auto bits_of = [&](auto&& f) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int c = 0; c < REGS; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m |= f(get(rank[c], e)) ? 1u << (4 * c + e) : 0u;
+        return m;
     };
     if constexpr (M > 0) {
 #pragma unroll
@@ -278,72 +285,125 @@ __global__ __launch_bounds__(evict::THREADS) void evict_select_kernel(PagedKv kv
     block_before(recent, sums[1], all_recent);
 
     // The rank of the last kept key, and how many keys of it are kept (`want`, the first ones). The recent ones are counted above (in the
-    // histogram they would all fall on one counter); of the others the want-th largest: 11 bits, 11, then 10.
+    // histogram they would all fall on one counter); of the others the want-th largest: a histogram of their range in 2048 equal bins (of the ranks'
+    // upper 11 bits a few are all that occur, and their counters are waited for), and of its bin, where that holds more than 64 keys, the same
+    // again; 64 keys are compared with one another.
     uint32_t last = kRecent;
     int want = a.budget;
     if (all_recent < a.budget) {
         want -= all_recent;
-        last = 0;
-        for (int pass = 0; pass < 3; ++pass) {
-            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-            const int known = pass == 1 ? 21 : 10;   // bits below those that are known (pass 0: none are)
-            const uint32_t mask = pass == 2 ? 1023u : 2047u;
-            each([&](int, uint32_t r) {
-                if (r != kRecent && (pass == 0 || (r >> known) == last)) atomicAdd(&hist[((r >> shift) & mask) * COPIES + (lane & (COPIES - 1))], 1);
-            });
+        uint32_t base = ~((uint32_t)bottom ^ 0x80000000u), range = ((uint32_t)top ^ 0x80000000u) - base;   // ranks base .. base + range
+        int shift = max(21 - __builtin_clz(range | 1), 0);
+        for (int pass = 0;; ++pass) {
+            const auto count_one = [&](uint32_t r) {
+                if (r - base <= range) atomicAdd(&hist[((r - base) >> shift) * COPIES + (lane & (COPIES - 1))], 1);
+            };
+            if constexpr (M > 0) {
+#pragma unroll
+                for (int c = 0; c < M; ++c)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) count_one(get(rank[c], e));
+            } else {
+                each([&](int, uint32_t r) { count_one(r); });
+            }
             __syncthreads();
             // thread t: the bins 2047 - 2t and 2046 - 2t; sums from the top
             int4v* at = (int4v*)(hist + (BINS - 2 - 2 * tid) * COPIES);
-            const int4v lo = at[0], hi = at[1];
-            at[0] = at[1] = int4v{0, 0, 0, 0};
-            const int h0 = hi[0] + hi[1] + hi[2] + hi[3], h1 = lo[0] + lo[1] + lo[2] + lo[3];
+            const int4v both = *at;
+            *at = int4v{0, 0, 0, 0};
+            const int h0 = both[2] + both[3], h1 = both[0] + both[1];
             int unused;
             const int before = block_before(h0 + h1, sums[2 + (pass & 1)], unused);
-            if (before < want && want <= before + h0) found[0] = BINS - 1 - 2 * tid, found[1] = want - before;
-            else if (before + h0 < want && want <= before + h0 + h1) found[0] = BINS - 2 - 2 * tid, found[1] = want - before - h0;
+            if (before < want && want <= before + h0) found[0] = BINS - 1 - 2 * tid, found[1] = want - before, found[2] = h0;
+            else if (before + h0 < want && want <= before + h0 + h1) found[0] = BINS - 2 - 2 * tid, found[1] = want - before - h0, found[2] = h1;
             __syncthreads();
-            last = pass == 0 ? (uint32_t)found[0] : (last << (pass == 1 ? 11 : 10)) | (uint32_t)found[0];
+            base += (uint32_t)found[0] << shift;
             want = found[1];
+            const int count = found[2];
+            last = base;
+            if (shift == 0) break;
+            range = (1u << shift) - 1;
+            if (count <= kCompared) {
+                if constexpr (M > 0) {
+                    if (bits_of([&](uint32_t r) { return r - base <= range; }) != 0) {
+#pragma unroll
+                        for (int c = 0; c < M; ++c)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (get(rank[c], e) - base <= range) list[0][atomicAdd(&near, 1)] = (int)get(rank[c], e);
+                    }
+                } else {
+                    each([&](int, uint32_t r) {
+                        if (r - base <= range) list[0][atomicAdd(&near, 1)] = (int)r;
+                    });
+                }
+                __syncthreads();
+                // each wave compares them all with four of them: how many are larger, how many equal (16 bits each)
+                const uint32_t mine = (uint32_t)list[0][min(lane, count - 1)];
+                int place = 0;
+#pragma unroll
+                for (int i = 0; i < kCompared / WAVES; ++i) {
+                    const int at = wave * (kCompared / WAVES) + i;
+                    const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)mine, at);
+                    place += at >= count ? 0 : other > mine ? 1 : other == mine ? 1 << 16 : 0;
+                }
+                if (place != 0) atomicAdd(&standing[lane], place);
+                __syncthreads();
+                place = standing[lane];
+                const int larger = place & 0xffff, equal = place >> 16;
+                // (the same of all lanes that hold it, and of all waves)
+                const int who = __builtin_ctzll(__builtin_amdgcn_ballot_w64(larger < want && want <= larger + equal));
+                last = (uint32_t)__builtin_amdgcn_readlane((int)mine, who);
+                want -= __builtin_amdgcn_readlane(larger, who);
+                break;
+            }
+            shift = max(shift - 11, 0);
         }
     }
-    int ties = 0, unused;
-    each([&](int, uint32_t r) { ties += r == last; });
-    const int tie0 = block_before(ties, sums[0], unused);
-    int holes = 0, movers = 0, tie = tie0;
-    each([&](int j, uint32_t r) {
-        const bool keep = r > last || (r == last && tie < want);
-        tie += r == last;
-        holes += !keep && j < a.budget;
-        movers += keep && j >= a.budget;
-    });
-    int total;
-    int hole, mover;
-    if constexpr (M > 0) {   // at most 16384 of each: one sum for both
-        hole = block_before(holes | movers << 16, sums[1], total);
-        mover = hole >> 16;
-        hole &= 0xffff;
-        total &= 0xffff;
-    } else {
-        hole = block_before(holes, sums[1], total);
-        mover = block_before(movers, sums[2], unused);
-    }
+    // Kept are the larger ranks and the first `want` of this one; of the slots in front of the budget those that are not kept are holes, and kept keys
+    // behind it move. `mine`: how many of this thread's own of this rank are kept.
     const bool here = a.cap <= kMovesHere;
-    if (tid == 0) a.counts[blockIdx.x] = here ? 0 : total;
     int* to = a.moves + (long)blockIdx.x * 2 * a.cap;
     int* from = to + a.cap;
-    tie = tie0;
-    each([&](int j, uint32_t r) {
-        const bool keep = r > last || (r == last && tie < want);
-        tie += r == last;
-        if (!keep && j < a.budget) {
-            if (here) list[0][hole++] = j;
-            else to[hole++] = j;
-        }
-        if (keep && j >= a.budget) {
-            if (here) list[1][mover++] = j;
-            else from[mover++] = j;
-        }
-    });
+    int total, unused;
+    if constexpr (M > 0) {
+        const uint32_t have = low_bits(min(len - j0, 4 * chunks)), front = low_bits(a.budget - j0);
+        const uint32_t equal = bits_of([&](uint32_t r) { return r == last; }) & have;
+        uint32_t keep = bits_of([&](uint32_t r) { return r > last; }) & have;
+        int mine = want - block_before(__builtin_popcount(equal), sums[0], unused);
+        for (uint32_t left = equal; left != 0 && mine > 0; left &= left - 1, --mine) keep |= left & -left;
+        uint32_t holes = ~keep & have & front, movers = keep & ~front;
+        // at most 16384 of each: one sum for both
+        const int before = block_before(__builtin_popcount(holes) | __builtin_popcount(movers) << 16, sums[1], total);
+        total &= 0xffff;
+        int* hole = (here ? list[0] : to) + (before & 0xffff);
+        int* mover = (here ? list[1] : from) + (before >> 16);
+        for (; holes != 0; holes &= holes - 1) *hole++ = j0 + __builtin_ctz(holes);
+        for (; movers != 0; movers &= movers - 1) *mover++ = j0 + __builtin_ctz(movers);
+    } else {
+        int ties = 0;
+        each([&](int, uint32_t r) { ties += r == last; });
+        const int tie0 = block_before(ties, sums[0], unused);
+        const auto keeps = [&](uint32_t r, int& tie) {
+            const bool keep = r > last || (r == last && tie < want);
+            tie += r == last;
+            return keep;
+        };
+        int holes = 0, movers = 0, tie = tie0;
+        each([&](int j, uint32_t r) {
+            const bool keep = keeps(r, tie);
+            holes += !keep && j < a.budget;
+            movers += keep && j >= a.budget;
+        });
+        int hole = block_before(holes, sums[1], total), mover = block_before(movers, sums[2], unused);
+        tie = tie0;
+        each([&](int j, uint32_t r) {
+            const bool keep = keeps(r, tie);
+            if (!keep && j < a.budget) (here ? list[0] : to)[hole++] = j;
+            if (keep && j >= a.budget) (here ? list[1] : from)[mover++] = j;
+        });
+    }
+    if (tid == 0) a.counts[blockIdx.x] = here ? 0 : total;
     if (!here) return;
     __syncthreads();
     for (int n = 0; n < total; n += 4 * THREADS / 32) move_keys(kv, b, hkv, list[0], list[1], n + (tid >> 5), THREADS / 32, total);
