@@ -61,6 +61,9 @@ CASES = [   # Hq, Hkv, S, page, lengths, new_lens, options
     (8, 4, 20, 16, [(97 * i) % 1100 for i in range(20)], None, {}),                       # more pairs than CUs could take in turn
     (32, 32, 130, 16, [700, 900, 130], [130, 100, 60], {}),                               # 192 triples: joined at the borders
     (32, 8, 512, 32, [1500, 513, 600, 2000], None, {}),                                   # workgroups of 256 columns
+    (32, 8, 512, 32, [600] * 7 + [550], [512] * 6 + [500, 512], {}),                      # whole triples in turn, two a workgroup
+    (32, 8, 128, 16, [1000, 1010, 990, 1000, 1000, 960, 1001, 999], None, {}),            # the same with two halves
+    (32, 8, 1000, 32, [2000], None, {}),                                                  # one sequence, a workgroup a triple
     (64, 8, 520, 64, [700, 520, 530, 0, 1000, 600, 521, 522], None, {}),                  # more triples than are cut
     (40, 8, 65, 16, [100, 480, 65, 20], [65, 65, 3, 65], {"max_pages": 32}),              # short ones, a workgroup each
     (32, 8, 500, 32, [500], None, {}),                                                    # a prompt from its start

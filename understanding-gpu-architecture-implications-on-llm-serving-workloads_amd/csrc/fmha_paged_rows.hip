@@ -15,7 +15,8 @@
 // The (block of columns, sequence, kv head) triples lie one behind the other on one axis, each with the tiles that its rows see (lengths are known to the device
 // only) and a head that stands for what a part costs beside them, and each of up to 256 workgroups takes an equal piece. A triple that a workgroup
 // walks alone is written out at once; the parts of the others go to the workspace, two for a workgroup at most (its first part and its last), and
-// paged_rows_join_kernel adds them up in order. Short sequences, and many triples, get a workgroup a triple and nothing to join.
+// paged_rows_join_kernel adds them up in order. Where triples of much the same length come out even, whole ones are dealt out in turn; short sequences,
+// one sequence of many rows, and many triples get a workgroup a triple and nothing to join.
 #include <algorithm>
 #include <type_traits>
 
@@ -105,16 +106,28 @@ struct Entries {
         keys = e0 + lane < a.entries ? seen.keys : 0;
         incl = wave_inclusive_sum(units_of(keys));
     }
-    // units (tiles and heads) of all, and of a workgroup
-    __device__ __forceinline__ int total() {
-        int n = 0;
+    // units (tiles and heads) of all, and the most of a triple
+    struct Sum {
+        int total, most;
+    };
+    __device__ __forceinline__ Sum sum() {
+        int n = 0, most = 0;
         for (int e0 = 0; e0 < a.entries; e0 += 64) {
             load(e0);
             n += __builtin_amdgcn_readlane(incl, 63);
+            most = max(most, wave_max(units_of(keys)));
         }
-        return n * kv.Hkv;
+        return {n * kv.Hkv, most};
     }
-    __device__ __forceinline__ int quota(int n) const { return max((int)((uint32_t)(n + a.workgroups - 1) / (uint32_t)a.workgroups), kMinKeys / TK); }
+    __device__ __forceinline__ int quota(const Sum& s) const {
+        return max((int)((uint32_t)(s.total + a.workgroups - 1) / (uint32_t)a.workgroups), kMinKeys / TK);
+    }
+    // whether whole triples, dealt to the workgroups in turn, take at most a quarter longer than equal pieces, which cost their parts' way through the
+    // workspace (8 x 512 rows of 32/8 heads over 2048 keys 162 us, cut 190; 8 x 128 over 1024 31 / 44)
+    __device__ __forceinline__ bool in_turn(const Sum& s) const {
+        const int rounds = (int)((uint32_t)(a.entries * kv.Hkv + a.workgroups - 1) / (uint32_t)a.workgroups);
+        return 4L * rounds * s.most <= 5L * (s.total / a.workgroups);
+    }
     struct Where {
         int e, len, n_new, keys, tiles, units, before;   // before: units of the entries in front, per kv head
     };
@@ -169,16 +182,31 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
     // This workgroup's piece of the axis: unit `at` of triple (seq.e, hkv) and the following ones
     Entries<COLS> entries(kv, a);
     typename Entries<COLS>::Where seq;
-    int hkv, at = 0, f = 0, f_end = 1;
-    if (a.direct) {   // (the blocks with the most keys first)
-        const int triple = a.entries * kv.Hkv - 1 - blockIdx.x, e = divide(triple, a.by_hkv);
-        hkv = triple - e * kv.Hkv;
-        entries.load(e);
-        seq = entries.pick(0, 0);
-    } else {
-        const int total = entries.total(), quota = entries.quota(total);
+    int hkv, at = 0, f = 0, f_end = 0;   // (whole triples: f counts them down, the blocks with the most keys first, f_end is the step)
+    bool whole = a.direct;
+    const auto take = [&]() {
+        const int e = divide(f, a.by_hkv);
+        hkv = f - e * kv.Hkv;
+        if (a.direct) {
+            entries.load(e);
+            seq = entries.pick(0, 0);
+        } else {
+            seq = entries.at(e);
+        }
+    };
+    if (!whole) {
+        const auto sum = entries.sum();
+        whole = entries.in_turn(sum);
+        const int quota = entries.quota(sum);
         f = blockIdx.x * quota;
-        f_end = min(f + quota, total);
+        f_end = min(f + quota, sum.total);
+    }
+    if (whole) {
+        f = a.entries * kv.Hkv - 1 - blockIdx.x;
+        f_end = a.workgroups;
+        if (f < 0) return;
+        take();
+    } else {
         if (f >= f_end) return;
         seq = entries.find(f);
         hkv = (int)((uint32_t)(f - seq.before * kv.Hkv) / (uint32_t)seq.units);
@@ -201,7 +229,7 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
 
     for (;;) {
         const int block = divide(seq.e, a.by_batch), b = seq.e - block * kv.B;
-        const int units = a.direct ? seq.units : min(seq.units - at, f_end - f);
+        const int units = whole ? seq.units : min(seq.units - at, f_end - f);
         const int tile0 = max(at - Entries<COLS>::HEAD, 0), n = at + units - Entries<COLS>::HEAD - tile0;   // (units of the head alone: nothing)
         if (n <= 0 && seq.units > 0) return;
         const int n_loc = max((n - kg + KG - 1) / KG, 0);   // tiles kg, kg + KG, .. of the part
@@ -530,7 +558,7 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
             __syncthreads();
         }
         if (kg == 0) {
-            if (n == seq.tiles || a.direct) {
+            if (n == seq.tiles || whole) {
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
                     const int col = col0 + 16 * nb + c16;
@@ -559,8 +587,14 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
                 }
             }
         }
+        if (whole) {
+            f -= f_end;
+            if (f < 0) return;
+            take();
+            continue;
+        }
         f += units;
-        if (a.direct || units <= 0 || f >= f_end) return;   // (nothing done ends the walk even where lengths change under the call)
+        if (units <= 0 || f >= f_end) return;   // (nothing done ends the walk even where lengths change under the call)
         ++parts;
         at = 0;
         if (++hkv == kv.Hkv) {
@@ -600,7 +634,9 @@ __global__ __launch_bounds__(256) void paged_rows_join_kernel(PagedKv kv, RowsAt
         return;
     }
     const int join = blockIdx.x / CW, cw = blockIdx.x % CW;
-    const int total = entries.total(), quota = entries.quota(total);
+    const auto sum = entries.sum();
+    if (entries.in_turn(sum)) return;
+    const int total = sum.total, quota = entries.quota(sum);
     typename Entries<COLS>::Where seq;
     int hkv;
     if (a.few) {   // a triple
@@ -678,9 +714,11 @@ static Plan plan_of(const mi355_paged_kv& c, int Hq, int Sq) {
     const int cols = 256 / p.kg, tk = 64 / p.kg;
     p.blocks = (ncols + cols - 1) / cols;
     p.units = pairs * p.blocks * ((max_len + tk - 1) / tk + kHeadKeys / tk);
-    // us, a workgroup a triple / cut: 500 rows over 500 keys 18 / 73, 8 x 1024 rows over 2048 247 / 288
-    p.direct = max_len <= kDirectLen || pairs * p.blocks >= kDirectTriples;
-    p.workgroups = p.direct ? (int)(pairs * p.blocks) : (int)std::min<long>(kWorkgroups, p.units / (kMinKeys / tk) + 1);
+    // us, a workgroup a triple / cut: 500 rows over 500 keys 18 / 73, 8 x 1024 rows over 2048 247 / 288, one sequence (whose triples are of nearly one
+    // length) of 2048 rows over 8191 300 / 320, of 1000 rows over 2000 42.7 / 58.5
+    const long triples = pairs * p.blocks, rounds = (triples + kWorkgroups - 1) / kWorkgroups;
+    p.direct = max_len <= kDirectLen || triples >= kDirectTriples || (c.B == 1 && 10 * triples >= 9 * rounds * kWorkgroups);
+    p.workgroups = p.direct ? (int)triples : (int)std::min<long>(kWorkgroups, p.units / (kMinKeys / tk) + 1);
     p.bytes = p.direct ? 0 : sizeof(float) * 2 * (size_t)p.workgroups * (WAVES / p.kg) * PART_FLOATS;
     return p;
 }
