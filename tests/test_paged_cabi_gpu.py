@@ -93,3 +93,37 @@ def test_filing_and_eviction(gpu, dtype):
     left = ops.fine_evict_paged(kv, table, lens, weights, positions, 128, 32)
     assert torch.equal(out, left) and out.tolist() == [128, 40, 128]
     assert torch.equal(mine[0], kv) and torch.equal(mine[1], weights) and torch.equal(mine[2], positions)
+
+
+@pytest.mark.parametrize("S", [2, 40])
+def test_scales_of_every_size(gpu, S):
+    """From one that makes all scores alike (the mean of the values that a row sees) to one that leaves the largest score alone."""
+    c = lib.load()
+    kv, table, lens, _, _ = pool(torch.float16, [700, 60])
+    B, Hq, Hkv, page = 2, 8, 2, 16
+    q = torch.randn(B, Hq, S, D, generator=torch.Generator().manual_seed(4)).half().cuda()
+    cache = lib.paged_kv(kv, table, lens)
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    size = c.mi355_fmha_paged_workspace_bytes(ctypes.byref(cache), Hq, S, 1)
+    for scale in (1e-38, 1e-30, 1e-6, 50.0, 1e6):
+        o, lse, ws = torch.empty_like(q), torch.empty(B, Hq, S, device="cuda"), workspace(size)
+        run(c.mi355_fmha_paged, ctypes.byref(cache), ptr(q), ptr(o), ptr(lse), Hq, S, None, scale, ptr(ws), size, stream)
+        for b, n in enumerate([700, 60]):
+            j = torch.arange(n, device="cuda")
+            x = kv[table[b].long()[j // page], :, j % page].double().repeat_interleave(Hq // Hkv, 1).transpose(0, 1)   # [2 Hq, n, D]
+            s = torch.matmul(q[b].double(), x[:Hq].transpose(1, 2).contiguous())
+            seen = j[None] <= torch.arange(S, device="cuda")[:, None] + n - S
+            if scale < 1e-5:   # the largest |score| is below 80: probabilities are alike but for 1.6e-4 of themselves, rounded to 16 bits (2^-11), and so is their mean
+                mean = torch.matmul(seen.double(), x[Hq:]) / seen.sum(1)[:, None]
+                spread = torch.matmul(seen.double(), x[Hq:].abs()) / seen.sum(1)[:, None]
+                assert ((o[b].double() - mean).abs() <= (2 * 2.0 ** -11 + 2e-4) * spread + 2.0 ** -11 * mean.abs() + 2.0 ** -24).all()
+                assert ((lse[b].double() - seen.sum(1).double().log()).abs() <= 2e-4).all()
+            else:              # rows whose two largest scores are more than 25 apart, after scaling, have the value of the first: the others have e^-25 n of the sum
+                top = torch.where(seen, s, -1e30).topk(2, -1)
+                alone = (top.values[..., 0] - top.values[..., 1]) * scale > 25
+                first = torch.gather(x[Hq:], 1, top.indices[..., :1].expand(-1, -1, D))
+                assert alone.float().mean() > 0.5
+                # its probability is 2^x against the exponent's reference, which may be any of the row's maxima so far (x up to 8): rounded to 16 bits in the
+                # product (2^-11), not in the sum; the quotient is rounded once more (2^-11)
+                assert ((o[b].double() - first).abs() <= 2.001 * 2.0 ** -11 * first.abs() + 1e-6)[alone].all()
+                assert torch.isfinite(o[b]).all()

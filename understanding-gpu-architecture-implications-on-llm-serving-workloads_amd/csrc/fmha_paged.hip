@@ -171,6 +171,7 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
         f_end = min(f + cut.quota, cut.total);
         if (f >= f_end) return;
         now.seq = lengths.find(f);
+        if (now.seq.tiles == 0) return;   // (where lengths change under the call)
         const int rest = f - now.seq.before * kv.Hkv;
         now.hkv = (int)((uint32_t)rest / (uint32_t)now.seq.tiles);
         now.tile0 = rest - now.hkv * now.seq.tiles;

@@ -209,6 +209,7 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
     } else {
         if (f >= f_end) return;
         seq = entries.find(f);
+        if (seq.units == 0) return;   // (where lengths change under the call)
         hkv = (int)((uint32_t)(f - seq.before * kv.Hkv) / (uint32_t)seq.units);
         at = f - seq.before * kv.Hkv - hkv * seq.units;
     }
@@ -325,7 +326,7 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
         float4v o[NB][8];
         // exponent reference of the running sums, the score above which it moves, -reference * scale
         float m_run[NB], m_top[NB], neg_ms[NB], l_run[NB];
-        const float margin = kLazyLog2 / a.scale_log2;
+        const float margin = fminf(kLazyLog2 / a.scale_log2, 3.0e38f);   // (finite: minus infinity stays that)
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             m_run[nb] = m_top[nb] = -INFINITY;
@@ -647,6 +648,7 @@ __global__ __launch_bounds__(256) void paged_rows_join_kernel(PagedKv kv, RowsAt
     } else {       // a border
         if (join == 0 || join * quota >= total) return;
         seq = entries.find(join * quota);
+        if (seq.units == 0) return;
         hkv = (int)((uint32_t)(join * quota - seq.before * kv.Hkv) / (uint32_t)seq.units);
     }
     const int f0 = seq.before * kv.Hkv + hkv * seq.units, first = (int)((uint32_t)(f0 + Entries<COLS>::HEAD) / (uint32_t)quota);
