@@ -420,6 +420,45 @@ def test_rows_that_saw_nothing_and_masked_nan_add_nothing(gpu):
     assert torch.equal(w3[pg[:-1], :, sl[:-1]], w[pg[:-1], :, sl[:-1]]) and w3[pg[-1], :, sl[-1]].isnan().all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("Hq,Hkv,S,page,lens,new,last", [
+    (4, 2, 10, 16, [90], None, 0),                                 # one tile of 10 rows, masked and not
+    (8, 2, 200, 16, [700, 200], [200, 150], 0),
+    (2, 1, 300, 16, [300], None, 100),
+    (8, 8, 640, 32, [2000] * 8, None, 0),                          # workgroups of four waves, several ranges
+])
+def test_rows_taken_out_of_an_account_add_nothing_whatever_they_scored(gpu, Hq, Hkv, S, page, lens, new, last, dtype):
+    """LSE = -inf takes a row out: an infinite score of it, or a NaN, leaves the weights as they are without the row."""
+    cache, clean = Cache(lens, Hkv, page, dtype), Cache(lens, Hkv, page, dtype)
+    q = queries(cache, Hq, S)
+    n = None if new is None else torch.tensor(new, dtype=torch.int32, device="cuda")
+    out = torch.arange(S) % 3 == 1
+    # the key at 2 is infinite in one direction: scores of the rows taken out are +inf, the others' -inf
+    size = q[..., 0].abs() + 0.5
+    q[..., 0] = torch.where(out.cuda(), size, -size)
+    for b in range(len(lens)):
+        pg, sl = cache.at(b)
+        cache.kv[pg[2], :Hkv, sl[2]] = 0
+        cache.kv[pg[2], :Hkv, sl[2], 0] = math.inf
+    _, lse = ops.fine_fmha_paged_with_lse(q, *clean.args, new_lens=n)
+    lse[:, :, out] = -math.inf
+    before, w, want = cache.weights.clone(), cache.weights.clone(), cache.weights.clone()
+    ops.fine_key_weights(q, lse, *cache.args, w, new_lens=n, last_rows=last)
+    ops.fine_key_weights(q, lse, *clean.args, want, new_lens=n, last_rows=last)
+    for b in range(len(lens)):
+        pg, sl = cache.at(b)
+        want[pg[2], :, sl[2]] = before[pg[2], :, sl[2]]            # (the other rows' probability of that key is nothing)
+    assert torch.equal(w.nan_to_num(7.0), want.nan_to_num(7.0))
+    for b in range(len(lens)):
+        pg, sl = cache.at(b)
+        cache.kv[pg[0], :Hkv, sl[0]] = math.nan
+        cache.kv[pg[-1], :Hkv, sl[-1]] = -math.inf
+    lse.fill_(-math.inf)
+    w = before.clone()
+    ops.fine_key_weights(q, lse, *cache.args, w, new_lens=n, last_rows=last)
+    assert torch.equal(w.nan_to_num(7.0), before.nan_to_num(7.0))
+
+
 # ---- eviction ------------------------------------------------------------------------------------------------------------
 
 

@@ -5,7 +5,7 @@
 // over the rows i < new (or the last `last_rows` of them) that see the key, j <= i + len - new. LSE is what the attention left: no
 // maximum is searched and no probability is written, so the work is one product (MFMA) and an exponential a (row, key).
 //
-// Bound by issue: of the 2440 cycles that a SIMD takes per 64 keys x 64 rows (2 x 32/8 heads, 4096 rows, causal: 160 us, 860 TFLOP/s), the matrix
+// Bound by issue: of the 2340 cycles that a SIMD takes per 64 keys x 64 rows (2 x 32/8 heads, 4096 rows, causal: 154 us, 890 TFLOP/s), the matrix
 // pipe is busy 1024 and the vector unit 1400 (a multiply-add, an exponential and an addition a score, 224 instructions), and the two
 // hardly overlap: a software pipeline of product and exponentials took 162 us, 32x32x16 instructions (2 waves to a SIMD instead of 3) 177.
 //
@@ -72,6 +72,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void key_weights_kernel(PagedKv kv, 
     constexpr int COPIES = 16 / WAVES;                     // of 4 rows, of a wave and tile
     __shared__ __attribute__((aligned(1024))) char smem[NSTAGE * STAGE_BYTES];
     __shared__ float refs[kMaxTiles * ROWS];   // the exponents' offsets of the range's rows
+    __shared__ int taken_out;                  // whether the LSE of one of them is -inf
     MI355_LDS char* lds = (MI355_LDS char*)smem;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -125,13 +126,18 @@ __global__ __launch_bounds__(WAVES * 64, 2) void key_weights_kernel(PagedKv kv, 
         const int q_base = c16 * 256 + ((g ^ c16) << 4);   // xor (ks << 6), + 16 cb rows
         issue(t_begin, 0);
         if (t_begin + 1 < t_end) issue(t_begin + 1, 1);
-        // All rows' offsets up front (a load among the copies would be waited for together with them). A row that sees no key (or is none)
-        // adds nothing: 2^(x - inf) = 0
+        // All rows' offsets up front (a load among the copies would be waited for together with them). A row whose LSE is -inf (or that is none)
+        // adds nothing: 2^(x - inf) = 0. That holds for a finite x alone, so a range with such an LSE takes the body with comparisons below (a row that is
+        // none repeats the first one, whose own term is not finite either where this one is not)
+        // (a flag of each wave's own, which needs no barrier in front of the loop: 2 x 32/8 heads, 4096 rows 156.3 us, this way 153.7, without a flag 155.7)
+        if (threadIdx.x == 0) taken_out = 0;
+        __syncthreads();
         for (int r = threadIdx.x; r < (t_end - t_begin) * ROWS; r += WAVES * 64) {
             const int t = t_begin + r / ROWS, back = divide(t, a.by_group), hq = hkv * a.group + t - back * a.group;
             const int row = n_new - (back + 1) * ROWS + r % ROWS;
             const float lse = row >= first ? LSE[(long)hq * a.Sq + row] : -INFINITY;
             refs[r] = lse == -INFINITY ? -INFINITY : -lse * 1.4426950408889634f;
+            if (row >= first && lse == -INFINITY) taken_out = 1;
         }
         // this wave's keys: lane holds K[16 kb + c16][32 ks + 8 g .. +7]; keys behind the last repeat it, those of a page outside the
         // pool read its first one (neither is written out)
@@ -149,6 +155,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void key_weights_kernel(PagedKv kv, 
             for (int ks = 0; ks < 4; ++ks) kf[kb][ks] = *(const V8*)(p + 64 * ks);
         }
         int slot = 0;
+        __syncthreads();
+        // a tile from this row on needs no comparisons
+        const int plain_from = __builtin_amdgcn_readfirstlane(taken_out) != 0 ? INT32_MAX : key0 + KEYS - 1 - shift;
         for (int t = t_begin; t < t_end; ++t) {
             if (t + 1 < t_end) wait_vmcnt<COPIES>();   // everything but the newest tile has landed
             else wait_vmcnt<0>();
@@ -158,8 +167,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void key_weights_kernel(PagedKv kv, 
             MI355_LDS char* st = lds + slot * STAGE_BYTES;
             const float* ref_of = refs + (t - t_begin) * ROWS;
             slot = slot == NSTAGE - 1 ? 0 : slot + 1;
-            // 16 rows against this wave's 64 keys, four times. MASKED: the tile holds rows that do not see all of them (a body of its own:
-            // the comparisons would double the vector instructions of the others)
+            // 16 rows against this wave's 64 keys, four times. MASKED: the tile holds rows that do not see all of them, or add nothing (a body of its
+            // own: the comparisons would double the vector instructions of the others)
             const auto tile = [&](auto mask) {
 #pragma unroll
                 for (int cb = 0; cb < 4; ++cb) {
@@ -175,7 +184,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void key_weights_kernel(PagedKv kv, 
                     for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
                         for (int kb = 0; kb < NKB; ++kb) s[kb] = Elem<T>::mfma16(kf[kb][ks], qf[ks], s[kb]);
-                    const int seen = row + 16 * cb + c16 + shift - key0 - 4 * g;   // of this lane's keys 16 kb + e, those up to here are seen
+                    // of this lane's keys 16 kb + e, those up to here count
+                    const int seen = ref == -INFINITY ? -1 : row + 16 * cb + c16 + shift - key0 - 4 * g;
 #pragma unroll
                     for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
@@ -186,7 +196,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void key_weights_kernel(PagedKv kv, 
                         }
                 }
             };
-            if (row + shift >= key0 + KEYS - 1) tile(std::false_type{});
+            if (row >= plain_from) tile(std::false_type{});
             else if (row + ROWS - 1 + shift >= key0) tile(std::true_type{});   // (a tile none of whose rows sees these keys is passed over)
         }
 #pragma unroll
