@@ -201,6 +201,25 @@ def test_what_a_row_does_not_see_has_no_influence(gpu):
         assert o[:, :, -1].isnan().all()
 
 
+@pytest.mark.parametrize("S,lens", [(4, [300]), (4, [5000, 70]), (3, [40, 1]), (40, [900])])
+def test_a_row_of_nan_leaves_the_account_of_keys_that_it_does_not_see(gpu, S, lens):
+    cache = Cache(lens, 2, 16)
+    q = queries(cache, 8, S)
+    w, want = cache.weights.clone(), cache.weights.clone()
+    ops.fine_fmha_paged_with_lse(q, *cache.args, weights=want)
+    q[:, :, 0] = math.nan
+    o, lse = ops.fine_fmha_paged_with_lse(q, *cache.args, weights=w)
+    for b, n in enumerate(lens):
+        pg, sl = cache.at(b)
+        seen = max(n - S + 1, 0)                                   # keys of the first row
+        assert o[b, :, 0].isnan().all() if seen else (o[b, :, 0] == 0).all()
+        assert torch.isfinite(o[b, :, max(S - n, 0) + (seen > 0):]).all()
+        assert w[pg[:seen], :, sl[:seen]].isnan().all()
+        # of the others' sums, up to 160 probabilities of at most one: the exponent's reference may be another one, which moves each by 2^-16 of itself
+        got, ref = w[pg[seen:], :, sl[seen:]], want[pg[seen:], :, sl[seen:]]
+        assert ((got - ref).abs() <= 160 * 2.0 ** -16).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
 def test_pages_outside_the_pool_hold_no_keys(gpu, dtype):
     lens = [300, 700, 64]

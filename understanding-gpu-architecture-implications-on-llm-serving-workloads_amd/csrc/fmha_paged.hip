@@ -648,12 +648,20 @@ __device__ __forceinline__ void add_weights(const PagedKv& kv, const PagedAttn& 
     __syncthreads();
     if (!there) return;
     float sum = 0.f;
-    // a row that sees no key adds nothing
-    const auto add = [&](int c, float x) { sum += lse[c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(x, a.scale_log2, -lse[c])); };
+    // a row that does not see the key adds nothing, whatever its log-sum-exp is
+    const auto add = [&](int c, float x) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x, a.scale_log2, -lse[c]));
+        sum += x == -INFINITY ? 0.f : p;
+    };
+    for (int c0 = 0;;) {
 #pragma unroll
-    for (int c = 0; c < AHEAD; ++c)
-        if (c < a.ncols) add(c, s[c]);
-    for (int c = AHEAD; c < a.ncols; ++c) add(c, sp[c * TK]);
+        for (int c = 0; c < AHEAD; ++c)
+            if (c0 + c < a.ncols) add(c0 + c, s[c]);
+        c0 += AHEAD;
+        if (c0 >= a.ncols) break;
+#pragma unroll
+        for (int c = 0; c < AHEAD; ++c) s[c] = sp[min(c0 + c, a.ncols - 1) * TK];
+    }
     *w = old + sum;
 }
 
