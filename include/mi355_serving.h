@@ -313,7 +313,8 @@ int mi355_fmha_fwd_noalloc(const void* Q, const void* K, const void* V, void* O,
  * Lengths, table and positions are read on the device: no call waits for it, and a captured call serves what the tensors hold when it
  * is replayed (they must not change while a call runs). No page may belong to two sequences of a call that writes it, to its weights among others.
  * Launches and workspaces are sized for max_pages, whatever the lengths are: a caller whose table is much wider than its sequences are long passes
- * the columns in use. B * Hkv <= 65535, max_pages * page_size <= 2^28.
+ * the columns in use. B * Hkv <= 65535, max_pages * page_size <= 2^28, B * Hkv * (max_pages * page_size / 32 + 1) < 2^31 - 2^16; the strides of rows
+ * below 2^24 elements, those of a page's rows together below 2^30.
  *
  * The library allocates nothing for these calls: what *_workspace_bytes says (0: NULL will do) is the caller's, 16-byte aligned, its
  * contents irrelevant before and after; calls that share a workspace must be ordered on one stream. The reference has no counterpart: its caller grows
@@ -338,7 +339,8 @@ typedef struct mi355_paged_kv {
  * Where cache->weights is given, each key's probabilities, summed over the query heads of its kv head and the rows, are added to
  * it. Sums and statistics are fp32, in an order that depends on the sizes and lengths alone; the probabilities are rounded to the element type for
  * the second product. What a row does not see has no influence on it, infinities and NaN included. new_lens of NULL with S rows and
- * a sequence shorter than S: its first rows see nothing.
+ * a sequence shorter than S: its first rows see nothing. Hq / Hkv * S < 2^24 (2^16 where S is more than max_pages * page_size), and
+ * B * Hq * S + B * Hkv * (max_pages * page_size / 256 + 1) < 2^24.
  */
 size_t mi355_fmha_paged_workspace_bytes(const mi355_paged_kv* cache, int Hq, int S, int want_lse);
 int mi355_fmha_paged(const mi355_paged_kv* cache, const void* Q, void* O, float* LSE, int Hq, int S, const int64_t* strides, float scale,
@@ -357,7 +359,8 @@ int mi355_rope_paged(const mi355_paged_kv* cache, void* qkv, int S, int q_heads,
 /*
  * What a prompt's rows attended to: for every key, cache->weights += the sum over the query heads of its kv head and the rows that see it of
  * exp(scale * q k - LSE), LSE [B, Hq, S] being what the attention over the same keys left. last_rows > 0: only the last `last_rows` tokens of
- * each sequence count. Rows whose LSE is -inf add nothing. q_strides: batch, head, row (NULL: contiguous [B, Hq, S, 128]).
+ * each sequence count. Rows whose LSE is -inf add nothing. q_strides: batch, head, row (NULL: contiguous [B, Hq, S, 128]). Hq / Hkv times the
+ * rows that count < 2^24 (2^16 where they are more than max_pages * page_size), S <= 2^28.
  */
 size_t mi355_fmha_key_weights_workspace_bytes(const mi355_paged_kv* cache, int Hq, int S, int last_rows);
 int mi355_fmha_key_weights(const mi355_paged_kv* cache, const void* Q, const float* LSE, int Hq, int S, const int64_t* q_strides,

@@ -89,6 +89,26 @@ def test_an_account_of_more_rows_than_a_launch_takes_is_refused(lib):
     assert b"more than a call takes" in cdll.mi355_last_error()
 
 
+def test_prompts_of_many_heads_and_tokens_are_taken(lib):
+    """The workspaces of calls of 65536 query columns a kv head and more are sized, and only a missing one is refused."""
+    cdll = lib.load()
+    for Hq, Hkv, S, last, pages in ((64, 8, 8192, 0, 512), (32, 8, 16384, 0, 1024), (32, 1, 2048, 0, 128), (64, 8, 8192, 64, 512), (32, 8, 1 << 20, 5, 1 << 16)):
+        c = cache(lib, B=1, Hkv=Hkv, max_pages=pages, table_stride=pages)
+        if last == 0:
+            need = cdll.mi355_fmha_paged_workspace_bytes(c, Hq, S, 1)
+            assert 0 < need < 1 << 32
+            assert cdll.mi355_fmha_paged(c, P, P, P, Hq, S, None, 0.1, None, need, None) == lib.ERR_BAD_ARGUMENT and b"workspace" in cdll.mi355_last_error()
+        need = cdll.mi355_fmha_key_weights_workspace_bytes(c, Hq, S, last)
+        assert (need > 0 or last > 0) and need < 1 << 32
+        if need:
+            assert cdll.mi355_fmha_key_weights(c, P, P, Hq, S, None, last, 0.1, None, need, None) == lib.ERR_BAD_ARGUMENT and b"workspace" in cdll.mi355_last_error()
+    # more rows than a sequence has keys, more columns than there may be
+    for Hq, S, last in ((64, 8193, 0), (8, 1 << 16, 0), (8, (1 << 28) + 1, 1)):
+        c = cache(lib, B=1, Hkv=8, max_pages=512, table_stride=512)
+        assert cdll.mi355_fmha_key_weights(c, P, P, Hq, S, None, last, 0.1, P, 1 << 60, None) == lib.ERR_UNSUPPORTED
+        assert cdll.mi355_fmha_key_weights_workspace_bytes(c, Hq, S, last) == 0
+
+
 def test_the_other_entry_points_refuse_bad_arguments(lib):
     cdll, c, big = lib.load(), cache(lib), 1 << 60
     row = 48 * 128

@@ -119,6 +119,19 @@ def test_steps_with_eviction_attend_to_what_is_kept(gpu):
     assert cache.lengths == [65, 64] and cache.positions == [151, 70] and cache.seq_lens.tolist() == [65, 64]
 
 
+def test_a_long_prompt_of_many_heads_with_an_account(gpu):
+    """8192 tokens of 64 query heads on 8 kv heads, as without an account; each row spreads a weight of one a head."""
+    H, n_q, n_kv, F, S = 512, 64, 8, 1024, 8192
+    layer = FineLlamaDecoderLayer({k: v.to(gpu) for k, v in layer_weights(H, n_q, n_kv, F, seed=90).items()}, n_q, n_kv, max_positions=S)
+    x = so.randn_fp16((1, S, H), 5).to(gpu)
+    caches = [FinePagedKVCache(1, S // 64, n_kv, page_size=64, device=gpu, account=account) for account in (False, True)]
+    plain, counted = [layer(x, kv_cache=c) for c in caches]
+    assert torch.equal(plain, counted)
+    cache = caches[1]
+    total = cache.weights[cache.block_table[0].long()].double().sum((0, 2))
+    assert ((total - 8 * S).abs() <= 8 * S * (2.0 ** -11 + 2.0 ** -16)).all()
+
+
 def test_layer_over_pages_refuses(gpu):
     H, n_q, n_kv, F = 512, 4, 2, 1024
     layer = FineLlamaDecoderLayer({k: v.to(gpu) for k, v in layer_weights(H, n_q, n_kv, F).items()}, n_q, n_kv, max_positions=64)

@@ -195,3 +195,40 @@ def test_chunks_on_two_streams_at_once(gpu):
     torch.cuda.synchronize()
     for k in range(2):
         assert all(torch.equal(o, alone[k]) for o in got[k])
+
+
+@pytest.mark.parametrize("Hq,Hkv,S,lens,new", [(32, 1, 2049, [2100], None), (64, 2, 2100, [2100, 2300], [2001, 2100])])
+def test_more_than_65535_columns(gpu, Hq, Hkv, S, lens, new):
+    """2049 rows of 32 query heads on a kv head: what the rows see, and the account from the scores worked out again."""
+    cache = Cache(lens, Hkv, 32)
+    q = queries(cache, Hq, S)
+    n = None if new is None else torch.tensor(new, dtype=torch.int32, device="cuda")
+    before = cache.weights.clone()
+    o, lse = ops.fine_fmha_paged_with_lse(q, *cache.args, new_lens=n, weights=cache.weights)
+    check(cache, q, o, lse, new)
+    again = before.clone()
+    ops.fine_key_weights(q, lse, *cache.args, again, new_lens=n)
+    assert torch.equal(again.nan_to_num(7.0), cache.weights.nan_to_num(7.0))
+    for b, length in enumerate(lens):
+        pg, sl = cache.at(b)
+        rows = S if new is None else new[b]
+        total = (cache.weights[pg, :, sl].double() - before[pg, :, sl].double()).sum(0)
+        # each row's probabilities sum to one: a score is off by 130 half steps of sums of magnitudes of 128 |q| |k| / 11.3 <= 60, the LSE as much, the account's
+        # additions by 2^-24 of values up to Hq / Hkv * rows a step
+        count = Hq // Hkv * rows
+        assert ((total - count).abs() <= count * (2 * 130 * 60 * EPS32 + 2.0 ** -16)).all()
+
+
+def test_the_last_rows_of_a_prompt_of_any_length_count(gpu):
+    Hq, Hkv, S, last = 32, 8, 16500, 64
+    cache = Cache([S], Hkv, 64)
+    q = queries(cache, Hq, last)
+    whole = torch.full((1, Hq, S, D), math.nan, dtype=torch.float16, device="cuda")
+    whole[:, :, -last:] = q
+    _, lse = ops.fine_fmha_paged_with_lse(q, *cache.args)
+    wide = torch.full((1, Hq, S), math.nan, device="cuda")
+    wide[:, :, -last:] = lse
+    a, b = cache.weights.clone(), cache.weights.clone()
+    ops.fine_key_weights(whole, wide, *cache.args, a, last_rows=last)
+    ops.fine_key_weights(q, lse, *cache.args, b)
+    assert torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0))

@@ -442,7 +442,14 @@ static bool paged_sizes(const mi355_paged_kv* c) {
     const int64_t pairs = (int64_t)c->B * c->Hkv, max_len = (int64_t)c->max_pages * c->page_size;
     return pairs <= 65535 && max_len <= (1 << 28) && pairs * (max_len / 32 + 1) <= INT32_MAX - 65536;
 }
-static bool paged_rows(const mi355_paged_kv* c, int Hq, int S) { return Hq >= c->Hkv && S >= 1 && (int64_t)(Hq / c->Hkv) * S <= 65535; }
+constexpr int64_t kMostWorkgroups = (1 << 24) - 1;   // of 256 threads in one launch
+// Likewise of the query columns of a kv head that a call works on: S rows, or the last `last_rows` of them, for each of its query heads. A sequence has no
+// more tokens than it has room for keys; a padded batch may be longer, up to 65535 columns
+static bool paged_rows(const mi355_paged_kv* c, int Hq, int S, int last_rows) {
+    if (Hq < c->Hkv || S < 1 || S > (1 << 28) || last_rows < 0) return false;
+    const int64_t rows = last_rows > 0 && last_rows < S ? last_rows : S, max_len = (int64_t)c->max_pages * c->page_size;
+    return Hq / c->Hkv * rows <= (rows <= max_len ? kMostWorkgroups : 65535);
+}
 
 static int paged_checked(const char* fn, const mi355_paged_kv* c) {
     if (!c || !c->pages || !c->block_table || !c->seq_lens) return fail(MI355_ERR_BAD_ARGUMENT, "%s: null pointer", fn);
@@ -469,12 +476,14 @@ static int paged_checked(const char* fn, const mi355_paged_kv* c) {
     return 0;
 }
 
-static int paged_queries_checked(const char* fn, const mi355_paged_kv* c, const void* Q, int Hq, int S, const int64_t* strides, int n, float scale) {
+static int paged_queries_checked(const char* fn, const mi355_paged_kv* c, const void* Q, int Hq, int S, int last_rows, const int64_t* strides, int n,
+                                 float scale) {
     if (!Q) return fail(MI355_ERR_BAD_ARGUMENT, "%s: null pointer", fn);
     if (Hq < 1 || S < 1) return fail(MI355_ERR_BAD_ARGUMENT, "%s: Hq and S must be >= 1", fn);
     if (Hq % c->Hkv != 0) return fail(MI355_ERR_BAD_ARGUMENT, "%s: Hq (%d) must be a multiple of Hkv (%d)", fn, Hq, c->Hkv);
-    if (!paged_rows(c, Hq, S))
-        return fail(MI355_ERR_UNSUPPORTED, "%s: Hq / Hkv * S must be at most 65535 (got %d / %d * %d)", fn, Hq, c->Hkv, S);
+    if (!paged_rows(c, Hq, S, last_rows))
+        return fail(MI355_ERR_UNSUPPORTED, "%s: Hq / Hkv * S must be below 2^24, and below 2^16 for more rows than a sequence may have keys (got %d / %d * %d, %lld keys)", fn,
+                    Hq, c->Hkv, S, (long long)c->max_pages * c->page_size);
     if (!(scale > 0.f) || scale > 3.0e38f) return fail(MI355_ERR_BAD_ARGUMENT, "%s: scale must be positive and finite (got %g)", fn, (double)scale);
     if (!aligned16(Q)) return fail(MI355_ERR_BAD_ARGUMENT, "%s: Q must be 16-byte aligned", fn);
     for (int i = 0; i < n; ++i)
@@ -484,8 +493,6 @@ static int paged_queries_checked(const char* fn, const mi355_paged_kv* c, const 
     return 0;
 }
 
-constexpr int64_t kMostWorkgroups = (1 << 24) - 1;   // of 256 threads in one launch
-
 static int workspace_checked(const char* fn, size_t need, const void* workspace, size_t bytes) {
     if (need > 0 && (workspace == nullptr || bytes < need || !aligned16(workspace)))
         return fail(MI355_ERR_BAD_ARGUMENT, "%s: workspace of %zu bytes at %p; this call needs %zu bytes, 16-byte aligned (%s_workspace_bytes)", fn, bytes,
@@ -494,7 +501,7 @@ static int workspace_checked(const char* fn, size_t need, const void* workspace,
 }
 
 size_t mi355_fmha_paged_workspace_bytes(const mi355_paged_kv* cache, int Hq, int S, int want_lse) {
-    if (!paged_sizes(cache) || !paged_rows(cache, Hq, S)) return 0;   // (the call is refused)
+    if (!paged_sizes(cache) || !paged_rows(cache, Hq, S, 0)) return 0;   // (the call is refused)
     return mi355::fmha_paged_workspace(*cache, Hq, S, want_lse != 0);
 }
 
@@ -505,7 +512,7 @@ int mi355_fmha_paged(const mi355_paged_kv* cache, const void* Q, void* O, float*
     if (!O) return fail(MI355_ERR_BAD_ARGUMENT, "%s: null pointer", fn);
     const int64_t dense[6] = {(int64_t)Hq * S * 128, (int64_t)S * 128, 128, (int64_t)Hq * S * 128, (int64_t)S * 128, 128};
     const int64_t* st = strides ? strides : dense;
-    if (int rc = paged_queries_checked(fn, cache, Q, Hq, S, st, 6, scale)) return rc;
+    if (int rc = paged_queries_checked(fn, cache, Q, Hq, S, 0, st, 6, scale)) return rc;
     if (!aligned16(O)) return fail(MI355_ERR_BAD_ARGUMENT, "%s: O must be 16-byte aligned", fn);
     // (the account of many rows is made by mi355_fmha_key_weights' kernel)
     if ((int64_t)cache->B * cache->Hkv * ((int64_t)(Hq / cache->Hkv) * S + (int64_t)cache->max_pages * cache->page_size / 256 + 1) > kMostWorkgroups ||
@@ -541,7 +548,7 @@ int mi355_rope_paged(const mi355_paged_kv* cache, void* qkv, int S, int q_heads,
 }
 
 size_t mi355_fmha_key_weights_workspace_bytes(const mi355_paged_kv* cache, int Hq, int S, int last_rows) {
-    if (!paged_sizes(cache) || !paged_rows(cache, Hq, S)) return 0;   // (the call is refused)
+    if (!paged_sizes(cache) || !paged_rows(cache, Hq, S, last_rows)) return 0;   // (the call is refused)
     return mi355::key_weights_workspace(*cache, Hq, S, last_rows);
 }
 
@@ -553,7 +560,7 @@ int mi355_fmha_key_weights(const mi355_paged_kv* cache, const void* Q, const flo
     if (last_rows < 0) return fail(MI355_ERR_BAD_ARGUMENT, "%s: last_rows must be >= 0 (got %d)", fn, last_rows);
     const int64_t dense[3] = {(int64_t)Hq * S * 128, (int64_t)S * 128, 128};
     const int64_t* st = q_strides ? q_strides : dense;
-    if (int rc = paged_queries_checked(fn, cache, Q, Hq, S, st, 3, scale)) return rc;
+    if (int rc = paged_queries_checked(fn, cache, Q, Hq, S, last_rows, st, 3, scale)) return rc;
     if (mi355::key_weights_workgroups(*cache, Hq, S, last_rows) > kMostWorkgroups / 2)
         return fail(MI355_ERR_UNSUPPORTED, "%s: %d sequences of %d rows over up to %lld keys are more than a call takes", fn, cache->B, S,
                     (long long)cache->max_pages * cache->page_size);

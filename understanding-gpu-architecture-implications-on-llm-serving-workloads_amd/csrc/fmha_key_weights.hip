@@ -257,7 +257,7 @@ static KeyWeightsPlan key_weights_plan(const mi355_paged_kv& c, int Hq, int Sq, 
     const long most = (long)(Hq / c.Hkv) * ((rows + ROWS - 1) / ROWS);
     // about as many workgroups as run at the same time, where that leaves them few enough tiles; of the tiles, those that the causal triangle
     // of the longest sequence leaves
-    const long seen = most * c.B * c.Hkv * p.max_blocks * (2L * max_len - std::min(rows, max_len)) / (2L * max_len);
+    const long seen = (long)((__int128)most * c.B * c.Hkv * p.max_blocks * (2L * max_len - std::min(rows, max_len)) / (2L * max_len));
     p.range_tiles = (int)std::max<long>(kMinTiles, std::min<long>(kMaxTiles, (seen + kWorkgroups - 1) / kWorkgroups));
     p.ranges = (int)((most + p.range_tiles - 1) / p.range_tiles);
     return p;

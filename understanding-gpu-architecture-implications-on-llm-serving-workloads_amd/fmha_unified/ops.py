@@ -52,7 +52,8 @@ def fine_fmha_with_lse(q: Tensor, k: Tensor, v: Tensor, causal: bool, is_decode=
 # weights, key_positions   [n_pages, Hkv, page_size] fp32 and int32: the attention each key has had, the position of its token
 #
 # Everything is read on the device: no call waits for it, and a captured call serves the lengths and tables that its tensors hold
-# when the graph is replayed. The reference keeps one growing tensor a layer instead (benchmarks/flashattn-cuda/modeling_llama.py:664-668).
+# when the graph is replayed. No page may belong to two sequences of a call that writes it, to its weights among others. Hq / Hkv * S is below
+# 2^24 (2^16 where S is more than max_pages * page_size); the other limits are those of include/mi355_serving.h. The reference keeps one growing tensor a layer instead (benchmarks/flashattn-cuda/modeling_llama.py:664-668).
 
 # The functions below call the extension module's own; `torch.ops.fmha_unified.{finefmha_paged, finefmha_paged_lse, rope_paged, key_weights,
 # evict_paged}` are the same through torch's dispatcher.
