@@ -197,3 +197,13 @@ def test_a_cache_hands_out_pages_and_takes_them_back():
     consistent()
     with pytest.raises(ValueError, match="account"):
         FinePagedKVCache(1, 4, 1, device="cpu").evict(3, 1)
+
+
+def test_calls_get_the_columns_in_use():
+    from llama_layer import FinePagedKVCache
+    c = FinePagedKVCache(2, 100, 1, page_size=48, device="cpu")          # steps of 6 pages, 288 keys
+    for new, rows, width in (([0, 0], 1, 6), ([288, 5], 5, 6), ([1, 0], 1, 12), ([0, 0], 2000, 42), ([0, 0], 1 << 20, 100)):
+        c.extend(new)
+        table = c.table_in_use(rows)
+        assert table.shape == (2, width) and table.data_ptr() == c.block_table.data_ptr() and table.stride(0) == 100
+    assert FinePagedKVCache(1, 4, 1, page_size=512, device="cpu").table_in_use().shape == (1, 1)

@@ -132,6 +132,37 @@ def test_a_long_prompt_of_many_heads_with_an_account(gpu):
     assert ((total - 8 * S).abs() <= 8 * S * (2.0 ** -11 + 2.0 ** -16)).all()
 
 
+def test_calls_cost_what_is_in_use_whatever_the_pool(gpu):
+    """A table as wide as a large pool: the workspaces of a step, a chunk of a prompt and an eviction do not grow with it, results are those of a narrow one."""
+    H, n_q, n_kv, F, B = 512, 8, 2, 1024, 8
+    layer = FineLlamaDecoderLayer({k: v.to(gpu) for k, v in layer_weights(H, n_q, n_kv, F, seed=30).items()}, n_q, n_kv, max_positions=512)
+    wide, narrow = FinePagedKVCache(B, 20000, n_kv, page_size=16, device=gpu, account=True), FinePagedKVCache(B, 200, n_kv, page_size=16, max_pages=64, device=gpu, account=True)
+    lens = [120, 50, 33, 1, 0, 99, 16, 17]
+
+    def both(call):
+        results = []
+        for cache in (wide, narrow):
+            torch.cuda.synchronize()
+            torch.cuda.reset_peak_memory_stats()
+            before = torch.cuda.memory_allocated()
+            results.append(call(cache))
+            torch.cuda.synchronize()
+            assert torch.cuda.max_memory_allocated() - before <= 64 << 20
+        return results
+
+    for S, new in ((120, lens), (1, None), (20, [20] * 7 + [3]), (1, None)):
+        x = so.randn_fp16((B, S, H), 40 + S).to(gpu)
+        a, b = both(lambda cache: layer(x, kv_cache=cache, new_lens=new))
+        assert torch.equal(a, b)
+    both(lambda cache: cache.evict(60, 20))
+    assert wide.lengths == narrow.lengths and wide.seq_lens.tolist() == wide.lengths
+    for b in range(B):
+        assert torch.equal(keys_of(wide, b), keys_of(narrow, b))
+    x = so.randn_fp16((B, 1, H), 9).to(gpu)
+    a, b = both(lambda cache: layer(x, kv_cache=cache))
+    assert torch.equal(a, b)
+
+
 def test_layer_over_pages_refuses(gpu):
     H, n_q, n_kv, F = 512, 4, 2, 1024
     layer = FineLlamaDecoderLayer({k: v.to(gpu) for k, v in layer_weights(H, n_q, n_kv, F).items()}, n_q, n_kv, max_positions=64)

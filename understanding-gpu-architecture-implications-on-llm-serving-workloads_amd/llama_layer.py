@@ -83,6 +83,13 @@ class FinePagedKVCache:
     def free_pages(self):
         return len(self._free)
 
+    def table_in_use(self, rows=0):
+        """The columns of the block table that the longest sequence needs, or one of `rows` keys, in steps of 256 keys: launches, workspaces and the choice
+        of kernels go by the width of the table that a call is given, and the pool's may be a thousand times what is in use."""
+        page = self.kv_pages.shape[2]
+        step = -(-256 // page)
+        return self.block_table[:, :-(-max(rows, 1, *self.lengths) // (step * page)) * step]
+
     def extend(self, new):
         """Room for new[b] more tokens of each sequence, whose lengths and positions go on by that many. ValueError, and nothing changed, where the
         pool or the table has no more."""
@@ -125,7 +132,7 @@ class FinePagedKVCache:
             raise ValueError("eviction needs a cache made with account=True")
         if all(n <= budget for n in self.lengths):
             return
-        self.seq_lens.copy_(fine_evict_paged(self.kv_pages, self.block_table, self.seq_lens, self.weights, self.key_positions, budget, recent))
+        self.seq_lens.copy_(fine_evict_paged(self.kv_pages, self.table_in_use(), self.seq_lens, self.weights, self.key_positions, budget, recent))
         self._in_order = [0 if n > budget else have for n, have in zip(self.lengths, self._in_order)]
         self.lengths = [min(n, budget) for n in self.lengths]
         self._give_back(range(len(self.lengths)))
@@ -242,7 +249,7 @@ class FineLlamaDecoderLayer:
         prompt = not any(cache.lengths)
         cache.extend(new)
         counts = None if all(n == S for n in new) else torch.tensor(new, dtype=torch.int32, device=hidden_states.device)
-        paged = (cache.kv_pages, cache.block_table, cache.seq_lens, counts, cache.weights, cache.key_positions)
+        paged = (cache.kv_pages, cache.table_in_use(S), cache.seq_lens, counts, cache.weights, cache.key_positions)
         try:
             out, ms = _C.layer_forward(hidden_states, self.w_qkv, self.w_o, self.w_gu, self.w_d, self.ln1, self.ln2, self.cos, self.sin, pos,
                                        0, (), 0, self.n_q, self.n_kv, self.eps, self.gu_block, time_attention, paged, prompt)
