@@ -207,3 +207,23 @@ def test_calls_get_the_columns_in_use():
         table = c.table_in_use(rows)
         assert table.shape == (2, width) and table.data_ptr() == c.block_table.data_ptr() and table.stride(0) == 100
     assert FinePagedKVCache(1, 4, 1, page_size=512, device="cpu").table_in_use().shape == (1, 1)
+
+
+def test_positions_of_a_cache_follow_those_that_were_given():
+    from llama_layer import FinePagedKVCache
+    c = FinePagedKVCache(3, 20, 1, page_size=16, device="cpu")
+    ids = lambda *rows: torch.tensor(rows, dtype=torch.int32)
+    for new, given, want in (([2, 2, 2], None, [2, 2, 2]), ([2, 2, 2], ids([7, 8], [90, 91], [4, 5]), [9, 92, 6]), ([1, 1, 1], None, [10, 93, 7]),
+                             ([0, 2, 1], ids([50, 51], [60, 61], [70, 71]), [10, 62, 71]), ([0, 0, 0], ids([1], [1], [1]), [10, 62, 71]),
+                             ([1, 0, 2], ids([30, 31]), [31, 62, 32]), ([3, 3, 3], ids([40, 41, 42]), [43, 43, 43])):
+        c.extend(new)
+        if given is not None:
+            c.went_to(given, new)
+        assert c.positions == want and c.next_positions.tolist() == want
+    c.went_to(ids([40, 41, 52]), [3, 3, 3])
+    c.take_back([1, 0, 3])
+    c.extend([0, 2, 0])
+    c.release(0)
+    assert c.positions == [0, 55, 50] and c.next_positions.tolist() == [0, 55, 50]
+    c.release(1)
+    assert c.positions == [0, 0, 50]

@@ -163,6 +163,43 @@ def test_calls_cost_what_is_in_use_whatever_the_pool(gpu):
     assert torch.equal(a, b)
 
 
+def test_positions_go_on_behind_those_that_were_given(gpu):
+    H, n_q, n_kv, F, B = 512, 4, 2, 1024, 2
+    layer = FineLlamaDecoderLayer({k: v.to(gpu) for k, v in layer_weights(H, n_q, n_kv, F, seed=11).items()}, n_q, n_kv, max_positions=1200)
+    make = lambda: FinePagedKVCache(B, 40, n_kv, page_size=16, device=gpu, account=True)
+    given, mixed = make(), make()
+    x = so.randn_fp16((B, 100, H), 1).to(gpu)
+    first = torch.stack((torch.arange(1000, 1100), torch.arange(500, 600))).to(gpu)
+    new = [100, 60]
+    for cache in (given, mixed):
+        layer(x, first, kv_cache=cache, new_lens=new)
+        assert cache.positions == [1100, 560] and cache.next_positions.tolist() == [1100, 560]
+        cache.evict(50, 20)
+        assert cache.positions == [1100, 560]
+    for t in range(8):
+        xt = so.randn_fp16((B, 1, H), 20 + t).to(gpu)
+        a = layer(xt, torch.tensor([[1100 + t], [560 + t]], device=gpu), kv_cache=given)
+        b = layer(xt, kv_cache=mixed)
+        assert torch.equal(a, b)
+    for cache in (given, mixed):
+        assert cache.positions == [1108, 568] and cache.next_positions.tolist() == [1108, 568]
+        cache.evict(50, 20)
+        for b in range(B):                             # the newest tokens are the last of the text
+            j = torch.arange(50, device=gpu)
+            where = cache.key_positions[cache.block_table[b].long()[j // 16], :, j % 16]
+            for h in range(n_kv):
+                assert set(range(cache.positions[b] - 20, cache.positions[b])) <= set(where[:, h].tolist())
+    # one row of positions for all sequences; sequences without a token stay where they are
+    layer(so.randn_fp16((B, 3, H), 50).to(gpu), torch.arange(1150, 1153)[None].to(gpu), kv_cache=mixed, new_lens=[0, 2])
+    assert mixed.positions == [1108, 1152]
+    mixed.take_back([0, 1])
+    assert mixed.positions == [1108, 1151] and mixed.next_positions.tolist() == [1108, 1151]
+    with pytest.raises(ValueError, match="max_positions"):
+        layer(so.randn_fp16((B, 50, H), 51).to(gpu), kv_cache=mixed)
+    mixed.release(0)
+    assert mixed.positions == [0, 1151]
+
+
 def test_layer_over_pages_refuses(gpu):
     H, n_q, n_kv, F = 512, 4, 2, 1024
     layer = FineLlamaDecoderLayer({k: v.to(gpu) for k, v in layer_weights(H, n_q, n_kv, F).items()}, n_q, n_kv, max_positions=64)

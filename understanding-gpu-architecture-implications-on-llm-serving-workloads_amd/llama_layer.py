@@ -60,9 +60,10 @@ class FineKVCache:
 class FinePagedKVCache:
     """Key/value cache of one layer in pages, for sequences of different lengths that come and go: a pool `kv_pages` [n_pages, 2 * n_kv,
     page_size, 128], of which each of `batch` sequences owns the pages in its row of `block_table` [batch, max_pages]. `seq_lens` and
-    `next_positions` (int32, on the device) hold each sequence's keys and the position of its next token; `lengths` and `positions` are the same
-    on the host, which hands out the pages. With `account`, `weights` and `key_positions` [n_pages, n_kv, page_size] keep what
-    `evict` goes by: the attention that each key has had, the position of its token.
+    `next_positions` (int32, on the device) hold each sequence's keys and the position of its next token, one behind its last; `lengths` and
+    `positions` are the same on the host, which hands out the pages (`positions` waits for the device once after a call with position_ids of its
+    own). With `account`, `weights` and `key_positions` [n_pages, n_kv, page_size] keep what `evict` goes by: the attention that each key has
+    had, the position of its token.
 
     The layer's forward makes room with `extend` and files its tokens; `evict` cuts long sequences, `release` frees one."""
 
@@ -74,7 +75,7 @@ class FinePagedKVCache:
         self.next_positions = torch.zeros(batch, dtype=torch.int32, device=device)
         self.weights = torch.zeros((n_pages, n_kv, page_size), device=device) if account else None
         self.key_positions = torch.zeros((n_pages, n_kv, page_size), dtype=torch.int32, device=device) if account else None
-        self.lengths, self.positions = [0] * batch, [0] * batch
+        self.lengths, self._positions = [0] * batch, [0] * batch   # (positions: None where the device alone knows them)
         self._in_order = [0] * batch      # tokens at the end of each sequence that no eviction has moved
         self._pages = [[] for _ in range(batch)]
         self._free = list(range(n_pages - 1, -1, -1))
@@ -82,6 +83,29 @@ class FinePagedKVCache:
     @property
     def free_pages(self):
         return len(self._free)
+
+    @property
+    def positions(self):
+        if self._positions is None:
+            self._positions = self.next_positions.tolist()
+        return self._positions
+
+    @positions.setter
+    def positions(self, positions):
+        self._positions = positions
+
+    def went_to(self, position_ids, new):
+        """The last new[b] tokens of each sequence, which `extend` made room for, are those at position_ids [1 or batch, new or more] (int32, on the
+        device): positions go on behind them."""
+        came = [b for b, n in enumerate(new) if n > 0]
+        if not came:
+            return
+        if len(came) == len(new) and min(new) == max(new):
+            self.next_positions.copy_(position_ids[:, new[0] - 1] + 1)
+        else:
+            index = torch.tensor([came, [b if position_ids.shape[0] > 1 else 0 for b in came], [new[b] - 1 for b in came]], device=position_ids.device)
+            self.next_positions[index[0]] = position_ids[index[1], index[2]] + 1
+        self._positions = None
 
     def table_in_use(self, rows=0):
         """The columns of the block table that the longest sequence needs, or one of `rows` keys, in steps of 256 keys: launches, workspaces and the choice
@@ -107,7 +131,8 @@ class FinePagedKVCache:
         if any(wanted):
             self._write_table([b for b, more in enumerate(wanted) if more])
         self.lengths = lengths
-        self.positions = [n + more for n, more in zip(self.positions, new)]
+        if self._positions is not None:
+            self._positions = [n + more for n, more in zip(self._positions, new)]
         self._in_order = [n + more for n, more in zip(self._in_order, new)]
         step = new[0] if all(n == new[0] for n in new) else torch.tensor(new, dtype=torch.int32, device=self.seq_lens.device)
         self.seq_lens += step
@@ -115,12 +140,13 @@ class FinePagedKVCache:
 
     def take_back(self, new):
         """The last new[b] tokens of each sequence are no longer its own (a call that failed; drafted tokens that were not accepted); ValueError for more
-        than have come since it was cut, which leaves no order. The account of the others keeps what those added to it."""
+        than have come since it was cut, which leaves no order. Positions go back by as many. The account of the others keeps what those added to it."""
         if len(new) != len(self.lengths) or any(not 0 <= n <= have for n, have in zip(new, self._in_order)):
             raise ValueError("cannot take %r tokens back where %r have come" % (new, self._in_order))
         self._in_order = [n - less for n, less in zip(self._in_order, new)]
         self.lengths = [n - less for n, less in zip(self.lengths, new)]
-        self.positions = [n - less for n, less in zip(self.positions, new)]
+        if self._positions is not None:
+            self._positions = [n - less for n, less in zip(self._positions, new)]
         step = new[0] if all(n == new[0] for n in new) else torch.tensor(new, dtype=torch.int32, device=self.seq_lens.device)
         self.seq_lens -= step
         self.next_positions -= step
@@ -139,7 +165,9 @@ class FinePagedKVCache:
 
     def release(self, b):
         """Sequence b is done: its pages are free, its place may be taken by another."""
-        self.lengths[b] = self.positions[b] = self._in_order[b] = 0
+        self.lengths[b] = self._in_order[b] = 0
+        if self._positions is not None:
+            self._positions[b] = 0
         self.seq_lens[b] = 0
         self.next_positions[b] = 0
         self._give_back([b])
@@ -207,7 +235,8 @@ class FineLlamaDecoderLayer:
 
     def forward(self, hidden_states, position_ids=None, kv_cache=None, time_attention=False, new_lens=None):
         """With a FinePagedKVCache `new_lens` (a list) may say how many of each sequence's S rows are tokens, the first ones (none: all); the rows behind
-        them must be finite and their results mean nothing. Its positions go on where each sequence's text is unless position_ids are given."""
+        them must be finite and their results mean nothing. Its positions go on where each sequence's text is unless position_ids are given, behind
+        which they go on from then."""
         B, S, H = hidden_states.shape
         if type(kv_cache) is FinePagedKVCache:
             return self._forward_paged(hidden_states, position_ids, kv_cache, time_attention, new_lens)
@@ -256,6 +285,8 @@ class FineLlamaDecoderLayer:
         except Exception:
             cache.take_back(new)
             raise
+        if position_ids is not None:
+            cache.went_to(pos, new)
         if time_attention:
             self.attn_ms["prefill" if prompt or S > 1 else "decode"].append(ms)
         return out
