@@ -200,6 +200,17 @@ def test_positions_go_on_behind_those_that_were_given(gpu):
     assert mixed.positions == [0, 1151]
 
 
+def test_a_subclass_of_the_cache_is_one(gpu):
+    class Mine(FinePagedKVCache):
+        pass
+
+    H, n_q, n_kv, F = 512, 4, 2, 1024
+    layer = FineLlamaDecoderLayer({k: v.to(gpu) for k, v in layer_weights(H, n_q, n_kv, F).items()}, n_q, n_kv, max_positions=64)
+    x = so.randn_fp16((2, 20, H), 3).to(gpu)
+    a, b = [layer(x, kv_cache=kind(2, 6, n_kv, page_size=16, device=gpu), new_lens=[20, 7]) for kind in (FinePagedKVCache, Mine)]
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1, :7], b[1, :7])
+
+
 def test_layer_over_pages_refuses(gpu):
     H, n_q, n_kv, F = 512, 4, 2, 1024
     layer = FineLlamaDecoderLayer({k: v.to(gpu) for k, v in layer_weights(H, n_q, n_kv, F).items()}, n_q, n_kv, max_positions=64)

@@ -238,7 +238,7 @@ class FineLlamaDecoderLayer:
         them must be finite and their results mean nothing. Its positions go on where each sequence's text is unless position_ids are given, behind
         which they go on from then."""
         B, S, H = hidden_states.shape
-        if type(kv_cache) is FinePagedKVCache:
+        if isinstance(kv_cache, FinePagedKVCache):
             return self._forward_paged(hidden_states, position_ids, kv_cache, time_attention, new_lens)
         if new_lens is not None:
             raise ValueError("new_lens goes with a FinePagedKVCache")
