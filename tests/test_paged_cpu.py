@@ -3,6 +3,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.utils._python_dispatch import TorchDispatchMode
 
 import fmha_unified
 
@@ -162,6 +163,32 @@ def test_operators_name_what_they_write():
                           ("key_weights", ["weights"]), ("evict_paged", ["kv_pages", "weights", "key_positions"])):
         schema = getattr(torch.ops.fmha_unified, name).default._schema
         assert [a.name for a in schema.arguments if a.alias_info is not None and a.alias_info.is_write] == written
+
+
+class Seen(TorchDispatchMode):
+    """Names of the operators that torch's dispatcher is asked for; none of them runs."""
+
+    def __init__(self):
+        super().__init__()
+        self.names = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        self.names.append(func.name())
+        return tuple(torch.zeros(1) for _ in func._schema.returns) if len(func._schema.returns) > 1 else torch.zeros(1) if func._schema.returns else None
+
+
+def test_what_watches_the_dispatcher_sees_the_functions():
+    t, one = tensors(), torch.ones(50, 64)
+    w, pos, p = torch.zeros(5, 2, 16), torch.zeros(5, 2, 16, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    pool = (t["kv_pages"], t["block_table"], t["seq_lens"])
+    qkv, lse = torch.zeros(2, 1, 12, 128, dtype=torch.float16), torch.zeros(2, 8, 1)
+    with Seen() as seen:
+        ops.fine_fmha_paged(**t)
+        ops.fine_fmha_paged_with_lse(**t, weights=w)
+        ops.fine_rope_paged(qkv, *pool, one, one, p, 8, key_positions=pos)
+        ops.fine_key_weights(t["q"], lse, *pool, w)
+        ops.fine_evict_paged(*pool, w, pos, 4, 2)
+    assert seen.names == ["fmha_unified::" + n for n in ("finefmha_paged", "finefmha_paged_lse", "rope_paged", "key_weights", "evict_paged")]
 
 
 def test_a_cache_hands_out_pages_and_takes_them_back():

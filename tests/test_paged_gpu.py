@@ -799,6 +799,25 @@ def test_operators_through_the_dispatcher_are_the_same(gpu):
     assert torch.equal(x, y) and torch.equal(a[0].nan_to_num(7.0), b[0].nan_to_num(7.0))
 
 
+def test_gradients_that_there_are_none_of_are_not_lost_in_silence(gpu):
+    """As with the operators that go through torch's dispatcher: the result of a tensor that needs a gradient needs one, and going back through it is not silent."""
+    cache = Cache([70, 31], 2, 16)
+    q = queries(cache, 8, 2)
+    want = ops.fine_fmha_paged(q, *cache.args)
+    k = torch.zeros(2, 2, 70, D, dtype=torch.float16, device="cuda")
+    other = q.clone().requires_grad_()
+    expected, _ = ops.fine_fmha_with_lse(other, k, k, True)
+    o = ops.fine_fmha_paged(other, *cache.args)
+    o2, lse = ops.fine_fmha_paged_with_lse(other, *cache.args)
+    assert o.requires_grad == o2.requires_grad == lse.requires_grad == expected.requires_grad
+    assert torch.equal(o, want) and torch.equal(o2, want)
+    with torch.no_grad():
+        assert not ops.fine_fmha_paged(other, *cache.args).requires_grad
+    # (torch has no way of its own to batch an operator that may write an argument, and says so)
+    with pytest.raises(RuntimeError, match="Batching rule not implemented for fmha_unified::finefmha_paged"):
+        torch.vmap(lambda x: ops.fine_fmha_paged(x, *cache.args))(torch.stack((q, -q)))
+
+
 def test_operators_refuse_wrong_tensors_on_the_gpu(gpu):
     c = Cache([40, 20], 2, 16)
     q = queries(c, 8, 1)

@@ -23,6 +23,7 @@
 #include <array>
 #include <cmath>
 #include <optional>
+#include <string>
 #include <tuple>
 
 #include "mi355_serving.h"
@@ -286,14 +287,35 @@ TORCH_LIBRARY_IMPL(fmha_unified, CPU, m) {
 
 // _C as a Python extension module. The operators of the paged cache are functions of it as well: with eight to twelve arguments, most of them tensors, a call
 // through the dispatcher takes the host 1 us longer than one of these, and a step's calls are a few us long on the GPU (64 tokens filed, calls one
-// behind the other: 6.4 us each, 7.5 through the dispatcher).
+// behind the other: 6.4 us each, 7.5 through the dispatcher). Where something is there that only the dispatcher shows a call to (a mode, a transform, a
+// tracer, a tensor that needs a gradient, whose result says on the way back that there is none), it is asked.
+namespace {
+
+const c10::DispatchKeySet kWatchers({c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot, c10::DispatchKey::PythonDispatcher, c10::DispatchKey::Functionalize,
+                                     c10::DispatchKey::FuncTorchDynamicLayerFrontMode, c10::DispatchKey::FuncTorchDynamicLayerBackMode,
+                                     c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::Batched, c10::DispatchKey::Tracer});
+
+bool watched(const at::Tensor& t) { return t.defined() && (t.key_set().has_any(kWatchers) || (t.requires_grad() && at::GradMode::is_enabled())); }
+bool watched(const std::optional<at::Tensor>& t) { return t.has_value() && watched(*t); }
+bool watched(int64_t) { return false; }
+
+template <typename R, typename... A>
+void def(py::module_& m, const char* name, R (*kernel)(A...)) {
+    const auto op = c10::Dispatcher::singleton().findSchemaOrThrow((std::string("fmha_unified::") + name).c_str(), "").typed<R(A...)>();
+    m.def(name, [=](A... a) -> R {
+        if (c10::impl::tls_local_dispatch_key_set().included_.has_any(kWatchers) || (watched(a) || ...)) return op.call(a...);
+        return kernel(a...);
+    }, py::call_guard<py::gil_scoped_release>());
+}
+
+}  // namespace
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-    const auto no_gil = py::call_guard<py::gil_scoped_release>();
-    m.def("finefmha_paged", &finefmha_paged, no_gil);
-    m.def("finefmha_paged_lse", &finefmha_paged_lse, no_gil);
-    m.def("rope_paged", &rope_paged, no_gil);
-    m.def("key_weights", &key_weights, no_gil);
-    m.def("evict_paged", &evict_paged, no_gil);
+    def(m, "finefmha_paged", &finefmha_paged);
+    def(m, "finefmha_paged_lse", &finefmha_paged_lse);
+    def(m, "rope_paged", &rope_paged);
+    def(m, "key_weights", &key_weights);
+    def(m, "evict_paged", &evict_paged);
 }
 
 }  // namespace fmha_unified
