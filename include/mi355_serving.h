@@ -371,7 +371,8 @@ int mi355_fmha_key_weights(const mi355_paged_kv* cache, const void* Q, const flo
  * the largest position that the kv head holds (position > largest - recent), then those of the largest weights (NaN lowest); of equals, the
  * lowest slots. The kept keys that lie behind the budget move, in order, into the slots of the dropped ones in front of it, with their
  * values, weights and positions, so the sequence is `budget` long afterwards and its keys lie in no particular order; each kv head keeps keys of its own. Slots
- * from `budget` on are left as they are. lens_out[b] = min(seq_lens[b], budget); lens_out may not overlap seq_lens, which is not written. Both
+ * from `budget` on are left as they are. Slots of pages outside the pool hold no key and take none: where there are some in front of the budget, so many keys
+ * fewer are kept. lens_out[b] = min(seq_lens[b], budget); lens_out may not overlap seq_lens, which is not written. Both
  * weights and key_positions are needed; new_lens is not read.
  */
 size_t mi355_cache_evict_workspace_bytes(const mi355_paged_kv* cache, int budget);

@@ -567,6 +567,40 @@ def test_eviction_of_weights_side_by_side(gpu, steps, outliers):
             assert torch.equal(x.nan_to_num(7.0), y.nan_to_num(7.0))
 
 
+@pytest.mark.parametrize("lens,budget,page,Hkv", [([300, 77], 130, 16, 2), ([5000], 2100, 32, 1), ([40000], 9000, 64, 1), ([90, 200], 33, 48, 2)])
+def test_eviction_moves_nothing_into_pages_outside_the_pool(gpu, lens, budget, page, Hkv):
+    """A slot of such a page holds no key: in front of the budget it stays as it is and so many keys fewer are kept, behind it there is nothing to keep."""
+    cache = Cache(lens, Hkv, page)
+    positions_of(cache, 3)
+    full = cache.table.clone()
+    for b, n in enumerate(lens):
+        pages = -(-n // page)
+        for i in {0, 2 % pages, pages - 1, pages // 2}:
+            cache.table[b, i] = (-1, cache.kv.shape[0], 2 ** 31 - 1)[i % 3]
+    recent = 10
+    kv, w, pos = cache.kv.clone(), cache.weights.clone(), cache.positions.clone()
+    there = [torch.tensor([0 <= int(x) < cache.kv.shape[0] for x in row]) for row in cache.table.tolist()]
+    for b, n in enumerate(lens):
+        if n <= budget:
+            continue
+        has = [bool(there[b][j // page]) for j in range(n)]
+        room = sum(has[:budget])
+        pg, sl = full[b].cpu().long()[torch.arange(n) // page].cuda(), (torch.arange(n) % page).cuda()
+        for h in range(Hkv):
+            wl, pl = cache.weights[pg, h, sl].tolist(), cache.positions[pg, h, sl].tolist()
+            newest = max((p for p, x in zip(pl, has) if x), default=0)
+            kept = set(sorted((j for j in range(n) if has[j]), key=lambda j: (0, 0.0, j) if pl[j] > newest - recent else (1, -wl[j], j))[:room])
+            holes, moved = [j for j in range(budget) if has[j] and j not in kept], [j for j in range(budget, n) if j in kept]
+            assert len(holes) == len(moved)
+            d, s = torch.tensor(holes, dtype=torch.long, device="cuda"), torch.tensor(moved, dtype=torch.long, device="cuda")
+            for t, i in ((kv, h), (kv, h + Hkv), (w, h), (pos, h)):
+                t[pg[d], i, sl[d]] = t[pg[s], i, sl[s]]
+    got = ops.fine_evict_paged(*cache.args, cache.weights, cache.positions, budget, recent)
+    assert got.tolist() == [min(n, budget) for n in lens]
+    for x, y in ((cache.kv, kv), (cache.weights, w), (cache.positions, pos)):
+        assert torch.equal(x.nan_to_num(7.0), y.nan_to_num(7.0))
+
+
 def test_eviction_with_positions_of_the_whole_range(gpu):
     cache = Cache([100], 1, 16)
     pg, sl = cache.at(0)

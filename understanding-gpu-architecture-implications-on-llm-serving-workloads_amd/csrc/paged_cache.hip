@@ -71,7 +71,8 @@ __global__ __launch_bounds__(pcache::THREADS) void rope_paged_kernel(PagedKv kv,
 // A kv head of a sequence longer than the budget keeps the `budget` keys of the largest rank: those whose position is within `recent` of its
 // largest one first, then by weight, ties to the lowest slot. Kept keys behind the budget fill the slots of the dropped ones in
 // front of it, in order: attention does not care how keys lie, their positions travel with them, and only as many rows move
-// as are dropped (closing ranks would move most of the cache for one dropped key).
+// as are dropped (closing ranks would move most of the cache for one dropped key). A slot of a page outside the pool holds no key and takes none: one
+// in front of the budget counts as kept, so that nothing moves there, one behind it is dropped before all keys.
 namespace evict {
 constexpr int THREADS = 1024, WAVES = THREADS / 64;
 constexpr int BINS = 2048, COPIES = 2;        // of the histogram, even and odd lanes' own
@@ -80,10 +81,10 @@ constexpr int kMostChunks = 8;                // of 4 keys whose ranks stay in a
 constexpr int kMovesHere = 256;               // up to this many moves are made by the selecting workgroup
 constexpr int MOVES = 32;                     // of a workgroup of the moving kernel, 8 at a time side by side
 
-// a weight as a whole number of the same order; NaN and the slots of pages outside the pool lowest, minus infinity next
+// a weight as a whole number of the same order; the slots of pages outside the pool lowest (0), then NaN, then minus infinity
 __device__ __forceinline__ uint32_t rank_of(float w) {
     const uint32_t u = __builtin_bit_cast(uint32_t, w == 0.f ? 0.f : w);   // (-0 is 0)
-    if (w != w) return 0u;
+    if (w != w) return 1u;
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 // the lowest n bits, n cut to 0 .. 32
@@ -240,11 +241,12 @@ __global__ __launch_bounds__(evict::THREADS) void evict_select_kernel(PagedKv kv
     const int bottom = row_max(extent[0][lane & 15]), top = row_max(extent[1][lane & 15]);
     const long old = (long)newest - a.recent;   // positions up to here are not recent
     int recent = 0;
-    const auto mark = [&](uint32_t there, uint4& r, const uint4& p) {
+    // (`none`: slots in front of the budget that hold no key)
+    const auto mark = [&](uint32_t there, uint32_t none, uint4& r, const uint4& p) {
         uint32_t x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const bool is = ((there >> e) & 1) && (int)get(p, e) > old;
+            const bool is = (there >> e) & 1 ? (int)get(p, e) > old : (none >> e) & 1;
             x[e] = is ? kRecent : get(r, e);
             recent += is;
         }
@@ -270,14 +272,22 @@ __global__ __launch_bounds__(evict::THREADS) void evict_select_kernel(PagedKv kv
     };
     if constexpr (M > 0) {
 #pragma unroll
-        for (int c = 0; c < M; ++c) mark((present >> (4 * c)) & 15, rank[c], position[c]);
+        for (int c = 0; c < M; ++c) mark((present >> (4 * c)) & 15, 0, rank[c], position[c]);
+        const uint32_t none = low_bits(min(len - j0, 4 * chunks)) & low_bits(a.budget - j0) & ~present;
+        if (__builtin_amdgcn_ballot_w64(none != 0) != 0) {
+#pragma unroll
+            for (int c = 0; c < M; ++c) mark(0, (none >> (4 * c)) & 15, rank[c], position[c]);
+        }
     } else {
         for (int c = 0; c < chunks; ++c) {
             const int j = j0 + 4 * c;
             if (j >= len) break;
             uint4 r = kept_ranks[c * THREADS + tid];
             const int page = table[divide(j, kv.by_page)];
-            mark(there_of(j, page), r, kept_positions[c * THREADS + tid]);
+            const uint32_t there = there_of(j, page);
+            const uint4 at = kept_positions[c * THREADS + tid];
+            mark(there, 0, r, at);
+            if (there != 15u) mark(0, low_bits(min(len, a.budget) - j) & ~there, r, at);
             kept_ranks[c * THREADS + tid] = r;
         }
     }

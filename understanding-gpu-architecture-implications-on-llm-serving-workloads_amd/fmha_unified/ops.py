@@ -97,5 +97,6 @@ def fine_evict_paged(kv_pages: Tensor, block_table: Tensor, seq_lens: Tensor, we
     """Cuts sequences longer than `budget` to it, every kv head on its own: kept are the keys whose position is within `recent` of the
     largest, then those of the largest weights (NaN lowest), of equals the lowest slots. Kept keys that lie behind the budget move, in order,
     into the slots of dropped ones in front of it, with their values, weights and positions. Returns the new lengths, min(seq_lens,
-    budget); seq_lens itself is left as it is, and so are the slots from `budget` on."""
+    budget); seq_lens itself is left as it is, and so are the slots from `budget` on. Slots of pages outside the pool hold no key and take
+    none: where there are some in front of the budget, so many keys fewer are kept."""
     return _C.evict_paged(kv_pages, block_table, seq_lens, weights, key_positions, budget, recent)
