@@ -339,7 +339,8 @@ typedef struct mi355_paged_kv {
  * Where cache->weights is given, each key's probabilities, summed over the query heads of its kv head and the rows, are added to
  * it. Sums and statistics are fp32, in an order that depends on the sizes and lengths alone; the probabilities are rounded to the element type for
  * the second product. What a row does not see has no influence on it, infinities and NaN included. new_lens of NULL with S rows and
- * a sequence shorter than S: its first rows see nothing. Hq / Hkv * S < 2^24 (2^16 where S is more than max_pages * page_size), and
+ * a sequence shorter than S: its first rows see nothing. scale: positive, at most 2.3e38 (times log2 e it is finite), and such that no score passes
+ * 2^26 (beyond, an exponent's argument in 32 bits is off by more than the 16 bits of a probability have room for). Hq / Hkv * S < 2^24 (2^16 where S is more than max_pages * page_size), and
  * B * Hq * S + B * Hkv * (max_pages * page_size / 256 + 1) < 2^24.
  */
 size_t mi355_fmha_paged_workspace_bytes(const mi355_paged_kv* cache, int Hq, int S, int want_lse);

@@ -110,6 +110,16 @@ def test_prompts_of_many_heads_and_tokens_are_taken(lib):
         assert cdll.mi355_fmha_key_weights_workspace_bytes(c, Hq, S, last) == 0
 
 
+def test_a_scale_that_is_infinite_in_powers_of_two_is_refused(lib):
+    """The kernels take exponentials to the base 2, of scores times scale * log2 e."""
+    cdll, c = lib.load(), cache(lib)
+    for scale, word in ((2.4e38, b"scale"), (3.0e38, b"scale"), (2.2e38, b"workspace"), (1e-45, b"workspace")):
+        assert cdll.mi355_fmha_paged(c, P, P, P, 32, 1, None, scale, None, 0, None) == lib.ERR_BAD_ARGUMENT and word in cdll.mi355_last_error()
+        need = cdll.mi355_fmha_key_weights_workspace_bytes(c, 32, 1000, 0)
+        assert need > 0
+        assert cdll.mi355_fmha_key_weights(c, P, P, 32, 1000, None, 0, scale, None, 0, None) == lib.ERR_BAD_ARGUMENT and word in cdll.mi355_last_error()
+
+
 def test_the_other_entry_points_refuse_bad_arguments(lib):
     cdll, c, big = lib.load(), cache(lib), 1 << 60
     row = 48 * 128

@@ -484,7 +484,8 @@ static int paged_queries_checked(const char* fn, const mi355_paged_kv* c, const 
     if (!paged_rows(c, Hq, S, last_rows))
         return fail(MI355_ERR_UNSUPPORTED, "%s: Hq / Hkv * S must be below 2^24, and below 2^16 for more rows than a sequence may have keys (got %d / %d * %d, %lld keys)", fn,
                     Hq, c->Hkv, S, (long long)c->max_pages * c->page_size);
-    if (!(scale > 0.f) || scale > 3.0e38f) return fail(MI355_ERR_BAD_ARGUMENT, "%s: scale must be positive and finite (got %g)", fn, (double)scale);
+    // (times log2 e it must be finite too)
+    if (!(scale > 0.f) || scale > 2.3e38f) return fail(MI355_ERR_BAD_ARGUMENT, "%s: scale must be positive and at most 2.3e38 (got %g)", fn, (double)scale);
     if (!aligned16(Q)) return fail(MI355_ERR_BAD_ARGUMENT, "%s: Q must be 16-byte aligned", fn);
     for (int i = 0; i < n; ++i)
         if (strides[i] < 0 || strides[i] % 8 != 0)
