@@ -601,6 +601,30 @@ def test_eviction_moves_nothing_into_pages_outside_the_pool(gpu, lens, budget, p
         assert torch.equal(x.nan_to_num(7.0), y.nan_to_num(7.0))
 
 
+@pytest.mark.parametrize("lens,max_pages,budget,recent,kind", [
+    ([32768, 20001], 512, 16384, 0, "rising"),        # all 32 keys of a thread, 16384 holes and as many movers
+    ([32767, 16387], 512, 5001, 64, "ties"),
+    ([30002, 300, 5000], 512, 257, 100, "any"),       # short sequences in a wide table: fewer keys a thread
+    ([16385], 257, 16384, 0, "rising"),               # the narrowest table of this kernel
+])
+def test_eviction_of_sixteen_to_thirty_two_thousand_keys(gpu, lens, max_pages, budget, recent, kind):
+    page, Hkv = 64, 2
+    cache = Cache(lens, Hkv, page, torch.bfloat16, max_pages=max_pages)
+    positions_of(cache, 11)
+    gen = torch.Generator().manual_seed(12)
+    for b, n in enumerate(lens):
+        pg, sl = cache.at(b)
+        if kind == "rising":
+            cache.weights[pg, :, sl] = torch.arange(n, device="cuda", dtype=torch.float32)[:, None].expand(n, Hkv)
+        elif kind == "ties":
+            cache.weights[pg, :, sl] = (torch.randint(0, 3, (n, Hkv), generator=gen).float() / 2).cuda()
+    want = evicted(cache, budget, recent)
+    got = ops.fine_evict_paged(*cache.args, cache.weights, cache.positions, budget, recent)
+    assert got.tolist() == want[0]
+    for x, y in zip((cache.kv, cache.weights, cache.positions), want[1:]):
+        assert torch.equal(x.nan_to_num(7.0), y.nan_to_num(7.0))
+
+
 def test_eviction_with_positions_of_the_whole_range(gpu):
     cache = Cache([100], 1, 16)
     pg, sl = cache.at(0)
