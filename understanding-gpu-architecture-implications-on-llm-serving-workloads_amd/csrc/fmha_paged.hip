@@ -35,7 +35,9 @@ constexpr int NTHREADS = WAVES * 64;
 constexpr int WAVE_BYTES = NSTAGE * STAGE_BYTES;
 constexpr int LDS_BYTES = WAVES * WAVE_BYTES;   // 128 KiB
 constexpr int kMeetBytes = 31 << 10;           // the rest of a CU's 160 KiB, less what the compiler may want
-constexpr int kMostScores = 32;               // columns of a kv head whose scores are kept for the account
+// columns of a kv head whose scores are kept for the account: those of one workgroup. us, kept / worked out again from K (which is what more columns take), 64 heads on 8:
+// 64 sequences of up to 8192 keys, 32 columns 409 / 554, 8 columns 293 / 519; 8 of 4096 keys, 32 columns 44.6 / 75.9; one of 8191, 32 columns 24.2 / 34.9
+constexpr int kMostScores = 32;
 constexpr int COPIES = 2 * (TILE_BYTES / 1024);
 constexpr int WINDOW = 32;                   // tiles whose addresses a wave holds at a time (64 half tiles, one a lane)
 constexpr float kLazyLog2 = 8.f;             // rescale only when a column maximum grows by more than 2^8

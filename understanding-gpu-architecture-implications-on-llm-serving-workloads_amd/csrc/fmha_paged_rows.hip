@@ -433,7 +433,8 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
         const int room = lim_min - 31 - (tile0 + kg) * TK;
         plain = min(plain, room < 0 ? 0 : room / (64 / NH) + 1);
         int h = 0;
-        // S is read by assembly (max3), in front of which the compiler puts no wait for the matrix pipe: 11 wait states for this instruction
+        // S is read by assembly (max3), in front of which the compiler puts no wait for the matrix pipe. It puts 8 wait states (s_nop 7) between a 16x16x32
+        // product and an instruction of its own that reads the result; these are 11. Another instruction in the product's place needs this looked at again.
         const auto pin_s = [&]() { asm volatile("s_nop 10" : "+v"(s[0][0]), "+v"(s[0][1]), "+v"(s[1][0]), "+v"(s[1][1])); };
         const auto softmax_phase = [&]() {
             landed(h);
