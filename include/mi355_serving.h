@@ -313,8 +313,8 @@ int mi355_fmha_fwd_noalloc(const void* Q, const void* K, const void* V, void* O,
  * Lengths, table and positions are read on the device: no call waits for it, and a captured call serves what the tensors hold when it
  * is replayed (they must not change while a call runs). No page may belong to two sequences of a call that writes it, to its weights among others.
  * Launches and workspaces are sized for max_pages, whatever the lengths are: a caller whose table is much wider than its sequences are long passes
- * the columns in use. B * Hkv <= 65535, max_pages * page_size <= 2^28, B * Hkv * (max_pages * page_size / 32 + 1) < 2^31 - 2^16; the strides of rows
- * below 2^24 elements, those of a page's rows together below 2^30.
+ * the columns in use. B * Hkv <= 65535, max_pages * page_size <= 2^28, B * Hkv * (max_pages * page_size / 32 + 1) < 2^31 - 2^16; strides of
+ * rows below 2^24 elements, page_size * row_stride below 2^30.
  *
  * The library allocates nothing for these calls: what *_workspace_bytes says (0: NULL will do) is the caller's, 16-byte aligned, its
  * contents irrelevant before and after; calls that share a workspace must be ordered on one stream. The reference has no counterpart: its caller grows
@@ -340,8 +340,8 @@ typedef struct mi355_paged_kv {
  * it. Sums and statistics are fp32, in an order that depends on the sizes and lengths alone; the probabilities are rounded to the element type for
  * the second product. What a row does not see has no influence on it, infinities and NaN included. new_lens of NULL with S rows and
  * a sequence shorter than S: its first rows see nothing. scale: positive, at most 2.3e38 (times log2 e it is finite), and such that no score passes
- * 2^26 (beyond, an exponent's argument in 32 bits is off by more than the 16 bits of a probability have room for). Hq / Hkv * S < 2^24 (2^16 where S is more than max_pages * page_size), and
- * B * Hq * S + B * Hkv * (max_pages * page_size / 256 + 1) < 2^24.
+ * 2^26 (beyond, an exponent's argument in 32 bits is off by more than the 16 bits of a probability have room for). Hq / Hkv * S < 2^24 (2^16
+ * where S is more than max_pages * page_size), and B * Hq * S + B * Hkv * (max_pages * page_size / 256 + 1) < 2^24.
  */
 size_t mi355_fmha_paged_workspace_bytes(const mi355_paged_kv* cache, int Hq, int S, int want_lse);
 int mi355_fmha_paged(const mi355_paged_kv* cache, const void* Q, void* O, float* LSE, int Hq, int S, const int64_t* strides, float scale,
@@ -372,8 +372,8 @@ int mi355_fmha_key_weights(const mi355_paged_kv* cache, const void* Q, const flo
  * the largest position that the kv head holds (position > largest - recent), then those of the largest weights (NaN lowest); of equals, the
  * lowest slots. The kept keys that lie behind the budget move, in order, into the slots of the dropped ones in front of it, with their
  * values, weights and positions, so the sequence is `budget` long afterwards and its keys lie in no particular order; each kv head keeps keys of its own. Slots
- * from `budget` on are left as they are. Slots of pages outside the pool hold no key and take none: where there are some in front of the budget, so many keys
- * fewer are kept. lens_out[b] = min(seq_lens[b], budget); lens_out may not overlap seq_lens, which is not written. Both
+ * from `budget` on are left as they are. Slots of pages outside the pool hold no key and take none: where there are some in front of the
+ * budget, so many keys fewer are kept. lens_out[b] = min(seq_lens[b], budget); lens_out may not overlap seq_lens, which is not written. Both
  * weights and key_positions are needed; new_lens is not read.
  */
 size_t mi355_cache_evict_workspace_bytes(const mi355_paged_kv* cache, int budget);

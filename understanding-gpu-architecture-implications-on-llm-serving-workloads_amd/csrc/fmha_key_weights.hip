@@ -298,8 +298,8 @@ hipError_t key_weights_dispatch(const mi355_paged_kv& c, const void* Q, const fl
     a.by_blocks = divisor_of(a.max_blocks);
     a.by_group = divisor_of(a.group);
     const dim3 grid((unsigned)key_weights_workgroups(c, Hq, Sq, last_rows));
-    // Eight waves of 32 keys where a CU has one or two workgroups (us, eight / four waves: 64 rows of 32/8 heads over 8191 keys 11.3 / 12.2, 1024
-    // rows 17.8 / 18.9), four of 64, which read the rows' tiles half as often, where more share one (2 x 32/8 heads, 4096 rows 164.6 / 159.9).
+    // Eight waves of 32 keys where a CU has one or two workgroups (us, eight / four waves: 64 rows of 32/8 heads over 8191 keys 10.2 / 10.5, 1024
+    // rows 16.8 / 17.0), four of 64, which read the rows' tiles half as often, where more share one (2 x 32/8 heads, 4096 rows 157.4 / 153.1).
     const bool few = (long)a.max_blocks * a.pairs * a.ranges <= 512;
     const auto launch = [&](auto type) {
         using T = decltype(type);

@@ -53,11 +53,12 @@ def fine_fmha_with_lse(q: Tensor, k: Tensor, v: Tensor, causal: bool, is_decode=
 #
 # Everything is read on the device: no call waits for it, and a captured call serves the lengths and tables that its tensors hold
 # when the graph is replayed. No page may belong to two sequences of a call that writes it, to its weights among others. Hq / Hkv * S is below
-# 2^24 (2^16 where S is more than max_pages * page_size); the other limits are those of include/mi355_serving.h. The reference keeps one growing tensor a layer instead (benchmarks/flashattn-cuda/modeling_llama.py:664-668).
+# 2^24 (2^16 where S is more than max_pages * page_size); the other limits are those of include/mi355_serving.h. The reference keeps one
+# growing tensor a layer instead (benchmarks/flashattn-cuda/modeling_llama.py:664-668).
 
 # The functions below call the extension module's own (which ask the dispatcher where a mode, a transform, a tracer or a gradient that is needed would not see
-# them otherwise); `torch.ops.fmha_unified.{finefmha_paged, finefmha_paged_lse, rope_paged, key_weights,
-# evict_paged}` are the same through torch's dispatcher.
+# them otherwise); `torch.ops.fmha_unified.{finefmha_paged, finefmha_paged_lse, rope_paged, key_weights, evict_paged}` are the same through torch's
+# dispatcher. Inference only: there is no backward.
 
 def fine_fmha_paged(q: Tensor, kv_pages: Tensor, block_table: Tensor, seq_lens: Tensor, new_lens: Optional[Tensor] = None,
                     weights: Optional[Tensor] = None) -> Tensor:
