@@ -109,7 +109,8 @@ class FinePagedKVCache:
 
     def table_in_use(self, rows=0):
         """The columns of the block table that the longest sequence needs, or one of `rows` keys, in steps of 256 keys: launches, workspaces and the choice
-        of kernels go by the width of the table that a call is given, and the pool's may be a thousand times what is in use."""
+        of kernels go by the width of the table that a call is given, and the pool's may be a thousand times what is in use. (A call that is captured keeps
+        its table: one that is replayed as the lengths go on needs as many columns as they will.)"""
         page = self.kv_pages.shape[2]
         step = -(-256 // page)
         return self.block_table[:, :-(-max(rows, 1, *self.lengths) // (step * page)) * step]
