@@ -831,6 +831,51 @@ def test_strides_that_mean_nothing_and_strides_that_are_too_large(gpu):
     assert torch.equal(ops.fine_fmha_paged(q, pool, one.table, one.lens), ops.fine_fmha_paged(q, *one.args))
 
 
+def test_as_many_sequences_as_a_call_takes(gpu):
+    """65528 (sequence, kv head) pairs: a call gives what calls of parts of the batch give."""
+    B, Hkv, page, P = 8191, 8, 16, 40
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    kv = torch.randn((B * P, 2 * Hkv, page, D), generator=gen, device="cuda", dtype=torch.float16)
+    table = torch.randperm(B * P, generator=gen, device="cuda").int().reshape(B, P)
+    lens = torch.randint(0, P * page + 1, (B,), generator=gen, device="cuda", dtype=torch.int32)
+    weights = torch.rand((B * P, Hkv, page), generator=gen, device="cuda")
+    positions = torch.randint(0, 5000, (B * P, Hkv, page), generator=gen, device="cuda", dtype=torch.int32)
+    parts = [slice(0, 3000), slice(3000, 8000), slice(8000, B)]
+    for S in (1, 40):                                              # one token; a chunk, whose account is worked out from the log-sum-exp
+        q = torch.randn((B, Hkv, S, D), generator=gen, device="cuda", dtype=torch.float16)
+        a, b = weights.clone(), weights.clone()
+        o, lse = ops.fine_fmha_paged_with_lse(q, kv, table, lens, weights=a)
+        for p in parts:
+            po, pl = ops.fine_fmha_paged_with_lse(q[p], kv, table[p], lens[p], weights=b)
+            # (a cut at another place: rounding of 16-bit probabilities and results, |v| <= 6, and of the sums)
+            assert ((o[p] - po).abs() <= 4 * 2.0 ** -11 * 6).all() and (lse[p] - pl).abs().nan_to_num(0.0).max() <= 1e-5
+            assert torch.equal(lse[p].isinf(), pl.isinf())
+        # a probability is off by 2^-16 of itself at most in each (a score and its row's log-sum-exp, 2^-17 each), their sum is below b
+        assert ((a - b).abs() <= 2 * 2.0 ** -16 * b + 1e-6).all()
+    two = [[t.clone() for t in (kv, weights, positions)] for _ in range(2)]
+    left = ops.fine_evict_paged(two[0][0], table, lens, two[0][1], two[0][2], 300, 40)
+    for p in parts:
+        assert torch.equal(left[p], ops.fine_evict_paged(two[1][0], table[p], lens[p], two[1][1], two[1][2], 300, 40))
+    assert all(torch.equal(x, y) for x, y in zip(*two)) and torch.equal(left, lens.clamp(max=300))
+    qkv = torch.randn((B, 2, 3 * Hkv, D), generator=gen, device="cuda", dtype=torch.float16)
+    t, other = torch.rand((5000, 64), generator=gen, device="cuda"), qkv.clone()
+    pos = torch.randint(0, 5000, (B, 2), generator=gen, device="cuda", dtype=torch.int32)
+    ops.fine_rope_paged(qkv, two[0][0], table, left, t, t, pos, Hkv, weights=two[0][1], key_positions=two[0][2])
+    for p in parts:
+        ops.fine_rope_paged(other[p], two[1][0], table[p], left[p], t, t, pos[p], Hkv, weights=two[1][1], key_positions=two[1][2])
+    assert torch.equal(qkv, other) and all(torch.equal(x, y) for x, y in zip(*two))
+
+
+def test_sequences_may_share_pages_that_are_only_read(gpu):
+    """A common beginning of two texts in the same pages, and a page that a sequence has twice."""
+    cache = Cache([320, 200, 97], 2, 16)
+    cache.table[1, :6] = cache.table[0, :6]
+    cache.table[2, 3] = cache.table[2, 1]
+    for S in (1, 40):
+        q = queries(cache, 8, S)
+        check_attention(cache, q, *ops.fine_fmha_paged_with_lse(q, *cache.args))
+
+
 def test_operators_through_the_dispatcher_are_the_same(gpu):
     cache = Cache([700, 31], 2, 16)
     q = queries(cache, 8, 2)
