@@ -380,6 +380,71 @@ size_t mi355_cache_evict_workspace_bytes(const mi355_paged_kv* cache, int budget
 int mi355_cache_evict(const mi355_paged_kv* cache, int budget, int recent, int32_t* lens_out, void* workspace, size_t workspace_bytes,
                       void* stream);
 
+/*
+ * A tree of drafted tokens: mi355_fmha_paged for S rows of which row i continues row parents[b*parents_batch + i] (0 <= parent < i; anything
+ * else: a root) and sees the keys in front of the draft, itself and the rows on its path to a root, instead of all rows in front of it. The drafted
+ * tokens are the sequence's last keys, in the order of the rows; new_lens as there. parents_batch: 0 for parents that all sequences share, or >= S. S <= 256.
+ * cache->weights is neither read nor written: no account is kept of drafted tokens. The other limits are those of mi355_fmha_paged. A chain (parent i - 1) sees what
+ * mi355_fmha_paged's rows see.
+ */
+size_t mi355_fmha_paged_tree_workspace_bytes(const mi355_paged_kv* cache, int Hq, int S);
+int mi355_fmha_paged_tree(const mi355_paged_kv* cache, const void* Q, void* O, float* LSE, int Hq, int S, const int64_t* strides, const int32_t* parents,
+                          int64_t parents_batch, float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The accepted path of such a tree closes ranks: of the last new_lens[b] keys of sequence b (new_lens is needed here; it may be larger than the sequence, whose
+ * first drafted tokens are then no keys), key seq_lens[b] - new_lens[b] + path[b*path_batch + j] moves to key seq_lens[b] - new_lens[b] + j (to key j where
+ * that is negative), with its value, and its weight and position where those are given. A path ascends; it ends in front of the first entry that does not,
+ * or is no drafted token that is a key. lens_out[b] = the keys in front of the draft and those of the path; seq_lens is not written and may not overlap lens_out.
+ * Keys behind the new length are left as they are. A key that moves from or to a page outside the pool does not move. length <= 2^28.
+ */
+int mi355_cache_keep_path(const mi355_paged_kv* cache, const int32_t* path, int length, int64_t path_batch, int32_t* lens_out, void* stream);
+
+/*
+ * ---- Packed batches ---------------------------------------------------------------------------------------------------------
+ *
+ * The tokens of sequences of different lengths lie one behind the other in one batch of `rows` rows: sequence b has rows offsets[b] .. offsets[b + 1] - 1, offsets being
+ * B + 1 numbers on the device that ascend from 0 (cut to 0 .. rows; one that is smaller than one in front of it counts as that). Rows behind the last sequence
+ * are no tokens. Everything is read on the device; launches go by B and rows alone.
+ *
+ * mi355_packed_plan: block tables and slot maps from the lengths of the requests. block_table, seq_lens (keys so far), free_pages, free_span and next_positions
+ * are read and brought up to date; offsets [B + 1], positions [rows], slots [rows] and taken [B] are written.
+ *   - free_pages [n_pages] is a ring: free_span[1] pages, the first at place free_span[0], are free. Pages are taken from its front and come back at its end.
+ *   - new_lens[b] (negative: 0) tokens come to sequence b, whose rows are offsets[b] .. as above. They are taken, taken[b] = new_lens[b], where the sequence has room for them
+ *     in its row of the table, they end within `rows`, and the ring holds the pages that they lack: the columns seq_lens[b] / page_size up to the last
+ *     key's whose entry is outside [0, n_pages) get one each, in the order of (sequence, column). A sequence that lacks none is taken whatever the others lack; one that lacks some is
+ *     where the ring holds what it and all sequences in front of it that have room lack. Otherwise taken[b] = 0 and the sequence stays as it is.
+ *   - seq_lens[b] and next_positions[b] (may be NULL) go on by taken[b]. Token t of the sequence gets position next_positions[b] + t (without one: the number of its
+ *     key) and slot page * page_size + row of the page; rows of sequences that are not taken, and those behind the last sequence, get -1 for both.
+ *   - Pages behind a sequence's end (columns from its new length / page_size, rounded up, on) go back to the ring, in the order of (sequence, column), and their entries become
+ *     -1. They can be taken by the next call. A sequence is released by seq_lens[b] = 0 and new_lens[b] = 0.
+ * No page may be held twice. B <= 65535, rows <= 2^28, max_pages * page_size <= 2^28, n_pages * page_size and B * max_pages < 2^31.
+ */
+size_t mi355_packed_plan_workspace_bytes(int B);
+int mi355_packed_plan(int32_t* block_table, int64_t table_stride, int32_t* seq_lens, const int32_t* new_lens, int32_t* next_positions, int32_t* free_pages,
+                      int32_t* free_span, int B, int max_pages, int n_pages, int page_size, int rows, int32_t* offsets, int32_t* positions, int32_t* slots,
+                      int32_t* taken, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * mi355_rope_paged for a packed batch: row t of the fused projection at qkv + t*x_row is a token at positions[t] whose rotated key and whose value go to slot slots[t] of
+ * the pool (page slots[t] / page_size, row slots[t] % page_size). A negative position: no token, the row stays as it is. A slot outside the pool: rotated, not
+ * filed. No two tokens have one slot. Of `pool`, block_table, seq_lens, new_lens, table_stride, max_pages and B are not used. rows < 2^24, n_pages * page_size < 2^31.
+ */
+int mi355_rope_packed(const mi355_paged_kv* pool, void* qkv, int rows, int q_heads, int keep_keys, int64_t x_row, const float* cos_table, const float* sin_table,
+                      const int32_t* positions, const int32_t* slots, int n_positions, void* stream);
+
+/*
+ * Attention of whole prompts: O = softmax(scale * Q K^T + mask) V of each sequence's rows over its own rows, causal (row i sees rows 0 .. i of its sequence) or
+ * not. Q, O [rows, Hq, 128], K, V [rows, Hkv, 128] with `strides` = q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head in elements (multiples of 8, not
+ * negative, rows' below 2^24; NULL: contiguous); slices of one fused projection will do. Query head h reads kv head h / (Hq / Hkv). LSE [Hq, rows] (may be NULL): the natural
+ * log-sum-exp. Rows that no sequence has give O = 0 and LSE = -inf. Sums and statistics are 32 bits wide; the probabilities are rounded to the element type for the
+ * second product. The same call gives the same bits. What a row does not see has no influence on it, infinities and NaN included. scale as in
+ * mi355_fmha_paged. (rows / 128 + B) * Hq < 2^30.
+ */
+size_t mi355_fmha_packed_workspace_bytes(int rows, int B, int Hq, int Hkv);
+int mi355_fmha_packed(const void* Q, const void* K, const void* V, void* O, float* LSE, const int32_t* offsets, int rows, int B, int Hq, int Hkv,
+                      const int64_t* strides, float scale, int causal, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Thread-local text for the last non-zero return of this thread ("" if none). */
 const char* mi355_last_error(void);
 

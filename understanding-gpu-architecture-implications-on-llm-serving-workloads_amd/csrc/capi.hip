@@ -451,6 +451,18 @@ static bool paged_rows(const mi355_paged_kv* c, int Hq, int S, int last_rows) {
     return Hq / c->Hkv * rows <= (rows <= max_len ? kMostWorkgroups : 65535);
 }
 
+// What a call needs of the pool itself
+static int pool_checked(const char* fn, const mi355_paged_kv* c) {
+    if (c->row_stride < 128 || c->row_stride % 8 != 0 || c->head_stride < 128 || c->head_stride % 8 != 0 || c->page_stride < 128 || c->page_stride % 8 != 0)
+        return fail(MI355_ERR_BAD_ARGUMENT, "%s: strides of the pages must be multiples of 8 elements, 128 or more (got %lld, %lld, %lld)", fn,
+                    (long long)c->page_stride, (long long)c->head_stride, (long long)c->row_stride);
+    if (c->row_stride >= (1 << 24) || c->row_stride * 2 * c->page_size > INT32_MAX)
+        return fail(MI355_ERR_UNSUPPORTED, "%s: row stride %lld of the pages is too large", fn, (long long)c->row_stride);
+    if (!aligned16(c->pages) || !aligned16(c->weights) || !aligned16(c->key_positions))
+        return fail(MI355_ERR_BAD_ARGUMENT, "%s: pages, weights and key_positions must be 16-byte aligned", fn);
+    return 0;
+}
+
 static int paged_checked(const char* fn, const mi355_paged_kv* c) {
     if (!c || !c->pages || !c->block_table || !c->seq_lens) return fail(MI355_ERR_BAD_ARGUMENT, "%s: null pointer", fn);
     if (c->dtype != MI355_DTYPE_FP16 && c->dtype != MI355_DTYPE_BF16) return fail(MI355_ERR_BAD_ARGUMENT, "%s: unknown dtype %d", fn, c->dtype);
@@ -464,16 +476,7 @@ static int paged_checked(const char* fn, const mi355_paged_kv* c) {
         return fail(MI355_ERR_UNSUPPORTED, "%s: %d sequences of up to %lld keys of %d heads are more than a call takes", fn, c->B, (long long)max_len, c->Hkv);
     if (c->B > 1 && c->table_stride < c->max_pages)
         return fail(MI355_ERR_BAD_ARGUMENT, "%s: rows of the block table overlap (stride %lld, %d entries)", fn, (long long)c->table_stride, c->max_pages);
-    const int64_t strides[3] = {c->page_stride, c->head_stride, c->row_stride};
-    for (int64_t x : strides)
-        if (x < 128 || x % 8 != 0)
-            return fail(MI355_ERR_BAD_ARGUMENT, "%s: strides of the pages must be multiples of 8 elements, 128 or more (got %lld, %lld, %lld)", fn,
-                        (long long)strides[0], (long long)strides[1], (long long)strides[2]);
-    if (c->row_stride >= (1 << 24) || c->row_stride * 2 * c->page_size > INT32_MAX)
-        return fail(MI355_ERR_UNSUPPORTED, "%s: row stride %lld of the pages is too large", fn, (long long)c->row_stride);
-    if (!aligned16(c->pages) || !aligned16(c->weights) || !aligned16(c->key_positions))
-        return fail(MI355_ERR_BAD_ARGUMENT, "%s: pages, weights and key_positions must be 16-byte aligned", fn);
-    return 0;
+    return pool_checked(fn, c);
 }
 
 static int paged_queries_checked(const char* fn, const mi355_paged_kv* c, const void* Q, int Hq, int S, int last_rows, const int64_t* strides, int n,
@@ -503,12 +506,12 @@ static int workspace_checked(const char* fn, size_t need, const void* workspace,
 
 size_t mi355_fmha_paged_workspace_bytes(const mi355_paged_kv* cache, int Hq, int S, int want_lse) {
     if (!paged_sizes(cache) || !paged_rows(cache, Hq, S, 0)) return 0;   // (the call is refused)
-    return mi355::fmha_paged_workspace(*cache, Hq, S, want_lse != 0);
+    return mi355::fmha_paged_workspace(*cache, Hq, S, want_lse != 0, false);
 }
 
-int mi355_fmha_paged(const mi355_paged_kv* cache, const void* Q, void* O, float* LSE, int Hq, int S, const int64_t* strides, float scale,
-                     void* workspace, size_t workspace_bytes, void* stream) {
-    const char* fn = "mi355_fmha_paged";
+// `parents`: the rows are a tree of drafted tokens (null otherwise)
+static int fmha_paged_impl(const char* fn, const mi355_paged_kv* cache, const void* Q, void* O, float* LSE, int Hq, int S, const int64_t* strides,
+                           const int32_t* parents, int64_t parents_batch, float scale, void* workspace, size_t workspace_bytes, void* stream) {
     if (int rc = paged_checked(fn, cache)) return rc;
     if (!O) return fail(MI355_ERR_BAD_ARGUMENT, "%s: null pointer", fn);
     const int64_t dense[6] = {(int64_t)Hq * S * 128, (int64_t)S * 128, 128, (int64_t)Hq * S * 128, (int64_t)S * 128, 128};
@@ -523,10 +526,33 @@ int mi355_fmha_paged(const mi355_paged_kv* cache, const void* Q, void* O, float*
                     (long long)cache->max_pages * cache->page_size);
     if ((S > 1 && st[5] < 128) || (Hq > 1 && st[4] < 128) || (cache->B > 1 && st[3] < 128))
         return fail(MI355_ERR_BAD_ARGUMENT, "%s: rows of O overlap (o strides %lld, %lld, %lld)", fn, (long long)st[3], (long long)st[4], (long long)st[5]);
-    if (int rc = workspace_checked(fn, mi355::fmha_paged_workspace(*cache, Hq, S, LSE != nullptr), workspace, workspace_bytes)) return rc;
+    if (int rc = workspace_checked(fn, mi355::fmha_paged_workspace(*cache, Hq, S, LSE != nullptr, parents != nullptr), workspace, workspace_bytes)) return rc;
     const long l[6] = {(long)st[0], (long)st[1], (long)st[2], (long)st[3], (long)st[4], (long)st[5]};
-    const hipError_t e = mi355::fmha_paged_dispatch(*cache, Q, O, LSE, Hq, S, l, scale, workspace, static_cast<hipStream_t>(stream));
+    const hipError_t e = mi355::fmha_paged_dispatch(*cache, Q, O, LSE, Hq, S, l, scale, parents, (long)parents_batch, workspace, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? 0 : hip_fail(e, fn);
+}
+
+int mi355_fmha_paged(const mi355_paged_kv* cache, const void* Q, void* O, float* LSE, int Hq, int S, const int64_t* strides, float scale,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+    return fmha_paged_impl("mi355_fmha_paged", cache, Q, O, LSE, Hq, S, strides, nullptr, 0, scale, workspace, workspace_bytes, stream);
+}
+
+size_t mi355_fmha_paged_tree_workspace_bytes(const mi355_paged_kv* cache, int Hq, int S) {
+    if (!paged_sizes(cache) || !paged_rows(cache, Hq, S, 0)) return 0;   // (the call is refused)
+    mi355_paged_kv c = *cache;
+    c.weights = nullptr;
+    return mi355::fmha_paged_workspace(c, Hq, S, true, true);
+}
+
+int mi355_fmha_paged_tree(const mi355_paged_kv* cache, const void* Q, void* O, float* LSE, int Hq, int S, const int64_t* strides, const int32_t* parents,
+                          int64_t parents_batch, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* fn = "mi355_fmha_paged_tree";
+    if (!cache || !parents) return fail(MI355_ERR_BAD_ARGUMENT, "%s: null pointer", fn);
+    if (S > mi355::kMostDrafted) return fail(MI355_ERR_UNSUPPORTED, "%s: a tree has at most %d tokens (got %d)", fn, mi355::kMostDrafted, S);
+    if (parents_batch != 0 && parents_batch < S) return fail(MI355_ERR_BAD_ARGUMENT, "%s: parents_batch must be 0 or >= S (got %lld)", fn, (long long)parents_batch);
+    mi355_paged_kv c = *cache;
+    c.weights = nullptr;   // (no account is kept of drafted tokens)
+    return fmha_paged_impl(fn, &c, Q, O, LSE, Hq, S, strides, parents, parents_batch, scale, workspace, workspace_bytes, stream);
 }
 
 int mi355_rope_paged(const mi355_paged_kv* cache, void* qkv, int S, int q_heads, int keep_keys, int64_t x_batch, int64_t x_row,
@@ -587,6 +613,109 @@ int mi355_cache_evict(const mi355_paged_kv* cache, int budget, int recent, int32
     if (int rc = workspace_checked(fn, mi355::evict_workspace(*cache, budget), workspace, workspace_bytes)) return rc;
     const hipError_t e = mi355::evict_dispatch(*cache, budget, recent, lens_out, workspace, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? 0 : hip_fail(e, fn);
+}
+
+int mi355_cache_keep_path(const mi355_paged_kv* cache, const int32_t* path, int length, int64_t path_batch, int32_t* lens_out, void* stream) {
+    const char* fn = "mi355_cache_keep_path";
+    if (int rc = paged_checked(fn, cache)) return rc;
+    if (!cache->new_lens || !path || !lens_out) return fail(MI355_ERR_BAD_ARGUMENT, "%s: null pointer", fn);
+    if (length < 1 || length > (1 << 28)) return fail(MI355_ERR_BAD_ARGUMENT, "%s: length of a path must be in 1 .. 2^28 (got %d)", fn, length);
+    if (path_batch < 0 || (cache->B > 1 && path_batch < length))
+        return fail(MI355_ERR_BAD_ARGUMENT, "%s: paths overlap (stride %lld, %d entries)", fn, (long long)path_batch, length);
+    if (lens_out < cache->seq_lens + cache->B && cache->seq_lens < lens_out + cache->B)
+        return fail(MI355_ERR_BAD_ARGUMENT, "%s: lens_out overlaps seq_lens", fn);
+    const hipError_t e = mi355::keep_path_dispatch(*cache, path, length, (long)path_batch, lens_out, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? 0 : hip_fail(e, fn);
+}
+
+// ---- packed batches ----
+size_t mi355_packed_plan_workspace_bytes(int B) { return B < 1 || B > 65535 ? 0 : mi355::packed_plan_workspace(B); }
+
+int mi355_packed_plan(int32_t* block_table, int64_t table_stride, int32_t* seq_lens, const int32_t* new_lens, int32_t* next_positions, int32_t* free_pages,
+                      int32_t* free_span, int B, int max_pages, int n_pages, int page_size, int rows, int32_t* offsets, int32_t* positions, int32_t* slots,
+                      int32_t* taken, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* fn = "mi355_packed_plan";
+    if (!block_table || !seq_lens || !new_lens || !free_pages || !free_span || !offsets || !taken || (rows > 0 && (!positions || !slots)))
+        return fail(MI355_ERR_BAD_ARGUMENT, "%s: null pointer", fn);
+    if (B < 1 || max_pages < 1 || n_pages < 1 || rows < 0)
+        return fail(MI355_ERR_BAD_ARGUMENT, "%s: B, max_pages, n_pages >= 1 and rows >= 0 required (got %d, %d, %d, %d)", fn, B, max_pages, n_pages, rows);
+    if (page_size < 16 || page_size % 16 != 0)
+        return fail(MI355_ERR_UNSUPPORTED, "%s: page_size must be a positive multiple of 16 (got %d)", fn, page_size);
+    if (B > 65535 || rows > (1 << 28) || (int64_t)max_pages * page_size > (1 << 28) || (int64_t)n_pages * page_size > INT32_MAX || n_pages > (1 << 30) ||
+        (int64_t)B * max_pages > INT32_MAX)
+        return fail(MI355_ERR_UNSUPPORTED, "%s: %d sequences of up to %lld keys, %lld slots and %d rows are more than a call takes", fn, B,
+                    (long long)max_pages * page_size, (long long)n_pages * page_size, rows);
+    if (B > 1 && table_stride < max_pages)
+        return fail(MI355_ERR_BAD_ARGUMENT, "%s: rows of the block table overlap (stride %lld, %d entries)", fn, (long long)table_stride, max_pages);
+    if (int rc = workspace_checked(fn, mi355::packed_plan_workspace(B), workspace, workspace_bytes)) return rc;
+    const hipError_t e = mi355::packed_plan_dispatch(block_table, (long)table_stride, seq_lens, new_lens, next_positions, free_pages, free_span, B, max_pages, n_pages,
+                                                     page_size, rows, offsets, positions, slots, taken, workspace, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? 0 : hip_fail(e, fn);
+}
+
+int mi355_rope_packed(const mi355_paged_kv* pool, void* qkv, int rows, int q_heads, int keep_keys, int64_t x_row, const float* cos_table, const float* sin_table,
+                      const int32_t* positions, const int32_t* slots, int n_positions, void* stream) {
+    const char* fn = "mi355_rope_packed";
+    if (!pool || !pool->pages || !qkv || !cos_table || !sin_table || !positions || !slots) return fail(MI355_ERR_BAD_ARGUMENT, "%s: null pointer", fn);
+    if (pool->dtype != MI355_DTYPE_FP16 && pool->dtype != MI355_DTYPE_BF16) return fail(MI355_ERR_BAD_ARGUMENT, "%s: unknown dtype %d", fn, pool->dtype);
+    if (rows < 1 || q_heads < 0 || n_positions < 1 || pool->Hkv < 1 || pool->n_pages < 1)
+        return fail(MI355_ERR_BAD_ARGUMENT, "%s: rows, n_positions, Hkv, n_pages >= 1 and q_heads >= 0 required", fn);
+    if (pool->page_size < 16 || pool->page_size % 16 != 0)
+        return fail(MI355_ERR_UNSUPPORTED, "%s: page_size must be a positive multiple of 16 (got %d)", fn, pool->page_size);
+    if (int rc = pool_checked(fn, pool)) return rc;
+    const int64_t heads = (int64_t)q_heads + 2 * (int64_t)pool->Hkv;
+    if (rows > kMostWorkgroups || heads > 65535 * 32 || (int64_t)pool->n_pages * pool->page_size > INT32_MAX)
+        return fail(MI355_ERR_UNSUPPORTED, "%s: too many tokens, heads or slots", fn);
+    if (x_row % 8 || (rows > 1 && x_row < heads * 128))
+        return fail(MI355_ERR_BAD_ARGUMENT, "%s: rows of qkv overlap or their stride is no multiple of 8 (%lld, %lld heads)", fn, (long long)x_row, (long long)heads);
+    if (!aligned16(qkv) || !aligned16(cos_table) || !aligned16(sin_table))
+        return fail(MI355_ERR_BAD_ARGUMENT, "%s: pointers must be 16-byte aligned", fn);
+    const hipError_t e = mi355::rope_packed_dispatch(*pool, qkv, rows, q_heads, keep_keys, (long)x_row, cos_table, sin_table, positions, slots, n_positions,
+                                                     static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? 0 : hip_fail(e, fn);
+}
+
+static bool packed_sizes(int rows, int B, int Hq, int Hkv) {
+    return rows >= 1 && B >= 1 && Hkv >= 1 && Hq >= Hkv && rows <= (1 << 28) && B <= (1 << 28) && Hq <= 65535 && mi355::packed_fits(rows, B, Hq);
+}
+
+size_t mi355_fmha_packed_workspace_bytes(int rows, int B, int Hq, int Hkv) { return packed_sizes(rows, B, Hq, Hkv) ? mi355::packed_workspace(rows, B) : 0; }
+
+static int fmha_packed_impl(const char* fn, const void* Q, const void* K, const void* V, void* O, float* LSE, const int32_t* offsets, int rows, int B, int Hq, int Hkv,
+                            const int64_t* strides, float scale, int causal, int dtype, void* workspace, size_t workspace_bytes, int variant, void* stream) {
+    if (!Q || !K || !V || !O || !offsets) return fail(MI355_ERR_BAD_ARGUMENT, "%s: null pointer", fn);
+    if (dtype != MI355_DTYPE_FP16 && dtype != MI355_DTYPE_BF16) return fail(MI355_ERR_BAD_ARGUMENT, "%s: unknown dtype %d", fn, dtype);
+    if (rows < 1 || B < 1 || Hq < 1 || Hkv < 1) return fail(MI355_ERR_BAD_ARGUMENT, "%s: rows, B, Hq, Hkv must be >= 1 (got %d, %d, %d, %d)", fn, rows, B, Hq, Hkv);
+    if (Hq % Hkv != 0) return fail(MI355_ERR_BAD_ARGUMENT, "%s: Hq (%d) must be a multiple of Hkv (%d)", fn, Hq, Hkv);
+    if (!packed_sizes(rows, B, Hq, Hkv)) return fail(MI355_ERR_UNSUPPORTED, "%s: %d rows of %d sequences and %d heads are more than a call takes", fn, rows, B, Hq);
+    if (!(scale > 0.f) || scale > 2.3e38f) return fail(MI355_ERR_BAD_ARGUMENT, "%s: scale must be positive and at most 2.3e38 (got %g)", fn, (double)scale);
+    const int64_t dense[8] = {(int64_t)Hq * 128, 128, (int64_t)Hkv * 128, 128, (int64_t)Hkv * 128, 128, (int64_t)Hq * 128, 128};
+    const int64_t* st = strides ? strides : dense;
+    for (int i = 0; i < 8; ++i)
+        if (st[i] < 0 || st[i] % 8 != 0)
+            return fail(MI355_ERR_BAD_ARGUMENT, "%s: stride %d is %lld; strides must be non-negative multiples of 8 elements", fn, i, (long long)st[i]);
+    for (int i = 0; i < 8; i += 2)
+        if (st[i] >= (1 << 24)) return fail(MI355_ERR_UNSUPPORTED, "%s: row strides must be below 2^24 elements (got %lld)", fn, (long long)st[i]);
+    if ((rows > 1 && st[6] < 128) || (Hq > 1 && st[7] < 128))
+        return fail(MI355_ERR_BAD_ARGUMENT, "%s: rows of O overlap (o strides %lld, %lld)", fn, (long long)st[6], (long long)st[7]);
+    if (!aligned16(Q) || !aligned16(K) || !aligned16(V) || !aligned16(O)) return fail(MI355_ERR_BAD_ARGUMENT, "%s: pointers must be 16-byte aligned", fn);
+    if (int rc = workspace_checked(fn, mi355::packed_workspace(rows, B), workspace, workspace_bytes)) return rc;
+    const mi355::FmhaStrides sd = {0, (long)st[1], (long)st[0], 0, (long)st[3], (long)st[2], 0, (long)st[5], (long)st[4], 0, (long)st[7], (long)st[6]};
+    const hipError_t e = mi355::packed_dispatch(Q, K, V, O, LSE, offsets, rows, B, Hq, Hkv, sd, scale, causal, dtype, workspace, variant, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? 0 : hip_fail(e, fn);
+}
+
+int mi355_fmha_packed(const void* Q, const void* K, const void* V, void* O, float* LSE, const int32_t* offsets, int rows, int B, int Hq, int Hkv,
+                      const int64_t* strides, float scale, int causal, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+    return fmha_packed_impl("mi355_fmha_packed", Q, K, V, O, LSE, offsets, rows, B, Hq, Hkv, strides, scale, causal, dtype, workspace, workspace_bytes, 0, stream);
+}
+
+int mi355_internal_fmha_packed_variant(const void* Q, const void* K, const void* V, void* O, float* LSE, const int32_t* offsets, int rows, int B, int Hq, int Hkv,
+                                       const int64_t* strides, float scale, int causal, int dtype, void* workspace, size_t workspace_bytes, int variant,
+                                       void* stream) {
+    const char* fn = "mi355_internal_fmha_packed_variant";
+    if (variant < 0 || variant > 2) return fail(MI355_ERR_BAD_ARGUMENT, "%s: unknown variant %d", fn, variant);
+    return fmha_packed_impl(fn, Q, K, V, O, LSE, offsets, rows, B, Hq, Hkv, strides, scale, causal, dtype, workspace, workspace_bytes, variant, stream);
 }
 
 const char* mi355_last_error(void) { return g_err; }

@@ -178,16 +178,82 @@ __device__ __forceinline__ void copy16_global_to_lds_at(const void* uniform_base
 // queries, which are a single block of rows of the first wave and are stored as they lie: through LDS they are a chain of its own behind the
 // item, and a branch in the other kernels costs those up to 2 %. us, through LDS / as they lie: 64 x 16/2 heads, 9 queries over 64 keys 17.1 /
 // 15.9, 24 x 32/8, 16 over 64 13.8 / 13.1, 12 x 64/8, 16 over 128 18.2 / 17.6.
-enum { kOneWalk = 0, kRanges = 1, kRangesF32 = 2, kFewRows = 3 };
+// kPacked: sequences of different lengths one behind the other in one batch; the work items are those of a list that packed_items_kernel made on the
+// device (below), and a row whose result is NaN is worked out again (see packed_row).
+enum { kOneWalk = 0, kRanges = 1, kRangesF32 = 2, kFewRows = 3, kPacked = 4 };
 constexpr int kFewRowsMax = 16;
+
+// The list of a packed batch: `entries` q tiles {first row of the sequence, its rows, q tile, 0}, those with the most keys first
+struct PackedItems {
+    const int4v* list;
+    const int* entries;
+    long rows;   // of the batch: row stride of LSE
+};
+// what a work item knows beside the others' fields
+template <bool PACKED>
+struct PackedItem {};
+template <>
+struct PackedItem<true> {
+    int rows;       // of its sequence
+    float* lse;     // of its head and the sequence's first row
+};
+
+// One row of a packed batch in 32 bits, key by key, with nothing of the keys that it does not see: 64 keys at a time, a lane scores one of them and then sums 2 of the 128 outputs.
+// For rows whose products came out as NaN: where an unseen value is infinite or NaN, 0 * v is not nothing. A row that sees such values comes out as it should
+// too, and ends at once where nothing can come of it but NaN.
+template <typename T>
+__device__ __forceinline__ void packed_row(const T* q, const T* K, const T* V, long k_row, long v_row, int keys, float scale_log2, T* out) {
+    using V8 = typename Elem<T>::v8;
+    using V2 = typename Elem<T>::v2;
+    const int lane = threadIdx.x & 63;
+    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+    for (int key0 = 0; key0 < keys; key0 += 64) {
+        const int n = min(64, keys - key0);
+        const T* kp = K + (key0 + min(lane, n - 1)) * k_row;
+        float s = 0.f;
+#pragma unroll 4
+        for (int d = 0; d < fmha::D; d += 8) {
+            const V8 a = *(const V8*)(q + d), b = *(const V8*)(kp + d);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s = __builtin_fmaf((float)a[e], (float)b[e], s);
+        }
+        s *= scale_log2;
+        if (lane >= n) s = -INFINITY;
+        float top = s;
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+        const float m_new = fmaxf(m, top), m_use = m_new == -INFINITY ? 0.f : m_new;
+        const float keep = fmha::fast_exp2(m - m_use), p = lane < n ? fmha::fast_exp2(s - m_use) : 0.f;
+        m = m_new;
+        l = l * keep + p;
+        o0 *= keep;
+        o1 *= keep;
+        for (int j = 0; j < n; ++j) {
+            const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p), j));
+            const V2 v = *(const V2*)(V + (key0 + j) * v_row + 2 * lane);
+            o0 = __builtin_fmaf(w, (float)v[0], o0);
+            o1 = __builtin_fmaf(w, (float)v[1], o1);
+        }
+        if (__builtin_amdgcn_ballot_w64(o0 == o0 || o1 == o1) == 0) break;
+    }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) l += __shfl_xor(l, off, 64);
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    V2 v;
+    v[0] = (T)(o0 * inv);
+    v[1] = (T)(o1 * inv);
+    *(V2*)(out + 2 * lane) = v;
+}
+
 template <typename T, int QB, int MODE = kOneWalk>
 __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __restrict__ Q, const T* __restrict__ K,
                                                                const T* __restrict__ V, T* __restrict__ O,
                                                                float* __restrict__ LSE, int B, int Hq, int Hkv, int Sq,
                                                                int Sk, float scale_log2, int causal, int kv_valid,
-                                                               int q_tiles, FmhaStrides sd, int segments, int seg_len, ItemMap map) {
+                                                               int q_tiles, FmhaStrides sd, int segments, int seg_len, ItemMap map,
+                                                               PackedItems packed) {
     using namespace fmha;
-    constexpr bool SEG = MODE == kRanges || MODE == kRangesF32;
+    constexpr bool SEG = MODE == kRanges || MODE == kRangesF32, PACKED = MODE == kPacked;
     using V8 = typename Elem<T>::v8;
     using V4 = typename Elem<T>::v4;
     constexpr int NWAVES = 8;
@@ -209,7 +275,7 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
     const int c16 = lane & 15;
 
     // ---- work items -------------------------------------------------------------------------------------------------
-    struct Item {
+    struct Item : PackedItem<PACKED> {
         const T *Qh, *Kh, *Vh;
         T* Oh;
         int lse_row;             // (batch, q head), of a range too: row of LSE / Sq
@@ -228,6 +294,29 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
         Item it;
         int b, hkv, hq, q_tile;
         it.n_tiles = 0;
+        if constexpr (PACKED) {   // the list's entries are ranked, the heads of an entry are what the (batch, head) groups are elsewhere
+            const int x = blockIdx.x & ((1 << map_.xcd_shift) - 1), wl = blockIdx.x >> map_.xcd_shift;
+            const int u = round * map_.wgs + ((round & 1) ? map_.wgs - 1 - wl : wl);
+            const int rank = divide(u, map_.by_rank), rem = u - rank * map_.per_rank;
+            const int4v entry = packed.list[min(rank, q_tiles_ - 1)];   // (q_tiles: the most entries that there may be)
+            it.exists = rank < *packed.entries;
+            if (!it.exists) return it;
+            const int gl = divide(rem, map_.by_group), kvh = x * map_.groups_per_xcd + gl;
+            const int head = kvh * map_.group + rem - gl * map_.group;
+            const long row0 = entry[0];
+            it.rows = entry[1];
+            it.lse = LSE == nullptr ? nullptr : LSE + head * packed.rows + row0;
+            it.lse_row = 0;
+            it.q_block0 = entry[2] * BM;
+            it.kv_valid = it.rows;
+            it.shift = 0;
+            it.Qh = Q + row0 * sd.q_row + head * sd.q_head;
+            it.Kh = K + row0 * sd.k_row + kvh * sd.k_head;
+            it.Vh = V + row0 * sd.v_row + kvh * sd.v_head;
+            it.Oh = O + row0 * sd.o_row + head * sd.o_head;
+            it.n_tiles = ((causal ? min(it.q_block0 + BM, it.rows) : it.rows) + BN - 1) / BN;
+            return it;
+        }
         it.exists = fmha_work_item(blockIdx.x, round, q_tiles_, map_, b, hkv, hq, q_tile);
         if (!it.exists) return it;
         it.q_block0 = q_tile * BM;
@@ -274,11 +363,18 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
     // steps of an item in which the pair that is copied (tiles j + 3 of K, j + 2 of V) is made of full tiles
     auto fast_steps = [](int n_tiles, int kv_valid) { return min(min(n_tiles, kv_valid / BN) - 3, n_tiles - 1); };
     Item cur = item_of(0);   // a launch has no more workgroups than items
+    if constexpr (PACKED) {  // (than there may be)
+        if (!cur.exists) return;
+    }
+    const auto rows_of = [&](const Item& it) {
+        if constexpr (PACKED) return it.rows;
+        else return Sq;
+    };
     int q_wave0 = cur.q_block0 + wave * WQ;
 
     // Q fragments (B operand of the first product): lane holds Q[16 qb + c][32 ks + 8 g .. +7]
     V8 qf[QB][4];
-    auto load_q = [&](const T* Qh, int q_wave0) {
+    auto load_q = [&](const T* Qh, int q_wave0, int Sq) {
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) {
             const int qrow = min(q_wave0 + qb * 16 + c16, Sq - 1);
@@ -347,7 +443,7 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
     }
 
     float4v o[8][QB];
-    constexpr bool kSumOnMatrixPipe = std::is_same<T, half_t>::value;
+    constexpr bool kSumOnMatrixPipe = std::is_same<T, half_t>::value && !PACKED;
     float4v l_acc[QB];
     V8 ones;
 #pragma unroll
@@ -586,9 +682,9 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
     // starts there, also where that means that its first pairs can only leave behind the last barrier of the item in front (a second copy
     // of the general step in front of the loop makes the 256-query instantiation spill 400 bytes a lane).
     MI355_TL(unsigned long long tl_tiles = 0, tl_end = 0, tl_between = 0;)   // cycles from an item's last barrier to the first of the next
-    load_q(cur.Qh, q_wave0);
+    load_q(cur.Qh, q_wave0, rows_of(cur));
     if (cur.n_tiles > 0) issue_first_pairs();
-    const bool more_items = (long)q_tiles * Hq * B * (SEG ? segments : 1) > gridDim.x;   // of the launch, than it has workgroups
+    const bool more_items = (PACKED ? (long)*packed.entries * Hq : (long)q_tiles * Hq * B * (SEG ? segments : 1)) > gridDim.x;   // of the launch, than it has workgroups
     bool landed = false;   // the current item's first pairs and Q fragments have been waited for
     for (int round = 0;;) {
 #pragma unroll
@@ -662,7 +758,7 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
             if (more_items) {
                 const Item next = item_from(listed_words(round));
                 more = next.exists;
-                if (more) load_q(next.Qh, next.q_block0 + wave * WQ);
+                if (more) load_q(next.Qh, next.q_block0 + wave * WQ, rows_of(next));
             }
             softmax_tile(s, n_tiles - 1, pf, std::integral_constant<int, -2>{});
             if (n_tiles == 2 && n_next > 0) {   // two tiles have no step that copies pair n_tiles: K(0) of the next item
@@ -688,14 +784,16 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
             if (more_items) {
                 const Item next = item_from(listed_words(round));
                 more = next.exists;
-                if (more) load_q(next.Qh, next.q_block0 + wave * WQ);
+                if (more) load_q(next.Qh, next.q_block0 + wave * WQ, rows_of(next));
             }
         }
 
         // what the epilogue needs of the item just finished, then on to the next one
         T* const o_item = cur.Oh;
         const int q_item0 = q_wave0;
-        float* const lse_item = LSE == nullptr ? nullptr : LSE + (long)cur.lse_row * Sq;
+        float* lse_item = LSE == nullptr ? nullptr : LSE + (long)cur.lse_row * Sq;
+        const int item_rows = rows_of(cur);
+        if constexpr (PACKED) lse_item = cur.lse;
         if (more) {
             landed = n_next > 0;
             ring = landed ? ring + cur.n_tiles : 0;
@@ -719,9 +817,10 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
         };
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) {
-            if (q_item0 + qb * 16 >= Sq) break;   // no such rows (a few queries are done 0.5 us sooner for it)
+            if (q_item0 + qb * 16 >= item_rows) break;   // no such rows (a few queries are done 0.5 us sooner for it)
             const float l_tot = kSumOnMatrixPipe ? l_acc[qb][0] : quad_sum(l_acc[qb][0]);
-            const float inv = (l_tot > 0.f) ? 1.f / l_tot : 0.f;
+            float inv = (l_tot > 0.f) ? 1.f / l_tot : 0.f;
+            if constexpr (PACKED) inv = l_tot != 0.f ? 1.f / l_tot : 0.f;   // (a sum that is NaN stays one)
             if constexpr (MODE == kFewRows) {
                 if (r16 < Sq) {
                     T* const row = o_item + r16 * o_row + 4 * r4;
@@ -754,14 +853,30 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
                 *(MI355_LDS V4*)(mine + (((2 * db + (r4 >> 1)) ^ r16) << 4) + (r4 & 1) * 8) = v;
             }
             const int q_first = q_item0 + qb * 16;
-            if (lse_item != nullptr && r4 == 0 && q_first + r16 < Sq)
-                lse_item[q_first + r16] = (l_tot > 0.f) ? (m_run[qb] * scale_log2 + __builtin_log2f(l_tot)) * 0.69314718055994531f : -INFINITY;
+            if (lse_item != nullptr && r4 == 0 && q_first + r16 < item_rows)
+                lse_item[q_first + r16] = (PACKED ? l_tot != 0.f : l_tot > 0.f) ? (m_run[qb] * scale_log2 + __builtin_log2f(l_tot)) * 0.69314718055994531f : -INFINITY;
             V8 row[4];
 #pragma unroll
             for (int a = 0; a < 4; ++a) row[a] = *(MI355_LDS const V8*)(park_row(4 * a + r4) + ((r16 ^ (4 * a + r4)) << 4));
 #pragma unroll
             for (int a = 0; a < 4; ++a)
-                if (q_first + 4 * a + r4 < Sq) *(V8*)(o_item + (q_first + 4 * a + r4) * o_row + 8 * r16) = row[a];
+                if (q_first + 4 * a + r4 < item_rows) *(V8*)(o_item + (q_first + 4 * a + r4) * o_row + 8 * r16) = row[a];
+            if constexpr (PACKED) {
+                bool nan = false;
+#pragma unroll
+                for (int db = 0; db < 8; ++db)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) nan = nan || o[db][qb][e] != o[db][qb][e];
+                uint64_t lanes = __builtin_amdgcn_ballot_w64(nan && q_first + r16 < item_rows);
+                if (lanes != 0) {
+                    const Item done = item_of(round - 1);
+                    uint32_t again = (uint32_t)(lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) & 0xffff;
+                    for (; again != 0; again &= again - 1) {
+                        const int i = q_first + __builtin_ctz(again);
+                        packed_row<T>(done.Qh + i * sd.q_row, done.Kh, done.Vh, sd.k_row, sd.v_row, causal ? i + 1 : done.rows, scale_log2, done.Oh + i * o_row);
+                    }
+                }
+            }
         }
         if (!more) break;
     }
@@ -808,7 +923,7 @@ static hipError_t launch_fmha_pingpong(const T* Q, const T* K, const T* V, T* O,
     if (((long)Hkv * B) % 8 == 0 && blocks >= 8) blocks &= ~7L;
     const float scale_log2 = scale * 1.4426950408889634f;
     kern<<<dim3((unsigned)blocks), dim3(512), LDS, stream>>>(Q, K, V, O, LSE, B, Hq, Hkv, Sq, Sk, scale_log2, causal, kv_valid,
-                                                             q_tiles, sd, 1, 0, item_map(B, Hq, Hkv, 1, blocks));
+                                                             q_tiles, sd, 1, 0, item_map(B, Hq, Hkv, 1, blocks), PackedItems{});
     return hipGetLastError();
 }
 
@@ -1027,7 +1142,7 @@ static hipError_t launch_fmha_segmented(const T* Q, const T* K, const T* V, T* O
     if (((long)Hkv * B * segments) % 8 == 0 && blocks >= 8) blocks &= ~7L;
     const float scale_log2 = scale * 1.4426950408889634f;
     kern<<<dim3((unsigned)blocks), dim3(512), LDS, stream>>>(Q, K, V, reinterpret_cast<T*>(o_part), lse_part, B, Hq, Hkv, Sq, Sk, scale_log2, causal, kv_valid,
-                                                             q_tiles, sd, segments, seg_len, item_map(B, Hq, Hkv, segments, blocks));
+                                                             q_tiles, sd, segments, seg_len, item_map(B, Hq, Hkv, segments, blocks), PackedItems{});
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     auto merge = fmha_merge_segments_kernel<T, P, SEG == kRangesF32 ? kMaxSegmentsF32 : kMaxSegments>;
     merge<<<dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, stream>>>(o_part, lse_part, O, LSE, B, Hq, Sq, segments, sd);
@@ -1111,6 +1226,167 @@ hipError_t fmha_fwd_dispatch(const void* Q, const void* K, const void* V, void* 
     if (dtype == MI355_DTYPE_BF16)
         return fmha_fwd_dispatch_t<bf16_t>(Q, K, V, O, LSE, B, Hq, Hkv, Sq, Sk, scale, causal, kv_valid_len, sd, variant, ws, stream);
     return fmha_fwd_dispatch_t<half_t>(Q, K, V, O, LSE, B, Hq, Hkv, Sq, Sk, scale, causal, kv_valid_len, sd, variant, ws, stream);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// A packed batch: sequences of different lengths, rows offsets[b] .. offsets[b + 1] - 1 of one batch each, known to the device only. Its first kernel makes the
+// list of q tiles, ordered by the keys that they see (a counting sort: of equal ones in no particular order, which decides which workgroup takes which, and nothing
+// else), and writes zeros to the rows that no sequence has; the second is the kernel above, which deals the list's entries out like q tiles of one sequence.
+// ---------------------------------------------------------------------------------------------------------------
+namespace packed {
+constexpr int THREADS = 1024, WAVES = THREADS / 64;
+constexpr int BINS = 1024;     // of key tiles, the heaviest first
+constexpr int kRowsAWorkgroup = 64;   // rows behind the last sequence
+constexpr int kMostTails = 256;
+
+// running maximum of a value a lane over the lanes up to this one
+__device__ __forceinline__ int wave_running_max(int x) {
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int y = __shfl_up(x, off, 64);
+        if ((int)(threadIdx.x & 63) >= off) x = max(x, y);
+    }
+    return x;
+}
+}  // namespace packed
+
+struct PackedList {
+    const int* offsets;
+    int4v* list;
+    int* entries;
+    int B, rows, tile, most, causal, shift;   // tile: rows of a q tile; most: entries that there may be; shift: key tiles of a bin
+};
+
+// Workgroup 0 makes the list, the others write zeros (O, LSE = -inf) to rows in front of the first sequence and behind the last
+template <typename T>
+__global__ __launch_bounds__(packed::THREADS) void packed_items_kernel(PackedList p, T* O, float* LSE, int Hq, long o_row, long o_head) {
+    using namespace packed;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const auto row_of = [&](int b) { return min(max(p.offsets[b], 0), p.rows); };
+    if (blockIdx.x > 0) {
+        // rows r .. of `row_of(0)` in front and behind: a wave a (row, head)
+        const int begin = row_of(0), end = row_of(p.B);
+        for (int r = (int)(blockIdx.x - 1) * kRowsAWorkgroup; r < p.rows; r += (int)(gridDim.x - 1) * kRowsAWorkgroup) {
+            if (r >= begin && r + kRowsAWorkgroup <= end) continue;
+            for (int i = tid; i < kRowsAWorkgroup * Hq * 16; i += THREADS) {
+                const int d = (i & 15) * 8, head = (i >> 4) % Hq, row = r + (i >> 4) / Hq;
+                if (row >= p.rows || (row >= begin && row < end)) continue;
+                *(int4v*)(O + row * o_row + head * o_head + d) = int4v{0, 0, 0, 0};
+                if (LSE != nullptr && d == 0) LSE[(long)head * p.rows + row] = -INFINITY;
+            }
+        }
+        return;
+    }
+    __shared__ int bins[BINS], sums[WAVES], tops[WAVES];
+    bins[tid] = 0;
+    static_assert(BINS == THREADS, "a bin a thread");
+    // Offsets that descend are taken for the largest one in front of them, so that no two sequences have a row in common. Each group of 1024 sequences
+    // needs the largest offset in front of it.
+    const auto each = [&](auto f) {   // f(first row, rows, q tile): a sequence of one tile by its lane, those of more by the whole wave
+        int front = 0;
+        for (int b0 = 0; b0 < p.B; b0 += THREADS) {
+            const int b = b0 + tid;
+            int start = b < p.B ? row_of(b) : 0, end = b < p.B ? row_of(b + 1) : 0;
+            start = wave_running_max(start);
+            if (p.B > 64) {   // (the waves of a group)
+                __syncthreads();
+                if (lane == 63) tops[wave] = start;
+                __syncthreads();
+                for (int w = 0; w < wave; ++w) start = max(start, tops[w]);
+                start = max(start, front);
+                for (int w = 0; w < WAVES; ++w) front = max(front, tops[w]);
+            }
+            const int n = b < p.B ? max(end - start, 0) : 0, tiles = (n + p.tile - 1) / p.tile;
+            if (tiles == 1) f(start, n, 0);
+            for (uint64_t left = __builtin_amdgcn_ballot_w64(tiles > 1); left != 0; left &= left - 1) {
+                const int i = __builtin_ctzll(left);
+                const int s = __builtin_amdgcn_readlane(start, i), m = __builtin_amdgcn_readlane(n, i), t = __builtin_amdgcn_readlane(tiles, i);
+                for (int k = lane; k < t; k += 64) f(s, m, k);
+            }
+        }
+    };
+    const auto bin_of = [&](int n, int k) {
+        const int keys = p.causal ? min((k + 1) * p.tile, n) : n;
+        return BINS - 1 - min(((keys + fmha::BN - 1) / fmha::BN - 1) >> p.shift, BINS - 1);
+    };
+    __syncthreads();
+    each([&](int, int n, int k) { atomicAdd(&bins[bin_of(n, k)], 1); });
+    __syncthreads();
+    const int mine = bins[tid];
+    int incl = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int y = __shfl_up(incl, off, 64);
+        if (lane >= off) incl += y;
+    }
+    if (lane == 63) sums[wave] = incl;
+    __syncthreads();
+    int front = 0, all = 0;
+    for (int w = 0; w < WAVES; ++w) {
+        if (w < wave) front += sums[w];
+        all += sums[w];
+    }
+    bins[tid] = front + incl - mine;
+    if (tid == 0) *p.entries = min(all, p.most);
+    __syncthreads();
+    each([&](int start, int n, int k) {
+        const int at = atomicAdd(&bins[bin_of(n, k)], 1);
+        if (at < p.most) p.list[at] = int4v{start, n, k, 0};
+    });
+}
+
+// q tiles of `tile` rows that B sequences of `rows` rows in all can have
+static long packed_entries(int rows, int B, int tile) { return (long)rows / tile + std::min(B, rows); }
+
+size_t packed_workspace(int rows, int B) { return 16 * ((size_t)packed_entries(rows, B, 128) + 1); }
+
+template <typename T, int QB>
+static hipError_t launch_packed(const T* Q, const T* K, const T* V, T* O, float* LSE, const int* offsets, int rows, int B, int Hq, int Hkv, const FmhaStrides& sd,
+                                float scale, int causal, void* workspace, hipStream_t stream) {
+    constexpr int BM = 128 * QB, LDS = 8 * fmha::TILE_BYTES;
+    auto kern = fmha_fwd_pingpong_kernel<T, QB, kPacked>;
+    static DynamicLdsOnce lds_once;
+    if (hipError_t e = lds_once.ensure(reinterpret_cast<const void*>(kern), LDS); e != hipSuccess) return e;
+    int cus = 0;
+    if (hipError_t e = compute_units(cus); e != hipSuccess) return e;
+    PackedList p = {};
+    p.offsets = offsets;
+    p.entries = (int*)workspace;
+    p.list = (int4v*)workspace + 1;
+    p.B = B;
+    p.rows = rows;
+    p.tile = BM;
+    p.most = (int)packed_entries(rows, B, BM);
+    p.causal = causal;
+    while ((rows + fmha::BN - 1) / fmha::BN >> p.shift > packed::BINS) ++p.shift;
+    const int tails = std::min(packed::kMostTails, (rows + packed::kRowsAWorkgroup - 1) / packed::kRowsAWorkgroup);
+    packed_items_kernel<T><<<dim3(1 + tails), dim3(packed::THREADS), 0, stream>>>(p, O, LSE, Hq, sd.o_row, sd.o_head);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    const long items = (long)p.most * Hq;
+    long blocks = items < cus ? items : cus;
+    if (Hkv % 8 == 0 && blocks >= 8) blocks &= ~7L;
+    kern<<<dim3((unsigned)blocks), dim3(512), LDS, stream>>>(Q, K, V, O, LSE, 1, Hq, Hkv, rows, rows, scale * 1.4426950408889634f, causal, rows, p.most, sd, 1, 0,
+                                                             item_map(1, Hq, Hkv, 1, blocks), PackedItems{p.list, p.entries, rows});
+    return hipGetLastError();
+}
+
+template <typename T>
+static hipError_t packed_t(const void* Q, const void* K, const void* V, void* O, float* LSE, const int* offsets, int rows, int B, int Hq, int Hkv,
+                           const FmhaStrides& sd, float scale, int causal, void* workspace, int variant, hipStream_t stream) {
+    int cus = 0;
+    if (hipError_t e = compute_units(cus); e != hipSuccess) return e;
+    const int mean = (rows + B - 1) / B;
+    if (variant == 0) variant = one_walk_us(2, cus, B, Hq, mean, mean, causal, mean) < one_walk_us(1, cus, B, Hq, mean, mean, causal, mean) ? 2 : 1;
+    const auto launch = variant == 2 ? &launch_packed<T, 2> : &launch_packed<T, 1>;
+    return launch((const T*)Q, (const T*)K, (const T*)V, (T*)O, LSE, offsets, rows, B, Hq, Hkv, sd, scale, causal, workspace, stream);
+}
+
+bool packed_fits(int rows, int B, int Hq) { return packed_entries(rows, B, 128) * Hq <= INT32_MAX / 2; }
+
+hipError_t packed_dispatch(const void* Q, const void* K, const void* V, void* O, float* LSE, const int* offsets, int rows, int B, int Hq, int Hkv,
+                           const FmhaStrides& sd, float scale, int causal, int dtype, void* workspace, int variant, hipStream_t stream) {
+    const auto run = dtype == MI355_DTYPE_BF16 ? &packed_t<bf16_t> : &packed_t<half_t>;
+    return run(Q, K, V, O, LSE, offsets, rows, B, Hq, Hkv, sd, scale, causal, workspace, variant, stream);
 }
 
 }  // namespace mi355

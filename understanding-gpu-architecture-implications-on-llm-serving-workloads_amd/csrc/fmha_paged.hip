@@ -34,6 +34,7 @@ constexpr int WAVES = 4, NSTAGE = 2;
 constexpr int NTHREADS = WAVES * 64;
 constexpr int WAVE_BYTES = NSTAGE * STAGE_BYTES;
 constexpr int LDS_BYTES = WAVES * WAVE_BYTES;   // 128 KiB
+constexpr int kTreeBytes = (4 * (kMostDrafted + 32 * kTreeWords) + 1023) / 1024 * 1024;   // parents and words of a tree; what follows is aligned to 1024 bytes
 constexpr int kMeetBytes = 31 << 10;           // the rest of a CU's 160 KiB, less what the compiler may want
 // columns of a kv head whose scores are kept for the account: those of one workgroup. us, kept / worked out again from K (which is what more columns take), 64 heads on 8:
 // 64 sequences of up to 8192 keys, 32 columns 409 / 554, 8 columns 293 / 519; 8 of 4096 keys, 32 columns 44.6 / 75.9; one of 8191, 32 columns 24.2 / 34.9
@@ -69,6 +70,7 @@ struct PagedAttn {
     int Hq, Sq, group, ncols, col_block;   // columns of a kv head, and of a workgroup
     int workgroups, min_tiles, direct, max_tiles;
     int apart;        // the waves' results meet behind the stages
+    PagedTree tree;   // of the drafted tokens, where they are one
     float scale_log2;
     int chunks;       // of 256 keys, of the longest sequence
     Divisor by_sq, by_hkv, by_ncols, by_chunks;
@@ -137,8 +139,8 @@ struct Lengths {
 }  // namespace pdec
 
 // Grid: (workgroups, blocks of columns). NB: blocks of 16 columns of a workgroup. SCORES: the scores are kept for the
-// account.
-template <typename T, int NB, bool SCORES>
+// account. TREE: the rows are drafted tokens of a.tree: in front of the draft a tile needs no mask, from there on a row's word has a bit a key.
+template <typename T, int NB, bool SCORES, bool TREE>
 __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, PagedAttn a) {
     using namespace pdec;
     using V8 = typename Elem<T>::v8;
@@ -293,6 +295,8 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) qf[nb][ks] = *(const V8*)(qp + ks * 32);
         }
+        const int base = len - n_new;       // (TREE) key of the first drafted token
+        if constexpr (TREE) lim_min = min(lim_min, base - 1);
         int row_min = a.Sq, row_max = -1;   // rows of the columns of this wave
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) row_min = min(row_min, qrow[nb]), row_max = max(row_max, qrow[nb]);
@@ -311,6 +315,24 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
         // iteration, for everything in flight
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) asm volatile("" : "+v"(qf[nb][0]), "+v"(qf[nb][1]), "+v"(qf[nb][2]), "+v"(qf[nb][3]));
+
+        // the words of this workgroup's columns, where the part reaches the draft
+        __shared__ int up[TREE ? kMostDrafted : 1];
+        __shared__ uint32_t words[TREE ? 32 * kTreeWords : 1];
+        if constexpr (TREE) {
+            if ((now.tile0 + n) * TK > base) {
+                const int* parents = a.tree.parents + b * a.tree.batch;
+                for (int i = tid; i < a.Sq; i += NTHREADS) up[i] = parents[i];
+                __syncthreads();
+                if (tid < ncols) {
+                    const int col = col0 + tid;
+                    tree_words((MI355_LDS const int*)up, col - divide(col, a.by_sq) * a.Sq, n_new, base, (MI355_LDS uint32_t*)words + tid * kTreeWords);
+                }
+                __syncthreads();
+            }
+        }
+        // the word of column c for a tile that reaches the draft
+        const auto seen = [&](int tile, int c) { return words[c * kTreeWords + tile - (max(base, 0) >> 5)]; };
 
         bool begun = false;   // the next part's first tile has been requested
         for (int i = 0; i < n_loc; ++i) {
@@ -344,7 +366,15 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
                     for (int nb = 0; nb < NB; ++nb) s[nb][kb] = Elem<T>::mfma16(kf, qf[nb][ks], s[nb][kb]);
                 }
             const bool masked = key0 + TK - 1 > lim_min || no_keys != 0;
-            if (masked) {
+            if (TREE && key0 + TK > base) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    const uint32_t mine = seen(tile, min(16 * nb + c16, ncols - 1)) >> (4 * g);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (!((mine >> (16 * (e >> 2) + (e & 3))) & 1) || ((no_keys >> (e >> 2)) & 1)) s[nb][e >> 2][e & 3] = -INFINITY;
+                }
+            } else if (masked) {
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -421,13 +451,23 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
                 // What a row does not see is taken out of V, row by row, and the sum is taken over for that row's columns alone.
                 for (int r = row_min; r <= row_max; ++r) {
                     const int last = r < n_new ? min(len - 1, r + len - n_new) : -1;
+                    uint32_t word = 0;   // (TREE)
+                    const bool drafted = TREE && key0 + TK > base;
+                    if (drafted) {
+                        int c = r - (col0 - divide(col0, a.by_sq) * a.Sq);   // a column of the row
+                        if (c < 0) c += a.Sq;
+                        if (c >= ncols) continue;
+                        word = seen(tile, c) >> (4 * g);
+                    }
 #pragma unroll
                     for (int db = 0; db < 8; ++db) {
                         MI355_LDS char* vp = st + (v_base ^ (db << 5));
                         V8 vf = Elem<T>::frag(concat(lds_read_tr16_b64(vp), lds_read_tr16_b64(vp + 16 * ROW_BYTES)));
 #pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (key0 + 16 * (e >> 2) + 4 * g + (e & 3) > last || ((no_keys >> (e >> 2)) & 1)) vf[e] = (T)0.f;
+                        for (int e = 0; e < 8; ++e) {
+                            const bool hidden = drafted ? !((word >> (16 * (e >> 2) + (e & 3))) & 1) : key0 + 16 * (e >> 2) + 4 * g + (e & 3) > last;
+                            if (hidden || ((no_keys >> (e >> 2)) & 1)) vf[e] = (T)0.f;
+                        }
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb) {   // (of the row's own columns)
                             const float4v sum = Elem<T>::mfma16(vf, pf[nb], o[nb][db]);
@@ -686,7 +726,7 @@ struct PagedPlan {
     int nb, col_block, blocks, workgroups, direct, max_tiles, scores, lds;
     size_t part_bytes, score_bytes, lse_bytes;
 };
-static PagedPlan paged_plan(int B, int Hkv, int max_len, int Hq, int Sq, bool weights, bool lse) {
+static PagedPlan paged_plan(int B, int Hkv, int max_len, int Hq, int Sq, bool weights, bool lse, bool tree) {
     using namespace pdec;
     PagedPlan p = {};
     const int ncols = Hq / Hkv * Sq;
@@ -704,7 +744,7 @@ static PagedPlan paged_plan(int B, int Hkv, int max_len, int Hq, int Sq, bool we
     if (!p.direct) p.part_bytes = sizeof(float) * (size_t)p.blocks * (p.workgroups + pairs) * p.col_block * PART_STRIDE;
     p.scores = weights && ncols <= kMostScores;
     const int meet = WAVES * (p.col_block * D + 64) * (int)sizeof(float);
-    p.lds = LDS_BYTES + (meet <= kMeetBytes ? meet : 0);
+    p.lds = LDS_BYTES + (meet <= kMeetBytes - (tree ? kTreeBytes : 0) ? meet : 0);
     if (p.scores) p.score_bytes = sizeof(float) * (size_t)pairs * p.max_tiles * ncols * TK;
     if (weights && !lse) p.lse_bytes = (sizeof(float) * (size_t)B * Hq * Sq + 15) & ~size_t(15);
     return p;
@@ -722,20 +762,20 @@ bool fmha_paged_many_rows(const mi355_paged_kv& c, int Hq, int Sq) {
 
 bool fmha_paged_keeps_scores(const mi355_paged_kv& c, int Hq, int Sq) { return Hq / c.Hkv * Sq <= pdec::kMostScores; }
 
-size_t fmha_paged_workspace(const mi355_paged_kv& c, int Hq, int Sq, bool lse) {
-    const PagedPlan p = paged_plan(c.B, c.Hkv, c.max_pages * c.page_size, Hq, Sq, c.weights != nullptr, lse);
+size_t fmha_paged_workspace(const mi355_paged_kv& c, int Hq, int Sq, bool lse, bool tree) {
+    const PagedPlan p = paged_plan(c.B, c.Hkv, c.max_pages * c.page_size, Hq, Sq, c.weights != nullptr, lse, tree);
     size_t first = fmha_paged_many_rows(c, Hq, Sq) ? paged_rows_workspace(c, Hq, Sq) : p.part_bytes + p.score_bytes;
     if (c.weights != nullptr && !p.scores) first = std::max(first, key_weights_workspace(c, Hq, Sq, 0));   // (one behind the other)
     return first + p.lse_bytes;
 }
 
-template <typename T, int NB, bool SCORES>
+template <typename T, int NB, bool SCORES, bool TREE>
 static hipError_t launch_paged(const PagedKv& kv, const PagedAttn& a, const PagedPlan& p, hipStream_t stream) {
     using namespace pdec;
     static DynamicLdsOnce once;
-    const hipError_t e = once.ensure(reinterpret_cast<const void*>(fmha_paged_kernel<T, NB, SCORES>), LDS_BYTES + kMeetBytes);
+    const hipError_t e = once.ensure(reinterpret_cast<const void*>(fmha_paged_kernel<T, NB, SCORES, TREE>), LDS_BYTES + kMeetBytes - (TREE ? kTreeBytes : 0));
     if (e != hipSuccess) return e;
-    fmha_paged_kernel<T, NB, SCORES><<<dim3(p.workgroups, p.blocks), dim3(NTHREADS), p.lds, stream>>>(kv, a);
+    fmha_paged_kernel<T, NB, SCORES, TREE><<<dim3(p.workgroups, p.blocks), dim3(NTHREADS), p.lds, stream>>>(kv, a);
     return hipGetLastError();
 }
 
@@ -743,8 +783,10 @@ template <typename T>
 static hipError_t fmha_paged_t(const PagedKv& kv, const PagedAttn& a, const PagedPlan& p, hipStream_t stream) {
     using namespace pdec;
     const unsigned pairs = (unsigned)(kv.B * kv.Hkv);
-    hipError_t e = p.nb == 1 ? (p.scores ? launch_paged<T, 1, true>(kv, a, p, stream) : launch_paged<T, 1, false>(kv, a, p, stream))
-                             : (p.scores ? launch_paged<T, 2, true>(kv, a, p, stream) : launch_paged<T, 2, false>(kv, a, p, stream));
+    const auto launch = a.tree.parents != nullptr ? (p.nb == 1 ? &launch_paged<T, 1, false, true> : &launch_paged<T, 2, false, true>)
+                        : p.nb == 1               ? (p.scores ? &launch_paged<T, 1, true, false> : &launch_paged<T, 1, false, false>)
+                                                  : (p.scores ? &launch_paged<T, 2, true, false> : &launch_paged<T, 2, false, false>);
+    hipError_t e = launch(kv, a, p, stream);
     const unsigned rest = pairs * ((p.direct ? 0u : (unsigned)a.ncols) + (p.scores ? (unsigned)a.chunks : 0u));
     if (e == hipSuccess && rest > 0) {
         paged_finish_kernel<T><<<dim3(rest), dim3(NTHREADS), 0, stream>>>(kv, a);
@@ -754,9 +796,9 @@ static hipError_t fmha_paged_t(const PagedKv& kv, const PagedAttn& a, const Page
 }
 
 hipError_t fmha_paged_dispatch(const mi355_paged_kv& c, const void* Q, void* O, float* LSE, int Hq, int Sq, const long* strides, float scale,
-                               void* workspace, hipStream_t stream) {
-    const PagedKv kv = paged_from(c);
-    const PagedPlan p = paged_plan(kv.B, kv.Hkv, kv.max_len, Hq, Sq, kv.weights != nullptr, LSE != nullptr);
+                               const int* parents, long parents_batch, void* workspace, hipStream_t stream) {
+    const PagedKv kv = paged_from(c);   // (a tree's call has no account)
+    const PagedPlan p = paged_plan(kv.B, kv.Hkv, kv.max_len, Hq, Sq, kv.weights != nullptr, LSE != nullptr, parents != nullptr);
     char* ws = (char*)workspace;
     PagedAttn a = {};
     a.Q = Q;
@@ -783,13 +825,14 @@ hipError_t fmha_paged_dispatch(const mi355_paged_kv& c, const void* Q, void* O, 
     a.apart = p.lds > pdec::LDS_BYTES;
     a.max_tiles = p.max_tiles;
     a.part_block = (long)(p.workgroups + kv.B * kv.Hkv) * p.col_block * pdec::PART_STRIDE;
+    a.tree = {parents, parents_batch};
     a.scale_log2 = scale * 1.4426950408889634f;
     a.by_sq = divisor_of(Sq);
     a.by_hkv = divisor_of(kv.Hkv);
     a.chunks = (kv.max_len + 255) / 256;
     a.by_ncols = divisor_of(a.ncols);
     a.by_chunks = divisor_of(a.chunks);
-    hipError_t e = fmha_paged_many_rows(c, Hq, Sq) ? paged_rows_dispatch(c, Q, O, a.LSE, Hq, Sq, strides, scale, ws, stream)
+    hipError_t e = fmha_paged_many_rows(c, Hq, Sq) ? paged_rows_dispatch(c, Q, O, a.LSE, Hq, Sq, strides, scale, parents, parents_batch, ws, stream)
                    : c.dtype == MI355_DTYPE_BF16      ? fmha_paged_t<bf16_t>(kv, a, p, stream)
                                                       : fmha_paged_t<half_t>(kv, a, p, stream);
     if (e == hipSuccess && kv.weights != nullptr && !p.scores)   // many rows: from the log-sum-exp, with the scores worked out again

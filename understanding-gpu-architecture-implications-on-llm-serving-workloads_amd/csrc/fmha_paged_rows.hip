@@ -69,6 +69,7 @@ struct RowsAttn {
     float* part;     // [2 workgroups][waves of columns][PART_FLOATS]
     long q_batch, q_head, q_row, o_batch, o_head, o_row;
     int Hq, Sq, group, ncols, entries, workgroups;   // entries: (block of columns, sequence)
+    PagedTree tree;  // of the drafted tokens, where they are one
     float scale_log2;
     int direct;      // a workgroup a triple
     int joins, few;  // triples or borders, which of them
@@ -158,7 +159,8 @@ struct Entries {
 
 }  // namespace prow
 
-template <typename T, int KG>
+// TREE: the rows are drafted tokens of a.tree (fmha_paged.hip)
+template <typename T, int KG, bool TREE>
 __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv kv, RowsAttn a) {
     using namespace prow;
     using V8 = typename Elem<T>::v8;
@@ -319,6 +321,22 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
         row_min = __builtin_amdgcn_readfirstlane(row_min);
         row_max = __builtin_amdgcn_readfirstlane(row_max);
         if (col0 >= a.ncols) lim_max = -1;   // (a wave without columns)
+        const int base = len - n_new;        // (TREE) key of the first drafted token
+        const int row0 = TREE ? divide(block * COLS, a.by_group) : 0;   // first row of the block
+        __shared__ int up[TREE ? kMostDrafted : 1];
+        __shared__ uint32_t words[TREE ? kMostDrafted * kTreeWords : 1];
+        if constexpr (TREE) {
+            lim_min = min(lim_min, base - 1);
+            if ((tile0 + n) * TK > base) {   // the words of the block's rows, where the part reaches the draft
+                const int* parents = a.tree.parents + b * a.tree.batch;
+                for (int i = tid; i < a.Sq; i += NTHREADS) up[i] = parents[i];
+                __syncthreads();
+                const int rows = divide(min(block * COLS + COLS, a.ncols) - 1, a.by_group) - row0 + 1;
+                if (tid < rows) tree_words((MI355_LDS const int*)up, row0 + tid, n_new, base, (MI355_LDS uint32_t*)words + tid * kTreeWords);
+            }   // (a barrier follows)
+        }
+        // the word of row r for 32 keys from key0 on, which reach the draft
+        const auto seen = [&](int key0, int r) { return words[(r - row0) * kTreeWords + (key0 >> 5) - (max(base, 0) >> 5)]; };
         // a use of the query fragments in front of the loop: their first use inside it would make the compiler wait there, on every
         // iteration, for everything in flight
 #pragma unroll
@@ -477,11 +495,22 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
             phase_barrier();
             if (work) {
                 const uint32_t none = none_of(h);
+                const bool drafted = TREE && key0 + 32 > base;
+                if (drafted) {
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
+                    for (int nb = 0; nb < NB; ++nb) {
+                        const uint32_t mine = seen(key0, qrow[nb]) >> (4 * g);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (key0 + 16 * (e >> 2) + 4 * g + (e & 3) > lim[nb] || ((none >> (e >> 2)) & 1)) s[nb][e >> 2][e & 3] = -INFINITY;
+                        for (int e = 0; e < 8; ++e)
+                            if (!((mine >> (16 * (e >> 2) + (e & 3))) & 1) || ((none >> (e >> 2)) & 1)) s[nb][e >> 2][e & 3] = -INFINITY;
+                    }
+                } else {
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (key0 + 16 * (e >> 2) + 4 * g + (e & 3) > lim[nb] || ((none >> (e >> 2)) & 1)) s[nb][e >> 2][e & 3] = -INFINITY;
+                }
                 softmax();
                 read_v(st);
                 // A product with p = 0 is not nothing where v is infinite or NaN: such values are taken out and go to the rows that see them, one
@@ -505,15 +534,18 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
 #pragma unroll 1
                     for (int r = row_min; r <= row_max; ++r) {
                         const int last = r < n_new ? min(len - 1, r + len - n_new) : -1;
+                        const uint32_t word = drafted ? seen(key0, r) >> (4 * g) : 0;
 #pragma unroll
                         for (int db = 0; db < 8; ++db) {
-                            V8 seen = v_frag(st, db);
+                            V8 vs = v_frag(st, db);
 #pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                if (is_finite(seen[e]) || key0 + 16 * (e >> 2) + 4 * g + (e & 3) > last || ((none >> (e >> 2)) & 1)) seen[e] = (T)0.f;
+                            for (int e = 0; e < 8; ++e) {
+                                const bool hidden = drafted ? !((word >> (16 * (e >> 2) + (e & 3))) & 1) : key0 + 16 * (e >> 2) + 4 * g + (e & 3) > last;
+                                if (is_finite(vs[e]) || hidden || ((none >> (e >> 2)) & 1)) vs[e] = (T)0.f;
+                            }
 #pragma unroll
                             for (int nb = 0; nb < NB; ++nb) {
-                                const float4v more = Elem<T>::mfma16(seen, pf[nb], float4v{0.f, 0.f, 0.f, 0.f});
+                                const float4v more = Elem<T>::mfma16(vs, pf[nb], float4v{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) o[nb][db][e] += qrow[nb] == r ? more[e] : 0.f;
                             }
@@ -731,13 +763,13 @@ bool paged_rows_fits(const mi355_paged_kv& c, int Hq, int Sq) { return prow::pla
 
 size_t paged_rows_workspace(const mi355_paged_kv& c, int Hq, int Sq) { return prow::plan_of(c, Hq, Sq).bytes; }
 
-template <typename T, int KG>
+template <typename T, int KG, bool TREE>
 static hipError_t launch_rows(const PagedKv& kv, const RowsAttn& a, hipStream_t stream) {
     using namespace prow;
     static DynamicLdsOnce once;
-    hipError_t e = once.ensure(reinterpret_cast<const void*>(paged_rows_kernel<T, KG>), LDS_BYTES);
+    hipError_t e = once.ensure(reinterpret_cast<const void*>(paged_rows_kernel<T, KG, TREE>), LDS_BYTES);
     if (e != hipSuccess) return e;
-    paged_rows_kernel<T, KG><<<dim3(a.workgroups), dim3(NTHREADS), LDS_BYTES, stream>>>(kv, a);
+    paged_rows_kernel<T, KG, TREE><<<dim3(a.workgroups), dim3(NTHREADS), LDS_BYTES, stream>>>(kv, a);
     e = hipGetLastError();
     if (e != hipSuccess || a.direct) return e;
     paged_rows_join_kernel<T, KG><<<dim3((unsigned)(a.joins * (WAVES / KG) + a.entries), a.few ? 4 : 1), dim3(256), 0, stream>>>(kv, a);
@@ -745,7 +777,7 @@ static hipError_t launch_rows(const PagedKv& kv, const RowsAttn& a, hipStream_t 
 }
 
 hipError_t paged_rows_dispatch(const mi355_paged_kv& c, const void* Q, void* O, float* LSE, int Hq, int Sq, const long* strides, float scale,
-                               void* workspace, hipStream_t stream) {
+                               const int* parents, long parents_batch, void* workspace, hipStream_t stream) {
     const PagedKv kv = paged_from(c);
     const prow::Plan p = prow::plan_of(c, Hq, Sq);
     RowsAttn a = {};
@@ -764,12 +796,17 @@ hipError_t paged_rows_dispatch(const mi355_paged_kv& c, const void* Q, void* O, 
     a.direct = p.direct;
     a.few = (long)a.entries * kv.Hkv <= a.workgroups / 2;
     a.joins = a.few ? a.entries * kv.Hkv : a.workgroups;
+    a.tree = {parents, parents_batch};
     a.scale_log2 = scale * 1.4426950408889634f;
     a.by_group = divisor_of(a.group);
     a.by_batch = divisor_of(kv.B);
     a.by_hkv = divisor_of(kv.Hkv);
-    if (c.dtype == MI355_DTYPE_BF16) return p.kg == 1 ? launch_rows<bf16_t, 1>(kv, a, stream) : launch_rows<bf16_t, 2>(kv, a, stream);
-    return p.kg == 1 ? launch_rows<half_t, 1>(kv, a, stream) : launch_rows<half_t, 2>(kv, a, stream);
+    const auto launch = [&](auto type, auto tree) {
+        using T = decltype(type);
+        return p.kg == 1 ? launch_rows<T, 1, decltype(tree)::value>(kv, a, stream) : launch_rows<T, 2, decltype(tree)::value>(kv, a, stream);
+    };
+    if (parents != nullptr) return c.dtype == MI355_DTYPE_BF16 ? launch(bf16_t{}, std::true_type{}) : launch(half_t{}, std::true_type{});
+    return c.dtype == MI355_DTYPE_BF16 ? launch(bf16_t{}, std::false_type{}) : launch(half_t{}, std::false_type{});
 }
 
 }  // namespace mi355

@@ -183,17 +183,18 @@ hipError_t silu_mul_dispatch(const void* in, void* out, long rows, int inter, in
 
 // The paged key-value cache (arguments as the entry points' after validation). `strides`: q (batch, head, row), o (batch, head, row).
 // `workspace` holds what the *_workspace functions say.
-size_t fmha_paged_workspace(const mi355_paged_kv& cache, int Hq, int Sq, bool lse);
+// `parents`: of the drafted tokens, where the rows are a tree of them (null otherwise; `tree` says so). A tree's call has no account.
+size_t fmha_paged_workspace(const mi355_paged_kv& cache, int Hq, int Sq, bool lse, bool tree);
 // whether the account is made from the attention's own scores (otherwise by key_weights_dispatch)
 bool fmha_paged_keeps_scores(const mi355_paged_kv& cache, int Hq, int Sq);
 hipError_t fmha_paged_dispatch(const mi355_paged_kv& cache, const void* Q, void* O, float* LSE, int Hq, int Sq, const long* strides, float scale,
-                               void* workspace, hipStream_t stream);
+                               const int* parents, long parents_batch, void* workspace, hipStream_t stream);
 // whether the kernel for many query columns a kv head takes a call (fmha_paged_rows.hip), and whether its tiles can be counted in an int
 bool fmha_paged_many_rows(const mi355_paged_kv& cache, int Hq, int Sq);
 bool paged_rows_fits(const mi355_paged_kv& cache, int Hq, int Sq);
 size_t paged_rows_workspace(const mi355_paged_kv& cache, int Hq, int Sq);
 hipError_t paged_rows_dispatch(const mi355_paged_kv& cache, const void* Q, void* O, float* LSE, int Hq, int Sq, const long* strides, float scale,
-                               void* workspace, hipStream_t stream);
+                               const int* parents, long parents_batch, void* workspace, hipStream_t stream);
 long key_weights_workgroups(const mi355_paged_kv& cache, int Hq, int Sq, int last_rows);
 size_t key_weights_workspace(const mi355_paged_kv& cache, int Hq, int Sq, int last_rows);
 hipError_t key_weights_dispatch(const mi355_paged_kv& cache, const void* Q, const float* LSE, int Hq, int Sq, const long* q_strides, int last_rows,
@@ -202,6 +203,21 @@ hipError_t rope_paged_dispatch(const mi355_paged_kv& cache, void* qkv, int S, in
                                const float* sin_t, const int* positions, long pos_batch, int n_pos, hipStream_t stream);
 size_t evict_workspace(const mi355_paged_kv& cache, int budget);
 hipError_t evict_dispatch(const mi355_paged_kv& cache, int budget, int recent, int* lens_out, void* workspace, hipStream_t stream);
+hipError_t keep_path_dispatch(const mi355_paged_kv& cache, const int* path, int length, long path_batch, int* lens_out, hipStream_t stream);
+
+// most tokens of a tree
+constexpr int kMostDrafted = 256;
+
+// Packed batches (likewise). packed_dispatch: `variant` 0 = by shape, 1 and 2 = q tiles of 128 and 256 rows; of `strides` the rows' and heads' count.
+size_t packed_plan_workspace(int B);
+hipError_t packed_plan_dispatch(int* table, long table_stride, int* seq_lens, const int* new_lens, int* next_positions, int* ring, int* span, int B, int columns,
+                                int n_pages, int page_size, int rows, int* offsets, int* positions, int* slots, int* taken, void* workspace, hipStream_t stream);
+hipError_t rope_packed_dispatch(const mi355_paged_kv& pool, void* qkv, int rows, int q_heads, int keep_keys, long x_row, const float* cos_t, const float* sin_t,
+                                const int* positions, const int* slots, int n_pos, hipStream_t stream);
+bool packed_fits(int rows, int B, int Hq);
+size_t packed_workspace(int rows, int B);
+hipError_t packed_dispatch(const void* Q, const void* K, const void* V, void* O, float* LSE, const int* offsets, int rows, int B, int Hq, int Hkv,
+                           const FmhaStrides& strides, float scale, int causal, int dtype, void* workspace, int variant, hipStream_t stream);
 
 }  // namespace mi355
 
@@ -247,6 +263,10 @@ int mi355_internal_step_qkv(const void* x, const void* norm_weight, float eps, c
                             const float* sin_table, const int32_t* positions, int64_t pos_batch, int n_positions, int dtype, void* stream);
 int mi355_internal_step_gate_up(const void* x, const void* norm_weight, float eps, const void* w_gu, void* out, int rows, int inter, int hidden,
                                 int dtype, void* stream);
+// mi355_fmha_packed with the q tiles pinned: variant 0 = by shape, 1 = 128 rows, 2 = 256 rows
+int mi355_internal_fmha_packed_variant(const void* Q, const void* K, const void* V, void* O, float* LSE, const int32_t* offsets, int rows, int B, int Hq, int Hkv,
+                                       const int64_t* strides, float scale, int causal, int dtype, void* workspace, size_t workspace_bytes, int variant,
+                                       void* stream);
 // how few queries over `kv_valid_len` keys are cut: key ranges per (batch, kv head), 0 = by the prefill kernel; waves per workgroup
 int mi355_internal_fmha_decode_plan(int B, int Hq, int Hkv, int Sq, int kv_valid_len, int* splits, int* waves);
 }

@@ -86,4 +86,30 @@ __device__ __forceinline__ int wave_max(int x) {
     return __builtin_amdgcn_readlane(x, 63);
 }
 
+// ---- a tree of drafted tokens -----------------------------------------------------------------------------------------
+//
+// The last n keys of a sequence are drafted tokens, of which token i continues parents[i], 0 <= parents[i] < i, or is a root (anything else). It sees the keys
+// in front of the draft, itself and the tokens on its path to a root; none of them lies behind it. What a row sees of 32 keys that begin at a multiple of 32 is
+// a word of bits; the words of a row begin with the one that holds the draft's first key, whose lower bits are keys in front of the draft.
+struct PagedTree {
+    const int* parents;
+    long batch;      // entries from one sequence's parents to the next's (0: the same for all)
+};
+constexpr int kTreeWords = kMostDrafted / 32 + 1;   // (odd: rows side by side in LDS lie in different banks)
+
+// The words of drafted token `row` of n, of which the first is key `base` (negative where the sequence is shorter than its draft: the first ones are no keys).
+// `parents` in LDS. Every step of the walk goes to a smaller number.
+__device__ __forceinline__ void tree_words(MI355_LDS const int* parents, int row, int n, int base, MI355_LDS uint32_t* words) {
+    const int skew = base >= 0 ? base & 31 : base;
+#pragma unroll
+    for (int w = 0; w < kTreeWords; ++w) words[w] = 0;
+    if (row < 0 || row >= n) return;
+    if (base > 0) words[0] = (1u << skew) - 1;
+    for (int i = row; i >= 0;) {
+        if (skew + i >= 0) words[(skew + i) >> 5] |= 1u << ((skew + i) & 31);
+        const int up = parents[i];
+        i = up < i ? up : -1;
+    }
+}
+
 }  // namespace mi355

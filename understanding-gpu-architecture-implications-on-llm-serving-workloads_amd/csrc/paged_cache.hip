@@ -10,6 +10,21 @@ namespace pcache {
 constexpr int THREADS = 256;
 }
 
+// (x, y) -> (x c - y s, y c + x s) for 8 values x of a head's lower half and their partners y, in 32 bits, each rounded once
+template <typename T>
+__device__ __forceinline__ void rotate8(typename Elem<T>::v8& lo, typename Elem<T>::v8& hi, const float* __restrict__ cp, const float* __restrict__ sp) {
+    const float4v c0 = *(const float4v*)cp, c1 = *(const float4v*)(cp + 4);
+    const float4v s0 = *(const float4v*)sp, s1 = *(const float4v*)(sp + 4);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float c = j < 4 ? c0[j] : c1[j - 4];
+        const float sn = j < 4 ? s0[j] : s1[j - 4];
+        const float x = (float)lo[j], y = (float)hi[j];
+        lo[j] = (T)(x * c - y * sn);
+        hi[j] = (T)(y * c + x * sn);
+    }
+}
+
 // Token (b, t) of a fused projection [q_heads | Hkv key heads | Hkv value heads] of 128: queries rotated in place, rotated keys and the values to row
 // seq_lens[b] - new + t of the sequence; keep_keys: the rotated keys also where they were read. A thread owns 8 values of the
 // lower half of a head and their 8 partners; 8 threads a head, 32 heads a workgroup. The arithmetic is that of rope_kernel (glue.hip). Bound by
@@ -31,18 +46,7 @@ __global__ __launch_bounds__(pcache::THREADS) void rope_paged_kernel(PagedKv kv,
     const int place = positions[b * pos_batch + t];
     if (head < q_heads + kv.Hkv) {
         const int pos = min(max(place, 0), n_pos - 1);
-        const float* cp = cos_t + (long)pos * 64 + i0;
-        const float* sp = sin_t + (long)pos * 64 + i0;
-        const float4v c0 = *(const float4v*)cp, c1 = *(const float4v*)(cp + 4);
-        const float4v s0 = *(const float4v*)sp, s1 = *(const float4v*)(sp + 4);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float c = j < 4 ? c0[j] : c1[j - 4];
-            const float sn = j < 4 ? s0[j] : s1[j - 4];
-            const float x = (float)lo[j], y = (float)hi[j];
-            lo[j] = (T)(x * c - y * sn);
-            hi[j] = (T)(y * c + x * sn);
-        }
+        rotate8<T>(lo, hi, cos_t + (long)pos * 64 + i0, sin_t + (long)pos * 64 + i0);
         if (head < q_heads || keep_keys) {
             *(V8*)xp = lo;
             *(V8*)(xp + 64) = hi;
@@ -64,6 +68,114 @@ __global__ __launch_bounds__(pcache::THREADS) void rope_paged_kernel(PagedKv kv,
         if (kv.weights != nullptr) kv.weights[at] = 0.f;
         if (kv.key_positions != nullptr) kv.key_positions[at] = place;
     }
+}
+
+// The same for a packed projection, [rows] tokens without padding: token t is filed in slot slots[t] = page * page_size + row of the page of the pool
+// (outside the pool: not filed); a row whose position is negative is no token and stays as it is. The slots are read where rope_paged_kernel reads a
+// length and a table one behind the other. Bound by HBM for prompts, by one chain of loads for a step.
+template <typename T>
+__global__ __launch_bounds__(pcache::THREADS) void rope_packed_kernel(PagedKv kv, T* qkv, int q_heads, int keep_keys, long x_row,
+                                                                      const float* __restrict__ cos_t, const float* __restrict__ sin_t,
+                                                                      const int* __restrict__ positions, const int* __restrict__ slots, int n_pos) {
+    using V8 = typename Elem<T>::v8;
+    const int head = blockIdx.y * 32 + (threadIdx.x >> 3);
+    if (head >= q_heads + 2 * kv.Hkv) return;
+    const int t = blockIdx.x, i0 = (threadIdx.x & 7) * 8;
+    const int place = positions[t], at = slots[t];
+    if (place < 0) return;
+    T* xp = qkv + t * x_row + (long)head * 128 + i0;
+    V8 lo = *(const V8*)xp;
+    V8 hi = *(const V8*)(xp + 64);
+    if (head < q_heads + kv.Hkv) {
+        const int pos = min(place, n_pos - 1);
+        rotate8<T>(lo, hi, cos_t + (long)pos * 64 + i0, sin_t + (long)pos * 64 + i0);
+        if (head < q_heads || keep_keys) {
+            *(V8*)xp = lo;
+            *(V8*)(xp + 64) = hi;
+        }
+        if (head < q_heads) return;
+    }
+    const int page = at < 0 ? kv.n_pages : divide(at, kv.by_page);
+    if (page >= kv.n_pages) return;
+    const int slot = at - page * kv.page_size;
+    char* op = kv.pages + (long)page * kv.page_bytes + (long)(head - q_heads) * kv.head_bytes + (uint32_t)slot * kv.row_bytes + 2 * i0;
+    *(V8*)op = lo;
+    *(V8*)(op + 128) = hi;
+    if (head < q_heads + kv.Hkv && i0 == 0) {   // what eviction goes by
+        const long w = ((long)page * kv.Hkv + (head - q_heads)) * kv.page_size + slot;
+        if (kv.weights != nullptr) kv.weights[w] = 0.f;
+        if (kv.key_positions != nullptr) kv.key_positions[w] = place;
+    }
+}
+
+// ---- the accepted path of drafted tokens ---------------------------------------------------------------------------------
+//
+// The last n keys of a sequence are a tree of drafted tokens; path[b] names the accepted ones, ascending: key len - n + path[j] moves to key
+// len - n + j, with its value, weight and position. The path ends in front of the first entry that does not ascend or is no drafted token of the sequence.
+// A key's new place is never behind its old one, and the old places of the keys that follow are behind both: a thread that owns 16 bytes of a head and
+// takes the path in order, reading a group of keys before it writes them, needs to wait for nobody. Bound by its chain of loads: length, path, table, keys.
+template <int GROUP>
+__global__ __launch_bounds__(pcache::THREADS) void keep_path_kernel(PagedKv kv, const int* __restrict__ path, int length, long path_batch, int* lens_out) {
+    const int b = blockIdx.y, lane = threadIdx.x & 63;
+    const int head = blockIdx.x * 16 + (threadIdx.x >> 4);
+    const int len = paged_len(kv, b), n = max(kv.new_lens[b], 0);
+    const int base = max(len - n, 0), missing = max(n - len, 0);   // (drafted tokens in front of the sequence's first key)
+    const int* mine = path + (long)b * path_batch;
+    const int* table = kv.table + (long)b * kv.table_stride;
+    const bool works = head < 2 * kv.Hkv;
+    char* const column = kv.pages + (long)(works ? head : 0) * kv.head_bytes + (threadIdx.x & 15) * 16;
+    const bool account = works && head < kv.Hkv && (threadIdx.x & 15) == 0;
+    const long account_row = (long)head * kv.page_size;
+    int kept = 0, last = missing - 1;
+    for (int j0 = 0; j0 < length; j0 += 64) {
+        // 64 entries, one a lane: where its key is and where it goes
+        const int j = j0 + lane, entry = j < length ? mine[j] : -1;
+        const int left = __shfl_up(entry, 1, 64), prev = lane == 0 ? last : left;
+        const uint64_t ends = __builtin_amdgcn_ballot_w64(!(entry > prev && entry < n));
+        const int count = ends == 0 ? 64 : __builtin_ctzll(ends);
+        last = __builtin_amdgcn_readlane(entry, 63);
+        const int from = base + entry - missing, to = base + j;
+        int from_page = -1, to_page = -1, from_slot = 0, to_slot = 0;
+        if (lane < count) {
+            const int fi = divide(from, kv.by_page), ti = divide(to, kv.by_page);
+            from_page = table[fi];
+            to_page = table[ti];
+            from_slot = from - fi * kv.page_size;
+            to_slot = to - ti * kv.page_size;
+        }
+        const bool moves = lane < count && from != to && (uint32_t)from_page < (uint32_t)kv.n_pages && (uint32_t)to_page < (uint32_t)kv.n_pages;
+        uint64_t left_to_move = __builtin_amdgcn_ballot_w64(moves);
+        while (left_to_move != 0) {
+            int4v row[GROUP];
+            float w[GROUP];
+            int pos[GROUP], at[GROUP];
+            int m = 0;
+#pragma unroll
+            for (int g = 0; g < GROUP; ++g) {
+                at[g] = left_to_move != 0 ? __builtin_ctzll(left_to_move) : -1;
+                if (at[g] < 0) continue;
+                left_to_move &= left_to_move - 1;
+                ++m;
+                const int page = __builtin_amdgcn_readlane(from_page, at[g]), slot = __builtin_amdgcn_readlane(from_slot, at[g]);
+                row[g] = *(const int4v*)(column + (long)page * kv.page_bytes + (uint32_t)slot * kv.row_bytes);
+                const long a = (long)page * kv.Hkv * kv.page_size + account_row + slot;
+                if (account && kv.weights != nullptr) w[g] = kv.weights[a];
+                if (account && kv.key_positions != nullptr) pos[g] = kv.key_positions[a];
+            }
+#pragma unroll
+            for (int g = 0; g < GROUP; ++g) {
+                if (g >= m) continue;
+                const int page = __builtin_amdgcn_readlane(to_page, at[g]), slot = __builtin_amdgcn_readlane(to_slot, at[g]);
+                if (works) *(int4v*)(column + (long)page * kv.page_bytes + (uint32_t)slot * kv.row_bytes) = row[g];
+                const long a = (long)page * kv.Hkv * kv.page_size + account_row + slot;
+                if (account && kv.weights != nullptr) kv.weights[a] = w[g];
+                if (account && kv.key_positions != nullptr) kv.key_positions[a] = pos[g];
+            }
+        }
+        kept += count;
+        if (count < 64) break;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) lens_out[b] = base + kept;
 }
 
 // ---- eviction ------------------------------------------------------------------------------------------------------------
@@ -439,6 +551,26 @@ hipError_t rope_paged_dispatch(const mi355_paged_kv& c, void* qkv, int S, int q_
     };
     if (c.dtype == MI355_DTYPE_BF16) launch(bf16_t{});
     else launch(half_t{});
+    return hipGetLastError();
+}
+
+hipError_t rope_packed_dispatch(const mi355_paged_kv& c, void* qkv, int rows, int q_heads, int keep_keys, long x_row, const float* cos_t, const float* sin_t,
+                                const int* positions, const int* slots, int n_pos, hipStream_t stream) {
+    const PagedKv kv = paged_from(c);
+    const dim3 grid((unsigned)rows, (unsigned)((q_heads + 2 * kv.Hkv + 31) / 32));
+    const auto launch = [&](auto type) {
+        using T = decltype(type);
+        rope_packed_kernel<T><<<grid, dim3(pcache::THREADS), 0, stream>>>(kv, (T*)qkv, q_heads, keep_keys, x_row, cos_t, sin_t, positions, slots, n_pos);
+    };
+    if (c.dtype == MI355_DTYPE_BF16) launch(bf16_t{});
+    else launch(half_t{});
+    return hipGetLastError();
+}
+
+hipError_t keep_path_dispatch(const mi355_paged_kv& c, const int* path, int length, long path_batch, int* lens_out, hipStream_t stream) {
+    const PagedKv kv = paged_from(c);
+    const dim3 grid((unsigned)((2 * kv.Hkv + 15) / 16), (unsigned)kv.B);
+    keep_path_kernel<8><<<grid, dim3(pcache::THREADS), 0, stream>>>(kv, path, length, path_batch, lens_out);
     return hipGetLastError();
 }
 

@@ -228,6 +228,164 @@ at::Tensor evict_paged(const at::Tensor& kv_pages, const at::Tensor& block_table
     return lens;
 }
 
+at::Tensor keep_path(const at::Tensor& kv_pages, const at::Tensor& block_table, const at::Tensor& seq_lens, const at::Tensor& new_lens, const at::Tensor& path,
+                     const std::optional<at::Tensor>& weights, const std::optional<at::Tensor>& key_positions) {
+    const char* name = "fine_keep_path";
+    const mi355_paged_kv c = paged_kv(name, kv_pages, block_table, seq_lens, new_lens, weights, key_positions);
+    check_like(name, "path", path, kv_pages, at::kInt);
+    TORCH_CHECK(path.dim() == 2 && path.size(0) == c.B && path.size(1) >= 1 && path.size(1) <= INT32_MAX && path.is_contiguous(), name, ": path must be a contiguous [", c.B,
+                ", length] tensor, got ", path.sizes());
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(kv_pages.device());
+    at::Tensor lens = gpu_empty({c.B}, at::kInt, kv_pages);
+    hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+    const int rc = mi355_cache_keep_path(&c, path.data_ptr<int32_t>(), (int)path.size(1), path.size(1), lens.data_ptr<int32_t>(), stream);
+    TORCH_CHECK(rc == 0, name, ": ", mi355_last_error(), " (code ", rc, ")");
+    return lens;
+}
+
+std::tuple<at::Tensor, at::Tensor> run_tree(const at::Tensor& q, const at::Tensor& kv_pages, const at::Tensor& block_table, const at::Tensor& seq_lens,
+                                            const at::Tensor& parents, const std::optional<at::Tensor>& new_lens, bool want_lse) {
+    const char* name = "fine_fmha_tree";
+    const mi355_paged_kv c = paged_kv(name, kv_pages, block_table, seq_lens, new_lens, std::nullopt, std::nullopt);
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(kv_pages.device());
+    const at::Tensor qc = paged_queries(name, q, kv_pages, c);
+    const int64_t Hq = q.size(1), S = q.size(2);
+    check_like(name, "parents", parents, kv_pages, at::kInt);
+    TORCH_CHECK(parents.is_contiguous() && ((parents.dim() == 2 && parents.size(0) == c.B && parents.size(1) == S) || (parents.dim() == 1 && parents.size(0) == S)), name,
+                ": parents must be a contiguous [", c.B, ", ", S, "] or [", S, "] tensor, got ", parents.sizes());
+    at::Tensor o = gpu_empty(q.sizes(), q.scalar_type(), q), lse;
+    if (want_lse) lse = gpu_empty({c.B, Hq, S}, at::kFloat, q);
+    const size_t need = mi355_fmha_paged_tree_workspace_bytes(&c, (int)Hq, (int)S);
+    const at::Tensor ws = workspace_of(need, q);
+    const auto st = query_strides(qc);
+    const int64_t strides[6] = {st[0], st[1], st[2], o.stride(0), o.stride(1), o.stride(2)};
+    hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+    const int rc = mi355_fmha_paged_tree(&c, qc.data_ptr(), o.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr, (int)Hq, (int)S, strides,
+                                         parents.data_ptr<int32_t>(), parents.dim() == 2 ? S : 0, 1.0f / std::sqrt(128.0f), need > 0 ? ws.data_ptr() : nullptr, need, stream);
+    TORCH_CHECK(rc == 0, name, ": ", mi355_last_error(), " (code ", rc, ")");
+    return {o, lse};
+}
+
+at::Tensor fmha_tree(const at::Tensor& q, const at::Tensor& kv_pages, const at::Tensor& block_table, const at::Tensor& seq_lens, const at::Tensor& parents,
+                     const std::optional<at::Tensor>& new_lens) {
+    return std::get<0>(run_tree(q, kv_pages, block_table, seq_lens, parents, new_lens, false));
+}
+
+std::tuple<at::Tensor, at::Tensor> fmha_tree_lse(const at::Tensor& q, const at::Tensor& kv_pages, const at::Tensor& block_table, const at::Tensor& seq_lens,
+                                                 const at::Tensor& parents, const std::optional<at::Tensor>& new_lens) {
+    return run_tree(q, kv_pages, block_table, seq_lens, parents, new_lens, true);
+}
+
+// ---- packed batches (include/mi355_serving.h: mi355_packed_plan, mi355_rope_packed, mi355_fmha_packed) -------------------------------------
+
+void check_ints(const char* name, const char* what, const at::Tensor& t, const at::Tensor& like, int64_t n) {
+    TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, ": ", what, " must be a GPU tensor on the device of the others");
+    TORCH_CHECK(t.scalar_type() == at::kInt, name, ": ", what, " must be ", at::kInt, ", got ", t.scalar_type());
+    TORCH_CHECK(t.dim() == 1 && t.size(0) == n && t.is_contiguous(), name, ": ", what, " must be a contiguous [", n, "] tensor, got ", t.sizes());
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> plan_packed(const at::Tensor& block_table, const at::Tensor& seq_lens, const at::Tensor& new_lens,
+                                                                      const at::Tensor& free_pages, const at::Tensor& free_span, int64_t page_size, int64_t rows,
+                                                                      const std::optional<at::Tensor>& next_positions) {
+    const char* name = "fine_plan_packed";
+    TORCH_CHECK(block_table.is_cuda() && block_table.scalar_type() == at::kInt && block_table.dim() == 2 && block_table.numel() > 0, name,
+                ": block_table must be a [B, max_pages] int32 GPU tensor, got ", block_table.sizes(), " of ", block_table.scalar_type());
+    const int64_t B = block_table.size(0), columns = block_table.size(1);
+    TORCH_CHECK(block_table.stride(1) == 1 || columns == 1, name, ": the rows of block_table must be contiguous");
+    check_ints(name, "seq_lens", seq_lens, block_table, B);
+    check_ints(name, "new_lens", new_lens, block_table, B);
+    TORCH_CHECK(free_pages.dim() == 1 && free_pages.size(0) >= 1, name, ": free_pages must be [n_pages], got ", free_pages.sizes());
+    check_ints(name, "free_pages", free_pages, block_table, free_pages.size(0));
+    check_ints(name, "free_span", free_span, block_table, 2);
+    if (next_positions.has_value()) check_ints(name, "next_positions", *next_positions, block_table, B);
+    TORCH_CHECK(rows >= 0 && rows <= INT32_MAX && page_size >= 1 && page_size <= INT32_MAX && B <= INT32_MAX && columns <= INT32_MAX && free_pages.size(0) <= INT32_MAX, name,
+                ": rows >= 0 and page_size >= 1 required (got ", rows, " and ", page_size, "), and no dimension beyond int32");
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(block_table.device());
+    at::Tensor offsets = gpu_empty({B + 1}, at::kInt, block_table), positions = gpu_empty({rows}, at::kInt, block_table);
+    at::Tensor slots = gpu_empty({rows}, at::kInt, block_table), taken = gpu_empty({B}, at::kInt, block_table);
+    const size_t need = mi355_packed_plan_workspace_bytes((int)B);
+    const at::Tensor ws = workspace_of(need, block_table);
+    hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+    const int rc = mi355_packed_plan(block_table.data_ptr<int32_t>(), block_table.stride(0), seq_lens.data_ptr<int32_t>(), new_lens.data_ptr<int32_t>(),
+                                     next_positions.has_value() ? next_positions->data_ptr<int32_t>() : nullptr, free_pages.data_ptr<int32_t>(),
+                                     free_span.data_ptr<int32_t>(), (int)B, (int)columns, (int)free_pages.size(0), (int)page_size, (int)rows, offsets.data_ptr<int32_t>(),
+                                     positions.data_ptr<int32_t>(), slots.data_ptr<int32_t>(), taken.data_ptr<int32_t>(), need > 0 ? ws.data_ptr() : nullptr, need, stream);
+    TORCH_CHECK(rc == 0, name, ": ", mi355_last_error(), " (code ", rc, ")");
+    return {offsets, positions, slots, taken};
+}
+
+void rope_packed(const at::Tensor& qkv, const at::Tensor& kv_pages, const at::Tensor& slots, const at::Tensor& cos, const at::Tensor& sin, const at::Tensor& positions,
+                 int64_t q_heads, const std::optional<at::Tensor>& weights, const std::optional<at::Tensor>& key_positions, bool keep_keys) {
+    const char* name = "fine_rope_packed";
+    const mi355_paged_kv c = mi355::paged_pool(name, kv_pages, weights, key_positions);
+    TORCH_CHECK(q_heads >= 0 && q_heads <= INT32_MAX && qkv.dim() == 3 && qkv.size(1) == q_heads + 2 * (int64_t)c.Hkv && qkv.size(2) == 128 && qkv.numel() > 0, name,
+                ": qkv must be [rows, ", q_heads + 2 * (int64_t)c.Hkv, ", 128], got ", qkv.sizes());
+    check_like(name, "qkv", qkv, kv_pages, kv_pages.scalar_type());
+    TORCH_CHECK(qkv.stride(2) == 1 && qkv.stride(1) == 128, name, ": the heads of a token of qkv must lie side by side");
+    const int64_t rows = qkv.size(0);
+    for (const at::Tensor* t : {&cos, &sin}) {
+        check_like(name, "cos and sin", *t, kv_pages, at::kFloat);
+        TORCH_CHECK(t->dim() == 2 && t->size(0) >= 1 && t->size(1) == 64 && t->is_contiguous() && t->sizes() == cos.sizes(), name,
+                    ": cos and sin must be contiguous [n_positions, 64] tensors");
+    }
+    check_ints(name, "positions", positions, kv_pages, rows);
+    check_ints(name, "slots", slots, kv_pages, rows);
+    TORCH_CHECK(rows <= INT32_MAX && cos.size(0) <= INT32_MAX, name, ": dimension exceeds int32");
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(kv_pages.device());
+    hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+    const int rc = mi355_rope_packed(&c, qkv.data_ptr(), (int)rows, (int)q_heads, keep_keys ? 1 : 0, rows > 1 ? qkv.stride(0) : (q_heads + 2 * (int64_t)c.Hkv) * 128,
+                                     cos.data_ptr<float>(), sin.data_ptr<float>(), positions.data_ptr<int32_t>(), slots.data_ptr<int32_t>(), (int)cos.size(0), stream);
+    TORCH_CHECK(rc == 0, name, ": ", mi355_last_error(), " (code ", rc, ")");
+}
+
+std::tuple<at::Tensor, at::Tensor> run_packed(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets, bool causal, bool want_lse) {
+    const char* name = "fine_fmha_packed";
+    TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && v.dim() == 3, name, ": q, k, v must be [rows, heads, 128] tensors");
+    const bool bf16 = q.scalar_type() == at::kBFloat16;
+    TORCH_CHECK(q.scalar_type() == at::kHalf || bf16, name, ": q must be float16 or bfloat16, got ", q.scalar_type());
+    TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), name, ": k and v must have q's dtype ", q.scalar_type());
+    const int64_t rows = q.size(0), Hq = q.size(1), Hkv = k.size(1);
+    TORCH_CHECK(q.size(2) == 128 && k.size(2) == 128, name, ": head embedding dimension must be 128, got ", q.size(2), " and ", k.size(2));
+    TORCH_CHECK(k.size(0) == rows && v.sizes() == k.sizes(), name, ": k and v must have q's rows and one shape, got ", q.sizes(), ", ", k.sizes(), ", ", v.sizes());
+    TORCH_CHECK(q.numel() > 0 && k.numel() > 0, name, ": empty tensors are not supported");
+    TORCH_CHECK(Hq % Hkv == 0, name, ": number of q heads (", Hq, ") must be a multiple of kv heads (", Hkv, ")");
+    TORCH_CHECK(rows <= INT32_MAX && Hq <= INT32_MAX, name, ": dimension exceeds int32");
+    TORCH_CHECK(q.is_cuda() && k.is_cuda() && v.is_cuda(), name, ": q, k, v must be GPU tensors");
+    TORCH_CHECK(q.device() == k.device() && q.device() == v.device(), name, ": q, k, v are on different devices");
+    TORCH_CHECK(offsets.dim() == 1 && offsets.size(0) >= 2 && offsets.size(0) <= INT32_MAX, name, ": offsets must be [B + 1] with B >= 1, got ", offsets.sizes());
+    check_ints(name, "offsets", offsets, q, offsets.size(0));
+    const int64_t B = offsets.size(0) - 1;
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+    // (of a dimension of one element the stride may be anything and is not used)
+    const auto row_of = [&](const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : 0; };
+    const auto head_of = [&](const at::Tensor& t) { return t.size(1) > 1 ? t.stride(1) : 0; };
+    const auto in_place = [&](const at::Tensor& t) {
+        return t.stride(2) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && row_of(t) >= 0 && head_of(t) >= 0 && (row_of(t) | head_of(t)) % 8 == 0 &&
+               row_of(t) < (1 << 24);
+    };
+    const at::Tensor qc = in_place(q) ? q : q.clone(at::MemoryFormat::Contiguous), kc = in_place(k) ? k : k.clone(at::MemoryFormat::Contiguous);
+    const at::Tensor vc = in_place(v) ? v : v.clone(at::MemoryFormat::Contiguous);
+    at::Tensor o = gpu_empty(q.sizes(), q.scalar_type(), q), lse;
+    if (want_lse) lse = gpu_empty({Hq, rows}, at::kFloat, q);
+    const size_t need = mi355_fmha_packed_workspace_bytes((int)rows, (int)B, (int)Hq, (int)Hkv);
+    const at::Tensor ws = workspace_of(need, q);
+    const int64_t strides[8] = {row_of(qc), head_of(qc), row_of(kc), head_of(kc), row_of(vc), head_of(vc), Hq * 128, 128};
+    hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+    const int rc = mi355_fmha_packed(qc.data_ptr(), kc.data_ptr(), vc.data_ptr(), o.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr, offsets.data_ptr<int32_t>(),
+                                     (int)rows, (int)B, (int)Hq, (int)Hkv, strides, 1.0f / std::sqrt(128.0f), causal ? 1 : 0, bf16 ? MI355_DTYPE_BF16 : MI355_DTYPE_FP16,
+                                     need > 0 ? ws.data_ptr() : nullptr, need, stream);
+    TORCH_CHECK(rc == 0, name, ": ", mi355_last_error(), " (code ", rc, ")");
+    return {o, lse};
+}
+
+at::Tensor fmha_packed(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets, bool causal) {
+    return std::get<0>(run_packed(q, k, v, offsets, causal, false));
+}
+
+std::tuple<at::Tensor, at::Tensor> fmha_packed_lse(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets, bool causal) {
+    return run_packed(q, k, v, offsets, causal, true);
+}
+
 }  // namespace
 
 // Defines the operators (the first eight schema strings are the reference's).
@@ -247,6 +405,15 @@ TORCH_LIBRARY(fmha_unified, m) {
           "Tensor? new_lens, Tensor(c!)? weights, Tensor(d!)? key_positions, bool keep_keys) -> ()");
     m.def("key_weights(Tensor q, Tensor lse, Tensor kv_pages, Tensor block_table, Tensor seq_lens, Tensor(a!) weights, Tensor? new_lens, int last_rows) -> ()");
     m.def("evict_paged(Tensor(a!) kv_pages, Tensor block_table, Tensor seq_lens, Tensor(b!) weights, Tensor(c!) key_positions, int budget, int recent) -> Tensor");
+    m.def("fmha_tree(Tensor q, Tensor kv_pages, Tensor block_table, Tensor seq_lens, Tensor parents, Tensor? new_lens) -> Tensor");
+    m.def("fmha_tree_lse(Tensor q, Tensor kv_pages, Tensor block_table, Tensor seq_lens, Tensor parents, Tensor? new_lens) -> (Tensor, Tensor)");
+    m.def("keep_path(Tensor(a!) kv_pages, Tensor block_table, Tensor seq_lens, Tensor new_lens, Tensor path, Tensor(b!)? weights, Tensor(c!)? key_positions) -> Tensor");
+    m.def("plan_packed(Tensor(a!) block_table, Tensor(b!) seq_lens, Tensor new_lens, Tensor(c!) free_pages, Tensor(d!) free_span, int page_size, int rows, "
+          "Tensor(e!)? next_positions) -> (Tensor, Tensor, Tensor, Tensor)");
+    m.def("rope_packed(Tensor(a!) qkv, Tensor(b!) kv_pages, Tensor slots, Tensor cos, Tensor sin, Tensor positions, int q_heads, Tensor(c!)? weights, "
+          "Tensor(d!)? key_positions, bool keep_keys) -> ()");
+    m.def("fmha_packed(Tensor q, Tensor k, Tensor v, Tensor offsets, bool causal) -> Tensor");
+    m.def("fmha_packed_lse(Tensor q, Tensor k, Tensor v, Tensor offsets, bool causal) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(fmha_unified, CUDA, m) {
@@ -264,6 +431,13 @@ TORCH_LIBRARY_IMPL(fmha_unified, CUDA, m) {
     m.impl("rope_paged", &rope_paged);
     m.impl("key_weights", &key_weights);
     m.impl("evict_paged", &evict_paged);
+    m.impl("fmha_tree", &fmha_tree);
+    m.impl("fmha_tree_lse", &fmha_tree_lse);
+    m.impl("keep_path", &keep_path);
+    m.impl("plan_packed", &plan_packed);
+    m.impl("rope_packed", &rope_packed);
+    m.impl("fmha_packed", &fmha_packed);
+    m.impl("fmha_packed_lse", &fmha_packed_lse);
 }
 
 // The same functions under the CPU key: CPU tensors then reach the argument validation above and are
@@ -283,6 +457,13 @@ TORCH_LIBRARY_IMPL(fmha_unified, CPU, m) {
     m.impl("rope_paged", &rope_paged);
     m.impl("key_weights", &key_weights);
     m.impl("evict_paged", &evict_paged);
+    m.impl("fmha_tree", &fmha_tree);
+    m.impl("fmha_tree_lse", &fmha_tree_lse);
+    m.impl("keep_path", &keep_path);
+    m.impl("plan_packed", &plan_packed);
+    m.impl("rope_packed", &rope_packed);
+    m.impl("fmha_packed", &fmha_packed);
+    m.impl("fmha_packed_lse", &fmha_packed_lse);
 }
 
 // _C as a Python extension module. The operators of the paged cache are functions of it as well: with eight to twelve arguments, most of them tensors, a call
@@ -316,6 +497,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     def(m, "rope_paged", &rope_paged);
     def(m, "key_weights", &key_weights);
     def(m, "evict_paged", &evict_paged);
+    def(m, "fmha_tree", &fmha_tree);
+    def(m, "fmha_tree_lse", &fmha_tree_lse);
+    def(m, "keep_path", &keep_path);
+    def(m, "plan_packed", &plan_packed);
+    def(m, "rope_packed", &rope_packed);
+    def(m, "fmha_packed", &fmha_packed);
+    def(m, "fmha_packed_lse", &fmha_packed_lse);
 }
 
 }  // namespace fmha_unified

@@ -21,11 +21,13 @@ EXPORTED_SYMBOLS = ("mi355_hgemm", "mi355_fmha_fwd", "mi355_fmha_fwd_strided", "
                     "mi355_fmha_fwd_workspace_bytes", "mi355_fmha_fwd_ws", "mi355_fmha_fwd_noalloc",
                     "mi355_fmha_paged_workspace_bytes", "mi355_fmha_paged", "mi355_rope_paged", "mi355_fmha_key_weights_workspace_bytes",
                     "mi355_fmha_key_weights", "mi355_cache_evict_workspace_bytes", "mi355_cache_evict",
+                    "mi355_fmha_paged_tree_workspace_bytes", "mi355_fmha_paged_tree", "mi355_cache_keep_path",
+                    "mi355_packed_plan_workspace_bytes", "mi355_packed_plan", "mi355_rope_packed", "mi355_fmha_packed_workspace_bytes", "mi355_fmha_packed",
                     "mi355_last_error", "mi355_serving_version")
 # exported for tests and tuning runs, declared in csrc/mi355_serving_internal.h and not in the public header
 INTERNAL_SYMBOLS = ("mi355_internal_hgemm_variant", "mi355_internal_hgemm_add_variant", "mi355_internal_hgemm_choice", "mi355_internal_hgemm_wide_ranges", "mi355_internal_hgemm_direct_choice",
                     "mi355_internal_gemm_copy_bytes",
-                    "mi355_internal_hgemm_silu_mul_variant", "mi355_internal_fmha_fwd_variant",
+                    "mi355_internal_hgemm_silu_mul_variant", "mi355_internal_fmha_fwd_variant", "mi355_internal_fmha_packed_variant",
                     "mi355_internal_fmha_decode_plan", "mi355_internal_step_qkv", "mi355_internal_step_gate_up")
 
 _lib = None
@@ -116,6 +118,24 @@ def load():
     lib.mi355_cache_evict_workspace_bytes.restype = size
     lib.mi355_cache_evict.argtypes = [cache, i32, i32, vp, vp, size, vp]
     lib.mi355_cache_evict.restype = i32
+    lib.mi355_fmha_paged_tree_workspace_bytes.argtypes = [cache, i32, i32]
+    lib.mi355_fmha_paged_tree_workspace_bytes.restype = size
+    lib.mi355_fmha_paged_tree.argtypes = [cache, vp, vp, vp, i32, i32, ctypes.POINTER(i64), vp, i64, f32, vp, size, vp]
+    lib.mi355_fmha_paged_tree.restype = i32
+    lib.mi355_cache_keep_path.argtypes = [cache, vp, i32, i64, vp, vp]
+    lib.mi355_cache_keep_path.restype = i32
+    lib.mi355_packed_plan_workspace_bytes.argtypes = [i32]
+    lib.mi355_packed_plan_workspace_bytes.restype = size
+    lib.mi355_packed_plan.argtypes = [vp, i64, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, size, vp]
+    lib.mi355_packed_plan.restype = i32
+    lib.mi355_rope_packed.argtypes = [cache, vp, i32, i32, i32, i64, vp, vp, vp, vp, i32, vp]
+    lib.mi355_rope_packed.restype = i32
+    lib.mi355_fmha_packed_workspace_bytes.argtypes = [i32, i32, i32, i32]
+    lib.mi355_fmha_packed_workspace_bytes.restype = size
+    lib.mi355_fmha_packed.argtypes = [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, ctypes.POINTER(i64), f32, i32, i32, vp, size, vp]
+    lib.mi355_fmha_packed.restype = i32
+    lib.mi355_internal_fmha_packed_variant.argtypes = [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, ctypes.POINTER(i64), f32, i32, i32, vp, size, i32, vp]
+    lib.mi355_internal_fmha_packed_variant.restype = i32
     lib.mi355_internal_hgemm_variant.argtypes = [vp, vp, vp, i32, i32, i32, i64, i64, i64, i32, i32, i32, vp]
     lib.mi355_internal_hgemm_variant.restype = i32
     lib.mi355_internal_hgemm_add_variant.argtypes = [vp, vp, vp, vp, i32, i32, i32, i64, i64, i64, i64, i32, i32, i32, vp]
