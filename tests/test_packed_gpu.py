@@ -156,7 +156,7 @@ def test_a_whole_batch_of_nan_ends(gpu):
 
 def test_offsets_that_are_wrong_leave_the_rest_alone(gpu):
     q, k, v = batch([200, 100], 8, 2, torch.float16)
-    for offsets, lens, first in (([0, 200, 100, 300], [200, 0, 100], 0), ([0, 200, 900], [200, 100], 0), ([-5, 200, 300], [200, 100], 0), ([50, 100, 120], [50, 20], 50), ([400, 500], [0], 300)):
+    for offsets, lens, first in (([0, 200, 100, 300], [200, 0, 100], 0), ([0, 200, 100], [200], 0), ([0, 200, 100, 250, 20], [200, 0, 50], 0), ([0, 200, 900], [200, 100], 0), ([-5, 200, 300], [200, 100], 0), ([50, 100, 120], [50, 20], 50), ([400, 500], [0], 300)):
         o, lse = ops.fine_fmha_packed_with_lse(q, k, v, ints(offsets))
         check_packed(q, k, v, lens, o, lse, first=first)
 

@@ -676,10 +676,10 @@ int mi355_rope_packed(const mi355_paged_kv* pool, void* qkv, int rows, int q_hea
 }
 
 static bool packed_sizes(int rows, int B, int Hq, int Hkv) {
-    return rows >= 1 && B >= 1 && Hkv >= 1 && Hq >= Hkv && rows <= (1 << 28) && B <= (1 << 28) && Hq <= 65535 && mi355::packed_fits(rows, B, Hq);
+    return rows >= 1 && B >= 1 && Hkv >= 1 && Hq >= Hkv && rows <= (1 << 28) && B <= (1 << 28) && Hq <= 65535 && mi355::packed_fits(rows, B, Hq, Hkv);
 }
 
-size_t mi355_fmha_packed_workspace_bytes(int rows, int B, int Hq, int Hkv) { return packed_sizes(rows, B, Hq, Hkv) ? mi355::packed_workspace(rows, B) : 0; }
+size_t mi355_fmha_packed_workspace_bytes(int rows, int B, int Hq, int Hkv) { return packed_sizes(rows, B, Hq, Hkv) ? mi355::packed_workspace(rows, B, Hq, Hkv) : 0; }
 
 static int fmha_packed_impl(const char* fn, const void* Q, const void* K, const void* V, void* O, float* LSE, const int32_t* offsets, int rows, int B, int Hq, int Hkv,
                             const int64_t* strides, float scale, int causal, int dtype, void* workspace, size_t workspace_bytes, int variant, void* stream) {
@@ -699,7 +699,7 @@ static int fmha_packed_impl(const char* fn, const void* Q, const void* K, const 
     if ((rows > 1 && st[6] < 128) || (Hq > 1 && st[7] < 128))
         return fail(MI355_ERR_BAD_ARGUMENT, "%s: rows of O overlap (o strides %lld, %lld)", fn, (long long)st[6], (long long)st[7]);
     if (!aligned16(Q) || !aligned16(K) || !aligned16(V) || !aligned16(O)) return fail(MI355_ERR_BAD_ARGUMENT, "%s: pointers must be 16-byte aligned", fn);
-    if (int rc = workspace_checked(fn, mi355::packed_workspace(rows, B), workspace, workspace_bytes)) return rc;
+    if (int rc = workspace_checked(fn, mi355::packed_workspace(rows, B, Hq, Hkv), workspace, workspace_bytes)) return rc;
     const mi355::FmhaStrides sd = {0, (long)st[1], (long)st[0], 0, (long)st[3], (long)st[2], 0, (long)st[5], (long)st[4], 0, (long)st[7], (long)st[6]};
     const hipError_t e = mi355::packed_dispatch(Q, K, V, O, LSE, offsets, rows, B, Hq, Hkv, sd, scale, causal, dtype, workspace, variant, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? 0 : hip_fail(e, fn);

@@ -178,16 +178,106 @@ __device__ __forceinline__ void copy16_global_to_lds_at(const void* uniform_base
 // queries, which are a single block of rows of the first wave and are stored as they lie: through LDS they are a chain of its own behind the
 // item, and a branch in the other kernels costs those up to 2 %. us, through LDS / as they lie: 64 x 16/2 heads, 9 queries over 64 keys 17.1 /
 // 15.9, 24 x 32/8, 16 over 64 13.8 / 13.1, 12 x 64/8, 16 over 128 18.2 / 17.6.
-// kPacked: sequences of different lengths one behind the other in one batch; the work items are those of a list that packed_items_kernel made on the
-// device (below), and a row whose result is NaN is worked out again (see packed_row).
+// kPacked: sequences of different lengths one behind the other in one batch, with work items of several heads (below); a row whose result is NaN is
+// worked out again (packed_row); the sums of probabilities are made from what they are in 32 bits (on the matrix pipe they are those of the rounded ones, which leaves
+// the log-sum-exp 3e-4 of a short row off; no slower here, and 20 bytes of registers fewer spilled).
 enum { kOneWalk = 0, kRanges = 1, kRangesF32 = 2, kFewRows = 3, kPacked = 4 };
 constexpr int kFewRowsMax = 16;
 
-// The list of a packed batch: `entries` q tiles {first row of the sequence, its rows, q tile, 0}, those with the most keys first
+// The list of a packed batch: `entries` q tiles {first row of the sequence, its rows, q tile, 0}, those with the most keys first. A work item is such a tile of
+// 2^head_shift query heads of one kv head, side by side: BM / 2^head_shift rows of each.
 struct PackedItems {
-    const int4v* list;
-    const int* entries;
-    long rows;   // of the batch: row stride of LSE
+    const int4v* list;    // null: few sequences, whose items a workgroup finds in the offsets itself (PackedOffsets)
+    const int* entries;   // and behind it the first row of the first sequence and the one behind the last's
+    const int* offsets;
+    long rows;            // of the batch: row stride of LSE
+    int B, head_shift;
+};
+// Up to 64 sequences, one a lane, and their q tiles, which every workgroup finds for itself: a launch less (6 us) for about 1 us of counting at the start (16 sequences)
+struct PackedOffsets {
+    static constexpr int kMost = 64, kMostTiles = 512;   // sequences, tiles of one of them
+    int start, rows, tiles;          // of this lane's sequence
+    int begin, end, entries;         // rows of all, q tiles
+    __device__ __forceinline__ PackedOffsets(const int* offsets, int B, int all_rows, int tile) {
+        const int lane = threadIdx.x & 63, first = offsets[min(lane, B)], last = offsets[min(lane + 1, B)];
+        // (offsets that descend are taken for the largest one in front of them; lanes behind the last sequence begin and end at the last offset)
+        start = min(max(first, 0), all_rows);
+        begin = __builtin_amdgcn_readfirstlane(start);
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int y = __shfl_up(start, off, 64);
+            if (lane >= off) start = max(start, y);
+        }
+        rows = max(min(last, all_rows) - start, 0);
+        end = __builtin_amdgcn_readlane(start + rows, 63);
+        tiles = (int)((uint32_t)(rows + tile - 1) / (uint32_t)tile);
+        entries = __builtin_amdgcn_readlane(up_to(tiles), 63);
+    }
+    static __device__ __forceinline__ int up_to(int x) {   // sum over the lanes up to this one
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int y = __shfl_up(x, off, 64);
+            if (lane >= off) x += y;
+        }
+        return x;
+    }
+    // {first row, rows, tile, 0} of tile `rank` in the order of (sequence, tile); the same for all lanes
+    __device__ __forceinline__ int4v in_order(int rank) const {
+        const int incl = up_to(tiles);
+        const uint64_t past = __builtin_amdgcn_ballot_w64(rank < incl);
+        const int i = past == 0 ? 0 : __builtin_ctzll(past);
+        return int4v{__builtin_amdgcn_readlane(start, i), __builtin_amdgcn_readlane(rows, i), rank - __builtin_amdgcn_readlane(incl, i) + __builtin_amdgcn_readlane(tiles, i), 0};
+    }
+};
+// Their tiles in the order of the keys that they see, most first, in LDS. The sequences are sorted by their rows. Causal: tiles of larger numbers come first, of equal
+// ones those of longer sequences: tile t of the k-th longest is behind the at_least[t + 1] = sum max(tiles - t - 1, 0) of larger numbers and k others. Otherwise the
+// tiles of longer sequences come first: at_least[k] of sequences in front of the k-th longest.
+struct PackedOrder {
+    int start[PackedOffsets::kMost], rows[PackedOffsets::kMost], place[PackedOffsets::kMost], at_least[PackedOffsets::kMostTiles + 1];
+    // all 8 waves
+    __device__ __forceinline__ void make(const PackedOffsets& s, int B, int tile, int causal) {
+        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+        if (tid < 64) place[tid] = 0;
+        __syncthreads();
+        int longer = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int b = wave * 8 + i, n = __builtin_amdgcn_readlane(s.rows, b);
+            longer += n > s.rows || (n == s.rows && b < lane);
+        }
+        atomicAdd(&place[lane], longer);
+        __syncthreads();
+        if (tid < 64) start[place[tid]] = s.start, rows[place[tid]] = s.rows;
+        __syncthreads();
+        const auto tiles_of = [&](int k) { return (int)((uint32_t)(rows[k] + tile - 1) / (uint32_t)tile); };
+        if (causal) {
+            const int tiles = tiles_of(lane);
+            int sum = 0;
+            for (int k = 0; k < B; ++k) sum += max(__builtin_amdgcn_readlane(tiles, k) - tid, 0);
+            at_least[tid] = sum;
+            if (tid == 0) at_least[PackedOffsets::kMostTiles] = 0;
+        } else if (wave == 0) {
+            const int tiles = tiles_of(lane);
+            at_least[lane] = PackedOffsets::up_to(tiles) - tiles;
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ int4v find(int rank, int causal) const {
+        int k = 0, t = 0;
+        if (causal) {
+#pragma unroll 1
+            for (int step = PackedOffsets::kMostTiles / 2; step > 0; step >>= 1)
+                if (at_least[t + step] > rank) t += step;
+            k = rank - at_least[t + 1];
+        } else {
+#pragma unroll
+            for (int step = PackedOffsets::kMost / 2; step > 0; step >>= 1)
+                if (at_least[k + step] <= rank) k += step;   // (sequences without rows are behind all others)
+            t = rank - at_least[k];
+        }
+        return int4v{start[k], rows[k], t, 0};
+    }
 };
 // what a work item knows beside the others' fields
 template <bool PACKED>
@@ -195,7 +285,7 @@ struct PackedItem {};
 template <>
 struct PackedItem<true> {
     int rows;       // of its sequence
-    float* lse;     // of its head and the sequence's first row
+    float* lse;     // of its first head and the sequence's first row
 };
 
 // One row of a packed batch in 32 bits, key by key, with nothing of the keys that it does not see: 64 keys at a time, a lane scores one of them and then sums 2 of the 128 outputs.
@@ -285,7 +375,9 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
         int exists;              // 0: no such item, nothing else is set
     };
     const long o_row = SEG ? (long)D : sd.o_row;
-    auto item_of = [&](int round) -> Item {
+    __shared__ typename std::conditional<PACKED, PackedOrder, char>::type order;
+    int packed_entries = 0;
+    auto item_of = [&](int round, const PackedOffsets* first = nullptr) -> Item {
         // (opaque copies: the compiler would form products of these once and keep them in registers through the loop over the keys, which
         // has none to spare)
         int q_tiles_ = q_tiles;
@@ -298,23 +390,32 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
             const int x = blockIdx.x & ((1 << map_.xcd_shift) - 1), wl = blockIdx.x >> map_.xcd_shift;
             const int u = round * map_.wgs + ((round & 1) ? map_.wgs - 1 - wl : wl);
             const int rank = divide(u, map_.by_rank), rem = u - rank * map_.per_rank;
-            const int4v entry = packed.list[min(rank, q_tiles_ - 1)];   // (q_tiles: the most entries that there may be)
-            it.exists = rank < *packed.entries;
+            int4v entry;
+            if (first != nullptr) {
+                it.exists = rank < first->entries;
+                entry = first->in_order(rank);
+            } else if (packed.list == nullptr) {
+                it.exists = rank < packed_entries;
+                entry = order.find(max(min(rank, packed_entries - 1), 0), causal);
+            } else {
+                entry = packed.list[min(rank, q_tiles_ - 1)];   // (q_tiles: the most entries that there may be)
+                it.exists = rank < *packed.entries;
+            }
             if (!it.exists) return it;
             const int gl = divide(rem, map_.by_group), kvh = x * map_.groups_per_xcd + gl;
-            const int head = kvh * map_.group + rem - gl * map_.group;
+            const int head = (kvh * map_.group + rem - gl * map_.group) << packed.head_shift;   // (map: of heads side by side)
             const long row0 = entry[0];
             it.rows = entry[1];
             it.lse = LSE == nullptr ? nullptr : LSE + head * packed.rows + row0;
             it.lse_row = 0;
-            it.q_block0 = entry[2] * BM;
+            it.q_block0 = entry[2] * (BM >> packed.head_shift);
             it.kv_valid = it.rows;
             it.shift = 0;
             it.Qh = Q + row0 * sd.q_row + head * sd.q_head;
             it.Kh = K + row0 * sd.k_row + kvh * sd.k_head;
             it.Vh = V + row0 * sd.v_row + kvh * sd.v_head;
             it.Oh = O + row0 * sd.o_row + head * sd.o_head;
-            it.n_tiles = ((causal ? min(it.q_block0 + BM, it.rows) : it.rows) + BN - 1) / BN;
+            it.n_tiles = ((causal ? min(it.q_block0 + (BM >> packed.head_shift), it.rows) : it.rows) + BN - 1) / BN;
             return it;
         }
         it.exists = fmha_work_item(blockIdx.x, round, q_tiles_, map_, b, hkv, hq, q_tile);
@@ -362,15 +463,58 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
     };
     // steps of an item in which the pair that is copied (tiles j + 3 of K, j + 2 of V) is made of full tiles
     auto fast_steps = [](int n_tiles, int kv_valid) { return min(min(n_tiles, kv_valid / BN) - 3, n_tiles - 1); };
-    Item cur = item_of(0);   // a launch has no more workgroups than items
-    if constexpr (PACKED) {  // (than there may be)
+    Item cur;
+    long packed_items = 0;   // of the launch, where a workgroup may have more than one
+    if constexpr (PACKED) {
+        int begin, end;
+        if (packed.list == nullptr) {
+            const PackedOffsets sequences(packed.offsets, packed.B, Sq, BM >> packed.head_shift);
+            begin = sequences.begin;
+            end = sequences.end;
+            packed_entries = sequences.entries;
+            if ((long)q_tiles * (Hq >> packed.head_shift) <= gridDim.x) {   // an item a workgroup at most, in any order
+                cur = item_of(0, &sequences);
+            } else {
+                packed_items = (long)packed_entries * (Hq >> packed.head_shift);
+                order.make(sequences, packed.B, BM >> packed.head_shift, causal);
+                cur = item_of(0);
+            }
+        } else {
+            begin = packed.entries[1];
+            end = packed.entries[2];
+            packed_items = (long)*packed.entries * (Hq >> packed.head_shift);
+            cur = item_of(0);
+        }
+        int words[sizeof(Item) / 4];   // (in scalar registers)
+        __builtin_memcpy(words, &cur, sizeof(Item));
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(Item) / 4); ++i) words[i] = __builtin_amdgcn_readfirstlane(words[i]);
+        __builtin_memcpy(&cur, words, sizeof(Item));
+        // zeros for the rows that no sequence has, in front of the first and behind the last
+        const int none = begin + Sq - end;
+        for (long i = blockIdx.x * 512L + tid; i < (long)none * Hq * 16; i += gridDim.x * 512L) {
+            const long rest = i >> 4, r = rest / Hq, head = rest - r * Hq, row = r < begin ? r : r + end - begin;
+            *(int4v*)(O + row * sd.o_row + head * sd.o_head + (i & 15) * 8) = int4v{0, 0, 0, 0};
+            if (LSE != nullptr && (i & 15) == 0) LSE[head * packed.rows + row] = -INFINITY;
+        }
+    }
+    if constexpr (PACKED) {
         if (!cur.exists) return;
+    } else {
+        cur = item_of(0);   // a launch has no more workgroups than items
     }
     const auto rows_of = [&](const Item& it) {
         if constexpr (PACKED) return it.rows;
         else return Sq;
     };
-    int q_wave0 = cur.q_block0 + wave * WQ;
+    // this wave's head of an item, and its first row
+    const int wave_head = PACKED ? wave >> (3 - packed.head_shift) : 0;
+    const int wave_row0 = PACKED ? (wave & ((NWAVES >> packed.head_shift) - 1)) * WQ : wave * WQ;
+    const auto queries_of = [&](const Item& it) {
+        if constexpr (PACKED) return it.Qh + wave_head * sd.q_head;
+        else return it.Qh;
+    };
+    int q_wave0 = cur.q_block0 + wave_row0;
 
     // Q fragments (B operand of the first product): lane holds Q[16 qb + c][32 ks + 8 g .. +7]
     V8 qf[QB][4];
@@ -682,9 +826,9 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
     // starts there, also where that means that its first pairs can only leave behind the last barrier of the item in front (a second copy
     // of the general step in front of the loop makes the 256-query instantiation spill 400 bytes a lane).
     MI355_TL(unsigned long long tl_tiles = 0, tl_end = 0, tl_between = 0;)   // cycles from an item's last barrier to the first of the next
-    load_q(cur.Qh, q_wave0, rows_of(cur));
+    load_q(queries_of(cur), q_wave0, rows_of(cur));
     if (cur.n_tiles > 0) issue_first_pairs();
-    const bool more_items = (PACKED ? (long)*packed.entries * Hq : (long)q_tiles * Hq * B * (SEG ? segments : 1)) > gridDim.x;   // of the launch, than it has workgroups
+    const bool more_items = (PACKED ? packed_items : (long)q_tiles * Hq * B * (SEG ? segments : 1)) > gridDim.x;   // of the launch, than it has workgroups
     bool landed = false;   // the current item's first pairs and Q fragments have been waited for
     for (int round = 0;;) {
 #pragma unroll
@@ -758,7 +902,7 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
             if (more_items) {
                 const Item next = item_from(listed_words(round));
                 more = next.exists;
-                if (more) load_q(next.Qh, next.q_block0 + wave * WQ, rows_of(next));
+                if (more) load_q(queries_of(next), next.q_block0 + wave_row0, rows_of(next));
             }
             softmax_tile(s, n_tiles - 1, pf, std::integral_constant<int, -2>{});
             if (n_tiles == 2 && n_next > 0) {   // two tiles have no step that copies pair n_tiles: K(0) of the next item
@@ -784,21 +928,22 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
             if (more_items) {
                 const Item next = item_from(listed_words(round));
                 more = next.exists;
-                if (more) load_q(next.Qh, next.q_block0 + wave * WQ, rows_of(next));
+                if (more) load_q(queries_of(next), next.q_block0 + wave_row0, rows_of(next));
             }
         }
 
         // what the epilogue needs of the item just finished, then on to the next one
-        T* const o_item = cur.Oh;
+        T* o_item = cur.Oh;
+        if constexpr (PACKED) o_item += wave_head * sd.o_head;
         const int q_item0 = q_wave0;
         float* lse_item = LSE == nullptr ? nullptr : LSE + (long)cur.lse_row * Sq;
         const int item_rows = rows_of(cur);
-        if constexpr (PACKED) lse_item = cur.lse;
+        if constexpr (PACKED) lse_item = cur.lse == nullptr ? nullptr : cur.lse + wave_head * packed.rows;
         if (more) {
             landed = n_next > 0;
             ring = landed ? ring + cur.n_tiles : 0;
             cur = item_from(listed_words(round));
-            q_wave0 = cur.q_block0 + wave * WQ;
+            q_wave0 = cur.q_block0 + wave_row0;
             src_k = {cur.Kh, 0, cur.n_tiles - 1, cur.kv_valid};
             src_v = {cur.Vh, 0, cur.n_tiles - 1, cur.kv_valid};
             if (cur.n_tiles > 0 && !landed) issue_first_pairs();
@@ -869,11 +1014,11 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
                     for (int e = 0; e < 4; ++e) nan = nan || o[db][qb][e] != o[db][qb][e];
                 uint64_t lanes = __builtin_amdgcn_ballot_w64(nan && q_first + r16 < item_rows);
                 if (lanes != 0) {
-                    const Item done = item_of(round - 1);
+                    const Item done = more ? item_of(round - 1) : cur;
                     uint32_t again = (uint32_t)(lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) & 0xffff;
                     for (; again != 0; again &= again - 1) {
                         const int i = q_first + __builtin_ctz(again);
-                        packed_row<T>(done.Qh + i * sd.q_row, done.Kh, done.Vh, sd.k_row, sd.v_row, causal ? i + 1 : done.rows, scale_log2, done.Oh + i * o_row);
+                        packed_row<T>(queries_of(done) + i * sd.q_row, done.Kh, done.Vh, sd.k_row, sd.v_row, causal ? i + 1 : done.rows, scale_log2, o_item + i * o_row);
                     }
                 }
             }
@@ -1229,25 +1374,19 @@ hipError_t fmha_fwd_dispatch(const void* Q, const void* K, const void* V, void* 
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// A packed batch: sequences of different lengths, rows offsets[b] .. offsets[b + 1] - 1 of one batch each, known to the device only. Its first kernel makes the
-// list of q tiles, ordered by the keys that they see (a counting sort: of equal ones in no particular order, which decides which workgroup takes which, and nothing
-// else), and writes zeros to the rows that no sequence has; the second is the kernel above, which deals the list's entries out like q tiles of one sequence.
+// A packed batch: sequences of different lengths, rows offsets[b] .. offsets[b + 1] - 1 of one batch each, known to the device only. Its q tiles, those that see the
+// most keys first, are dealt out like those of one sequence. Up to 64 sequences every workgroup works the order out for itself (PackedOrder); for more of them this kernel makes a list
+// (a counting sort: of equal tiles in no particular order, which decides which workgroup takes which, and nothing else).
+//
+// A work item is a q tile of up to 8 query heads of a kv head, side by side: 32 rows of 8 heads see fewer keys that none of them sees than 256 rows of one (of 512 rows 147 of
+// 197 k pairs are worked out, 131 k are seen), and a sequence's last tile is a smaller part of it. Bound by the matrix pipes and the vector unit in turn, like one long sequence, and for
+// short ones by the way of an item's operands and results to and from memory. us, 256 rows of a head and a list / now: 16 sequences of up to 1000 rows of 32/8 heads 119 / 90 (520
+// TFLOP/s of those seen), 4 of up to 8192 1091 / 1054 (1167), 64 of up to 200 74 / 52, 3 of up to 77 of 8/2 heads 12.0 / 8.3 (one launch).
 // ---------------------------------------------------------------------------------------------------------------
 namespace packed {
 constexpr int THREADS = 1024, WAVES = THREADS / 64;
 constexpr int BINS = 1024;     // of key tiles, the heaviest first
-constexpr int kRowsAWorkgroup = 64;   // rows behind the last sequence
-constexpr int kMostTails = 256;
 
-// running maximum of a value a lane over the lanes up to this one
-__device__ __forceinline__ int wave_running_max(int x) {
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const int y = __shfl_up(x, off, 64);
-        if ((int)(threadIdx.x & 63) >= off) x = max(x, y);
-    }
-    return x;
-}
 }  // namespace packed
 
 struct PackedList {
@@ -1257,52 +1396,71 @@ struct PackedList {
     int B, rows, tile, most, causal, shift;   // tile: rows of a q tile; most: entries that there may be; shift: key tiles of a bin
 };
 
-// Workgroup 0 makes the list, the others write zeros (O, LSE = -inf) to rows in front of the first sequence and behind the last
-template <typename T>
-__global__ __launch_bounds__(packed::THREADS) void packed_items_kernel(PackedList p, T* O, float* LSE, int Hq, long o_row, long o_head) {
+// One workgroup
+__global__ __launch_bounds__(packed::THREADS) void packed_items_kernel(PackedList p) {
     using namespace packed;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const auto row_of = [&](int b) { return min(max(p.offsets[b], 0), p.rows); };
-    if (blockIdx.x > 0) {
-        // rows r .. of `row_of(0)` in front and behind: a wave a (row, head)
-        const int begin = row_of(0), end = row_of(p.B);
-        for (int r = (int)(blockIdx.x - 1) * kRowsAWorkgroup; r < p.rows; r += (int)(gridDim.x - 1) * kRowsAWorkgroup) {
-            if (r >= begin && r + kRowsAWorkgroup <= end) continue;
-            for (int i = tid; i < kRowsAWorkgroup * Hq * 16; i += THREADS) {
-                const int d = (i & 15) * 8, head = (i >> 4) % Hq, row = r + (i >> 4) / Hq;
-                if (row >= p.rows || (row >= begin && row < end)) continue;
-                *(int4v*)(O + row * o_row + head * o_head + d) = int4v{0, 0, 0, 0};
-                if (LSE != nullptr && d == 0) LSE[(long)head * p.rows + row] = -INFINITY;
-            }
-        }
-        return;
-    }
-    __shared__ int bins[BINS], sums[WAVES], tops[WAVES];
+    __shared__ int bins[BINS], sums[2][WAVES], starts[THREADS], counts[THREADS], before[THREADS];
     bins[tid] = 0;
     static_assert(BINS == THREADS, "a bin a thread");
-    // Offsets that descend are taken for the largest one in front of them, so that no two sequences have a row in common. Each group of 1024 sequences
-    // needs the largest offset in front of it.
-    const auto each = [&](auto f) {   // f(first row, rows, q tile): a sequence of one tile by its lane, those of more by the whole wave
+    int last_row = 0;
+    // sum over the threads up to this one
+    const auto block_sum = [&](int x, int (&per_wave)[WAVES], int& all) {
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int y = __shfl_up(x, off, 64);
+            if (lane >= off) x += y;
+        }
+        if (lane == 63) per_wave[wave] = x;
+        __syncthreads();
+        all = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            if (w == wave) x += all;
+            all += per_wave[w];
+        }
+        return x;
+    };
+    // f(first row, rows, q tile) of every q tile, one a thread: 1024 sequences at a time, a thread finds its tile's in the sums of their tiles. Offsets that descend are
+    // taken for the largest one in front of them, so that no two sequences have a row in common.
+    const auto each = [&](auto f) {
         int front = 0;
         for (int b0 = 0; b0 < p.B; b0 += THREADS) {
-            const int b = b0 + tid;
-            int start = b < p.B ? row_of(b) : 0, end = b < p.B ? row_of(b + 1) : 0;
-            start = wave_running_max(start);
-            if (p.B > 64) {   // (the waves of a group)
+            const int b = b0 + tid, here = min(p.B - b0, THREADS);
+            int start = b < p.B ? row_of(b) : 0;
+            const int end = b < p.B ? row_of(b + 1) : 0;
+            if (b0 == 0 && tid == 0) last_row = start;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const int y = __shfl_up(start, off, 64);
+                if (lane >= off) start = max(start, y);
+            }
+            if (here > 64 || b0 > 0) {   // (the waves of a group)
                 __syncthreads();
-                if (lane == 63) tops[wave] = start;
+                if (lane == 63) sums[0][wave] = start;
                 __syncthreads();
-                for (int w = 0; w < wave; ++w) start = max(start, tops[w]);
+                for (int w = 0; w < wave; ++w) start = max(start, sums[0][w]);
                 start = max(start, front);
-                for (int w = 0; w < WAVES; ++w) front = max(front, tops[w]);
+                for (int w = 0; w < WAVES; ++w) front = max(front, sums[0][w]);
             }
-            const int n = b < p.B ? max(end - start, 0) : 0, tiles = (n + p.tile - 1) / p.tile;
-            if (tiles == 1) f(start, n, 0);
-            for (uint64_t left = __builtin_amdgcn_ballot_w64(tiles > 1); left != 0; left &= left - 1) {
-                const int i = __builtin_ctzll(left);
-                const int s = __builtin_amdgcn_readlane(start, i), m = __builtin_amdgcn_readlane(n, i), t = __builtin_amdgcn_readlane(tiles, i);
-                for (int k = lane; k < t; k += 64) f(s, m, k);
+            const int n = b < p.B ? max(end - start, 0) : 0, tiles = (int)((uint32_t)(n + p.tile - 1) / (uint32_t)p.tile);
+            int all;
+            const int incl = block_sum(tiles, sums[1], all);
+            starts[tid] = start;
+            counts[tid] = n;
+            before[tid] = incl - tiles;
+            __syncthreads();
+            int span = 1;
+            while (span < here) span <<= 1;
+            for (int e = tid; e < all; e += THREADS) {
+                int i = 0;   // the last sequence with no more than e tiles in front of it
+                for (int step = span >> 1; step > 0; step >>= 1)
+                    if (i + step < here && before[i + step] <= e) i += step;
+                f(starts[i], counts[i], e - before[i]);
             }
+            if (n > 0) last_row = max(last_row, start + n);
+            __syncthreads();
         }
     };
     const auto bin_of = [&](int n, int k) {
@@ -1311,23 +1469,18 @@ __global__ __launch_bounds__(packed::THREADS) void packed_items_kernel(PackedLis
     };
     __syncthreads();
     each([&](int, int n, int k) { atomicAdd(&bins[bin_of(n, k)], 1); });
-    __syncthreads();
-    const int mine = bins[tid];
-    int incl = mine;
+    int all;
+    const int mine = bins[tid], incl = block_sum(mine, sums[0], all);
+    bins[tid] = incl - mine;
+    // the row behind the last sequence
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const int y = __shfl_up(incl, off, 64);
-        if (lane >= off) incl += y;
-    }
-    if (lane == 63) sums[wave] = incl;
+    for (int off = 32; off >= 1; off >>= 1) last_row = max(last_row, __shfl_xor(last_row, off, 64));
+    if (lane == 0) sums[1][wave] = last_row;
     __syncthreads();
-    int front = 0, all = 0;
-    for (int w = 0; w < WAVES; ++w) {
-        if (w < wave) front += sums[w];
-        all += sums[w];
+    if (tid == 0) {
+        for (int w = 0; w < WAVES; ++w) last_row = max(last_row, sums[1][w]);
+        p.entries[0] = min(all, p.most), p.entries[1] = row_of(0), p.entries[2] = last_row;
     }
-    bins[tid] = front + incl - mine;
-    if (tid == 0) *p.entries = min(all, p.most);
     __syncthreads();
     each([&](int start, int n, int k) {
         const int at = atomicAdd(&bins[bin_of(n, k)], 1);
@@ -1338,7 +1491,13 @@ __global__ __launch_bounds__(packed::THREADS) void packed_items_kernel(PackedLis
 // q tiles of `tile` rows that B sequences of `rows` rows in all can have
 static long packed_entries(int rows, int B, int tile) { return (long)rows / tile + std::min(B, rows); }
 
-size_t packed_workspace(int rows, int B) { return 16 * ((size_t)packed_entries(rows, B, 128) + 1); }
+// heads of a kv head that are side by side in a work item: 2^this, the largest power of two up to 8 that divides them
+static int packed_head_shift(int Hq, int Hkv) {
+    const int group = Hq / Hkv;
+    return group % 8 == 0 ? 3 : group % 4 == 0 ? 2 : group % 2 == 0 ? 1 : 0;
+}
+
+size_t packed_workspace(int rows, int B, int Hq, int Hkv) { return 16 * ((size_t)packed_entries(rows, B, 128 >> packed_head_shift(Hq, Hkv)) + 1); }
 
 template <typename T, int QB>
 static hipError_t launch_packed(const T* Q, const T* K, const T* V, T* O, float* LSE, const int* offsets, int rows, int B, int Hq, int Hkv, const FmhaStrides& sd,
@@ -1355,33 +1514,53 @@ static hipError_t launch_packed(const T* Q, const T* K, const T* V, T* O, float*
     p.list = (int4v*)workspace + 1;
     p.B = B;
     p.rows = rows;
-    p.tile = BM;
-    p.most = (int)packed_entries(rows, B, BM);
+    const int shift = packed_head_shift(Hq, Hkv);
+    p.tile = BM >> shift;
+    p.most = (int)packed_entries(rows, B, p.tile);
     p.causal = causal;
     while ((rows + fmha::BN - 1) / fmha::BN >> p.shift > packed::BINS) ++p.shift;
-    const int tails = std::min(packed::kMostTails, (rows + packed::kRowsAWorkgroup - 1) / packed::kRowsAWorkgroup);
-    packed_items_kernel<T><<<dim3(1 + tails), dim3(packed::THREADS), 0, stream>>>(p, O, LSE, Hq, sd.o_row, sd.o_head);
-    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-    const long items = (long)p.most * Hq;
+    const long items = (long)p.most * (Hq >> shift);
+    if (B <= PackedOffsets::kMost && rows <= PackedOffsets::kMostTiles * p.tile) {
+        p.list = nullptr;
+    } else {
+        packed_items_kernel<<<dim3(1), dim3(packed::THREADS), 0, stream>>>(p);
+        if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
     long blocks = items < cus ? items : cus;
     if (Hkv % 8 == 0 && blocks >= 8) blocks &= ~7L;
     kern<<<dim3((unsigned)blocks), dim3(512), LDS, stream>>>(Q, K, V, O, LSE, 1, Hq, Hkv, rows, rows, scale * 1.4426950408889634f, causal, rows, p.most, sd, 1, 0,
-                                                             item_map(1, Hq, Hkv, 1, blocks), PackedItems{p.list, p.entries, rows});
+                                                             item_map(1, Hq >> shift, Hkv, 1, blocks), PackedItems{p.list, p.entries, offsets, rows, B, shift});
     return hipGetLastError();
+}
+
+// Whether work items are of 256 (row, head) pairs, whose K and V fragments feed two MFMAs, or of 128: where sequences of the mean length make 256 items or more that see 2.5 key
+// tiles on average. Over 342 drawn calls (1 .. 64 sequences, 1 .. 6000 rows, 8 .. 64 heads, causal and not) the choice is 0.8 % behind the better one on average, at worst
+// 27 %; 128 throughout 3.9 %. us, 128 / 256: 16 sequences of up to 1000 rows, 32/8 heads 99.8 / 92.3, 4 of up to 8192 1243 / 1040; 1 of 512 14.0 / 21.0, 64 of up to 200 51.7 /
+// 54.5, 8 of up to 600, 40/8 heads 47.2 / 54.6.
+static bool packed_large_tiles(int rows, int B, int Hq, int Hkv, int causal) {
+    const int shift = packed_head_shift(Hq, Hkv), tile = 256 >> shift, mean = (rows + B - 1) / B, tiles = (mean + tile - 1) / tile;
+    long keys = 0;   // key tiles of a sequence's q tiles
+    if (tiles > 64)
+        keys = 3L * tiles;   // (more than that)
+    else if (causal)
+        for (int t = 1; t <= tiles; ++t) keys += (std::min(t * tile, mean) + fmha::BN - 1) / fmha::BN;
+    else
+        keys = (long)tiles * ((mean + fmha::BN - 1) / fmha::BN);
+    return (long)B * tiles * (Hq >> shift) >= 256 && 2 * keys >= 5 * tiles;
 }
 
 template <typename T>
 static hipError_t packed_t(const void* Q, const void* K, const void* V, void* O, float* LSE, const int* offsets, int rows, int B, int Hq, int Hkv,
                            const FmhaStrides& sd, float scale, int causal, void* workspace, int variant, hipStream_t stream) {
-    int cus = 0;
-    if (hipError_t e = compute_units(cus); e != hipSuccess) return e;
-    const int mean = (rows + B - 1) / B;
-    if (variant == 0) variant = one_walk_us(2, cus, B, Hq, mean, mean, causal, mean) < one_walk_us(1, cus, B, Hq, mean, mean, causal, mean) ? 2 : 1;
+    if (variant == 0) variant = packed_large_tiles(rows, B, Hq, Hkv, causal) ? 2 : 1;
     const auto launch = variant == 2 ? &launch_packed<T, 2> : &launch_packed<T, 1>;
     return launch((const T*)Q, (const T*)K, (const T*)V, (T*)O, LSE, offsets, rows, B, Hq, Hkv, sd, scale, causal, workspace, stream);
 }
 
-bool packed_fits(int rows, int B, int Hq) { return packed_entries(rows, B, 128) * Hq <= INT32_MAX / 2; }
+bool packed_fits(int rows, int B, int Hq, int Hkv) {
+    const int shift = packed_head_shift(Hq, Hkv);
+    return packed_entries(rows, B, 128 >> shift) * (Hq >> shift) <= INT32_MAX / 2;
+}
 
 hipError_t packed_dispatch(const void* Q, const void* K, const void* V, void* O, float* LSE, const int* offsets, int rows, int B, int Hq, int Hkv,
                            const FmhaStrides& sd, float scale, int causal, int dtype, void* workspace, int variant, hipStream_t stream) {

@@ -214,8 +214,8 @@ hipError_t packed_plan_dispatch(int* table, long table_stride, int* seq_lens, co
                                 int n_pages, int page_size, int rows, int* offsets, int* positions, int* slots, int* taken, void* workspace, hipStream_t stream);
 hipError_t rope_packed_dispatch(const mi355_paged_kv& pool, void* qkv, int rows, int q_heads, int keep_keys, long x_row, const float* cos_t, const float* sin_t,
                                 const int* positions, const int* slots, int n_pos, hipStream_t stream);
-bool packed_fits(int rows, int B, int Hq);
-size_t packed_workspace(int rows, int B);
+bool packed_fits(int rows, int B, int Hq, int Hkv);
+size_t packed_workspace(int rows, int B, int Hq, int Hkv);
 hipError_t packed_dispatch(const void* Q, const void* K, const void* V, void* O, float* LSE, const int* offsets, int rows, int B, int Hq, int Hkv,
                            const FmhaStrides& strides, float scale, int causal, int dtype, void* workspace, int variant, hipStream_t stream);
 
