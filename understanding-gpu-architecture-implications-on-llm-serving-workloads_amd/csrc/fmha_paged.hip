@@ -290,13 +290,12 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
             const T* qp = Q + b * a.q_batch + (long)(hkv * a.group + head) * a.q_head + qi * a.q_row + 8 * g;
             qrow[nb] = qi;
             lim[nb] = qi < n_new ? min(len - 1, qi + len - n_new) : -1;
-            lim_min = min(lim_min, lim[nb]);
+            if (!TREE || lim[nb] >= 0) lim_min = min(lim_min, lim[nb]);   // (TREE: what the columns of rows that are no tokens see is taken out at the end)
             lim_max = max(lim_max, lim[nb]);
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) qf[nb][ks] = *(const V8*)(qp + ks * 32);
         }
         const int base = len - n_new;       // (TREE) key of the first drafted token
-        if constexpr (TREE) lim_min = min(lim_min, base - 1);
         int row_min = a.Sq, row_max = -1;   // rows of the columns of this wave
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) row_min = min(row_min, qrow[nb]), row_max = max(row_max, qrow[nb]);
@@ -309,6 +308,7 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
         }
         lim_min = __builtin_amdgcn_readfirstlane(lim_min);
         lim_max = __builtin_amdgcn_readfirstlane(lim_max);
+        if constexpr (TREE) lim_min = lim_max < 0 ? -1 : min(lim_min, base - 1);
         row_min = __builtin_amdgcn_readfirstlane(row_min);
         row_max = __builtin_amdgcn_readfirstlane(row_max);
         // a use of the query fragments in front of the loop: their first use inside it would make the compiler wait there, on every
@@ -479,12 +479,24 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
             wait_lgkmcnt<0>();  // the reads of this slot are complete before a later copy refills it
         }
 
+        if constexpr (TREE) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+                if (lim[nb] < 0) {
+                    m_run[nb] = -INFINITY;
+                    l_run[nb] = 0.f;
+#pragma unroll
+                    for (int db = 0; db < 8; ++db) o[nb][db] = float4v{0.f, 0.f, 0.f, 0.f};
+                }
+        }
         if (a.apart && more && !begun) begin_next(slot);   // (a wave without a tile of this part)
         // ---- the waves' results meet in LDS, behind the stages where there is room (a.apart: the next part's first tiles are on their way into
         // those), otherwise in them: per wave O~ [ncols][128] floats, then m [32], l [32] ----
         __syncthreads();
         MI355_LDS float* cmb = (MI355_LDS float*)(smem_raw + (a.apart ? LDS_BYTES : 0));
-        const int wave_floats = ncols * D + 64;
+        // (a tree's: of two blocks of columns with a stride of 132 floats, so that no two of 16 lanes write to one bank)
+        constexpr int CSTRIDE = TREE && NB == 2 ? D + 4 : D;
+        const int wave_floats = ncols * CSTRIDE + 64;
         {
             MI355_LDS float* mine = cmb + wave * wave_floats;
 #pragma unroll
@@ -493,10 +505,10 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
                 const float l_tot = quad_sum(l_run[nb]);
                 if (col < ncols) {
 #pragma unroll
-                    for (int db = 0; db < 8; ++db) *(MI355_LDS float4v*)(mine + col * D + db * 16 + 4 * g) = o[nb][db];
+                    for (int db = 0; db < 8; ++db) *(MI355_LDS float4v*)(mine + col * CSTRIDE + db * 16 + 4 * g) = o[nb][db];
                     if (g == 0) {
-                        mine[ncols * D + col] = m_run[nb];
-                        mine[ncols * D + 32 + col] = l_tot;
+                        mine[ncols * CSTRIDE + col] = m_run[nb];
+                        mine[ncols * CSTRIDE + 32 + col] = l_tot;
                     }
                 }
             }
@@ -510,9 +522,9 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
             float4v ow[WAVES];
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
-                mw[w] = cmb[w * wave_floats + ncols * D + c];
-                lw[w] = cmb[w * wave_floats + ncols * D + 32 + c];
-                ow[w] = *(MI355_LDS const float4v*)(cmb + w * wave_floats + 4 * e4);
+                mw[w] = cmb[w * wave_floats + ncols * CSTRIDE + c];
+                lw[w] = cmb[w * wave_floats + ncols * CSTRIDE + 32 + c];
+                ow[w] = *(MI355_LDS const float4v*)(cmb + w * wave_floats + c * CSTRIDE + d);
             }
             float m = -INFINITY, l = 0.f;
             float4v acc = float4v{0.f, 0.f, 0.f, 0.f};
@@ -764,7 +776,7 @@ bool fmha_paged_keeps_scores(const mi355_paged_kv& c, int Hq, int Sq) { return H
 
 size_t fmha_paged_workspace(const mi355_paged_kv& c, int Hq, int Sq, bool lse, bool tree) {
     const PagedPlan p = paged_plan(c.B, c.Hkv, c.max_pages * c.page_size, Hq, Sq, c.weights != nullptr, lse, tree);
-    size_t first = fmha_paged_many_rows(c, Hq, Sq) ? paged_rows_workspace(c, Hq, Sq) : p.part_bytes + p.score_bytes;
+    size_t first = fmha_paged_many_rows(c, Hq, Sq) ? paged_rows_workspace(c, Hq, Sq, tree) : p.part_bytes + p.score_bytes;
     if (c.weights != nullptr && !p.scores) first = std::max(first, key_weights_workspace(c, Hq, Sq, 0));   // (one behind the other)
     return first + p.lse_bytes;
 }

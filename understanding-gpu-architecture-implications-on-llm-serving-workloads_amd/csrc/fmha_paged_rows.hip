@@ -38,6 +38,7 @@ constexpr int PART_FLOATS = NB * 8 * 64 * 4 + 2 * WCOLS;   // of a wave: its acc
 constexpr int kWorkgroups = 256;              // one per CU
 constexpr int kMinKeys = 256;                 // of a piece
 constexpr int kHeadKeys = 512;                // what a part costs beside its keys, in keys (~9 us: its first tiles' way, its accumulators' way out)
+constexpr int kPieceKeys = 512, kJoinKeys = 256;   // what a piece of a tree's triple costs beside its keys, and what cutting does, in keys (Pieces)
 constexpr int kDirectLen = 512;               // up to this many keys, and from that many triples on, none is cut (plan_of)
 constexpr long kDirectTriples = 1024;
 constexpr long kWholeColumns = 256 * 256;     // from this many columns of all pairs on a workgroup is one of 256 (plan_of)
@@ -73,6 +74,8 @@ struct RowsAttn {
     float scale_log2;
     int direct;      // a workgroup a triple
     int joins, few;  // triples or borders, which of them
+    int blocks;      // of columns
+    int* cuts;       // (a tree's) how many triples are cut, and a CutTriple of each
     Divisor by_group, by_batch, by_hkv;
 };
 
@@ -92,6 +95,9 @@ struct Entries {
     struct Seen {
         int len, n_new, keys;
     };
+    struct Where {
+        int e, len, n_new, keys, tiles, units, before;   // before: units of the entries in front, per kv head
+    };
     __device__ __forceinline__ Seen keys_of(int e) const {
         const int block = divide(e, a.by_batch), b = e - block * kv.B;
         const int len = paged_len(kv, b), n_new = paged_new(kv, b, a.Sq);
@@ -106,6 +112,12 @@ struct Entries {
         n_new = seen.n_new;
         keys = e0 + lane < a.entries ? seen.keys : 0;
         incl = wave_inclusive_sum(units_of(keys));
+    }
+    // block `block` of a sequence
+    __device__ __forceinline__ Where block_of(int block, int b, int len, int n_new) const {
+        const int row0 = divide(block * COLS, a.by_group), row1 = min(divide(min(block * COLS + COLS, a.ncols) - 1, a.by_group), n_new - 1);
+        const int keys = row0 >= n_new ? 0 : max(min(len, len - n_new + row1 + 1), 0);
+        return {block * kv.B + b, len, n_new, keys, tiles_of(keys), units_of(keys), 0};
     }
     // units (tiles and heads) of all, and the most of a triple
     struct Sum {
@@ -129,9 +141,6 @@ struct Entries {
         const int rounds = (int)((uint32_t)(a.entries * kv.Hkv + a.workgroups - 1) / (uint32_t)a.workgroups);
         return 4L * rounds * s.most <= 5L * (s.total / a.workgroups);
     }
-    struct Where {
-        int e, len, n_new, keys, tiles, units, before;   // before: units of the entries in front, per kv head
-    };
     __device__ __forceinline__ Where pick(int i, int before) const {
         const int n = __builtin_amdgcn_readlane(keys, i), u = units_of(n);
         return {first + i, __builtin_amdgcn_readlane(len, i), __builtin_amdgcn_readlane(n_new, i), n, tiles_of(n), u, before + __builtin_amdgcn_readlane(incl, i) - u};
@@ -156,6 +165,96 @@ struct Entries {
         }
     }
 };
+
+// How the triples of a tree's call of up to 64 sequences are cut: into `pieces` of equal length where they are longer than a piece may be, and dealt out largest
+// first, in rounds that run forwards and backwards in turn. Every wave of every workgroup works the same out from the lengths: lane r has the sequence whose pieces are the r-th
+// longest, and the sums up to it. The longest piece is one of the longest sequence's 1 / 1 .. 1 / 64 that is no shorter than an equal share (so that at most two pieces a
+// workgroup are parts of a triple): the one whose heaviest workgroup is expected to have the least to do. Equal shares of the axis, of which most workgroups have two parts, / this, us, 32/8
+// heads: 32 tokens, 8 sequences of up to 8191 keys 51 / 46, 16 of up to 4097 55 / 54, 32 of up to 2000 59 / 52, 24 of 2000 67 / 50; 64 tokens, 16 of up to 4097 87 / 72, 20 of up to 1000
+// 53 / 37; 64/8 heads, 64 tokens, 16 of up to 4097 125 / 116. More sequences get a workgroup a triple.
+template <int COLS>
+struct Pieces {
+    static constexpr int TK = COLS / 4, HEAD = kPieceKeys / TK, JOIN = kJoinKeys / TK, kLeast = 128 / TK;   // in tiles; kLeast: of a piece
+    int b, len, n_new, tiles, pieces, length;   // of this lane's sequence; tiles of a piece
+    int items, parts, cut;                      // pieces, pieces of triples that are cut, such triples, up to this lane's
+    int all, all_cut;
+    __device__ __forceinline__ Pieces() {}
+    __device__ __forceinline__ void store(int (*to)[64]) const {
+        const int lane = threadIdx.x & 63, all_of[9] = {b, len, n_new, tiles, pieces, length, items, parts, cut};
+#pragma unroll
+        for (int i = 0; i < 9; ++i) to[i][lane] = all_of[i];
+    }
+    __device__ __forceinline__ void load(const int (*from)[64]) {
+        const int lane = threadIdx.x & 63;
+        int* const all_of[9] = {&b, &len, &n_new, &tiles, &pieces, &length, &items, &parts, &cut};
+#pragma unroll
+        for (int i = 0; i < 9; ++i) *all_of[i] = from[i][lane];
+    }
+    __device__ __forceinline__ Pieces(const PagedKv& kv, const RowsAttn& a) {
+        const int lane = threadIdx.x & 63, each = a.blocks * kv.Hkv;   // triples of a sequence
+        int my_len = 0, my_new = 0;
+        if (lane < kv.B) my_len = paged_len(kv, lane), my_new = paged_new(kv, lane, a.Sq);
+        const int my_tiles = my_new > 0 ? (my_len + TK - 1) / TK : 0;
+        const int most = max(wave_max(my_tiles), 1), total = __builtin_amdgcn_readlane(wave_inclusive_sum(my_tiles), 63) * each;
+        const int share = (int)((uint32_t)(total + a.workgroups - 1) / (uint32_t)a.workgroups);
+        int longest = max(max((int)ceilf((float)most / (float)(lane + 1)), share), kLeast);
+        const float per = 1.f / (float)longest;
+        float n = 0.f, small = 0.f;   // pieces, those of less than half the length
+        for (int s = 0; s < kv.B; ++s) {
+            const float share_of = (float)__builtin_amdgcn_readlane(my_tiles, s) * per;
+            n += ceilf(share_of);
+            small += share_of < .5f ? 1.f : 0.f;
+        }
+        n *= (float)each;
+        small *= (float)each;
+        // tiles that the heaviest workgroup counts
+        const float load = ((float)total + (float)HEAD * n) / (float)a.workgroups * 1.1f;
+        float cost = (float)min(longest, most) + (float)HEAD + (longest < most ? (float)JOIN : 0.f);
+        if (n > (float)a.workgroups) {   // (in rounds: the smallest pieces come last)
+            const float rounds = n - (float)a.workgroups <= small ? (float)min(longest, most) + 2.f * (float)HEAD
+                                                                  : ceilf(n / (float)a.workgroups) * (.9f * (float)total / n + (float)HEAD);
+            cost = fmaxf(cost, fmaxf(load, rounds) + (longest < most ? (float)JOIN : 0.f));
+        }
+        const int best = -wave_max(-(int)fminf(cost * 64.f, 1e9f));
+        const int choice = __builtin_ctzll(__builtin_amdgcn_ballot_w64((int)fminf(cost * 64.f, 1e9f) == best));
+        longest = __builtin_amdgcn_readlane(longest, choice);
+        const int my_pieces = max((int)((uint32_t)(my_tiles + longest - 1) / (uint32_t)longest), 1);
+        const int my_length = (int)((uint32_t)(my_tiles + my_pieces - 1) / (uint32_t)my_pieces);
+        int longer = 0;
+        for (int s = 0; s < kv.B; ++s) {
+            const int x = __builtin_amdgcn_readlane(my_length, s);
+            longer += x > my_length || (x == my_length && s < lane);
+        }
+        const int to = lane < kv.B ? longer * 4 : lane * 4;
+        b = __builtin_amdgcn_ds_permute(to, lane);
+        len = __builtin_amdgcn_ds_permute(to, my_len);
+        n_new = __builtin_amdgcn_ds_permute(to, my_new);
+        tiles = __builtin_amdgcn_ds_permute(to, my_tiles);
+        pieces = __builtin_amdgcn_ds_permute(to, my_pieces);
+        length = __builtin_amdgcn_ds_permute(to, my_length);
+        const bool there = tiles > 0;
+        items = wave_inclusive_sum(there ? pieces * each : 0);
+        parts = wave_inclusive_sum(there && pieces > 1 ? pieces * each : 0);
+        cut = wave_inclusive_sum(there && pieces > 1 ? each : 0);
+        all = __builtin_amdgcn_readlane(items, 63);
+        all_cut = __builtin_amdgcn_readlane(cut, 63);
+    }
+    struct Piece {
+        int b, triple, len, n_new, piece, pieces, length, part0, cut;   // triple: (block, kv head) of its sequence; part0: its first part; cut: which of those that are cut
+    };
+    // item u < all
+    __device__ __forceinline__ Piece item(int u, int each) const {
+        const int r = __builtin_ctzll(__builtin_amdgcn_ballot_w64(u < items)), p = __builtin_amdgcn_readlane(pieces, r);
+        const int i = u - __builtin_amdgcn_readlane(items, r) + p * each, triple = __builtin_amdgcn_readfirstlane((int)((uint32_t)i / (uint32_t)p));
+        return {__builtin_amdgcn_readlane(b, r), triple, __builtin_amdgcn_readlane(len, r), __builtin_amdgcn_readlane(n_new, r), i - triple * p, p, __builtin_amdgcn_readlane(length, r),
+                __builtin_amdgcn_readlane(parts, r) - p * each + triple * p, __builtin_amdgcn_readlane(cut, r) - each + triple};
+    }
+};
+// What the second kernel needs of a triple that was cut
+struct CutTriple {
+    int b, triple, pieces, part0;
+};
+constexpr int kCutBytes = 16 * (kWorkgroups + 1);   // how many there are, and which, in front of the parts
 
 }  // namespace prow
 
@@ -186,6 +285,33 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
     typename Entries<COLS>::Where seq;
     int hkv, at = 0, f = 0, f_end = 0;   // (whole triples: f counts them down, the blocks with the most keys first, f_end is the step)
     bool whole = a.direct;
+    // (TREE) tile `at` and the n_piece - 1 behind it, the piece's number among the parts
+    int n_piece = 0, part_number = 0, round = 0, all_pieces = 0;
+    __shared__ int held[TREE ? 9 : 1][64];   // `Pieces`, from one piece to the next
+    const auto take_piece = [&]() {          // this workgroup's next; false: none is left
+        if constexpr (TREE) {
+            const int each = a.blocks * kv.Hkv;
+            for (;;) {
+                const int u = round * a.workgroups + (round & 1 ? a.workgroups - 1 - (int)blockIdx.x : (int)blockIdx.x);
+                if (u >= all_pieces) return false;
+                Pieces<COLS> p;
+                p.load(held);
+                const auto x = p.item(u, each);
+                ++round;
+                const int block = divide(x.triple, a.by_hkv);
+                seq = entries.block_of(block, x.b, x.len, x.n_new);
+                if (x.pieces > 1 && x.piece == 0 && tid == 0) ((CutTriple*)a.cuts)[1 + x.cut] = {x.b, x.triple, x.pieces, x.part0};
+                if (seq.keys == 0) continue;   // (zeros: the second kernel's)
+                hkv = x.triple - block * kv.Hkv;
+                at = x.piece * x.length;
+                n_piece = max(min(x.length, seq.tiles - at), 0);
+                whole = x.pieces == 1;
+                part_number = x.part0 + x.piece;
+                return true;
+            }
+        }
+        return false;
+    };
     const auto take = [&]() {
         const int e = divide(f, a.by_hkv);
         hkv = f - e * kv.Hkv;
@@ -196,24 +322,40 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
             seq = entries.at(e);
         }
     };
-    if (!whole) {
-        const auto sum = entries.sum();
-        whole = entries.in_turn(sum);
-        const int quota = entries.quota(sum);
-        f = blockIdx.x * quota;
-        f_end = min(f + quota, sum.total);
-    }
-    if (whole) {
-        f = a.entries * kv.Hkv - 1 - blockIdx.x;
-        f_end = a.workgroups;
-        if (f < 0) return;
-        take();
+    if constexpr (TREE) {
+        if (whole) {   // a workgroup a triple, the blocks with the most keys first
+            const int i = a.entries * kv.Hkv - 1 - blockIdx.x, e = divide(i, a.by_hkv), block = divide(e, a.by_batch), b = e - block * kv.B;
+            hkv = i - e * kv.Hkv;
+            seq = entries.block_of(block, b, __builtin_amdgcn_readfirstlane(paged_len(kv, b)), __builtin_amdgcn_readfirstlane(paged_new(kv, b, a.Sq)));
+            n_piece = seq.tiles;
+        } else {
+            const Pieces<COLS> p(kv, a);
+            all_pieces = p.all;
+            if (blockIdx.x == 0 && tid == 0) *a.cuts = p.all_cut;
+            if (wave == 0) p.store(held);
+            __syncthreads();
+            if (!take_piece()) return;
+        }
     } else {
-        if (f >= f_end) return;
-        seq = entries.find(f);
-        if (seq.units == 0) return;   // (where lengths change under the call)
-        hkv = (int)((uint32_t)(f - seq.before * kv.Hkv) / (uint32_t)seq.units);
-        at = f - seq.before * kv.Hkv - hkv * seq.units;
+        if (!whole) {
+            const auto sum = entries.sum();
+            whole = entries.in_turn(sum);
+            const int quota = entries.quota(sum);
+            f = blockIdx.x * quota;
+            f_end = min(f + quota, sum.total);
+        }
+        if (whole) {
+            f = a.entries * kv.Hkv - 1 - blockIdx.x;
+            f_end = a.workgroups;
+            if (f < 0) return;
+            take();
+        } else {
+            if (f >= f_end) return;
+            seq = entries.find(f);
+            if (seq.units == 0) return;   // (where lengths change under the call)
+            hkv = (int)((uint32_t)(f - seq.before * kv.Hkv) / (uint32_t)seq.units);
+            at = f - seq.before * kv.Hkv - hkv * seq.units;
+        }
     }
 
     uint32_t k_lane[2], v_lane[2];   // of this wave's copies of a tile: rows 8 (cw & 1) + 4 c + lane / 16 of a 16-key block
@@ -232,9 +374,9 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
 
     for (;;) {
         const int block = divide(seq.e, a.by_batch), b = seq.e - block * kv.B;
-        const int units = whole ? seq.units : min(seq.units - at, f_end - f);
-        const int tile0 = max(at - Entries<COLS>::HEAD, 0), n = at + units - Entries<COLS>::HEAD - tile0;   // (units of the head alone: nothing)
-        if (n <= 0 && seq.units > 0) return;
+        const int units = TREE ? 0 : whole ? seq.units : min(seq.units - at, f_end - f);
+        const int tile0 = TREE ? at : max(at - Entries<COLS>::HEAD, 0), n = TREE ? n_piece : at + units - Entries<COLS>::HEAD - tile0;   // (units of the head alone: nothing)
+        if (!TREE && n <= 0 && seq.units > 0) return;
         const int n_loc = max((n - kg + KG - 1) / KG, 0);   // tiles kg, kg + KG, .. of the part
         const int keys = seq.keys;                          // those that some row of the block sees
         const int* table = kv.table + (long)b * kv.table_stride;
@@ -300,7 +442,7 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
             const T* qp = Q + b * a.q_batch + (long)(hkv * a.group + head) * a.q_head + qi * a.q_row + 8 * g;
             qrow[nb] = qi;
             lim[nb] = qi < n_new ? min(len - 1, qi + len - n_new) : -1;
-            lim_min = min(lim_min, lim[nb]);
+            if (!TREE || lim[nb] >= 0) lim_min = min(lim_min, lim[nb]);   // (TREE: what the columns of rows that are no tokens see is taken out at the end)
             lim_max = max(lim_max, lim[nb]);
             row_min = min(row_min, qi);
             row_max = max(row_max, qi);
@@ -326,7 +468,7 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
         __shared__ int up[TREE ? kMostDrafted : 1];
         __shared__ uint32_t words[TREE ? kMostDrafted * kTreeWords : 1];
         if constexpr (TREE) {
-            lim_min = min(lim_min, base - 1);
+            lim_min = lim_max < 0 ? -1 : min(lim_min, base - 1);
             if ((tile0 + n) * TK > base) {   // the words of the block's rows, where the part reaches the draft
                 const int* parents = a.tree.parents + b * a.tree.batch;
                 for (int i = tid; i < a.Sq; i += NTHREADS) up[i] = parents[i];
@@ -562,6 +704,16 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
         float l_tot[NB];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) l_tot[nb] = quad_sum(l_run[nb]);
+        if constexpr (TREE) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+                if (lim[nb] < 0) {
+                    m_run[nb] = -INFINITY;
+                    l_tot[nb] = 0.f;
+#pragma unroll
+                    for (int db = 0; db < 8; ++db) o[nb][db] = float4v{0.f, 0.f, 0.f, 0.f};
+                }
+        }
         __syncthreads();   // the stages are free
         if constexpr (KG == 2) {   // the halves meet
             MI355_LDS float* theirs = (MI355_LDS float*)smem_raw + cw * PART_FLOATS;
@@ -592,7 +744,7 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
             __syncthreads();
         }
         if (kg == 0) {
-            if (n == seq.tiles || whole) {
+            if (whole || (!TREE && n == seq.tiles)) {
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
                     const int col = col0 + 16 * nb + c16;
@@ -612,7 +764,7 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
                             l_tot[nb] != 0.f ? (m_run[nb] * a.scale_log2 + __builtin_log2f(l_tot[nb])) * 0.69314718055994531f : -INFINITY;
                 }
             } else {
-                float* part = a.part + ((long)(2 * blockIdx.x + (parts > 0)) * CW + cw) * PART_FLOATS;
+                float* part = a.part + ((long)(TREE ? part_number : 2 * blockIdx.x + (parts > 0)) * CW + cw) * PART_FLOATS;
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
@@ -620,6 +772,10 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
                     if (g == 0) part[NB * 8 * 256 + nb * 16 + c16] = m_run[nb], part[NB * 8 * 256 + WCOLS + nb * 16 + c16] = l_tot[nb];
                 }
             }
+        }
+        if constexpr (TREE) {
+            if (a.direct || !take_piece()) return;
+            continue;
         }
         if (whole) {
             f -= f_end;
@@ -642,8 +798,8 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
 // 2^((m_p - max m) c), a thread 4 d of a column: with few triples of many parts (a.few) four for each (triple, wave of columns), with many triples, of which only
 // those between two workgroups' pieces are cut, one for each (border, wave of columns), of which that of a triple's first border does it (32 x 32 triples of
 // 256 columns in 256 pieces: one workgroup or more a triple 74 us, a border 14). Then one per entry writes zeros where no key is seen.
-template <typename T, int KG>
-__global__ __launch_bounds__(256) void paged_rows_join_kernel(PagedKv kv, RowsAttn a) {
+template <typename T, int KG, bool TREE>
+__global__ __launch_bounds__(256, TREE ? 4 : 1) void paged_rows_join_kernel(PagedKv kv, RowsAttn a) {
     using namespace prow;
     using V4 = typename Elem<T>::v4;
     constexpr int CW = WAVES / KG, COLS = CW * WCOLS;
@@ -668,37 +824,50 @@ __global__ __launch_bounds__(256) void paged_rows_join_kernel(PagedKv kv, RowsAt
         return;
     }
     const int join = blockIdx.x / CW, cw = blockIdx.x % CW;
-    const auto sum = entries.sum();
-    if (entries.in_turn(sum)) return;
-    const int total = sum.total, quota = entries.quota(sum);
-    typename Entries<COLS>::Where seq;
-    int hkv;
-    if (a.few) {   // a triple
-        const int e = divide(join, a.by_hkv);
-        hkv = join - e * kv.Hkv;
-        seq = entries.at(e);
-        if (seq.units == 0) return;
-    } else {       // a border
-        if (join == 0 || join * quota >= total) return;
-        seq = entries.find(join * quota);
-        if (seq.units == 0) return;
-        hkv = (int)((uint32_t)(join * quota - seq.before * kv.Hkv) / (uint32_t)seq.units);
+    int n, hkv, b, col0;
+    const float *part0, *part1;   // its first part, and the one that stands in front of the others' places
+    long stride = 2 * CW * PART_FLOATS;
+    if constexpr (TREE) {
+        if (join >= *a.cuts) return;
+        const CutTriple cut = ((const CutTriple*)a.cuts)[1 + join];
+        const int block = divide(cut.triple, a.by_hkv);
+        n = cut.pieces, b = cut.b, hkv = cut.triple - block * kv.Hkv, col0 = block * COLS + cw * WCOLS;
+        if (col0 >= a.ncols || entries.keys_of(block * kv.B + b).keys == 0) return;
+        stride = CW * PART_FLOATS;
+        part0 = part1 = a.part + ((long)cut.part0 * CW + cw) * PART_FLOATS;
+    } else {
+        const auto sum = entries.sum();
+        if (entries.in_turn(sum)) return;
+        const int total = sum.total, quota = entries.quota(sum);
+        typename Entries<COLS>::Where seq;
+        if (a.few) {   // a triple
+            const int e = divide(join, a.by_hkv);
+            hkv = join - e * kv.Hkv;
+            seq = entries.at(e);
+            if (seq.units == 0) return;
+        } else {       // a border
+            if (join == 0 || join * quota >= total) return;
+            seq = entries.find(join * quota);
+            if (seq.units == 0) return;
+            hkv = (int)((uint32_t)(join * quota - seq.before * kv.Hkv) / (uint32_t)seq.units);
+        }
+        const int f0 = seq.before * kv.Hkv + hkv * seq.units, first = (int)((uint32_t)(f0 + Entries<COLS>::HEAD) / (uint32_t)quota);
+        n = (int)((uint32_t)(f0 + seq.units - 1) / (uint32_t)quota) - first + 1;   // (workgroups that have tiles of it)
+        if (n == 1 || (!a.few && first != join - 1)) return;
+        const int block = divide(seq.e, a.by_batch);
+        b = seq.e - block * kv.B, col0 = block * COLS + cw * WCOLS;
+        if (col0 >= a.ncols) return;
+        // its part is the last of the first workgroup (unless that begins inside it) and the first of the others
+        part0 = a.part + ((long)(2 * first + (first * quota < f0)) * CW + cw) * PART_FLOATS;
+        part1 = a.part + ((long)(2 * first) * CW + cw) * PART_FLOATS;
     }
-    const int f0 = seq.before * kv.Hkv + hkv * seq.units, first = (int)((uint32_t)(f0 + Entries<COLS>::HEAD) / (uint32_t)quota);
-    const int n = (int)((uint32_t)(f0 + seq.units - 1) / (uint32_t)quota) - first + 1;   // (workgroups that have tiles of it)
-    if (n == 1 || (!a.few && first != join - 1)) return;
-    const int block = divide(seq.e, a.by_batch), b = seq.e - block * kv.B, col0 = block * COLS + cw * WCOLS;
-    if (col0 >= a.ncols) return;
-    // its part is the last of the first workgroup (unless that begins inside it) and the first of the others
-    const float* part0 = a.part + ((long)(2 * first + (first * quota < f0)) * CW + cw) * PART_FLOATS;
-    const float* part1 = a.part + ((long)(2 * first) * CW + cw) * PART_FLOATS;
-    const auto part_of = [&](int p) { return p == 0 ? part0 : part1 + (long)p * (2 * CW * PART_FLOATS); };
+    const auto part_of = [&](int p) { return p == 0 ? part0 : part1 + (long)p * stride; };
     const auto weight = [&](float x, float ref) { return x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((x - ref) * a.scale_log2); };
     for (int quarter = blockIdx.y; quarter < 4; quarter += gridDim.y) {
         const int nb = quarter >> 1, db = (quarter & 1) * 4 + (threadIdx.x >> 6);
         float m = -INFINITY, l = 0.f;
         float4v acc = float4v{0.f, 0.f, 0.f, 0.f};
-        constexpr int ROUND = 8;   // parts in flight
+        constexpr int ROUND = TREE ? 4 : 8;   // parts in flight
         for (int p0 = 0; p0 < n; p0 += ROUND) {
             float4v v[ROUND];
             float mp[ROUND], lp[ROUND];
@@ -739,7 +908,7 @@ struct Plan {
     long units;    // of all triples, at most
     size_t bytes;
 };
-static Plan plan_of(const mi355_paged_kv& c, int Hq, int Sq) {
+static Plan plan_of(const mi355_paged_kv& c, int Hq, int Sq, bool tree) {
     Plan p;
     const int ncols = Hq / c.Hkv * Sq, max_len = c.max_pages * c.page_size;
     const long pairs = (long)c.B * c.Hkv;
@@ -752,16 +921,19 @@ static Plan plan_of(const mi355_paged_kv& c, int Hq, int Sq) {
     // us, a workgroup a triple / cut: 500 rows over 500 keys 18 / 73, 8 x 1024 rows over 2048 247 / 288, one sequence (whose triples are of nearly one
     // length) of 2048 rows over 8191 300 / 320, of 1000 rows over 2000 42.7 / 58.5
     const long triples = pairs * p.blocks, rounds = (triples + kWorkgroups - 1) / kWorkgroups;
-    p.direct = max_len <= kDirectLen || triples >= kDirectTriples || (c.B == 1 && 10 * triples >= 9 * rounds * kWorkgroups);
+    p.direct = max_len <= kDirectLen || triples >= kDirectTriples || (c.B == 1 && 10 * triples >= 9 * rounds * kWorkgroups) || (tree && c.B > 64);   // (Pieces)
     p.workgroups = p.direct ? (int)triples : (int)std::min<long>(kWorkgroups, p.units / (kMinKeys / tk) + 1);
     p.bytes = p.direct ? 0 : sizeof(float) * 2 * (size_t)p.workgroups * (WAVES / p.kg) * PART_FLOATS;
     return p;
 }
 }  // namespace prow
 
-bool paged_rows_fits(const mi355_paged_kv& c, int Hq, int Sq) { return prow::plan_of(c, Hq, Sq).units <= INT32_MAX - 65536; }
+bool paged_rows_fits(const mi355_paged_kv& c, int Hq, int Sq) { return prow::plan_of(c, Hq, Sq, false).units <= INT32_MAX - 65536; }
 
-size_t paged_rows_workspace(const mi355_paged_kv& c, int Hq, int Sq) { return prow::plan_of(c, Hq, Sq).bytes; }
+size_t paged_rows_workspace(const mi355_paged_kv& c, int Hq, int Sq, bool tree) {
+    const size_t bytes = prow::plan_of(c, Hq, Sq, tree).bytes;
+    return bytes + (bytes > 0 && tree ? prow::kCutBytes : 0);
+}
 
 template <typename T, int KG, bool TREE>
 static hipError_t launch_rows(const PagedKv& kv, const RowsAttn& a, hipStream_t stream) {
@@ -772,14 +944,14 @@ static hipError_t launch_rows(const PagedKv& kv, const RowsAttn& a, hipStream_t 
     paged_rows_kernel<T, KG, TREE><<<dim3(a.workgroups), dim3(NTHREADS), LDS_BYTES, stream>>>(kv, a);
     e = hipGetLastError();
     if (e != hipSuccess || a.direct) return e;
-    paged_rows_join_kernel<T, KG><<<dim3((unsigned)(a.joins * (WAVES / KG) + a.entries), a.few ? 4 : 1), dim3(256), 0, stream>>>(kv, a);
+    paged_rows_join_kernel<T, KG, TREE><<<dim3((unsigned)(a.joins * (WAVES / KG) + a.entries), a.few ? 4 : 1), dim3(256), 0, stream>>>(kv, a);
     return hipGetLastError();
 }
 
 hipError_t paged_rows_dispatch(const mi355_paged_kv& c, const void* Q, void* O, float* LSE, int Hq, int Sq, const long* strides, float scale,
                                const int* parents, long parents_batch, void* workspace, hipStream_t stream) {
     const PagedKv kv = paged_from(c);
-    const prow::Plan p = prow::plan_of(c, Hq, Sq);
+    const prow::Plan p = prow::plan_of(c, Hq, Sq, parents != nullptr);
     RowsAttn a = {};
     a.Q = Q;
     a.O = O;
@@ -794,8 +966,13 @@ hipError_t paged_rows_dispatch(const mi355_paged_kv& c, const void* Q, void* O, 
     a.entries = p.blocks * kv.B;
     a.workgroups = p.workgroups;
     a.direct = p.direct;
+    a.blocks = p.blocks;
+    if (parents != nullptr && !a.direct) {
+        a.cuts = (int*)workspace;
+        a.part = (float*)((char*)workspace + prow::kCutBytes);
+    }
     a.few = (long)a.entries * kv.Hkv <= a.workgroups / 2;
-    a.joins = a.few ? a.entries * kv.Hkv : a.workgroups;
+    a.joins = a.few || parents != nullptr ? std::min(a.entries * kv.Hkv, a.workgroups) : a.workgroups;
     a.tree = {parents, parents_batch};
     a.scale_log2 = scale * 1.4426950408889634f;
     a.by_group = divisor_of(a.group);

@@ -192,7 +192,7 @@ hipError_t fmha_paged_dispatch(const mi355_paged_kv& cache, const void* Q, void*
 // whether the kernel for many query columns a kv head takes a call (fmha_paged_rows.hip), and whether its tiles can be counted in an int
 bool fmha_paged_many_rows(const mi355_paged_kv& cache, int Hq, int Sq);
 bool paged_rows_fits(const mi355_paged_kv& cache, int Hq, int Sq);
-size_t paged_rows_workspace(const mi355_paged_kv& cache, int Hq, int Sq);
+size_t paged_rows_workspace(const mi355_paged_kv& cache, int Hq, int Sq, bool tree);
 hipError_t paged_rows_dispatch(const mi355_paged_kv& cache, const void* Q, void* O, float* LSE, int Hq, int Sq, const long* strides, float scale,
                                const int* parents, long parents_batch, void* workspace, hipStream_t stream);
 long key_weights_workgroups(const mi355_paged_kv& cache, int Hq, int Sq, int last_rows);
