@@ -258,6 +258,10 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
         return any;
     };
 
+    // (TREE) a parent a thread, requested in front of what the first tile waits for
+    static_assert(NTHREADS >= kMostDrafted, "");
+    const auto parent = [&](int b) { return TREE && tid < a.Sq ? a.tree.parents[b * a.tree.batch + tid] : 0; };
+    int up_mine = parent(now.seq.b);
     if (count_of(now) > 0) issue_tile(0, 0);
     int slot = 0;   // stage of the next tile
     for (;;) {      // the parts
@@ -296,6 +300,24 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
             for (int ks = 0; ks < 4; ++ks) qf[nb][ks] = *(const V8*)(qp + ks * 32);
         }
         const int base = len - n_new;       // (TREE) key of the first drafted token
+        // the words of this workgroup's columns, where the part reaches the draft (the barriers wait for LDS alone: copies are on their way)
+        __shared__ int up[TREE ? kMostDrafted : 1];
+        __shared__ uint32_t words[TREE ? 32 * kTreeWords : 1];
+        if constexpr (TREE) {
+            const auto barrier = []() {
+                wait_lgkmcnt<0>();
+                asm volatile("s_barrier" ::: "memory");
+            };
+            if ((now.tile0 + n) * TK > base) {
+                if (tid < a.Sq) up[tid] = up_mine;
+                barrier();
+                if (tid < ncols) {
+                    const int col = col0 + tid;
+                    tree_words((MI355_LDS const int*)up, col - divide(col, a.by_sq) * a.Sq, n_new, base, (MI355_LDS uint32_t*)words + tid * kTreeWords);
+                }
+                barrier();
+            }
+        }
         int row_min = a.Sq, row_max = -1;   // rows of the columns of this wave
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) row_min = min(row_min, qrow[nb]), row_max = max(row_max, qrow[nb]);
@@ -316,21 +338,6 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) asm volatile("" : "+v"(qf[nb][0]), "+v"(qf[nb][1]), "+v"(qf[nb][2]), "+v"(qf[nb][3]));
 
-        // the words of this workgroup's columns, where the part reaches the draft
-        __shared__ int up[TREE ? kMostDrafted : 1];
-        __shared__ uint32_t words[TREE ? 32 * kTreeWords : 1];
-        if constexpr (TREE) {
-            if ((now.tile0 + n) * TK > base) {
-                const int* parents = a.tree.parents + b * a.tree.batch;
-                for (int i = tid; i < a.Sq; i += NTHREADS) up[i] = parents[i];
-                __syncthreads();
-                if (tid < ncols) {
-                    const int col = col0 + tid;
-                    tree_words((MI355_LDS const int*)up, col - divide(col, a.by_sq) * a.Sq, n_new, base, (MI355_LDS uint32_t*)words + tid * kTreeWords);
-                }
-                __syncthreads();
-            }
-        }
         // the word of column c for a tile that reaches the draft
         const auto seen = [&](int tile, int c) { return words[c * kTreeWords + tile - (max(base, 0) >> 5)]; };
 
@@ -561,6 +568,7 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
         }
         f += n;
         now = ahead;
+        up_mine = parent(now.seq.b);
     }
 }
 
@@ -744,7 +752,9 @@ static PagedPlan paged_plan(int B, int Hkv, int max_len, int Hq, int Sq, bool we
     const int ncols = Hq / Hkv * Sq;
     const long pairs = (long)B * Hkv;
     p.nb = ncols > 16 ? 2 : 1;
-    p.col_block = std::min(ncols, 32);
+    // a tree over few keys: a workgroup's chain is shorter with 16 columns than with 32 (us: 26 tokens of 8/2 heads over 300 keys 9.8 / 11.6, 100 of 32/8 over 512 12.0 / 14.1)
+    if (tree && max_len <= kDirectLen && pairs * ((ncols + 15) / 16) <= kWorkgroups) p.nb = 1;
+    p.col_block = std::min(ncols, 16 * p.nb);
     p.blocks = (ncols + p.col_block - 1) / p.col_block;
     p.max_tiles = (max_len + TK - 1) / TK;
     // A workgroup per pair needs no joining, but walks the longest sequence alone. us, so / in equal shares, sequences as long as the table is wide: 8 pairs

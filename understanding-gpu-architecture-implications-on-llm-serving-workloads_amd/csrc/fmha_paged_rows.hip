@@ -429,6 +429,7 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
                 }
             }
         };
+        const int up_mine = TREE && tid < a.Sq ? a.tree.parents[b * a.tree.batch + tid] : 0;   // (a parent a thread)
         // this wave's columns; their loads are under way together with the table's
         const int len = seq.len, n_new = seq.n_new;
         const int col0 = block * COLS + cw * WCOLS;
@@ -451,6 +452,19 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
         }
         for (int i = 0; i < NSTAGE - 1 && i < n_loc; ++i) issue(i);
 
+        const int base = len - n_new;        // (TREE) key of the first drafted token
+        const int row0 = TREE ? divide(block * COLS, a.by_group) : 0;   // first row of the block
+        __shared__ int up[TREE ? kMostDrafted : 1];
+        __shared__ uint32_t words[TREE ? kMostDrafted * kTreeWords : 1];
+        if constexpr (TREE) {
+            if ((tile0 + n) * TK > base) {   // the words of the block's rows, where the part reaches the draft (the barrier waits for LDS alone; another one follows)
+                if (tid < a.Sq) up[tid] = up_mine;
+                wait_lgkmcnt<0>();
+                asm volatile("s_barrier" ::: "memory");
+                const int rows = divide(min(block * COLS + COLS, a.ncols) - 1, a.by_group) - row0 + 1;
+                if (tid < rows) tree_words((MI355_LDS const int*)up, row0 + tid, n_new, base, (MI355_LDS uint32_t*)words + tid * kTreeWords);
+            }
+        }
 #pragma unroll
         for (int off = 8; off >= 1; off >>= 1) {
             lim_min = min(lim_min, __shfl_xor(lim_min, off, 64));
@@ -463,20 +477,7 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
         row_min = __builtin_amdgcn_readfirstlane(row_min);
         row_max = __builtin_amdgcn_readfirstlane(row_max);
         if (col0 >= a.ncols) lim_max = -1;   // (a wave without columns)
-        const int base = len - n_new;        // (TREE) key of the first drafted token
-        const int row0 = TREE ? divide(block * COLS, a.by_group) : 0;   // first row of the block
-        __shared__ int up[TREE ? kMostDrafted : 1];
-        __shared__ uint32_t words[TREE ? kMostDrafted * kTreeWords : 1];
-        if constexpr (TREE) {
-            lim_min = lim_max < 0 ? -1 : min(lim_min, base - 1);
-            if ((tile0 + n) * TK > base) {   // the words of the block's rows, where the part reaches the draft
-                const int* parents = a.tree.parents + b * a.tree.batch;
-                for (int i = tid; i < a.Sq; i += NTHREADS) up[i] = parents[i];
-                __syncthreads();
-                const int rows = divide(min(block * COLS + COLS, a.ncols) - 1, a.by_group) - row0 + 1;
-                if (tid < rows) tree_words((MI355_LDS const int*)up, row0 + tid, n_new, base, (MI355_LDS uint32_t*)words + tid * kTreeWords);
-            }   // (a barrier follows)
-        }
+        if (TREE) lim_min = lim_max < 0 ? -1 : min(lim_min, base - 1);
         // the word of row r for 32 keys from key0 on, which reach the draft
         const auto seen = [&](int key0, int r) { return words[(r - row0) * kTreeWords + (key0 >> 5) - (max(base, 0) >> 5)]; };
         // a use of the query fragments in front of the loop: their first use inside it would make the compiler wait there, on every
