@@ -373,13 +373,13 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
                     for (int nb = 0; nb < NB; ++nb) s[nb][kb] = Elem<T>::mfma16(kf, qf[nb][ks], s[nb][kb]);
                 }
             const bool masked = key0 + TK - 1 > lim_min || no_keys != 0;
+            const uint32_t there = ~((no_keys & 1 ? 0xffffu : 0u) | (no_keys & 2 ? 0xffff0000u : 0u));   // (TREE: a word's)
             if (TREE && key0 + TK > base) {
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
-                    const uint32_t mine = seen(tile, min(16 * nb + c16, ncols - 1)) >> (4 * g);
+                    const uint32_t mine = (seen(tile, min(16 * nb + c16, ncols - 1)) & there) >> (4 * g);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (!((mine >> (16 * (e >> 2) + (e & 3))) & 1) || ((no_keys >> (e >> 2)) & 1)) s[nb][e >> 2][e & 3] = -INFINITY;
+                    for (int e = 0; e < 8; ++e) s[nb][e >> 2][e & 3] = mine & (1u << (16 * (e >> 2) + (e & 3))) ? s[nb][e >> 2][e & 3] : -INFINITY;
                 }
             } else if (masked) {
 #pragma unroll
@@ -435,7 +435,23 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
             // O^T += V^T P^T; the 8 keys of a lane of P are 4 g + 0..3 and 16 + 4 g + 0..3, V^T is gathered in that order
             // A product with p = 0 is not nothing where v is infinite or NaN: a masked tile that holds such values takes the way below.
             bool finite = true;
-            if (masked) {
+            V8 vfs[TREE ? 8 : 1];
+            if constexpr (TREE) {   // (the matrix pipe asks whether there are any: 0 * v is 0 but for those)
+#pragma unroll
+                for (int db = 0; db < 8; ++db) {
+                    MI355_LDS char* vp = st + (v_base ^ (db << 5));
+                    vfs[db] = Elem<T>::frag(concat(lds_read_tr16_b64(vp), lds_read_tr16_b64(vp + 16 * ROW_BYTES)));
+                }
+                if (masked) {
+                    V8 zero;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) zero[e] = (T)0.f;
+                    float4v sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int db = 0; db < 8; ++db) sum = Elem<T>::mfma16(vfs[db], zero, sum);
+                    finite = __builtin_amdgcn_ballot_w64(!(sum[0] == 0.f && sum[1] == 0.f && sum[2] == 0.f && sum[3] == 0.f)) == 0;
+                }
+            } else if (masked) {
                 ushort2v top = {0, 0};
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
@@ -449,8 +465,13 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
             if (finite) {
 #pragma unroll
                 for (int db = 0; db < 8; ++db) {
-                    MI355_LDS char* vp = st + (v_base ^ (db << 5));
-                    V8 vf = Elem<T>::frag(concat(lds_read_tr16_b64(vp), lds_read_tr16_b64(vp + 16 * ROW_BYTES)));
+                    V8 vf;
+                    if constexpr (TREE) {
+                        vf = vfs[db];
+                    } else {
+                        MI355_LDS char* vp = st + (v_base ^ (db << 5));
+                        vf = Elem<T>::frag(concat(lds_read_tr16_b64(vp), lds_read_tr16_b64(vp + 16 * ROW_BYTES)));
+                    }
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) o[nb][db] = Elem<T>::mfma16(vf, pf[nb], o[nb][db]);
                 }
@@ -464,7 +485,7 @@ __global__ __launch_bounds__(pdec::NTHREADS) void fmha_paged_kernel(PagedKv kv, 
                         int c = r - (col0 - divide(col0, a.by_sq) * a.Sq);   // a column of the row
                         if (c < 0) c += a.Sq;
                         if (c >= ncols) continue;
-                        word = seen(tile, c) >> (4 * g);
+                        word = (seen(tile, c) & there) >> (4 * g);
                     }
 #pragma unroll
                     for (int db = 0; db < 8; ++db) {

@@ -639,13 +639,13 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
             if (work) {
                 const uint32_t none = none_of(h);
                 const bool drafted = TREE && key0 + 32 > base;
+                const uint32_t there = ~((none & 1 ? 0xffffu : 0u) | (none & 2 ? 0xffff0000u : 0u));   // (a word's)
                 if (drafted) {
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
-                        const uint32_t mine = seen(key0, qrow[nb]) >> (4 * g);
+                        const uint32_t mine = (seen(key0, qrow[nb]) & there) >> (4 * g);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (!((mine >> (16 * (e >> 2) + (e & 3))) & 1) || ((none >> (e >> 2)) & 1)) s[nb][e >> 2][e & 3] = -INFINITY;
+                        for (int e = 0; e < 8; ++e) s[nb][e >> 2][e & 3] = mine & (1u << (16 * (e >> 2) + (e & 3))) ? s[nb][e >> 2][e & 3] : -INFINITY;
                     }
                 } else {
 #pragma unroll
@@ -658,14 +658,25 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
                 read_v(st);
                 // A product with p = 0 is not nothing where v is infinite or NaN: such values are taken out and go to the rows that see them, one
                 // after the other.
-                ushort2v top = {0, 0};
+                bool finite;
+                if constexpr (TREE) {   // (the matrix pipe asks: 0 * v is 0 but for those)
+                    V8 zero;
 #pragma unroll
-                for (int db = 0; db < 8; ++db) {
-                    const int4v x = __builtin_bit_cast(int4v, vf[db]);
+                    for (int e = 0; e < 8; ++e) zero[e] = (T)0.f;
+                    float4v sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(ushort2v, x[e] & 0x7fff7fff));
+                    for (int db = 0; db < 8; ++db) sum = Elem<T>::mfma16(vf[db], zero, sum);
+                    finite = __builtin_amdgcn_ballot_w64(!(sum[0] == 0.f && sum[1] == 0.f && sum[2] == 0.f && sum[3] == 0.f)) == 0;
+                } else {
+                    ushort2v top = {0, 0};
+#pragma unroll
+                    for (int db = 0; db < 8; ++db) {
+                        const int4v x = __builtin_bit_cast(int4v, vf[db]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(ushort2v, x[e] & 0x7fff7fff));
+                    }
+                    finite = __builtin_amdgcn_ballot_w64(top[0] >= kInfinity || top[1] >= kInfinity) == 0;
                 }
-                const bool finite = __builtin_amdgcn_ballot_w64(top[0] >= kInfinity || top[1] >= kInfinity) == 0;
                 if (!finite) {
 #pragma unroll
                     for (int db = 0; db < 8; ++db)
@@ -677,7 +688,7 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
 #pragma unroll 1
                     for (int r = row_min; r <= row_max; ++r) {
                         const int last = r < n_new ? min(len - 1, r + len - n_new) : -1;
-                        const uint32_t word = drafted ? seen(key0, r) >> (4 * g) : 0;
+                        const uint32_t word = drafted ? (seen(key0, r) & there) >> (4 * g) : 0;
 #pragma unroll
                         for (int db = 0; db < 8; ++db) {
                             V8 vs = v_frag(st, db);
@@ -800,7 +811,7 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
 // those between two workgroups' pieces are cut, one for each (border, wave of columns), of which that of a triple's first border does it (32 x 32 triples of
 // 256 columns in 256 pieces: one workgroup or more a triple 74 us, a border 14). Then one per entry writes zeros where no key is seen.
 template <typename T, int KG, bool TREE>
-__global__ __launch_bounds__(256, TREE ? 4 : 1) void paged_rows_join_kernel(PagedKv kv, RowsAttn a) {
+__global__ __launch_bounds__(256, TREE ? 3 : 1) void paged_rows_join_kernel(PagedKv kv, RowsAttn a) {
     using namespace prow;
     using V4 = typename Elem<T>::v4;
     constexpr int CW = WAVES / KG, COLS = CW * WCOLS;
@@ -868,7 +879,7 @@ __global__ __launch_bounds__(256, TREE ? 4 : 1) void paged_rows_join_kernel(Page
         const int nb = quarter >> 1, db = (quarter & 1) * 4 + (threadIdx.x >> 6);
         float m = -INFINITY, l = 0.f;
         float4v acc = float4v{0.f, 0.f, 0.f, 0.f};
-        constexpr int ROUND = TREE ? 4 : 8;   // parts in flight
+        constexpr int ROUND = 8;   // parts in flight
         for (int p0 = 0; p0 < n; p0 += ROUND) {
             float4v v[ROUND];
             float mp[ROUND], lp[ROUND];
