@@ -395,7 +395,7 @@ int mi355_fmha_paged_tree(const mi355_paged_kv* cache, const void* Q, void* O, f
  * The accepted path of such a tree closes ranks: of the last new_lens[b] keys of sequence b (new_lens is needed here; it may be larger than the sequence, whose
  * first drafted tokens are then no keys), key seq_lens[b] - new_lens[b] + path[b*path_batch + j] moves to key seq_lens[b] - new_lens[b] + j (to key j where
  * that is negative), with its value, and its weight and position where those are given. A path ascends; it ends in front of the first entry that does not,
- * or is no drafted token that is a key. lens_out[b] = the keys in front of the draft and those of the path; seq_lens is not written and may not overlap lens_out.
+ * or is no drafted token that is a key. lens_out[b] = the keys in front of the draft and those of the path; seq_lens and new_lens are not written and may not overlap lens_out.
  * Keys behind the new length are left as they are. A key that moves from or to a page outside the pool does not move. length <= 2^28.
  */
 int mi355_cache_keep_path(const mi355_paged_kv* cache, const int32_t* path, int length, int64_t path_batch, int32_t* lens_out, void* stream);
@@ -418,7 +418,7 @@ int mi355_cache_keep_path(const mi355_paged_kv* cache, const int32_t* path, int 
  *     key) and slot page * page_size + row of the page; rows of sequences that are not taken, and those behind the last sequence, get -1 for both.
  *   - Pages behind a sequence's end (columns from its new length / page_size, rounded up, on) go back to the ring, in the order of (sequence, column), and their entries become
  *     -1. They can be taken by the next call. A sequence is released by seq_lens[b] = 0 and new_lens[b] = 0.
- * No page may be held twice. B <= 65535, rows <= 2^28, max_pages * page_size <= 2^28, n_pages * page_size and B * max_pages < 2^31.
+ * No page may be held twice; next_positions may not overlap seq_lens. B <= 65535, rows <= 2^28, max_pages * page_size <= 2^28, n_pages * page_size and B * max_pages < 2^31.
  */
 size_t mi355_packed_plan_workspace_bytes(int B);
 int mi355_packed_plan(int32_t* block_table, int64_t table_stride, int32_t* seq_lens, const int32_t* new_lens, int32_t* next_positions, int32_t* free_pages,

@@ -46,14 +46,14 @@ def test_a_path_refuses_bad_arguments(lib):
         return cdll.mi355_cache_keep_path(cc, path, length, batch, out, None)
 
     for kw in (dict(path=None), dict(out=None), dict(length=0), dict(length=(1 << 28) + 1), dict(batch=3), dict(batch=-4), dict(out=P), dict(out=P + 12),
-               dict(cc=cache(lib, new_lens=None))):
+               dict(cc=cache(lib, new_lens=None)), dict(cc=cache(lib, new_lens=P * 16 + 8))):
         assert call(**kw) == lib.ERR_BAD_ARGUMENT, kw
 
 
 def test_a_plan_refuses_bad_arguments(lib):
     cdll = lib.load()
     names = ("table", "stride", "lens", "new", "next", "ring", "span", "B", "columns", "n_pages", "page", "rows", "offsets", "positions", "slots", "taken", "ws", "size")
-    good = dict(zip(names, (P, 8, P, P, P, P, P, 4, 8, 32, 16, 100, P, P, P, P, P, BIG)))
+    good = dict(zip(names, (P, 8, P, P, 2 * P, P, P, 4, 8, 32, 16, 100, P, P, P, P, P, BIG)))
 
     def call(**kw):
         return cdll.mi355_packed_plan(*dict(good, **kw).values(), None)
@@ -62,7 +62,7 @@ def test_a_plan_refuses_bad_arguments(lib):
     assert need > 0 and cdll.mi355_packed_plan_workspace_bytes(0) == 0 and cdll.mi355_packed_plan_workspace_bytes(65536) == 0
     for kw in ([{n: None} for n in ("table", "lens", "new", "ring", "span", "offsets", "positions", "slots", "taken", "ws")] +
                [dict(B=0), dict(columns=0), dict(n_pages=0), dict(rows=-1), dict(page=0), dict(page=24), dict(stride=7), dict(size=need - 1), dict(ws=P + 8), dict(B=65536),
-                dict(rows=(1 << 28) + 1), dict(columns=(1 << 24) + 1, stride=1 << 25), dict(n_pages=1 << 27, page=16), dict(B=60000, columns=1 << 16, stride=1 << 16)]):
+                dict(rows=(1 << 28) + 1), dict(next=P + 12, lens=P), dict(columns=(1 << 24) + 1, stride=1 << 25), dict(n_pages=1 << 27, page=16), dict(B=60000, columns=1 << 16, stride=1 << 16)]):
         assert call(**kw) in (lib.ERR_BAD_ARGUMENT, lib.ERR_UNSUPPORTED), kw
 
 

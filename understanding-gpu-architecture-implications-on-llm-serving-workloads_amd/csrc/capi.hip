@@ -622,8 +622,8 @@ int mi355_cache_keep_path(const mi355_paged_kv* cache, const int32_t* path, int 
     if (length < 1 || length > (1 << 28)) return fail(MI355_ERR_BAD_ARGUMENT, "%s: length of a path must be in 1 .. 2^28 (got %d)", fn, length);
     if (path_batch < 0 || (cache->B > 1 && path_batch < length))
         return fail(MI355_ERR_BAD_ARGUMENT, "%s: paths overlap (stride %lld, %d entries)", fn, (long long)path_batch, length);
-    if (lens_out < cache->seq_lens + cache->B && cache->seq_lens < lens_out + cache->B)
-        return fail(MI355_ERR_BAD_ARGUMENT, "%s: lens_out overlaps seq_lens", fn);
+    for (const int32_t* lens : {cache->seq_lens, cache->new_lens})
+        if (lens_out < lens + cache->B && lens < lens_out + cache->B) return fail(MI355_ERR_BAD_ARGUMENT, "%s: lens_out overlaps seq_lens or new_lens", fn);
     const hipError_t e = mi355::keep_path_dispatch(*cache, path, length, (long)path_batch, lens_out, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? 0 : hip_fail(e, fn);
 }
@@ -647,6 +647,8 @@ int mi355_packed_plan(int32_t* block_table, int64_t table_stride, int32_t* seq_l
                     (long long)max_pages * page_size, (long long)n_pages * page_size, rows);
     if (B > 1 && table_stride < max_pages)
         return fail(MI355_ERR_BAD_ARGUMENT, "%s: rows of the block table overlap (stride %lld, %d entries)", fn, (long long)table_stride, max_pages);
+    if (next_positions && next_positions < seq_lens + B && seq_lens < next_positions + B)
+        return fail(MI355_ERR_BAD_ARGUMENT, "%s: next_positions overlaps seq_lens (null: a token's position is the number of its key)", fn);
     if (int rc = workspace_checked(fn, mi355::packed_plan_workspace(B), workspace, workspace_bytes)) return rc;
     const hipError_t e = mi355::packed_plan_dispatch(block_table, (long)table_stride, seq_lens, new_lens, next_positions, free_pages, free_span, B, max_pages, n_pages,
                                                      page_size, rows, offsets, positions, slots, taken, workspace, static_cast<hipStream_t>(stream));
