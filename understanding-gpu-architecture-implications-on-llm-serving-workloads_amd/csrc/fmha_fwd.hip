@@ -26,6 +26,7 @@
 #include "mi355_common.h"
 #include "mi355_serving_internal.h"
 #include "mi355_timeline.h"
+#include "paged.h"
 
 namespace mi355 {
 
@@ -203,28 +204,15 @@ struct PackedOffsets {
         // (offsets that descend are taken for the largest one in front of them; lanes behind the last sequence begin and end at the last offset)
         start = min(max(first, 0), all_rows);
         begin = __builtin_amdgcn_readfirstlane(start);
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int y = __shfl_up(start, off, 64);
-            if (lane >= off) start = max(start, y);
-        }
+        start = wave_running_max(start);
         rows = max(min(last, all_rows) - start, 0);
         end = __builtin_amdgcn_readlane(start + rows, 63);
         tiles = (int)((uint32_t)(rows + tile - 1) / (uint32_t)tile);
-        entries = __builtin_amdgcn_readlane(up_to(tiles), 63);
-    }
-    static __device__ __forceinline__ int up_to(int x) {   // sum over the lanes up to this one
-        const int lane = threadIdx.x & 63;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int y = __shfl_up(x, off, 64);
-            if (lane >= off) x += y;
-        }
-        return x;
+        entries = __builtin_amdgcn_readlane(wave_inclusive_sum(tiles), 63);
     }
     // {first row, rows, tile, 0} of tile `rank` in the order of (sequence, tile); the same for all lanes
     __device__ __forceinline__ int4v in_order(int rank) const {
-        const int incl = up_to(tiles);
+        const int incl = wave_inclusive_sum(tiles);
         const uint64_t past = __builtin_amdgcn_ballot_w64(rank < incl);
         const int i = past == 0 ? 0 : __builtin_ctzll(past);
         return int4v{__builtin_amdgcn_readlane(start, i), __builtin_amdgcn_readlane(rows, i), rank - __builtin_amdgcn_readlane(incl, i) + __builtin_amdgcn_readlane(tiles, i), 0};
@@ -259,7 +247,7 @@ struct PackedOrder {
             if (tid == 0) at_least[PackedOffsets::kMostTiles] = 0;
         } else if (wave == 0) {
             const int tiles = tiles_of(lane);
-            at_least[lane] = PackedOffsets::up_to(tiles) - tiles;
+            at_least[lane] = wave_inclusive_sum(tiles) - tiles;
         }
         __syncthreads();
     }
@@ -472,7 +460,7 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
             begin = sequences.begin;
             end = sequences.end;
             packed_entries = sequences.entries;
-            if ((long)q_tiles * (Hq >> packed.head_shift) <= gridDim.x) {   // an item a workgroup at most, in any order
+            if ((long)packed_entries * (Hq >> packed.head_shift) <= gridDim.x) {   // an item a workgroup at most, in any order
                 cur = item_of(0, &sequences);
             } else {
                 packed_items = (long)packed_entries * (Hq >> packed.head_shift);
@@ -1407,11 +1395,7 @@ __global__ __launch_bounds__(packed::THREADS) void packed_items_kernel(PackedLis
     int last_row = 0;
     // sum over the threads up to this one
     const auto block_sum = [&](int x, int (&per_wave)[WAVES], int& all) {
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int y = __shfl_up(x, off, 64);
-            if (lane >= off) x += y;
-        }
+        x = wave_inclusive_sum(x);
         if (lane == 63) per_wave[wave] = x;
         __syncthreads();
         all = 0;
@@ -1431,11 +1415,7 @@ __global__ __launch_bounds__(packed::THREADS) void packed_items_kernel(PackedLis
             int start = b < p.B ? row_of(b) : 0;
             const int end = b < p.B ? row_of(b + 1) : 0;
             if (b0 == 0 && tid == 0) last_row = start;
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const int y = __shfl_up(start, off, 64);
-                if (lane >= off) start = max(start, y);
-            }
+            start = wave_running_max(start);
             if (here > 64 || b0 > 0) {   // (the waves of a group)
                 __syncthreads();
                 if (lane == 63) sums[0][wave] = start;

@@ -70,6 +70,15 @@ __device__ __forceinline__ int wave_inclusive_sum(int x) {
     x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
     return x;
 }
+// the largest value up to this lane
+__device__ __forceinline__ int wave_running_max(int x) {
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x111, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x112, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x114, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x118, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x142, 0xa, 0xf, false));
+    return max(x, __builtin_amdgcn_update_dpp(x, x, 0x143, 0xc, 0xf, false));
+}
 // the largest of the first 16 lanes' values, and of all lanes', in every lane (likewise)
 __device__ __forceinline__ int row_running_max(int x) {
     x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x111, 0xf, 0xf, false));
