@@ -71,6 +71,9 @@ PACKED = [   # Hq, Hkv, lengths, options
     (4, 1, [(37 * i) % 41 for i in range(70)], dict(spare=7)),            # more than 64 sequences
     (2, 1, [(7 * i) % 5 for i in range(2500)], dict(spare=70)),           # more than 1024
     (32, 8, [0, 0, 0], dict(spare=5)),
+    (16, 1, [100, 33, 5], {}),                                             # more heads a kv head than lie side by side
+    (8, 1, [(53 * i) % 150 for i in range(64)], dict(spare=1)),           # as many sequences as a workgroup orders
+    (12, 4, [(53 * i) % 150 for i in range(65)], {}),
     (16, 8, [1100, 900, 1300], {}),
 ]
 
@@ -172,10 +175,36 @@ def test_scores_of_every_size(gpu):
             assert o.isfinite().all() and lse.isfinite().all() and (o[0] == v[0].repeat_interleave(4, 0)).all()
 
 
-def test_a_long_prompt(gpu):
-    lens = [8191, 100]
-    q, k, v = batch(lens, 4, 1, torch.bfloat16)
-    check_packed(q, k, v, lens, *ops.fine_fmha_packed_with_lse(q, k, v, offsets_of(lens)))
+@pytest.mark.parametrize("Hq, lens, variant", [(4, [8191, 100], 0), (8, [8192], 1), (8, [5, 8191, 0, 100], 1)], ids=["8191", "512-tiles", "more-tiles"])
+def test_a_long_prompt(gpu, Hq, lens, variant):
+    """Tiles of 16 rows of 8 heads: a sequence of as many as a workgroup orders by itself, and a batch that may have more."""
+    q, k, v = batch(lens, Hq, 1, torch.bfloat16)
+    check_packed(q, k, v, lens, *pinned(q, k, v, offsets_of(lens), True, variant))
+
+
+def test_more_rows_than_the_list_has_bins_for(gpu):
+    lens = [(97 * i) % 500 for i in range(300)]
+    q, k, v = batch(lens, 1, 1, torch.float16)
+    assert sum(lens) > 64 * 1024
+    for causal in (True, False):
+        check_packed(q, k, v, lens, *ops.fine_fmha_packed_with_lse(q, k, v, offsets_of(lens), causal), causal)
+
+
+def test_rows_that_lie_beyond_32_bits(gpu):
+    """Rows 2^20 elements apart, 4.4 GB from first to last."""
+    rows, lens = 2200, [2000, 200]
+    whole = torch.empty(rows << 20, dtype=torch.float16, device="cuda")
+    x = torch.as_strided(whole, (rows, 6, D), (1 << 20, D, 1))
+    x.copy_(torch.randn(rows, 6, D, generator=torch.Generator().manual_seed(4)).half())
+    q, k, v = x.split((4, 1, 1), 1)
+    o, lse = ops.fine_fmha_packed_with_lse(q, k, v, offsets_of(lens))
+    want, want_lse = ops.fine_fmha_packed_with_lse(*(t.contiguous() for t in (q, k, v)), offsets_of(lens))
+    assert torch.equal(o, want) and torch.equal(lse, want_lse)
+    kv, (cos, sin) = torch.zeros(140, 2, 16, D, dtype=torch.float16, device="cuda"), tables(rows)
+    at, other, kv2 = torch.arange(rows, dtype=torch.int32, device="cuda"), x.contiguous(), torch.zeros_like(kv)
+    ops.fine_rope_packed(x, kv, at, cos, sin, at, 4)
+    ops.fine_rope_packed(other, kv2, at, cos, sin, at, 4)
+    assert torch.equal(x, other) and torch.equal(kv, kv2) and (kv != 0).any()
 
 
 def test_captured_calls_serve_the_lengths_of_their_tensors(gpu):

@@ -89,6 +89,9 @@ TREES = [   # Hq, Hkv, S, page, lengths, new_lens, options
     (64, 8, 255, 32, [2500] * 9, None, {}),
     (32, 8, 8, 16, [300, 20], None, dict(max_pages=900)),
     (8, 4, 3, 16, [(37 * i) % 97 + 3 for i in range(70)], None, {}),
+    (8, 2, 20, 16, [(37 * i) % 600 + 20 for i in range(70)], None, {}),     # more sequences than are ordered: a workgroup a triple
+    (8, 1, 24, 16, [(191 * i) % 1500 for i in range(40)], [(7 * i) % 25 for i in range(40)], {}),   # some without keys, some without tokens
+    (16, 2, 32, 32, [3000] + [40] * 20, None, {}),                         # one that is cut, and others
 ]
 
 
@@ -165,9 +168,10 @@ def test_pages_outside_the_pool_hold_no_keys(gpu, S, dtype):
     check_tree(cache, q, trees, o, lse, hidden=hidden)
 
 
-def test_captured_trees(gpu):
+@pytest.mark.parametrize("Hq", [2, 8, 32], ids=["12-columns", "48-columns", "192-columns"])
+def test_captured_trees(gpu, Hq):
     cache = Cache([900, 300], 2, 16)
-    q, parents, new = queries(cache, 8, 12), ints([a_tree("some", 12, b) for b in range(2)]), ints([12, 12])
+    q, parents, new = queries(cache, Hq, 12), ints([a_tree("some", 12, b) for b in range(2)]), ints([12, 12])
     side = torch.cuda.Stream()
     with torch.cuda.stream(side):
         ops.fine_fmha_tree_with_lse(q, *cache.args, parents, new_lens=new)
@@ -186,6 +190,24 @@ def test_captured_trees(gpu):
         torch.cuda.synchronize()
         assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
         check_tree(cache, q, trees, o, lse, n)
+
+
+def test_pages_that_lie_beyond_32_bits(gpu):
+    """Pages 2^23 elements apart, 5 GB from first to last."""
+    small = Cache([700, 90], 2, 16)
+    n_pages = 320
+    whole = torch.empty(n_pages << 23, dtype=torch.float16, device="cuda")
+    far = torch.as_strided(whole, (n_pages, 4, 16, D), (1 << 23, 16 * D, D, 1))
+    far[-small.kv.shape[0]:].copy_(small.kv)
+    table = small.table + (n_pages - small.kv.shape[0]) * (small.table >= 0)
+    for S in (6, 60):
+        q, trees = queries(small, 8, S), ints([a_tree("some", S, b) for b in range(2)])
+        a, b = ops.fine_fmha_tree_with_lse(q, *small.args, trees), ops.fine_fmha_tree_with_lse(q, far, table.int(), small.lens, trees)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    path = ints([[0, 5, 6, 50], [1, 3, -1, -1]])
+    ops.fine_keep_path(*small.args, ints([60, 60]), path)
+    ops.fine_keep_path(far, table.int(), small.lens, ints([60, 60]), path)
+    assert torch.equal(far[-small.kv.shape[0]:].nan_to_num(9.0), small.kv.nan_to_num(9.0))
 
 
 # ---- accepted paths ----------------------------------------------------------------------------------------------------
