@@ -40,35 +40,50 @@ namespace plan {
 __device__ __forceinline__ bool holds(const Plan& p, int page) { return (uint32_t)page < (uint32_t)p.n_pages; }
 __device__ __forceinline__ int pages_of(const Plan& p, int keys) { return divide(keys + p.page_size - 1, p.by_page); }
 
-// Sum over the threads in front of this one and over all (x >= 0), cut to `most` at every step: with that the sum of any number of terms fits an int.
-// `sums` is free again behind the caller's next barrier.
-__device__ __forceinline__ int before_and_all(int x, int most, int (&sums)[WAVES], int& all) {
+// Inclusive sum over a wave (x >= 0), cut to `most` at every step: with that the sum of any number of terms fits an int.
+__device__ __forceinline__ int cut_inclusive_sum(int x, int most) {
+    const auto add = [&](int y) { x = min(x + y, most); };
+    add(__builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true));   // (the steps of wave_inclusive_sum)
+    add(__builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true));
+    add(__builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true));
+    add(__builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true));
+    add(__builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+    add(__builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+    return x;
+}
+// What the waves in front of this one have, and all of them. `incl`: inclusive sums over this wave, of which the last lane's is its own.
+// `sums` is free again behind the caller's next barrier but one.
+template <int N>
+__device__ __forceinline__ void over_waves(const int (&incl)[N], int most, int (&sums)[WAVES][N], int (&front)[N], int (&all)[N]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int incl = x;
+    if (lane == 63) {
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const int y = __shfl_up(incl, off, 64);
-        incl = lane >= off ? min(incl + y, most) : incl;
+        for (int i = 0; i < N; ++i) sums[wave][i] = incl[i];
     }
-    const int left = __shfl_up(incl, 1, 64);   // of the lanes in front
-    if (lane == 63) sums[wave] = incl;
     __syncthreads();
-    int front = lane > 0 ? left : 0;
-    all = 0;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-        if (w == wave) front = min(front + all, most);
-        all = min(all + sums[w], most);
+    for (int i = 0; i < N; ++i) {
+        front[i] = all[i] = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            if (w == wave) front[i] = all[i];
+            all[i] = min(all[i] + sums[w][i], most);
+        }
     }
-    return front;
+}
+// Sum over the threads in front of this one, and over all
+__device__ __forceinline__ int before_and_all(int x, int most, int (&sums)[WAVES][1], int& all) {
+    const int incl[1] = {cut_inclusive_sum(x, most)};
+    int front[1], whole[1];
+    over_waves(incl, most, sums, front, whole);
+    all = whole[0];
+    const int left = __builtin_amdgcn_update_dpp(0, incl[0], 0x138, 0xf, 0xf, true);   // wave_shr:1, of the lane in front
+    return min(left + front[0], most);
 }
 
 // What the sequences in front of some sequence took
 struct Before {
     int rows, lacks, used, back;   // `used`: pages taken
-};
-struct Own {
-    int len, n, lacks, taken;
 };
 
 }  // namespace plan
@@ -118,13 +133,21 @@ __global__ __launch_bounds__(plan::THREADS) void plan_count_kernel(Plan p) {
 // Workgroups 0 .. B - 1: a sequence each; behind them the rows that are no sequence's, and the ring's new span
 __global__ __launch_bounds__(plan::THREADS) void plan_write_kernel(Plan p) {
     using namespace plan;
-    __shared__ int sums[4][WAVES];
+    __shared__ int sums[3][WAVES][1], pairs[WAVES][2];
     __shared__ int found[8];
     __shared__ int pages[THREADS];
-    const int tid = threadIdx.x, target = min((int)blockIdx.x, p.B);   // (B: the sums over all)
+    const int tid = threadIdx.x, lane = tid & 63, target = min((int)blockIdx.x, p.B);   // (B: the sums over all)
+    // the first entries of this sequence's row are requested beside the counts
+    constexpr int AHEAD = 4;
+    const int own = min((int)blockIdx.x, p.B - 1);
+    int* row = p.table + (long)own * p.table_stride;
+    const int c0 = divide(min(max(p.seq_lens[own], 0), p.columns * p.page_size), p.by_page);
+    const int next_position = p.next_positions != nullptr ? p.next_positions[own] : -1;
+    int ahead[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) ahead[i] = c0 + i * THREADS + tid < p.columns ? row[c0 + i * THREADS + tid] : -1;
     const int first = p.counts[0], count = p.counts[1], most_rows = p.rows + 1;
     Before sum = {0, 0, 0, 0};
-    Own own = {0, 0, 0, 0};
     for (int b0 = 0; b0 < p.B && b0 <= target; b0 += THREADS) {
         const int b = b0 + tid;
         int4v c = {0, 0, 0, 0};
@@ -143,7 +166,7 @@ __global__ __launch_bounds__(plan::THREADS) void plan_write_kernel(Plan p) {
         const bool taken = fits && (lacks == 0 || front + lacks <= count);
         const int used = sum.used + before_and_all(taken ? lacks : 0, INT32_MAX, sums[2], all);
         sum.used += all;
-        const int back = sum.back + before_and_all(taken ? c[3] : back0, INT32_MAX, sums[3], all);
+        const int back = sum.back + before_and_all(taken ? c[3] : back0, INT32_MAX, sums[0], all);
         sum.back += all;
         if (b == target && target < p.B) {
             found[0] = off, found[1] = used, found[2] = back, found[3] = c[0], found[4] = c[1], found[5] = taken;
@@ -164,28 +187,32 @@ __global__ __launch_bounds__(plan::THREADS) void plan_write_kernel(Plan p) {
     const int b = blockIdx.x, off = found[0], used0 = found[1], back0 = found[2], len = found[3], n = found[4];
     const bool taken = found[5] != 0;
     const int len1 = taken ? len + n : len;
-    const int next = p.next_positions != nullptr ? p.next_positions[b] : len;
+    const int next = p.next_positions != nullptr ? next_position : len;
     if (tid == 0) {
         p.offsets[b] = min(off, p.rows);
         p.taken[b] = taken ? n : 0;
-        p.seq_lens[b] = len1;
+        p.seq_lens[b] = len1;   // (everyone has passed a barrier since the old ones were read)
+        if (p.next_positions != nullptr) p.next_positions[b] = next + len1 - len;
     }
     if (!taken)
         for (int r = off + tid; r < min(off + n, p.rows); r += THREADS) p.positions[r] = p.slots[r] = -1;
-    __syncthreads();   // (everyone has the position)
-    if (tid == 0 && p.next_positions != nullptr) p.next_positions[b] = next + len1 - len;
-
-    int* row = p.table + (long)b * p.table_stride;
-    const int c0 = divide(len, p.by_page), c1 = pages_of(p, len1);
+    const int c1 = pages_of(p, len1);
     int used = used0, back = back0;
     for (int base = c0; base < p.columns; base += THREADS) {
         const int c = base + tid;
-        int page = c < p.columns ? row[c] : -1;
+        int page = ahead[0];
+#pragma unroll
+        for (int i = 1; i < AHEAD; ++i) ahead[i - 1] = ahead[i];
+        ahead[AHEAD - 1] = c + AHEAD * THREADS < p.columns ? row[c + AHEAD * THREADS] : -1;
         const bool held = holds(p, page), wanted = !held && c < c1 && len1 > len, behind = held && c >= c1;
-        int n_wanted, n_behind;
-        const int i = used + before_and_all(wanted, THREADS, sums[0], n_wanted), j = back + before_and_all(behind, THREADS, sums[1], n_behind);
-        used += n_wanted;
-        back += n_behind;
+        const uint64_t all_wanted = __builtin_amdgcn_ballot_w64(wanted), all_behind = __builtin_amdgcn_ballot_w64(behind);
+        const int wave_has[2] = {__builtin_popcountll(all_wanted), __builtin_popcountll(all_behind)};
+        int in_front[2], in_all[2];
+        over_waves(wave_has, THREADS, pairs, in_front, in_all);
+        const uint64_t lanes_below = ((uint64_t)1 << lane) - 1;
+        const int i = used + in_front[0] + __builtin_popcountll(all_wanted & lanes_below), j = back + in_front[1] + __builtin_popcountll(all_behind & lanes_below);
+        used += in_all[0];
+        back += in_all[1];
         if (wanted) {
             const int at = first + i;
             page = p.ring[at >= p.n_pages ? at - p.n_pages : at];
