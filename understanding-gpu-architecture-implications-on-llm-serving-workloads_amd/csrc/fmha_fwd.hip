@@ -1513,20 +1513,20 @@ static hipError_t launch_packed(const T* Q, const T* K, const T* V, T* O, float*
     return hipGetLastError();
 }
 
-// Whether work items are of 256 (row, head) pairs, whose K and V fragments feed two MFMAs, or of 128: where sequences of the mean length make 256 items or more that see 2.5 key
-// tiles on average. Over 342 drawn calls (1 .. 64 sequences, 1 .. 6000 rows, 8 .. 64 heads, causal and not) the choice is 0.8 % behind the better one on average, at worst
-// 27 %; 128 throughout 3.9 %. us, 128 / 256: 16 sequences of up to 1000 rows, 32/8 heads 99.8 / 92.3, 4 of up to 8192 1243 / 1040; 1 of 512 14.0 / 21.0, 64 of up to 200 51.7 /
-// 54.5, 8 of up to 600, 40/8 heads 47.2 / 54.6.
+// Whether work items are of 256 (row, head) pairs, whose K and V fragments feed two MFMAs, or of 128, which fill more workgroups and cost less beside their key tiles: by an
+// estimate for sequences of the mean length. us of an item of x key tiles: 128 pairs 3 + 1.1 x, 256 pairs 6 + 1.6 x; a launch of up to 256 items takes as long as one that
+// sees all keys, one of n items as long as n / 256 + 0.75 of the mean. Over 2104 drawn calls (1 .. 64 sequences, 1 .. 6000 rows, 8 .. 64 heads, causal and not) the choice is 0.4 %
+// behind the better one on average, at worst 50 %; 128 throughout 3.5 %, 256 throughout 18 %. us, 128 / 256: 16 sequences of up to 1000 rows, 32/8 heads 97.9 / 89.7, 4 of up to 8192 1243 / 1040;
+// 1 of 512 13.5 / 20.5, 8 of up to 600, 40/8 heads 47.9 / 54.3.
 static bool packed_large_tiles(int rows, int B, int Hq, int Hkv, int causal) {
-    const int shift = packed_head_shift(Hq, Hkv), tile = 256 >> shift, mean = (rows + B - 1) / B, tiles = (mean + tile - 1) / tile;
-    long keys = 0;   // key tiles of a sequence's q tiles
-    if (tiles > 64)
-        keys = 3L * tiles;   // (more than that)
-    else if (causal)
-        for (int t = 1; t <= tiles; ++t) keys += (std::min(t * tile, mean) + fmha::BN - 1) / fmha::BN;
-    else
-        keys = (long)tiles * ((mean + fmha::BN - 1) / fmha::BN);
-    return (long)B * tiles * (Hq >> shift) >= 256 && 2 * keys >= 5 * tiles;
+    const int shift = packed_head_shift(Hq, Hkv), mean = (rows + B - 1) / B, keys = (mean + fmha::BN - 1) / fmha::BN;
+    const auto estimate = [&](int tile, float item, float key_tile) {
+        const int first = (std::min(tile, mean) + fmha::BN - 1) / fmha::BN;   // key tiles of the first q tile, causal
+        const float items = (float)B * (float)((mean + tile - 1) / tile) * (float)(Hq >> shift);
+        if (items <= 256.f) return item + key_tile * (float)keys;
+        return (item + key_tile * (causal ? 0.5f * (float)(first + keys) : (float)keys)) * (items / 256.f + 0.75f);
+    };
+    return estimate(256 >> shift, 6.f, 1.6f) < estimate(128 >> shift, 3.f, 1.1f);
 }
 
 template <typename T>
