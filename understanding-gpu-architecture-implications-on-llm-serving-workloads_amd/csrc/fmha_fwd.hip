@@ -1516,8 +1516,8 @@ static hipError_t launch_packed(const T* Q, const T* K, const T* V, T* O, float*
 // Whether work items are of 256 (row, head) pairs, whose K and V fragments feed two MFMAs, or of 128, which fill more workgroups and cost less beside their key tiles: by an
 // estimate for sequences of the mean length. us of an item of x key tiles: 128 pairs 3 + 1.1 x, 256 pairs 6 + 1.6 x; a launch of up to 256 items takes as long as one that
 // sees all keys, one of n items as long as n / 256 + 0.75 of the mean. Over 2104 drawn calls (1 .. 64 sequences, 1 .. 6000 rows, 8 .. 64 heads, causal and not) the choice is 0.4 %
-// behind the better one on average, at worst 50 %; 128 throughout 3.5 %, 256 throughout 18 %. us, 128 / 256: 16 sequences of up to 1000 rows, 32/8 heads 97.9 / 89.7, 4 of up to 8192 1243 / 1040;
-// 1 of 512 13.5 / 20.5, 8 of up to 600, 40/8 heads 47.9 / 54.3.
+// behind the better one on average, at worst 50 %; 128 throughout 3.5 %, 256 throughout 18 %. us, 128 / 256: 16 sequences of up to 1000 rows, 32/8 heads 91.0 / 86.6, 4 of up to 8192 1302 / 1085;
+// 1 of 512 13.5 / 20.5, 8 of up to 600, 40/8 heads 45.8 / 53.3.
 static bool packed_large_tiles(int rows, int B, int Hq, int Hkv, int causal) {
     const int shift = packed_head_shift(Hq, Hkv), mean = (rows + B - 1) / B, keys = (mean + fmha::BN - 1) / fmha::BN;
     const auto estimate = [&](int tile, float item, float key_tile) {
