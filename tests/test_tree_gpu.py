@@ -192,6 +192,25 @@ def test_captured_trees(gpu, Hq):
         check_tree(cache, q, trees, o, lse, n)
 
 
+def test_trees_on_two_streams_at_once(gpu):
+    """Each with parts of its own on their way through a workspace of its own."""
+    calls = []
+    for lens, S in (([900, 300], 12), ([2000, 5, 700], 40)):
+        cache = Cache(lens, 2, 16)
+        q, trees = queries(cache, 16, S), ints([a_tree("some", S, b) for b in range(len(lens))])
+        calls.append((lambda c=cache, q=q, t=trees: ops.fine_fmha_tree_with_lse(q, *c.args, t), torch.cuda.Stream()))
+    want = [call() for call, _ in calls]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, (call, stream) in enumerate(calls):
+            with torch.cuda.stream(stream):
+                got[i].append(call())
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i][0]) and torch.equal(lse, want[i][1]) for o, lse in got[i])
+
+
 def test_pages_that_lie_beyond_32_bits(gpu):
     """Pages 2^23 elements apart, 5 GB from first to last."""
     small = Cache([700, 90], 2, 16)
