@@ -1369,7 +1369,7 @@ hipError_t fmha_fwd_dispatch(const void* Q, const void* K, const void* V, void* 
 // A work item is a q tile of up to 8 query heads of a kv head, side by side: 32 rows of 8 heads see fewer keys that none of them sees than 256 rows of one (of 512 rows 147 of
 // 197 k pairs are worked out, 131 k are seen), and a sequence's last tile is a smaller part of it. Bound by the matrix pipes and the vector unit in turn, like one long sequence, and for
 // short ones by the way of an item's operands and results to and from memory. us, 256 rows of a head and a list / now: 16 sequences of up to 1000 rows of 32/8 heads 119 / 90 (520
-// TFLOP/s of those seen), 4 of up to 8192 1091 / 1054 (1167), 64 of up to 200 74 / 52, 3 of up to 77 of 8/2 heads 12.0 / 8.3 (one launch).
+// TFLOP/s of those seen), 4 of up to 8192 1091 / 1054 (1167), 64 of up to 200 74 / 52, 3 of up to 77 of 8/2 heads 12.0 / 8.0 (one launch).
 // ---------------------------------------------------------------------------------------------------------------
 namespace packed {
 constexpr int THREADS = 1024, WAVES = THREADS / 64;

@@ -9,7 +9,9 @@
 //
 // Bound by launches and chains of memory round trips, not by bytes (a table of 256 x 1024 entries is 1 MB): one kernel counts per sequence (a workgroup each), the
 // second adds up the counts of all sequences in every workgroup, 256 at a time, and writes its own sequence's part. Places of the ring that are read and that
-// are written differ (it holds `count` pages from `first` on and no more than n_pages in all), so nothing waits for anything but the launch in front.
+// are written differ (it holds `count` pages from `first` on and no more than n_pages in all), so nothing waits for anything but the launch in front. us: a step of 64
+// sequences of up to 512 pages 3.1 + 4.2, 64 prompts and 192 running sequences of up to 1024 pages 3.7 + 5.6 (lane sums through LDS, and the table read behind the
+// counts: 5.8 and 8.0 for the second).
 #include <algorithm>
 
 #include "paged.h"

