@@ -302,14 +302,17 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> plan_packed(const at:
                 ": rows >= 0 and page_size >= 1 required (got ", rows, " and ", page_size, "), and no dimension beyond int32");
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(block_table.device());
     at::Tensor offsets = gpu_empty({B + 1}, at::kInt, block_table), positions = gpu_empty({rows}, at::kInt, block_table);
-    at::Tensor slots = gpu_empty({rows}, at::kInt, block_table), taken = gpu_empty({B}, at::kInt, block_table);
+    // the workspace lies behind `taken`, in its storage (the host takes longer than the kernels do: an allocation less, 8.85 -> 8.4 us a call)
     const size_t need = mi355_packed_plan_workspace_bytes((int)B);
-    const at::Tensor ws = workspace_of(need, block_table);
+    const int64_t first = (B + 3) & ~int64_t(3);
+    at::Tensor slots = gpu_empty({rows}, at::kInt, block_table), taken = gpu_empty({first + (int64_t)(need / 4)}, at::kInt, block_table);
+    taken.unsafeGetTensorImpl()->set_sizes_contiguous({B});
+    int32_t* const taken_at = taken.data_ptr<int32_t>();
     hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
     const int rc = mi355_packed_plan(block_table.data_ptr<int32_t>(), block_table.stride(0), seq_lens.data_ptr<int32_t>(), new_lens.data_ptr<int32_t>(),
                                      next_positions.has_value() ? next_positions->data_ptr<int32_t>() : nullptr, free_pages.data_ptr<int32_t>(),
                                      free_span.data_ptr<int32_t>(), (int)B, (int)columns, (int)free_pages.size(0), (int)page_size, (int)rows, offsets.data_ptr<int32_t>(),
-                                     positions.data_ptr<int32_t>(), slots.data_ptr<int32_t>(), taken.data_ptr<int32_t>(), need > 0 ? ws.data_ptr() : nullptr, need, stream);
+                                     positions.data_ptr<int32_t>(), slots.data_ptr<int32_t>(), taken_at, need > 0 ? taken_at + first : nullptr, need, stream);
     TORCH_CHECK(rc == 0, name, ": ", mi355_last_error(), " (code ", rc, ")");
     return {offsets, positions, slots, taken};
 }
