@@ -390,9 +390,10 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
         // the pool's first page to read.
         uint32_t adr_lo = 0, adr_hi = 0;
         uint64_t bad = 0;
-        const auto load_window = [&](int i) {
-            const int key = ((tile0 + kg + (i + lane / NKB) * KG) * NKB + lane % NKB) * 16, index = divide(key, kv.by_page);
-            const int page = table[min(index, kv.max_pages - 1)];
+        const auto key_of_lane = [&](int i) { return ((tile0 + kg + (i + lane / NKB) * KG) * NKB + lane % NKB) * 16; };
+        const auto page_of_lane = [&](int i) { return table[min(divide(key_of_lane(i), kv.by_page), kv.max_pages - 1)]; };
+        const auto load_window = [&](int i, int page) {
+            const int key = key_of_lane(i), index = divide(key, kv.by_page);
             const bool ok = key < keys && (uint32_t)page < (uint32_t)kv.n_pages;
             bad = __builtin_amdgcn_ballot_w64(!ok);
             const uint64_t adr = (uint64_t)(uintptr_t)heads + (ok ? (uint64_t)page * kv.page_bytes + (uint32_t)(key - index * kv.page_size) * kv.row_bytes : 0);
@@ -404,7 +405,7 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
         // this half's tile i into its stage; rows behind the last key repeat it (masked later)
         const auto issue = [&](int i) {
             const int in_window = i & (TILES_AHEAD - 1);
-            if (in_window == 0) load_window(i);
+            if (in_window == 0 && i > 0) load_window(i, page_of_lane(i));
             const int slot = i & (NSTAGE - 1);
             const uint32_t none = (uint32_t)(bad >> (in_window * NKB)) & ((1u << NKB) - 1);
             empty = (empty & ~(15u << (4 * slot))) | none << (4 * slot);
@@ -433,6 +434,7 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
                 }
             }
         };
+        const int first_page = page_of_lane(0);   // (in front of the queries: its wait is not theirs)
         const int up_mine = TREE && tid < a.Sq ? a.tree.parents[b * a.tree.batch + tid] : 0;   // (a parent a thread)
         // this wave's columns; their loads are under way together with the table's
         const int len = seq.len, n_new = seq.n_new;
@@ -454,6 +456,7 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) qf[nb][ks] = *(const V8*)(qp + ks * 32);
         }
+        load_window(0, first_page);
         for (int i = 0; i < NSTAGE - 1 && i < n_loc; ++i) issue(i);
 
         const int base = len - n_new;        // (TREE) key of the first drafted token
@@ -469,17 +472,10 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
                 if (tid < rows) tree_words((MI355_LDS const int*)up, row0 + tid, n_new, base, (MI355_LDS uint32_t*)words + tid * kTreeWords);
             }
         }
-#pragma unroll
-        for (int off = 8; off >= 1; off >>= 1) {
-            lim_min = min(lim_min, __shfl_xor(lim_min, off, 64));
-            lim_max = max(lim_max, __shfl_xor(lim_max, off, 64));
-            row_min = min(row_min, __shfl_xor(row_min, off, 64));
-            row_max = max(row_max, __shfl_xor(row_max, off, 64));
-        }
-        lim_min = __builtin_amdgcn_readfirstlane(lim_min);
-        lim_max = __builtin_amdgcn_readfirstlane(lim_max);
-        row_min = __builtin_amdgcn_readfirstlane(row_min);
-        row_max = __builtin_amdgcn_readfirstlane(row_max);
+        lim_min = -mi355::row_max(-lim_min);
+        lim_max = mi355::row_max(lim_max);
+        row_min = -mi355::row_max(-row_min);
+        row_max = mi355::row_max(row_max);
         if (col0 >= a.ncols) lim_max = -1;   // (a wave without columns)
         if (TREE) lim_min = lim_max < 0 ? -1 : min(lim_min, base - 1);
         // the word of row r for 32 keys from key0 on, which reach the draft
@@ -591,8 +587,11 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
             if (h % NH == NH - 1 && h / NH + NSTAGE - 1 < n_loc) issue(h / NH + NSTAGE - 1);
         };
         const int steps = (n + KG - 1) / KG * NH;
-        wait_vmcnt<0>();
-        __syncthreads();
+        if (n_loc >= 3) wait_vmcnt<2 * COPIES>();   // (the first tile)
+        else if (n_loc == 2) wait_vmcnt<COPIES>();
+        else wait_vmcnt<0>();
+        wait_lgkmcnt<0>();
+        phase_barrier();
         if (wave >= 4) phase_barrier();
         // the steps whose keys all columns of the wave see, up to the first that holds a page outside the pool
         const int room = lim_min - 31 - (tile0 + kg) * TK;
@@ -731,62 +730,70 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
                 }
         }
         __syncthreads();   // the stages are free
-        if constexpr (KG == 2) {   // the halves meet
-            MI355_LDS float* theirs = (MI355_LDS float*)smem_raw + cw * PART_FLOATS;
+        // The halves meet: the first one finishes the lower 16 columns of a wave, the second one the upper ones.
+        constexpr int FINISHED = KG == 2 ? 1 : NB, COLUMN_FLOATS = 8 * 64 * 4 + 32;   // blocks of columns that a wave finishes; what a wave hands over
+        if constexpr (KG == 2) {
             if (kg == 1) {
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-                    for (int db = 0; db < 8; ++db) *(MI355_LDS float4v*)(theirs + ((nb * 8 + db) * 64 + lane) * 4) = o[nb][db];
-                    if (g == 0) theirs[NB * 8 * 256 + nb * 16 + c16] = m_run[nb], theirs[NB * 8 * 256 + WCOLS + nb * 16 + c16] = l_tot[nb];
+                for (int db = 0; db < 8; ++db) {
+                    const float4v x = o[0][db];
+                    o[0][db] = o[1][db];
+                    o[1][db] = x;
                 }
+                const float m = m_run[0], l = l_tot[0];
+                m_run[0] = m_run[1], l_tot[0] = l_tot[1], m_run[1] = m, l_tot[1] = l;
+                qrow[0] = qrow[1];
             }
+            MI355_LDS float* mine = (MI355_LDS float*)smem_raw + wave * COLUMN_FLOATS;
+            MI355_LDS const float* theirs = (MI355_LDS const float*)smem_raw + (wave ^ CW) * COLUMN_FLOATS;
+#pragma unroll
+            for (int db = 0; db < 8; ++db) *(MI355_LDS float4v*)(mine + (db * 64 + lane) * 4) = o[1][db];
+            if (g == 0) mine[8 * 256 + c16] = m_run[1], mine[8 * 256 + 16 + c16] = l_tot[1];
             __syncthreads();
-            if (kg == 0) {
+            const float m1 = theirs[8 * 256 + c16], l1 = theirs[8 * 256 + 16 + c16];
+            const float m = fmaxf(m_run[0], m1);
+            // of a half that saw no key: its outputs and l are 0 (or NaN, which stays)
+            const float w0 = m_run[0] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run[0] - m) * a.scale_log2);
+            const float w1 = m1 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m1 - m) * a.scale_log2);
+            const auto meet = [&](float own, float other) {   // (the second half's share rounded first, on both sides)
+                return kg == 0 ? __builtin_fmaf(w0, own, w1 * other) : __builtin_fmaf(w1, other, w0 * own);
+            };
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    const float m1 = theirs[NB * 8 * 256 + nb * 16 + c16], l1 = theirs[NB * 8 * 256 + WCOLS + nb * 16 + c16];
-                    const float m = fmaxf(m_run[nb], m1);
-                    // of a half that saw no key: its outputs and l are 0 (or NaN, which stays)
-                    const float w0 = m_run[nb] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run[nb] - m) * a.scale_log2);
-                    const float w1 = m1 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m1 - m) * a.scale_log2);
+            for (int db = 0; db < 8; ++db) {
+                const float4v x = *(MI355_LDS const float4v*)(theirs + (db * 64 + lane) * 4);
 #pragma unroll
-                    for (int db = 0; db < 8; ++db)
-                        o[nb][db] = w0 * o[nb][db] + w1 * *(MI355_LDS const float4v*)(theirs + ((nb * 8 + db) * 64 + lane) * 4);
-                    l_tot[nb] = w0 * l_tot[nb] + w1 * l1;
-                    m_run[nb] = m;
-                }
+                for (int e = 0; e < 4; ++e) o[0][db][e] = meet(o[0][db][e], x[e]);
             }
+            l_tot[0] = meet(l_tot[0], l1);
+            m_run[0] = m;
             __syncthreads();
         }
-        if (kg == 0) {
-            if (whole || (!TREE && n == seq.tiles)) {
+        if (whole || (!TREE && n == seq.tiles)) {
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    const int col = col0 + 16 * nb + c16;
-                    if (col >= a.ncols) continue;
-                    const int qi = qrow[nb], hq = hkv * a.group + col - qi * a.group;
-                    const float inv = l_tot[nb] != 0.f ? 1.f / l_tot[nb] : 0.f;
-                    T* op = O + b * a.o_batch + (long)hq * a.o_head + qi * a.o_row + 4 * g;
+            for (int i = 0; i < FINISHED; ++i) {
+                const int col = col0 + 16 * (KG == 2 ? kg : i) + c16;
+                if (col >= a.ncols) continue;
+                const int qi = qrow[i], hq = hkv * a.group + col - qi * a.group;
+                const float inv = l_tot[i] != 0.f ? 1.f / l_tot[i] : 0.f;
+                T* op = O + b * a.o_batch + (long)hq * a.o_head + qi * a.o_row + 4 * g;
 #pragma unroll
-                    for (int db = 0; db < 8; ++db) {
-                        V4 ov;
+                for (int db = 0; db < 8; ++db) {
+                    V4 ov;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) ov[e] = (T)(o[nb][db][e] * inv);
-                        *(V4*)(op + 16 * db) = ov;
-                    }
-                    if (a.LSE != nullptr && g == 0)
-                        a.LSE[((long)b * a.Hq + hq) * a.Sq + qi] =
-                            l_tot[nb] != 0.f ? (m_run[nb] * a.scale_log2 + __builtin_log2f(l_tot[nb])) * 0.69314718055994531f : -INFINITY;
+                    for (int e = 0; e < 4; ++e) ov[e] = (T)(o[i][db][e] * inv);
+                    *(V4*)(op + 16 * db) = ov;
                 }
-            } else {
-                float* part = a.part + ((long)(TREE ? part_number : 2 * blockIdx.x + (parts > 0)) * CW + cw) * PART_FLOATS;
+                if (a.LSE != nullptr && g == 0)
+                    a.LSE[((long)b * a.Hq + hq) * a.Sq + qi] = l_tot[i] != 0.f ? (m_run[i] * a.scale_log2 + __builtin_log2f(l_tot[i])) * 0.69314718055994531f : -INFINITY;
+            }
+        } else {
+            float* part = a.part + ((long)(TREE ? part_number : 2 * blockIdx.x + (parts > 0)) * CW + cw) * PART_FLOATS;
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
+            for (int i = 0; i < FINISHED; ++i) {
+                const int nb = KG == 2 ? kg : i;
 #pragma unroll
-                    for (int db = 0; db < 8; ++db) *(float4v*)(part + ((nb * 8 + db) * 64 + lane) * 4) = o[nb][db];
-                    if (g == 0) part[NB * 8 * 256 + nb * 16 + c16] = m_run[nb], part[NB * 8 * 256 + WCOLS + nb * 16 + c16] = l_tot[nb];
-                }
+                for (int db = 0; db < 8; ++db) *(float4v*)(part + ((nb * 8 + db) * 64 + lane) * 4) = o[i][db];
+                if (g == 0) part[NB * 8 * 256 + nb * 16 + c16] = m_run[i], part[NB * 8 * 256 + WCOLS + nb * 16 + c16] = l_tot[i];
             }
         }
         if constexpr (TREE) {
