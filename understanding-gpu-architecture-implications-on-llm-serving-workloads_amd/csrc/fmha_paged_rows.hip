@@ -19,8 +19,9 @@
 // one sequence of many rows, and many triples get a workgroup a triple and nothing to join.
 //
 // Drafted tokens that are a tree (TREE): words of bits as in fmha_paged.hip, a row's in LDS, and triples cut by rules of their own (Pieces). 32 tokens of 32 sequences of up to 4097
-// keys, 32/8 heads: 74 us and 6.8 for the join; the keys, each read once, come at 4.1 TB/s, a workgroup takes 1.36 us for 64 keys of 128 columns. 64 tokens over
-// 8191 keys: 22 + 6, of which 7 are the keys at the memory's rate; the rest is the chain in front of the first tile and 17 MB of parts on their way out and in.
+// keys, 32/8 heads: 72 us and 6.8 for the join; the keys, each read once, come at 4.2 TB/s, a workgroup takes 1.3 us for 64 keys of 128 columns. 64 tokens over
+// 8191 keys: 21.5 + 5.5, of which 10 are the steps; the rest is what comes in front of the first tile (8 us, the queries and three tiles of every workgroup on their way together), the halves'
+// meeting, and 17 MB of parts on their way out and in.
 #include <algorithm>
 #include <type_traits>
 
@@ -174,8 +175,8 @@ struct Entries {
 // first, in rounds that run forwards and backwards in turn. Every wave of every workgroup works the same out from the lengths: lane r has the sequence whose pieces are the r-th
 // longest, and the sums up to it. The longest piece is one of the longest sequence's 1 / 1 .. 1 / 64 that is no shorter than an equal share (so that at most two pieces a
 // workgroup are parts of a triple): the one whose heaviest workgroup is expected to have the least to do. Equal shares of the axis, of which most workgroups have two parts, / this, us, 32/8
-// heads: 32 tokens, 8 sequences of up to 8191 keys 51 / 46, 16 of up to 4097 55 / 54, 32 of up to 2000 59 / 52, 24 of 2000 67 / 50; 64 tokens, 16 of up to 4097 87 / 72, 20 of up to 1000
-// 53 / 37; 64/8 heads, 64 tokens, 16 of up to 4097 125 / 116. More sequences get a workgroup a triple.
+// heads (both 1 .. 3 us less since): 32 tokens, 8 sequences of up to 8191 keys 51 / 46, 16 of up to 4097 55 / 54, 32 of up to 2000 59 / 52, 24 of 2000 67 / 50; 64 tokens, 16 of up to 4097
+// 87 / 72, 20 of up to 1000 53 / 37; 64/8 heads, 64 tokens, 16 of up to 4097 125 / 116. More sequences get a workgroup a triple.
 template <int COLS>
 struct Pieces {
     static constexpr int TK = COLS / 4, HEAD = kPieceKeys / TK, JOIN = kJoinKeys / TK, kLeast = 128 / TK;   // in tiles; kLeast: of a piece
@@ -254,7 +255,7 @@ struct Pieces {
                 __builtin_amdgcn_readlane(parts, r) - p * each + triple * p, __builtin_amdgcn_readlane(cut, r) - each + triple};
     }
 };
-// What the second kernel needs of a triple that was cut
+// What the second kernel needs of a triple that was cut (pieces: 0 where its columns see no key)
 struct CutTriple {
     int b, triple, pieces, part0;
 };
@@ -304,7 +305,7 @@ __global__ __launch_bounds__(prow::NTHREADS, 2) void paged_rows_kernel(PagedKv k
                 ++round;
                 const int block = divide(x.triple, a.by_hkv);
                 seq = entries.block_of(block, x.b, x.len, x.n_new);
-                if (x.pieces > 1 && x.piece == 0 && tid == 0) ((CutTriple*)a.cuts)[1 + x.cut] = {x.b, x.triple, x.pieces, x.part0};
+                if (x.pieces > 1 && x.piece == 0 && tid == 0) ((CutTriple*)a.cuts)[1 + x.cut] = {x.b, x.triple, seq.keys == 0 ? 0 : x.pieces, x.part0};
                 if (seq.keys == 0) continue;   // (zeros: the second kernel's)
                 hkv = x.triple - block * kv.Hkv;
                 at = x.piece * x.length;
@@ -851,11 +852,11 @@ __global__ __launch_bounds__(256, TREE ? 3 : 1) void paged_rows_join_kernel(Page
     const float *part0, *part1;   // its first part, and the one that stands in front of the others' places
     long stride = 2 * CW * PART_FLOATS;
     if constexpr (TREE) {
-        if (join >= *a.cuts) return;
-        const CutTriple cut = ((const CutTriple*)a.cuts)[1 + join];
+        const CutTriple cut = ((const CutTriple*)a.cuts)[1 + join];   // (requested together with how many there are)
+        if (join >= *a.cuts || cut.pieces == 0) return;
         const int block = divide(cut.triple, a.by_hkv);
         n = cut.pieces, b = cut.b, hkv = cut.triple - block * kv.Hkv, col0 = block * COLS + cw * WCOLS;
-        if (col0 >= a.ncols || entries.keys_of(block * kv.B + b).keys == 0) return;
+        if (col0 >= a.ncols) return;
         stride = CW * PART_FLOATS;
         part0 = part1 = a.part + ((long)cut.part0 * CW + cw) * PART_FLOATS;
     } else {
