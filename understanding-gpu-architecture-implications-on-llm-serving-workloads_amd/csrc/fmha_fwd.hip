@@ -376,18 +376,30 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
         it.n_tiles = 0;
         if constexpr (PACKED) {   // the list's entries are ranked, the heads of an entry are what the (batch, head) groups are elsewhere
             const int x = blockIdx.x & ((1 << map_.xcd_shift) - 1), wl = blockIdx.x >> map_.xcd_shift;
-            const int u = round * map_.wgs + ((round & 1) ? map_.wgs - 1 - wl : wl);
+            const int entries = packed.list == nullptr ? packed_entries : *packed.entries;
+            int u = wl;
+            if (first == nullptr) {
+                // Forwards and backwards in turn. The workgroups that have an item more than the others take the lightest of the last full rounds, of as many as
+                // make up for that item: a causal one costs about as much as 4 key tiles, and between the ends of a round lie the longest sequence's over the rounds. us, without that /
+                // with it: 16 sequences of up to 1000 rows 88 / 83, 6 of up to 606 of 64/8 heads 42.6 / 36.4; with it in all rounds 4 of up to 8192 1079, without 1046, so 1041.
+                const int items = entries * map_.per_rank, rounds = (int)((uint32_t)items / (uint32_t)map_.wgs), rest = items - rounds * map_.wgs;
+                const int spread = max(((packed.list == nullptr ? order.rows[0] : packed.list[0][1]) - 1) / BN, 1);
+                const int apart = causal ? min((int)((uint32_t)(8 * rounds + spread / 2) / (uint32_t)spread), rounds) : rounds;
+                const int few = round < rounds - apart ? map_.wgs : map_.wgs - rest;   // in the first group
+                const bool another = wl >= few;
+                const int size = another ? rest : few, i = another ? wl - few : wl, at = round & 1 ? size - 1 - i : i;
+                u = round * map_.wgs + at + (another && round < rounds ? few : 0);
+                if (round == rounds && !another) u = items;   // (none)
+            }
             const int rank = divide(u, map_.by_rank), rem = u - rank * map_.per_rank;
             int4v entry;
+            it.exists = rank < entries;
             if (first != nullptr) {
-                it.exists = rank < first->entries;
                 entry = first->in_order(rank);
             } else if (packed.list == nullptr) {
-                it.exists = rank < packed_entries;
                 entry = order.find(max(min(rank, packed_entries - 1), 0), causal);
             } else {
                 entry = packed.list[min(rank, q_tiles_ - 1)];   // (q_tiles: the most entries that there may be)
-                it.exists = rank < *packed.entries;
             }
             if (!it.exists) return it;
             const int gl = divide(rem, map_.by_group), kvh = x * map_.groups_per_xcd + gl;
@@ -1368,8 +1380,8 @@ hipError_t fmha_fwd_dispatch(const void* Q, const void* K, const void* V, void* 
 //
 // A work item is a q tile of up to 8 query heads of a kv head, side by side: 32 rows of 8 heads see fewer keys that none of them sees than 256 rows of one (of 512 rows 147 of
 // 197 k pairs are worked out, 131 k are seen), and a sequence's last tile is a smaller part of it. Bound by the matrix pipes and the vector unit in turn, like one long sequence, and for
-// short ones by the way of an item's operands and results to and from memory. us, 256 rows of a head and a list / now: 16 sequences of up to 1000 rows of 32/8 heads 119 / 90 (520
-// TFLOP/s of those seen), 4 of up to 8192 1091 / 1054 (1167), 64 of up to 200 74 / 52, 3 of up to 77 of 8/2 heads 12.0 / 8.0 (one launch).
+// short ones by the way of an item's operands and results to and from memory. us, 256 rows of a head and a list / now: 16 sequences of up to 1000 rows of 32/8 heads 119 / 83 (565
+// TFLOP/s of those seen), 4 of up to 8192 1091 / 1041 (1180), 64 of up to 200 74 / 52, 3 of up to 77 of 8/2 heads 12.0 / 8.0 (one launch).
 // ---------------------------------------------------------------------------------------------------------------
 namespace packed {
 constexpr int THREADS = 1024, WAVES = THREADS / 64;
