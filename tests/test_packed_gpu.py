@@ -74,6 +74,9 @@ PACKED = [   # Hq, Hkv, lengths, options
     (16, 1, [100, 33, 5], {}),                                             # more heads a kv head than lie side by side
     (8, 1, [(53 * i) % 150 for i in range(64)], dict(spare=1)),           # as many sequences as a workgroup orders
     (12, 4, [(53 * i) % 150 for i in range(65)], {}),
+    (32, 8, [256] * 16, {}),                                               # as many items for every workgroup
+    (16, 16, [2000, 30, 700, 1], {}),                                      # few and long ones, workgroups of which have one more than others
+    (24, 8, [(71 * i) % 400 for i in range(40)], {}),
     (16, 8, [1100, 900, 1300], {}),
 ]
 
