@@ -179,8 +179,8 @@ __device__ __forceinline__ void copy16_global_to_lds_at(const void* uniform_base
 // queries, which are a single block of rows of the first wave and are stored as they lie: through LDS they are a chain of its own behind the
 // item, and a branch in the other kernels costs those up to 2 %. us, through LDS / as they lie: 64 x 16/2 heads, 9 queries over 64 keys 17.1 /
 // 15.9, 24 x 32/8, 16 over 64 13.8 / 13.1, 12 x 64/8, 16 over 128 18.2 / 17.6.
-// kPacked: sequences of different lengths one behind the other in one batch, with work items of several heads (below); a row whose result is NaN is
-// worked out again (packed_row); the sums of probabilities are those of what they are in 32 bits, in fp16 too (on the matrix pipe, which sums up the rounded
+// kPacked: sequences of different lengths one behind the other in one batch, with work items of several heads (below); infinities and NaN of V
+// are kept from the rows that do not see them (NonFinite); the sums of probabilities are those of what they are in 32 bits, in fp16 too (on the matrix pipe, which sums up the rounded
 // ones, each up to 2^-11 off, a call takes 3 % less: 16 prompts of up to 1000 rows 88 us, 4 of up to 8192 1035; but the log-sum-exp would have that error in it).
 enum { kOneWalk = 0, kRanges = 1, kRangesF32 = 2, kFewRows = 3, kPacked = 4 };
 constexpr int kFewRowsMax = 16;
@@ -276,52 +276,90 @@ struct PackedItem<true> {
     float* lse;     // of its first head and the sequence's first row
 };
 
-// One row of a packed batch in 32 bits, key by key, with nothing of the keys that it does not see: 64 keys at a time, a lane scores one of them and then sums 2 of the 128 outputs.
-// For rows whose products came out as NaN: where an unseen value is infinite or NaN, 0 * v is not nothing. A row that sees such values comes out as it should
-// too, and ends at once where nothing can come of it but NaN.
+// Infinities and NaN among the values of a packed batch. A product takes every row of a tile with every key of it, and 0 * v is not nothing for such a v: a value that a
+// row does not see can make its output NaN, and so can one that it sees, where its probability is 0 in 16 bits. So a wave asks its outputs for NaN, and a workgroup that has found
+// some looks at these items again behind its last one, outside the loop over the items (in it such code costs all calls 2-5 %, whether it runs or not). It goes through
+// the values for the first key of each kind in every column (FirstNonFinite). An output that is NaN where its row sees a NaN, or two infinities of different
+// signs, is right; one whose row sees an infinity becomes that. For the others the items are worked out once more with zeros in the place of all such
+// values, and their outputs then become what is found in front of each row. us, 16 prompts of 1000 rows of 32/8 heads (clean: 190 .. 200): a NaN in the first value of each 310, in the
+// middle one 290, in the last one 230, 1 of 1000 elements infinite 600; 4 prompts of up to 8192 (1097) 1340, 1500, 1410, 2510.
 template <typename T>
-__device__ __forceinline__ void packed_row(const T* q, const T* K, const T* V, long k_row, long v_row, int keys, float scale_log2, T* out) {
-    using V8 = typename Elem<T>::v8;
-    using V2 = typename Elem<T>::v2;
-    const int lane = threadIdx.x & 63;
-    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int key0 = 0; key0 < keys; key0 += 64) {
-        const int n = min(64, keys - key0);
-        const T* kp = K + (key0 + min(lane, n - 1)) * k_row;
-        float s = 0.f;
-#pragma unroll 4
-        for (int d = 0; d < fmha::D; d += 8) {
-            const V8 a = *(const V8*)(q + d), b = *(const V8*)(kp + d);
+struct NonFinite {
+    static constexpr unsigned short kInfinity = std::is_same<T, half_t>::value ? 0x7c00 : 0x7f80;
+    static __device__ __forceinline__ bool is(T x) { return (__builtin_bit_cast(unsigned short, x) & 0x7fff) >= kInfinity; }
+    static __device__ __forceinline__ bool nan(T x) { return (__builtin_bit_cast(unsigned short, x) & 0x7fff) > kInfinity; }
+    template <int N>
+    static __device__ __forceinline__ bool any(const int4v (&x)[N]) {
+        ushort2v top = {0, 0};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s = __builtin_fmaf((float)a[e], (float)b[e], s);
-        }
-        s *= scale_log2;
-        if (lane >= n) s = -INFINITY;
-        float top = s;
+        for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-        const float m_new = fmaxf(m, top), m_use = m_new == -INFINITY ? 0.f : m_new;
-        const float keep = fmha::fast_exp2(m - m_use), p = lane < n ? fmha::fast_exp2(s - m_use) : 0.f;
-        m = m_new;
-        l = l * keep + p;
-        o0 *= keep;
-        o1 *= keep;
-        for (int j = 0; j < n; ++j) {
-            const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p), j));
-            const V2 v = *(const V2*)(V + (key0 + j) * v_row + 2 * lane);
-            o0 = __builtin_fmaf(w, (float)v[0], o0);
-            o1 = __builtin_fmaf(w, (float)v[1], o1);
-        }
-        if (__builtin_amdgcn_ballot_w64(o0 == o0 || o1 == o1) == 0) break;
+            for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(ushort2v, x[i][e] & 0x7fff7fff));
+        return top[0] >= kInfinity || top[1] >= kInfinity;
     }
+};
+// The first key of a sequence whose value is NaN, +infinity, -infinity, in each of the 8 columns from 8 (lane % 16) on. An infinity whose key is not finite either is NaN: its
+// score is infinite or NaN, and so its weight 0 or NaN.
+template <typename T>
+struct FirstNonFinite {
+    static constexpr int kNone = INT32_MAX, kInts = 3 * fmha::D;
+    int of[3][8];
+    // by all 8 waves, 32 keys a wave in turn, which meet in `table` (kInts, each kNone)
+    __device__ __forceinline__ FirstNonFinite(const T* K, const T* V, long k_row, long v_row, int keys, int wave, int lane, MI355_LDS int* table) {
+        constexpr int AHEAD = 8;   // loads, of four rows each
+        const int column = 8 * (lane & 15);
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) l += __shfl_xor(l, off, 64);
-    const float inv = l != 0.f ? 1.f / l : 0.f;
-    V2 v;
-    v[0] = (T)(o0 * inv);
-    v[1] = (T)(o1 * inv);
-    *(V2*)(out + 2 * lane) = v;
-}
+        for (int e = 0; e < 8; ++e) of[0][e] = of[1][e] = of[2][e] = kNone;
+#pragma unroll 1
+        for (int k0 = 4 * AHEAD * wave; k0 < keys; k0 += 4 * AHEAD * 8) {
+            const auto key_of = [&](int i) { return min(k0 + 4 * i + (lane >> 4), keys - 1); };
+            int4v v[AHEAD], k[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) v[i] = *(const int4v*)(V + key_of(i) * v_row + column);
+            if (__builtin_amdgcn_ballot_w64(NonFinite<T>::any(v)) == 0) continue;
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) k[i] = *(const int4v*)(K + key_of(i) * k_row + column);
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const int4v one[1] = {k[i]};
+                const bool no_key = (__builtin_amdgcn_ballot_w64(NonFinite<T>::any(one)) >> (lane & 48) & 0xffff) != 0;
+                const uint32_t most = NonFinite<T>::kInfinity - no_key, up = no_key ? ~0u : (uint32_t)NonFinite<T>::kInfinity, down = no_key ? ~0u : 0x8000u | NonFinite<T>::kInfinity;
+                const int key = key_of(i);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t x = (uint32_t)v[i][e >> 1] >> (16 * (e & 1)) & 0xffff;
+                    of[0][e] = min(of[0][e], (x & 0x7fff) > most ? key : kNone);
+                    of[1][e] = min(of[1][e], x == up ? key : kNone);
+                    of[2][e] = min(of[2][e], x == down ? key : kNone);
+                }
+            }
+        }
+#pragma unroll
+        for (int kind = 0; kind < 3; ++kind)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (of[kind][e] != kNone) atomicMin((int*)(table + kind * fmha::D + column + e), of[kind][e]);
+        __syncthreads();
+#pragma unroll
+        for (int kind = 0; kind < 3; ++kind)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) of[kind][e] = table[kind * fmha::D + column + e];
+    }
+    // whether there is any, in any column
+    __device__ __forceinline__ bool some() const {
+        int least = kNone;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) least = min(least, min(of[0][e], min(of[1][e], of[2][e])));
+        return __builtin_amdgcn_ballot_w64(least != kNone) != 0;
+    }
+    // what a row that sees the first `keys` keys has in a column, if there are some among them
+    static __device__ __forceinline__ bool found(int nan, int above, int below, int keys, float& x) {
+        const bool up = above < keys, down = below < keys, none = nan < keys || (up && down);
+        x = none ? __builtin_nanf("") : up ? INFINITY : -INFINITY;
+        return none || up || down;
+    }
+    __device__ __forceinline__ bool found(int e, int keys, float& x) const { return found(of[0][e], of[1][e], of[2][e], keys, x); }
+};
 
 template <typename T, int QB, int MODE = kOneWalk>
 __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __restrict__ Q, const T* __restrict__ K,
@@ -364,6 +402,7 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
     };
     const long o_row = SEG ? (long)D : sd.o_row;
     __shared__ typename std::conditional<PACKED, PackedOrder, char>::type order;
+    __shared__ int nan_rounds[3];   // (PACKED) the first and the last round whose outputs hold NaN; the last that is worked out again
     int packed_entries = 0;
     auto item_of = [&](int round, const PackedOffsets* first = nullptr) -> Item {
         // (opaque copies: the compiler would form products of these once and keep them in registers through the loop over the keys, which
@@ -464,8 +503,17 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
     // steps of an item in which the pair that is copied (tiles j + 3 of K, j + 2 of V) is made of full tiles
     auto fast_steps = [](int n_tiles, int kv_valid) { return min(min(n_tiles, kv_valid / BN) - 3, n_tiles - 1); };
     Item cur;
+    const auto in_scalars = [](Item it) {   // (what is the same for all lanes, in scalar registers)
+        int words[sizeof(Item) / 4];
+        __builtin_memcpy(words, &it, sizeof(Item));
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(Item) / 4); ++i) words[i] = __builtin_amdgcn_readfirstlane(words[i]);
+        __builtin_memcpy(&it, words, sizeof(Item));
+        return it;
+    };
     long packed_items = 0;   // of the launch, where a workgroup may have more than one
     if constexpr (PACKED) {
+        if (tid < 3) nan_rounds[tid] = tid == 0 ? INT32_MAX : -1;
         int begin, end;
         if (packed.list == nullptr) {
             const PackedOffsets sequences(packed.offsets, packed.B, Sq, BM >> packed.head_shift);
@@ -485,11 +533,7 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
             packed_items = (long)*packed.entries * (Hq >> packed.head_shift);
             cur = item_of(0);
         }
-        int words[sizeof(Item) / 4];   // (in scalar registers)
-        __builtin_memcpy(words, &cur, sizeof(Item));
-#pragma unroll
-        for (int i = 0; i < (int)(sizeof(Item) / 4); ++i) words[i] = __builtin_amdgcn_readfirstlane(words[i]);
-        __builtin_memcpy(&cur, words, sizeof(Item));
+        cur = in_scalars(cur);
         // zeros for the rows that no sequence has, in front of the first and behind the last
         const int none = begin + Sq - end;
         for (long i = blockIdx.x * 512L + tid; i < (long)none * Hq * 16; i += gridDim.x * 512L) {
@@ -815,6 +859,18 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
         }
     };
 
+    // (PACKED) what this wave copied of V(tile), which has landed and nobody has read yet, without infinities and NaN
+    const auto take_out = [&](int tile) {
+        MI355_LDS char* const mine = smem + VBUF0 + ((ring + tile + 1) & (NBUF - 1)) * TILE_BYTES + wave * 1024 + lane * 16;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            V8 v = *(MI355_LDS const V8*)(mine + i * NWAVES * 1024);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = NonFinite<T>::is(v[e]) ? (T)0.f : v[e];
+            *(MI355_LDS V8*)(mine + i * NWAVES * 1024) = v;
+        }
+    };
+
     // ---- persistent loop over the work items of this workgroup ----------------------------------------------------------
     // The first pairs of the next item ride in the last softmax phases of the current one and its Q fragments are loaded behind the last
     // use of the current ones, so that the next item starts, when O has been normalised and stored (nothing waits for the stores), on
@@ -844,7 +900,7 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
         bool more = false;   // this workgroup has another item
         int n_next = 0;      // its key tiles, if its first pairs are copied while the current item is worked on
         if (more_items && ListedItems::refill(round) && wave == NWAVES - 1) write_listed(round + lane, item_of(round + lane));
-        if (cur.n_tiles > 0) {
+        if (PACKED || cur.n_tiles > 0) {   // (an item of a packed batch has tiles. The way without would make the compiler wait for the next item's Q, and with it for its first pairs, behind it)
             const int n_tiles = cur.n_tiles;
             if (!landed) wait_vmcnt<0>();
             wait_lgkmcnt<0>();
@@ -960,6 +1016,17 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
             const int a = row >> 2;
             return park + (a >> 1) * VBUF0 + (a & 1) * (NWAVES * 1024) + (row & 3) * ROW_BYTES;
         };
+        if constexpr (PACKED) {
+            float sum = 0.f;   // NaN where an output is
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+                for (int db = 0; db < 8; ++db) sum += (o[db][qb][0] + o[db][qb][1]) + (o[db][qb][2] + o[db][qb][3]);
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(sum != sum) != 0, 0) && lane_ == 0) {
+                atomicMin(&nan_rounds[0], round - 1);
+                atomicMax(&nan_rounds[1], round - 1);
+            }
+        }
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) {
             if (q_item0 + qb * 16 >= item_rows) break;   // no such rows (a few queries are done 0.5 us sooner for it)
@@ -1006,24 +1073,111 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
 #pragma unroll
             for (int a = 0; a < 4; ++a)
                 if (q_first + 4 * a + r4 < item_rows) *(V8*)(o_item + (q_first + 4 * a + r4) * o_row + 8 * r16) = row[a];
-            if constexpr (PACKED) {
-                bool nan = false;
+        }
+        if (!more) break;
+    }
+    if constexpr (PACKED) {   // outputs that are NaN (NonFinite)
+        wait_lgkmcnt<0>();
+        phase_barrier();
+        const int nan0 = __builtin_amdgcn_readfirstlane(nan_rounds[0]), nan1 = __builtin_amdgcn_readfirstlane(nan_rounds[1]);
+        if (__builtin_expect(nan0 <= nan1, 0)) {
+            int lane_ = lane, wave_head_ = wave_head, wave_row0_ = wave_row0, causal_ = causal;
+            asm volatile("" : "+v"(lane_), "+s"(wave_head_), "+s"(wave_row0_), "+s"(causal_));   // (or what follows from them is kept in registers through the loop above)
+            const int r16 = lane_ & 15, r4 = lane_ >> 4;
+            MI355_LDS int* const table = (MI355_LDS int*)&listed[0][0];
+            static_assert(sizeof(listed) >= sizeof(int) * FirstNonFinite<T>::kInts, "");
+            wait_vmcnt<0>();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");   // (outputs that were in this CU's cache before they were written)
+#pragma unroll 1
+            for (int r = nan0; r <= nan1; ++r) {
+                cur = in_scalars(more_items ? item_of(r) : cur);   // (otherwise it is the only one)
+                __syncthreads();
+                for (int i = lane_; i < FirstNonFinite<T>::kInts; i += 64) table[i] = FirstNonFinite<T>::kNone;
+                __syncthreads();
+                const FirstNonFinite<T> first(cur.Kh, cur.Vh, sd.k_row, sd.v_row, min(cur.n_tiles * BN, cur.kv_valid), wave, lane_, table);
+                const bool some = first.some();
+                q_wave0 = cur.q_block0 + wave_row0_;
+                const int rows_end = min(q_wave0 + WQ, rows_of(cur));
+                T* const out = cur.Oh + wave_head_ * sd.o_head;
+                bool open = false;   // an output that neither the values that its row sees nor, as far as one can tell, the scores make NaN
+#pragma unroll 1
+                for (int i0 = q_wave0; i0 < rows_end; i0 += 4) {   // four rows, 8 columns a lane
+                    const int i = min(i0 + r4, rows_end - 1);
+                    T* const at = out + i * sd.o_row + 8 * r16;
+                    const V8 x = *(const V8*)at;
+                    bool all = true;
 #pragma unroll
-                for (int db = 0; db < 8; ++db)
+                    for (int e = 0; e < 8; ++e) all = all && NonFinite<T>::nan(x[e]);
+                    all = (__builtin_amdgcn_ballot_w64(all) >> (lane_ & 48) & 0xffff) == 0xffff;   // throughout: the scores may be
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) nan = nan || o[db][qb][e] != o[db][qb][e];
-                uint64_t lanes = __builtin_amdgcn_ballot_w64(nan && q_first + r16 < item_rows);
-                if (lanes != 0) {
-                    const Item done = more ? item_of(round - 1) : cur;
-                    uint32_t again = (uint32_t)(lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) & 0xffff;
-                    for (; again != 0; again &= again - 1) {
-                        const int i = q_first + __builtin_ctz(again);
-                        packed_row<T>(queries_of(done) + i * sd.q_row, done.Kh, done.Vh, sd.k_row, sd.v_row, causal ? i + 1 : done.rows, scale_log2, o_item + i * o_row);
+                    for (int e = 0; e < 8; ++e) {
+                        float y;
+                        const bool found = first.found(e, causal_ ? i + 1 : cur.kv_valid, y), none = NonFinite<T>::nan(x[e]);
+                        if (none && found && !all) at[e] = (T)y;
+                        open = open || (none && (all ? some && !(found && y != y) : !found));
+                    }
+                }
+                if (__builtin_amdgcn_ballot_w64(open) != 0 && lane_ == 0) nan_rounds[2] = r;
+                wait_vmcnt<0>();
+                __syncthreads();
+                if (__builtin_amdgcn_readfirstlane(nan_rounds[2]) != r) continue;
+                // Once more without such values, one tile behind the other, in the arithmetic of the loop above
+                ring = 0;
+                src_k = {cur.Kh, 0, cur.n_tiles - 1, cur.kv_valid};
+                src_v = {cur.Vh, 0, cur.n_tiles - 1, cur.kv_valid};
+                const auto issue = [&](int tile) { issue_k1(tile, 0), issue_k1(tile, 1), issue_v1(tile + 1, 0), issue_v1(tile + 1, 1); };
+                load_q(queries_of(cur), q_wave0, rows_of(cur));
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb) {
+                    m_run[qb] = m_thr[qb] = -INFINITY;
+                    neg_ms[qb] = 0.f;
+                    l_acc[qb] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int db = 0; db < 8; ++db) o[db][qb] = float4v{0.f, 0.f, 0.f, 0.f};
+                }
+#pragma unroll 1
+                for (int next = 0; next <= cur.n_tiles; ++next) {
+                    const int tile = next - 1;
+                    if (tile >= 0) {
+                        wait_vmcnt<0>();
+                        take_out(tile);
+                        __syncthreads();
+                    }
+                    if (next < cur.n_tiles) issue(next);
+                    if (tile < 0) continue;
+                    float4v s[4][QB];
+                    V8 pf[2][QB], fr[AHEAD];
+                    preload(I0{}, Dyn{}, tile & (NBUF - 1), fr);
+                    mfma_phase(I0{}, I16{}, Dyn{}, tile & (NBUF - 1), s, pf, fr);
+                    // S is read by assembly, in front of which the compiler puts no wait for the matrix pipe; behind the last product (a 16x16x32, which writes s[2]) 8 wait
+                    // states are enough. (In the loop above a barrier lies between.)
+                    asm volatile("s_nop 10" : "+v"(s[2][QB - 1]), "+v"(s[3][QB - 1]));
+                    pin_s(s);
+                    softmax_tile(s, tile, pf, std::integral_constant<int, -2>{});
+                    pin_p(pf);
+                    preload(I16{}, Dyn{}, (tile + 1) & (NBUF - 1), fr);
+                    mfma_phase(I16{}, I32{}, Dyn{}, (tile + 1) & (NBUF - 1), s, pf, fr);
+                }
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb) {
+                    const int i = q_wave0 + qb * 16 + r16;
+                    const float l_tot = quad_sum(l_acc[qb][0]), inv = l_tot != 0.f ? 1.f / l_tot : 0.f;
+                    if (i >= rows_end || l_tot != l_tot) continue;
+                    const int keys = causal_ ? i + 1 : cur.kv_valid;
+#pragma unroll
+                    for (int db = 0; db < 8; ++db) {
+                        const int column = 16 * db + 4 * r4;
+                        V4 v;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float y;
+                            v[e] = FirstNonFinite<T>::found(table[column + e], table[D + column + e], table[2 * D + column + e], keys, y) ? (T)y : (T)(o[db][qb][e] * inv);
+                        }
+                        *(V4*)(out + i * sd.o_row + column) = v;
                     }
                 }
             }
         }
-        if (!more) break;
     }
     MI355_TL(
         wait_vmcnt<0>();   // the stores of this wave have been accepted

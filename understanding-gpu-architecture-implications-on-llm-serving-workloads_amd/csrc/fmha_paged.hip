@@ -28,7 +28,6 @@ namespace mi355 {
 
 namespace pdec {
 typedef float float2v __attribute__((ext_vector_type(2)));
-typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
 constexpr int D = 128;
 constexpr int TK = 32;                       // keys per tile
 constexpr int ROW_BYTES = D * 2;             // 256

@@ -30,7 +30,6 @@
 namespace mi355 {
 
 namespace prow {
-typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
 constexpr int D = 128, ROW_BYTES = D * 2;
 constexpr int WAVES = 8, NTHREADS = WAVES * 64;
 constexpr int NB = 2, WCOLS = 16 * NB;        // columns of a wave

@@ -24,6 +24,7 @@ typedef float float4v __attribute__((ext_vector_type(4)));
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef int int4v __attribute__((ext_vector_type(4)));
 typedef int int2v __attribute__((ext_vector_type(2)));
+typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
 
 #define MI355_LDS __attribute__((address_space(3)))
 #define MI355_GLOBAL __attribute__((address_space(1)))
