@@ -181,7 +181,8 @@ __device__ __forceinline__ void copy16_global_to_lds_at(const void* uniform_base
 // 15.9, 24 x 32/8, 16 over 64 13.8 / 13.1, 12 x 64/8, 16 over 128 18.2 / 17.6.
 // kPacked: sequences of different lengths one behind the other in one batch, with work items of several heads (below); infinities and NaN of V
 // are kept from the rows that do not see them (NonFinite); the sums of probabilities are those of what they are in 32 bits, in fp16 too (on the matrix pipe, which sums up the rounded
-// ones, each up to 2^-11 off, a call takes 3 % less: 16 prompts of up to 1000 rows 88 us, 4 of up to 8192 1035; but the log-sum-exp would have that error in it).
+// ones, each up to 2^-11 off, calls of long prompts take 2 to 4 % less: 4 of up to 8192 rows 1025 us / 981, 2 of up to 2000 of 64/8 heads 101.5 / 98.0, 16 of up to 1000 79.3 /
+// 79.6; but the log-sum-exp would have that error in it).
 enum { kOneWalk = 0, kRanges = 1, kRangesF32 = 2, kFewRows = 3, kPacked = 4 };
 constexpr int kFewRowsMax = 16;
 
@@ -419,7 +420,7 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
             int u = wl;
             if (first == nullptr) {
                 // Forwards and backwards in turn. The workgroups that have an item more than the others take the lightest of the last full rounds, of as many as
-                // make up for that item: a causal one costs about as much as 4 key tiles, and between the ends of a round lie the longest sequence's over the rounds. us, without that /
+                // make up for that item: a causal one costs about as much as 4 key tiles, and between the ends of a round lie the longest sequence's over the rounds. us when it came, without that /
                 // with it: 16 sequences of up to 1000 rows 88 / 83, 6 of up to 606 of 64/8 heads 42.6 / 36.4; with it in all rounds 4 of up to 8192 1079, without 1046, so 1041.
                 const int items = entries * map_.per_rank, rounds = (int)((uint32_t)items / (uint32_t)map_.wgs), rest = items - rounds * map_.wgs;
                 const int spread = max(((packed.list == nullptr ? order.rows[0] : packed.list[0][1]) - 1) / BN, 1);
@@ -1534,8 +1535,8 @@ hipError_t fmha_fwd_dispatch(const void* Q, const void* K, const void* V, void* 
 //
 // A work item is a q tile of up to 8 query heads of a kv head, side by side: 32 rows of 8 heads see fewer keys that none of them sees than 256 rows of one (of 512 rows 147 of
 // 197 k pairs are worked out, 131 k are seen), and a sequence's last tile is a smaller part of it. Bound by the matrix pipes and the vector unit in turn, like one long sequence, and for
-// short ones by the way of an item's operands and results to and from memory. us, 256 rows of a head and a list / now: 16 sequences of up to 1000 rows of 32/8 heads 119 / 83 (565
-// TFLOP/s of those seen), 4 of up to 8192 1091 / 1041 (1180), 64 of up to 200 74 / 52, 3 of up to 77 of 8/2 heads 12.0 / 8.0 (one launch).
+// short ones by the way of an item's operands and results to and from memory. us, 256 rows of a head and a list / now: 16 sequences of up to 1000 rows of 32/8 heads 119 / 77 .. 82 (590
+// TFLOP/s of those seen), 4 of up to 8192 1091 / 1034 (1190), 64 of up to 200 74 / 50, 3 of up to 77 of 8/2 heads 12.0 / 8.0 (one launch).
 // ---------------------------------------------------------------------------------------------------------------
 namespace packed {
 constexpr int THREADS = 1024, WAVES = THREADS / 64;
@@ -1681,9 +1682,10 @@ static hipError_t launch_packed(const T* Q, const T* K, const T* V, T* O, float*
 
 // Whether work items are of 256 (row, head) pairs, whose K and V fragments feed two MFMAs, or of 128, which fill more workgroups and cost less beside their key tiles: by an
 // estimate for sequences of the mean length. us of an item of x key tiles: 128 pairs 3 + 1.1 x, 256 pairs 6 + 1.6 x; a launch of up to 256 items takes as long as one that
-// sees all keys, one of n items as long as n / 256 + 0.75 of the mean. Over 2104 drawn calls (1 .. 64 sequences, 1 .. 6000 rows, 8 .. 64 heads, causal and not) the choice is 0.4 %
-// behind the better one on average, at worst 50 %; 128 throughout 3.5 %, 256 throughout 18 %. us, 128 / 256: 16 sequences of up to 1000 rows, 32/8 heads 91.0 / 86.6, 4 of up to 8192 1302 / 1085;
-// 1 of 512 13.5 / 20.5, 8 of up to 600, 40/8 heads 45.8 / 53.3.
+// sees all keys, one of n items as long as n / 256 + 0.75 of the mean. Over 526 drawn calls (1 .. 64 sequences, 1 .. 6000 rows, 8 .. 64 heads, causal and not) the choice is 0.5 %
+// behind the better one on average, at worst 51 % (55 of up to 55 rows, 16/4 heads 16.4 us for 10.9: 316 items where the mean makes 220); 128 throughout 4.1 %, 256 throughout 17 %. us, 128 / 256:
+// 16 sequences of up to 1000 rows, 32/8 heads 91.0 / 78.3, 4 of up to 8192 1242 / 1035; 1 of 512 13.7 / 20.4, 8 of up to 600, 40/8 heads 42.0 / 49.4. Sequences without rows count into
+// the mean: one of 4096 rows among 63 without takes 148 where it takes 123 by itself, 4 of 8192 among 60 without 1810 either way.
 static bool packed_large_tiles(int rows, int B, int Hq, int Hkv, int causal) {
     const int shift = packed_head_shift(Hq, Hkv), mean = (rows + B - 1) / B, keys = (mean + fmha::BN - 1) / fmha::BN;
     const auto estimate = [&](int tile, float item, float key_tile) {

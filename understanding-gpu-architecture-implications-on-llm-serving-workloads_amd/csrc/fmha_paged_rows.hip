@@ -175,7 +175,8 @@ struct Entries {
 // longest, and the sums up to it. The longest piece is one of the longest sequence's 1 / 1 .. 1 / 64 that is no shorter than an equal share (so that at most two pieces a
 // workgroup are parts of a triple): the one whose heaviest workgroup is expected to have the least to do. Equal shares of the axis, of which most workgroups have two parts, / this, us, 32/8
 // heads (both 1 .. 3 us less since): 32 tokens, 8 sequences of up to 8191 keys 51 / 46, 16 of up to 4097 55 / 54, 32 of up to 2000 59 / 52, 24 of 2000 67 / 50; 64 tokens, 16 of up to 4097
-// 87 / 72, 20 of up to 1000 53 / 37; 64/8 heads, 64 tokens, 16 of up to 4097 125 / 116. More sequences get a workgroup a triple.
+// 87 / 72, 20 of up to 1000 53 / 37; 64/8 heads, 64 tokens, 16 of up to 4097 125 / 116. More sequences get a workgroup a triple, which walks a long one alone: 32 tokens, 64 / 65 / 128 sequences of up to 4097 keys 127 / 149 / 252, one of
+// 16384 keys among others of 200 69 / 259 / 277.
 template <int COLS>
 struct Pieces {
     static constexpr int TK = COLS / 4, HEAD = kPieceKeys / TK, JOIN = kJoinKeys / TK, kLeast = 128 / TK;   // in tiles; kLeast: of a piece

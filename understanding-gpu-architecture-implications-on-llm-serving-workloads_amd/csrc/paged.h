@@ -107,7 +107,8 @@ struct PagedTree {
 constexpr int kTreeWords = kMostDrafted / 32 + 1;   // (odd: rows side by side in LDS lie in different banks)
 
 // The words of drafted token `row` of n, of which the first is key `base` (negative where the sequence is shorter than its draft: the first ones are no keys).
-// `parents` in LDS. Every step of the walk goes to a smaller number.
+// `parents` in LDS. Every step of the walk goes to a smaller number; the last token of a chain walks all of them. us, steps back by 1 .. 8 / a chain: 26 tokens over 300 keys 9.3 /
+// 11.5, 64 over 8191 28.7 / 33.2, 256 over 8191 56 / 77, 32 of 32 sequences of up to 4097 80.8 / 81.7.
 __device__ __forceinline__ void tree_words(MI355_LDS const int* parents, int row, int n, int base, MI355_LDS uint32_t* words) {
     const int skew = base >= 0 ? base & 31 : base;
 #pragma unroll
