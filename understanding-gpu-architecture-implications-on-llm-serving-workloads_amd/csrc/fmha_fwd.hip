@@ -282,8 +282,8 @@ struct PackedItem<true> {
 // some looks at these items again behind its last one, outside the loop over the items (in it such code costs all calls 2-5 %, whether it runs or not). It goes through
 // the values for the first key of each kind in every column (FirstNonFinite). An output that is NaN where its row sees a NaN, or two infinities of different
 // signs, is right; one whose row sees an infinity becomes that. For the others the items are worked out once more with zeros in the place of all such
-// values, and their outputs then become what is found in front of each row. us, 16 prompts of 1000 rows of 32/8 heads (clean: 190 .. 200): a NaN in the first value of each 310, in the
-// middle one 290, in the last one 230, 1 of 1000 elements infinite 600; 4 prompts of up to 8192 (1097) 1340, 1500, 1410, 2510.
+// values, and their outputs then become what is found in front of each row. us, 16 prompts of 1000 rows of 32/8 heads (clean: 177): a NaN in the first value of each 291, in the
+// middle one 281, in the last one 235, 1 of 1000 elements infinite 570; 4 prompts of up to 8192 (1088) 1297, 1468, 1408, 2510; one of 1000, an item a workgroup (20.4), 33, 38, 54.
 template <typename T>
 struct NonFinite {
     static constexpr unsigned short kInfinity = std::is_same<T, half_t>::value ? 0x7c00 : 0x7f80;
@@ -340,7 +340,8 @@ struct FirstNonFinite {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 if (of[kind][e] != kNone) atomicMin((int*)(table + kind * fmha::D + column + e), of[kind][e]);
-        __syncthreads();
+        wait_lgkmcnt<0>();
+        asm volatile("s_barrier" ::: "memory");
 #pragma unroll
         for (int kind = 0; kind < 3; ++kind)
 #pragma unroll
@@ -1092,30 +1093,44 @@ __global__ __launch_bounds__(512, 2) void fmha_fwd_pingpong_kernel(const T* __re
 #pragma unroll 1
             for (int r = nan0; r <= nan1; ++r) {
                 cur = in_scalars(more_items ? item_of(r) : cur);   // (otherwise it is the only one)
-                __syncthreads();
-                for (int i = lane_; i < FirstNonFinite<T>::kInts; i += 64) table[i] = FirstNonFinite<T>::kNone;
-                __syncthreads();
-                const FirstNonFinite<T> first(cur.Kh, cur.Vh, sd.k_row, sd.v_row, min(cur.n_tiles * BN, cur.kv_valid), wave, lane_, table);
-                const bool some = first.some();
                 q_wave0 = cur.q_block0 + wave_row0_;
                 const int rows_end = min(q_wave0 + WQ, rows_of(cur));
                 T* const out = cur.Oh + wave_head_ * sd.o_head;
+                // this wave's outputs, of which a lane has 8 columns of every fourth row: asked for in front of the values, looked at behind them
+                V8 x[WQ / 4];
+#pragma unroll
+                for (int a = 0; a < WQ / 4; ++a) x[a] = *(const V8*)(out + max(min(q_wave0 + 4 * a + r4, rows_end - 1), 0) * sd.o_row + 8 * r16);
+                phase_barrier();   // (the table of the item in front has been read)
+                for (int i = lane_; i < FirstNonFinite<T>::kInts; i += 64) table[i] = FirstNonFinite<T>::kNone;
+                wait_lgkmcnt<0>();
+                phase_barrier();
+                const FirstNonFinite<T> first(cur.Kh, cur.Vh, sd.k_row, sd.v_row, min(cur.n_tiles * BN, cur.kv_valid), wave, lane_, table);
+                const bool some = first.some();
+                uint64_t nans = 0;    // bit 8 a + e
+                uint32_t whole = 0;   // bit a: throughout a row
+#pragma unroll
+                for (int a = 0; a < WQ / 4; ++a) {
+                    uint32_t row = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) row |= NonFinite<T>::nan(x[a][e]) ? 1u << e : 0u;
+                    if (q_wave0 >= rows_end) row = 0;   // (no rows)
+                    nans |= (uint64_t)row << (8 * a);
+                    whole |= (__builtin_amdgcn_ballot_w64(row == 0xff) >> (lane_ & 48) & 0xffff) == 0xffff ? 1u << a : 0u;
+                }
                 bool open = false;   // an output that neither the values that its row sees nor, as far as one can tell, the scores make NaN
 #pragma unroll 1
-                for (int i0 = q_wave0; i0 < rows_end; i0 += 4) {   // four rows, 8 columns a lane
-                    const int i = min(i0 + r4, rows_end - 1);
-                    T* const at = out + i * sd.o_row + 8 * r16;
-                    const V8 x = *(const V8*)at;
-                    bool all = true;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) all = all && NonFinite<T>::nan(x[e]);
-                    all = (__builtin_amdgcn_ballot_w64(all) >> (lane_ & 48) & 0xffff) == 0xffff;   // throughout: the scores may be
+                for (int a = 0; a < WQ / 4; ++a) {
+                    const uint32_t row = (uint32_t)(nans >> (8 * a)) & 0xff;
+                    if (__builtin_amdgcn_ballot_w64(row != 0) == 0) continue;
+                    const int i = min(q_wave0 + 4 * a + r4, rows_end - 1);
+                    const bool all = whole >> a & 1;   // (the scores may be NaN)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         float y;
-                        const bool found = first.found(e, causal_ ? i + 1 : cur.kv_valid, y), none = NonFinite<T>::nan(x[e]);
-                        if (none && found && !all) at[e] = (T)y;
-                        open = open || (none && (all ? some && !(found && y != y) : !found));
+                        const bool found = first.found(e, causal_ ? i + 1 : cur.kv_valid, y), none = row >> e & 1;
+                        if (!none || (found && y != y)) continue;   // (right)
+                        if (found && !all) out[i * sd.o_row + 8 * r16 + e] = (T)y;
+                        open = open || (all ? some : !found);
                     }
                 }
                 if (__builtin_amdgcn_ballot_w64(open) != 0 && lane_ == 0) nan_rounds[2] = r;
